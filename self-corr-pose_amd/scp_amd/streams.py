@@ -16,12 +16,9 @@ probes over all 51 combinations, profiles/r05_packed_fp32_erratum.txt).  hipcc's
   * every file of the library that is not itself a bf16 GEMM is compiled with the packed-fp32 feature switched off (build.py NO_PACKED) and
     a CPU test disassembles the shipped code objects: no packed-fp32 instruction with ANY op_sel in 220 kernels
     (tests/test_capi_symbols.py);
-  * of the 110 ATen / rocprim kernels a step launches none carries the form (libtorch_hip.so scanned: 767 of its kernels do, none of them on
-    this path; profiles/r05_torch_kernel_scan.txt) -- re-scan when torch is upgraded (tools/packed_census.py);
-  * the fp32 GEMM kernels rocBLAS / hipBLASLt can serve the step's remaining library products with (20 169 kernels in 30 gfx950 code
-    objects, helper kernels included) carry the form nowhere but in rocBLAS's complex-single PostGSU reduction, which no fp32 GEMM
-    launches (tools/library_gemm_scan.py, profiles/r06_library_gemm_scan.txt); the scan is stamped with the torch / HIP version and a
-    digest of those files, and an installation the stamp does not describe DEFAULTS TO `serial` (stamp_status below) -- round 6, ADVICE;
+  * the library kernels of the step (ATen, rocprim, the remaining fp32 rocBLAS / hipBLASLt products, RCCL) are held by the screen below, by
+    running them; the installation it ran on is stamped (torch / HIP version and a digest of the GEMM files' names and sizes,
+    tools/library_gemm_scan.py), and an installation the stamp does not describe DEFAULTS TO `serial` (stamp_status below);
   * tests/test_coresidency_gpu.py screens every stage of the B = 32 step (forward AND backward, clip + fused AdamW, a 1-rank RCCL
     all-reduce) and the whole step under a persistent bf16-MFMA load, bit-exact where the stage is deterministic, with two positive
     controls that must FAIL on the box the test runs on (the self-checking erratum kernel; the rasteriser as compiled until round 4).
@@ -32,11 +29,10 @@ STAMP = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def stamp_status():
-    """(ok, why): does the static scan this build ships (tuning/coresidency_stamp.json: torch / HIP version and a digest over the names
-    and sizes of the gfx950 fp32 rocBLAS / hipBLASLt code objects, written by tools/library_gemm_scan.py) describe the installation
-    that is running?  Which library GEMM kernel serves a call is the library's choice (heuristics, TunableOp), so the rule "no kernel
-    of the step carries the erratum form" can only be vouched for per library build: a different torch / ROCm needs a re-scan
-    No GPU and no torch.cuda call needed."""
+    """(ok, why): does the stamp this build ships (tuning/coresidency_stamp.json: torch / HIP version and a digest over the names and
+    sizes of the gfx950 fp32 rocBLAS / hipBLASLt files, written by tools/library_gemm_scan.py) describe the installation that is
+    running?  Which library GEMM kernel serves a call is the library's choice (heuristics, TunableOp), so the co-residency screen can
+    only vouch for the library build it ran beside: a different torch / ROCm needs a new screen.  No GPU and no torch.cuda call needed."""
     import hashlib
     import json
     try:
@@ -68,8 +64,8 @@ def _default_mode():
     if ok:
         return "overlap"
     import warnings
-    warnings.warn("scp_amd.streams: SCP_STREAMS defaults to 'serial' here -- %s; re-run tools/library_gemm_scan.py and "
-                  "tools/packed_census.py for this installation (DESIGN 5.2), or set SCP_STREAMS=overlap" % why)
+    warnings.warn("scp_amd.streams: SCP_STREAMS defaults to 'serial' here -- %s; screen this installation with "
+                  "tests/coresidency.py and renew the stamp (tools/library_gemm_scan.py), or set SCP_STREAMS=overlap" % why)
     return "serial"
 
 

@@ -1,5 +1,6 @@
 """tools/packed_census.py -- per kernel of a built library: packed-fp32 instructions (v_pk_*_f32, with / without op_sel), K-doubled 16-bit
-MFMAs, vector registers.  `python tools/packed_census.py [lib.so]`; tests/test_capi_symbols.py imports census() for the static half of the
+MFMAs, vector registers.  `python tools/packed_census.py [lib.so]` on a library built here from source (installed libraries are refused:
+their code is not read); tests/test_capi_symbols.py imports census() for the static half of the
 co-residency rule: a kernel that does not itself issue bf16 MFMAs carries no packed-fp32 instruction."""
 import os
 import re
@@ -19,7 +20,10 @@ SYM = re.compile(r"^[0-9a-f]+ <([^>]+)>:$")
 
 
 def census(lib=DEFAULT):
-    """{kernel symbol: dict(packed, op_sel, bad, mfma16)} over every gfx950 code object embedded in `lib` (a .so or a .o)"""
+    """{kernel symbol: dict(packed, op_sel, bad, mfma16)} over every gfx950 code object embedded in `lib` (a .so or a .o built here)"""
+    real = os.path.realpath(lib)
+    if real.startswith(("/opt/", "/usr/", "/lib")) or "site-packages" in real or "dist-packages" in real:
+        raise RuntimeError("packed_census: %s is an installed library; only objects built here from source are read" % lib)
     out = {}
     tmp = tempfile.mkdtemp(prefix="scp_census_")
     try:
