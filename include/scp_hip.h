@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define SCP_ABI_VERSION 8
+#define SCP_ABI_VERSION 9
 
 /* enum values = the integer ids the reference passes (functional/soft_rasterize.py:22-25) */
 enum { SCP_DIST_HARD = 0, SCP_DIST_BARYCENTRIC = 1, SCP_DIST_EUCLIDEAN = 2 };
@@ -627,6 +627,54 @@ int scp_image_losses_backward_scale(const float* depth_out, const float* parts, 
 int scp_texture_loss_forward(const float* tex_out, const float* img, const float* mask, int B, int H, int W, float* rowsum, void* stream);
 int scp_texture_loss_backward(const float* tex_out, const float* img, const float* mask, const float* g_tex, int B, int H, int W,
                               float* grad_tex_out, void* stream);
+
+/* ---- ViT operators with gradients ------------------------------------------------------------------------------------------------
+ * The training forms of what a transformer block is made of (vision_transformer_flexible.py:54-132 is an nn.Module: the reference can train
+ * it, its pipeline keeps it frozen).  Tensors are dense rows in fp32 or bf16 (`dtype`), all sums and statistics in fp32, no atomics. */
+enum { SCP_DTYPE_F32 = 0, SCP_DTYPE_BF16 = 1 };
+
+/* LayerNorm over C channels (C <= 8192), the residual add in front of it fused (csrc/layernorm_train.hip).
+ *   forward:  s = x + resid rounded to `dtype` (s = x when resid is NULL), y = (s - mean) rstd gamma + beta; sum_out receives s (NULL
+ *     without resid); stats [rows,2] = (mean, rstd), may be NULL; gamma / beta [C] may be NULL (1 / 0), fp32 or `dtype` (wdtype).
+ *   backward: gx [rows,C] = gradient w.r.t. s (= w.r.t. x and resid) with gsum (may be NULL) added, may be NULL; g_gamma / g_beta [C] fp32,
+ *     each may be NULL.  workspace >= scp_layernorm_backward_workspace(rows, C) bytes when either is wanted. */
+int scp_layernorm_forward(const void* x, const void* resid, const void* gamma, const void* beta, float eps, long rows, int C, int dtype,
+                          int wdtype, void* sum_out, void* y, float* stats, void* stream);
+size_t scp_layernorm_backward_workspace(long rows, int C);
+int scp_layernorm_backward(const void* s, const void* gamma, const void* gy, const void* gsum, const float* stats, long rows, int C, int dtype,
+                           int wdtype, void* gx, float* g_gamma, float* g_beta, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of `queries` tokens to `keys` tokens of another set (csrc/cross_attn.hip): out = softmax(scale q k^T over the keys whose
+ * key_mask byte is not zero) v per head; query head h reads key / value head h / (heads / kv_heads).  q, k, v, g_out are addressed through
+ * strides in ELEMENTS (batch, token, head; a stride may be 0; channels contiguous; strides and pointers multiples of 16 bytes); out, g_q
+ * [batch,queries,heads,head_dim], g_k, g_v [batch,keys,kv_heads,head_dim] are contiguous.  key_mask [batch,keys] or NULL.  A batch entry
+ * without a key gives zeros and zero gradients; values stored at masked keys, NaN included, never reach a result.
+ *   lse [batch,kv_heads,queries * heads / kv_heads]: log2 of the softmax denominator per row, kept for the backward pass; may be NULL.
+ *   head_dim: a multiple of 8, <= 128.  g_q / g_k / g_v may each be NULL. */
+typedef struct scp_cross_attn_params {
+    int batch, queries, keys, heads, kv_heads, head_dim, dtype;
+    float scale;
+    long long q_stride[3], k_stride[3], v_stride[3], g_stride[3];      /* g_stride: g_out's (backward only) */
+} scp_cross_attn_params;
+size_t scp_cross_attention_forward_workspace(const scp_cross_attn_params* p);
+int scp_cross_attention_forward(const void* q, const void* k, const void* v, const unsigned char* key_mask, const scp_cross_attn_params* p,
+                                void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+size_t scp_cross_attention_backward_workspace(const scp_cross_attn_params* p);
+int scp_cross_attention_backward(const void* q, const void* k, const void* v, const unsigned char* key_mask, const void* out, const float* lse,
+                                 const void* g_out, const scp_cross_attn_params* p, void* g_q, void* g_k, void* g_v, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/* Activation checkpoints in 8 bits (csrc/act8.hip): x [rows,C] -> codes [rows,C] int8 and exps [rows,ceil(C/32)]; 32 neighbouring
+ * channels share the step 2^(exps - 127), value = code * step; exps = 255: the group held an infinity or a NaN (every value reads as NaN).
+ *   gelu8: y = erf GELU of x, with the checkpoint of x written in the same pass (codes and exps NULL: none); backward: gx = gy gelu'(value).
+ *   weight_grad8 (csrc/act8_wgrad.hip): gw [N,K] = sum over rows of gy[:,n] value[:,k], gb [N] (may be NULL) = sum over rows of gy; fp32. */
+int scp_pack8(const void* x, long rows, int C, int dtype, signed char* codes, unsigned char* exps, void* stream);
+int scp_unpack8(const signed char* codes, const unsigned char* exps, long rows, int C, int dtype, void* x, void* stream);
+int scp_gelu8_forward(const void* x, long rows, int C, int dtype, void* y, signed char* codes, unsigned char* exps, void* stream);
+int scp_gelu8_backward(const signed char* codes, const unsigned char* exps, const void* gy, long rows, int C, int dtype, void* gx, void* stream);
+size_t scp_weight_grad8_workspace(long rows, int N, int K, int dtype);
+int scp_weight_grad8(const void* gy, const signed char* codes, const unsigned char* exps, long rows, int N, int K, int dtype, float* gw,
+                     float* gb, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -12,7 +12,7 @@ import torch
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 # SCP_HIP_LIB: an alternative build of the same library (A/B of kernel variants from tools/); the default is the in-tree build
 LIB_PATH = os.environ.get("SCP_HIP_LIB") or os.path.join(_PKG, "lib", "libscp_hip.so")
-ABI_VERSION = 8
+ABI_VERSION = 9
 CONV_PLANES_TILE = 32     # include/scp_hip.h: SCP_CONV_PLANES_TILE
 
 
@@ -56,6 +56,15 @@ class CropDesc(ctypes.Structure):
                 ("in_h", ctypes.c_int), ("in_w", ctypes.c_int), ("pad_top", ctypes.c_int), ("pad_left", ctypes.c_int),
                 ("virt_h", ctypes.c_int), ("virt_w", ctypes.c_int)]
 
+
+class CrossAttnParams(ctypes.Structure):
+    """struct scp_cross_attn_params"""
+    _fields_ = [("batch", ctypes.c_int), ("queries", ctypes.c_int), ("keys", ctypes.c_int), ("heads", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("head_dim", ctypes.c_int), ("dtype", ctypes.c_int), ("scale", ctypes.c_float), ("q_stride", ctypes.c_longlong * 3),
+                ("k_stride", ctypes.c_longlong * 3), ("v_stride", ctypes.c_longlong * 3), ("g_stride", ctypes.c_longlong * 3)]
+
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1}      # include/scp_hip.h: SCP_DTYPE_*
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -165,6 +174,19 @@ SYMBOLS = {
     "scp_vit_attention_split_forward_presplit": (ctypes.c_int, [_P, _P, _P, _I, _I, _I, _I, _F, _P, _P, _P, ctypes.c_size_t, _P]),
     "scp_vit_linear_qkv": (ctypes.c_int, [_P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _I, _F, _I, _P]),
     "scp_vit_attention_split_forward": (ctypes.c_int, [_P, _P, _I, _I, _I, _I, _F, _P, _P, _I, _P, ctypes.c_size_t, _P]),
+    "scp_layernorm_forward": (ctypes.c_int, [_P] * 4 + [_F, ctypes.c_long, _I, _I, _I] + [_P] * 4),
+    "scp_layernorm_backward_workspace": (ctypes.c_size_t, [ctypes.c_long, _I]),
+    "scp_layernorm_backward": (ctypes.c_int, [_P] * 5 + [ctypes.c_long, _I, _I, _I] + [_P] * 4 + [ctypes.c_size_t, _P]),
+    "scp_cross_attention_forward_workspace": (ctypes.c_size_t, [ctypes.POINTER(CrossAttnParams)]),
+    "scp_cross_attention_forward": (ctypes.c_int, [_P] * 4 + [ctypes.POINTER(CrossAttnParams)] + [_P] * 3 + [ctypes.c_size_t, _P]),
+    "scp_cross_attention_backward_workspace": (ctypes.c_size_t, [ctypes.POINTER(CrossAttnParams)]),
+    "scp_cross_attention_backward": (ctypes.c_int, [_P] * 7 + [ctypes.POINTER(CrossAttnParams)] + [_P] * 4 + [ctypes.c_size_t, _P]),
+    "scp_pack8": (ctypes.c_int, [_P, ctypes.c_long, _I, _I, _P, _P, _P]),
+    "scp_unpack8": (ctypes.c_int, [_P, _P, ctypes.c_long, _I, _I, _P, _P]),
+    "scp_gelu8_forward": (ctypes.c_int, [_P, ctypes.c_long, _I, _I] + [_P] * 4),
+    "scp_gelu8_backward": (ctypes.c_int, [_P, _P, _P, ctypes.c_long, _I, _I, _P, _P]),
+    "scp_weight_grad8_workspace": (ctypes.c_size_t, [ctypes.c_long, _I, _I, _I]),
+    "scp_weight_grad8": (ctypes.c_int, [_P, _P, _P, ctypes.c_long, _I, _I, _I, _P, _P, _P, ctypes.c_size_t, _P]),
     "scp_dual_softmax_backward": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _F, _P, _P, _P, _P, _I, _F,
                                                 _I, _I, _I, _P]),
 }

@@ -1,0 +1,388 @@
+"""scp_amd/vit_ops.py -- the operators of a transformer block WITH gradients: what training a ViT, or a decoder that attends to its tokens,
+needs next to the forward-only operators of scp_amd.dino (the reference's blocks, vision_transformer_flexible.py:54-132, are ordinary
+modules; its pipeline keeps them frozen).
+
+  layer_norm       LayerNorm, alone or with the residual add in front of it          (csrc/layernorm_train.hip)
+  cross_attention  queries of one length against keys / values of another            (csrc/cross_attn.hip)
+  gelu8            erf GELU whose input is kept for the backward pass in 8 bits       (csrc/act8.hip)
+  linear8          linear layer whose input is kept for the backward pass in 8 bits   (csrc/act8_wgrad.hip)
+  pack8, Packed8, weight_grad8: the 8-bit checkpoint by itself, and the weight gradient taken from it
+
+float32 and bfloat16 GPU tensors on the current device only, anything else raises RuntimeError (no CPU fallback).  Statistics, softmax and
+sums are fp32; results are rounded once to the type they are returned in.  No atomics: a call repeated gives the same bits.  Launches
+go to the current stream; workspaces come from torch's allocator, so a call can be captured into a HIP graph.  Once differentiable."""
+import ctypes
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import capi
+
+_NULL = ctypes.c_void_p(0)
+
+
+def _tensor(t, name, dtypes=(torch.float32, torch.bfloat16)):
+    if not torch.is_tensor(t) or not t.is_cuda:
+        raise RuntimeError("%s must be a CUDA tensor (no CPU fallback)" % name)
+    if t.dtype not in dtypes:
+        raise RuntimeError("%s must be %s, not %s" % (name, " or ".join(str(d)[6:] for d in dtypes), t.dtype))
+    if t.device.index != torch.cuda.current_device():
+        raise RuntimeError("%s lives on cuda:%d but the current device is cuda:%d (torch.cuda.set_device first)"
+                           % (name, t.device.index, torch.cuda.current_device()))
+
+
+def _ptr(t):
+    return _NULL if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+def _wants_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+# ---- layer norm ------------------------------------------------------------------------------------------------------------------------
+def _norm_forward(x, residual, weight, bias, eps, want_stats):
+    c = x.shape[-1]
+    rows = x.numel() // c
+    y = torch.empty_like(x)
+    total = None if residual is None else torch.empty_like(x)
+    stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if want_stats else None
+    if rows:
+        w = weight if weight is not None else bias
+        wdtype = capi.DTYPES[x.dtype if w is None else w.dtype]
+        capi.check(capi.lib().scp_layernorm_forward(_ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), eps, rows, c, capi.DTYPES[x.dtype], wdtype,
+                                                    _ptr(total), _ptr(y), _ptr(stats), capi.current_stream()), "scp_layernorm_forward")
+    return total, y, stats
+
+
+class _LayerNorm(Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps):
+        total, y, stats = _norm_forward(x, residual, weight, bias, eps, True)
+        ctx.save_for_backward(x if total is None else total, weight, stats)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.has_residual = residual is not None
+        ctx.set_materialize_grads(False)
+        return (total, y) if ctx.has_residual else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        gsum, gy = grads if ctx.has_residual else (None, grads[0])
+        s, weight, stats = ctx.saved_tensors
+        want_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        want_w, want_b = ctx.needs_input_grad[2], ctx.needs_input_grad[3]
+        if gy is None:                                           # only the sum was used
+            gx = gsum if want_x else None
+            return gx, gx if ctx.has_residual else None, None, None, None
+        c = s.shape[-1]
+        rows = s.numel() // c
+        gy = gy.contiguous()
+        gsum = None if gsum is None else gsum.contiguous()
+        gx = torch.empty_like(s) if want_x else None
+        if rows:
+            gw = torch.empty(c, dtype=torch.float32, device=s.device) if want_w else None
+            gb = torch.empty(c, dtype=torch.float32, device=s.device) if want_b else None
+            L = capi.lib()
+            nbytes = L.scp_layernorm_backward_workspace(rows, c) if want_w or want_b else 0
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=s.device) if nbytes else None
+            wdtype = capi.DTYPES[s.dtype if weight is None else weight.dtype]
+            capi.check(L.scp_layernorm_backward(_ptr(s), _ptr(weight), _ptr(gy), _ptr(gsum), _ptr(stats), rows, c, capi.DTYPES[s.dtype], wdtype,
+                                                _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), nbytes, capi.current_stream()), "scp_layernorm_backward")
+        else:
+            gw = torch.zeros(c, dtype=torch.float32, device=s.device) if want_w else None
+            gb = torch.zeros(c, dtype=torch.float32, device=s.device) if want_b else None
+        gw = None if gw is None else gw.to(weight.dtype)
+        gb = None if gb is None else gb.to(ctx.bias_dtype)
+        return gx, gx if ctx.has_residual else None, gw, gb, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-6, residual=None):
+    """y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension (biased variance, at most 8192 channels).  weight / bias
+    [C], float32 or of x's type, None = 1 / 0.  With `residual` (x's shape and type): s = x + residual is rounded to x's type and
+    normalised, and (s, y) is returned -- the residual stream and its normalised copy in one pass, as scp_amd.dino.add_layernorm does
+    for the frozen ViT.  Any strides; the results are contiguous."""
+    _tensor(x, "layer_norm: x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError("layer_norm: x needs a last dimension of at least one channel")
+    c = x.shape[-1]
+    if c > 8192:
+        raise RuntimeError("layer_norm: at most 8192 channels, got %d" % c)
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _tensor(t, "layer_norm: " + name, (torch.float32, x.dtype))
+            if t.dim() != 1 or t.shape[0] != c:
+                raise RuntimeError("layer_norm: %s must have %d entries" % (name, c))
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise RuntimeError("layer_norm: weight and bias must have one type")
+    if residual is not None:
+        _tensor(residual, "layer_norm: residual", (x.dtype,))
+        if residual.shape != x.shape:
+            raise RuntimeError("layer_norm: residual must have x's shape %s, not %s" % (tuple(x.shape), tuple(residual.shape)))
+        residual = residual.contiguous()
+    x = x.contiguous()
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if _wants_grad(x, residual, weight, bias):
+        return _LayerNorm.apply(x, residual, weight, bias, float(eps))
+    total, y, _ = _norm_forward(x, residual, weight, bias, float(eps), False)
+    return y if residual is None else (total, y)
+
+
+# ---- cross attention ---------------------------------------------------------------------------------------------------------------------
+def _addressable(t):
+    """t itself when the kernels can address it (channels contiguous, pointer and strides multiples of 16 bytes), else a contiguous copy"""
+    unit = 16 // t.element_size()
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(s % unit for s in t.stride()[:3]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)      # contiguous() would return a misaligned tensor as it is
+
+
+def _attn_params(q, k, v, scale, g=None):
+    p = capi.CrossAttnParams()
+    p.batch, p.queries, p.heads, p.head_dim = q.shape
+    p.keys, p.kv_heads = k.shape[1], k.shape[2]
+    p.dtype, p.scale = capi.DTYPES[q.dtype], scale
+    for f, t in (("q_stride", q), ("k_stride", k), ("v_stride", v), ("g_stride", g)):
+        if t is not None:
+            getattr(p, f)[:] = t.stride()[:3]
+    return p
+
+
+def _attn_forward(q, k, v, mask, scale, want_lse):
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=q.device) if want_lse else None
+    if out.numel() == 0:
+        return out, lse
+    if k.shape[1] == 0:
+        return out.zero_(), lse
+    L = capi.lib()
+    p = _attn_params(q, k, v, scale)
+    nbytes = L.scp_cross_attention_forward_workspace(ctypes.byref(p))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    capi.check(L.scp_cross_attention_forward(_ptr(q), _ptr(k), _ptr(v), _ptr(mask), ctypes.byref(p), _ptr(out), _ptr(lse), _ptr(ws), nbytes,
+                                             capi.current_stream()), "scp_cross_attention_forward")
+    return out, lse
+
+
+class _CrossAttention(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, mask, scale):
+        out, lse = _attn_forward(q, k, v, mask, scale, True)
+        ctx.save_for_backward(q, k, v, mask, out, lse)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        q, k, v, mask, out, lse = ctx.saved_tensors
+        want = ctx.needs_input_grad[:3]
+        gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((q, k, v), want))
+        if q.numel() == 0 or k.shape[1] == 0:                   # no query or no key: nothing depends on the other side
+            return tuple(None if t is None else t.zero_() for t in (gq, gk, gv)) + (None, None)
+        g = _addressable(g)
+        L = capi.lib()
+        p = _attn_params(q, k, v, ctx.scale, g)
+        nbytes = L.scp_cross_attention_backward_workspace(ctypes.byref(p))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        capi.check(L.scp_cross_attention_backward(_ptr(q), _ptr(k), _ptr(v), _ptr(mask), _ptr(out), _ptr(lse), _ptr(g), ctypes.byref(p), _ptr(gq),
+                                                  _ptr(gk), _ptr(gv), _ptr(ws), nbytes, capi.current_stream()), "scp_cross_attention_backward")
+        return gq, gk, gv, None, None
+
+
+def cross_attention(q, k, v, scale=None, key_mask=None):
+    """softmax(scale * q k^T) v per head: q [B, Nq, H, D] against an encoder's k, v [B, Nk, Hkv, D] of another length -> [B, Nq, H, D]
+    (contiguous).  H a multiple of Hkv: query head h reads key / value head h // (H // Hkv).  D a multiple of 8, at most 128.  `scale`
+    defaults to D ** -0.5.  `key_mask` (bool [B, Nk], True = attend): an image's padding; values stored at masked keys, NaN included,
+    reach no result; a batch entry without a key gives zeros, and zero gradients.  Any strides (slices of a fused qkv projection, an
+    expanded batch); gradients for q, k and v."""
+    _tensor(q, "cross_attention: q")
+    for t, name in ((k, "k"), (v, "v")):
+        _tensor(t, "cross_attention: " + name, (q.dtype,))
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise RuntimeError("cross_attention: q, k and v must be [batch, tokens, heads, channels]")
+    b, nq, h, d = q.shape
+    nk, hk = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise RuntimeError("cross_attention: q %s does not go with k %s and v %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if hk == 0 or h % hk:
+        raise RuntimeError("cross_attention: %d query heads are no multiple of %d key heads" % (h, hk))
+    if d < 8 or d > 128 or d % 8:
+        raise RuntimeError("cross_attention: head dimension %d; a multiple of 8 up to 128 is needed" % d)
+    mask = None
+    if key_mask is not None:
+        _tensor(key_mask, "cross_attention: key_mask", (torch.bool,))
+        if key_mask.shape != (b, nk):
+            raise RuntimeError("cross_attention: key_mask must be [%d, %d], not %s" % (b, nk, tuple(key_mask.shape)))
+        mask = key_mask.contiguous()
+    scale = float(d) ** -0.5 if scale is None else float(scale)
+    q, k, v = _addressable(q), _addressable(k), _addressable(v)
+    if _wants_grad(q, k, v):
+        return _CrossAttention.apply(q, k, v, mask, scale)
+    return _attn_forward(q, k, v, mask, scale, False)[0]
+
+
+# ---- 8-bit activation checkpoints ----------------------------------------------------------------------------------------------------------
+class Packed8:
+    """An activation [..., C] held in 8 bits: `codes` int8 of its shape and `exps` uint8 [..., ceil(C / 32)]; 32 neighbouring channels share
+    the step 2 ** (exps - 127), value = code * step (exact in float32 and bfloat16).  exps 255: the group held an infinity or a NaN."""
+
+    def __init__(self, codes, exps, dtype):
+        self.codes, self.exps, self.dtype = codes, exps, dtype
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    def nbytes(self):
+        return self.codes.numel() + self.exps.numel()
+
+    def unpack(self, dtype=None):
+        """the values the codes stand for, in `dtype` (default: the type that was packed)"""
+        dtype = self.dtype if dtype is None else dtype
+        if dtype not in capi.DTYPES:
+            raise RuntimeError("Packed8.unpack: float32 or bfloat16, not %s" % dtype)
+        _check_packed(self, "Packed8.unpack")
+        out = torch.empty(self.codes.shape, dtype=dtype, device=self.codes.device)
+        if out.numel():
+            c = out.shape[-1]
+            capi.check(capi.lib().scp_unpack8(_ptr(self.codes), _ptr(self.exps), out.numel() // c, c, capi.DTYPES[dtype], _ptr(out),
+                                              capi.current_stream()), "scp_unpack8")
+        return out
+
+
+def _packed_like(x):
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    exps = torch.empty(tuple(x.shape[:-1]) + ((x.shape[-1] + 31) // 32,), dtype=torch.uint8, device=x.device)
+    return codes, exps
+
+
+def _check_packed(p, what):
+    _tensor(p.codes, what + ": codes", (torch.int8,))
+    _tensor(p.exps, what + ": exps", (torch.uint8,))
+    if p.codes.dim() < 1 or tuple(p.exps.shape) != tuple(p.codes.shape[:-1]) + ((p.codes.shape[-1] + 31) // 32,):
+        raise RuntimeError("%s: exps %s do not go with codes %s" % (what, tuple(p.exps.shape), tuple(p.codes.shape)))
+    if not (p.codes.is_contiguous() and p.exps.is_contiguous()):
+        raise RuntimeError("%s: codes and exps must be contiguous" % what)
+
+
+def _check_rows(x, what):
+    _tensor(x, what)
+    if x.dim() < 1 or x.shape[-1] < 1 or x.shape[-1] > 1 << 24:
+        raise RuntimeError("%s needs a last dimension of 1 to 2^24 channels" % what)
+
+
+def pack8(x):
+    """x [..., C] -> Packed8: per 32 channels a power-of-two step with max|x| in [64, 128) steps, codes rounded to nearest (ties to
+    even) and clamped to +-127.  1 + 1/32 bytes per value; not differentiable (it is what an autograd node keeps)."""
+    _check_rows(x, "pack8: x")
+    x = x.detach().contiguous()
+    codes, exps = _packed_like(x)
+    if x.numel():
+        c = x.shape[-1]
+        capi.check(capi.lib().scp_pack8(_ptr(x), x.numel() // c, c, capi.DTYPES[x.dtype], _ptr(codes), _ptr(exps), capi.current_stream()), "scp_pack8")
+    return Packed8(codes, exps, x.dtype)
+
+
+def _gelu_forward(x, keep):
+    y = torch.empty_like(x)
+    codes, exps = _packed_like(x) if keep else (None, None)
+    if x.numel():
+        c = x.shape[-1]
+        capi.check(capi.lib().scp_gelu8_forward(_ptr(x), x.numel() // c, c, capi.DTYPES[x.dtype], _ptr(y), _ptr(codes), _ptr(exps),
+                                                capi.current_stream()), "scp_gelu8_forward")
+    return y, codes, exps
+
+
+class _Gelu8(Function):
+    @staticmethod
+    def forward(ctx, x):
+        y, codes, exps = _gelu_forward(x, True)
+        ctx.save_for_backward(codes, exps)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        codes, exps = ctx.saved_tensors
+        gy = gy.contiguous()
+        gx = torch.empty_like(gy)
+        if gy.numel():
+            c = gy.shape[-1]
+            capi.check(capi.lib().scp_gelu8_backward(_ptr(codes), _ptr(exps), _ptr(gy), gy.numel() // c, c, capi.DTYPES[gy.dtype], _ptr(gx),
+                                                     capi.current_stream()), "scp_gelu8_backward")
+        return gx
+
+
+def gelu8(x):
+    """erf GELU of x [..., C] (the MLP's activation, vision_transformer_flexible.py:54-70).  The backward pass takes the slope at the
+    8-bit checkpoint of x instead of keeping x: 1 + 1/32 bytes per value held between the passes.  The forward value is exact."""
+    _check_rows(x, "gelu8: x")
+    x = x.contiguous()
+    if _wants_grad(x):
+        return _Gelu8.apply(x)
+    return _gelu_forward(x, False)[0]
+
+
+def weight_grad8(grad, packed, bias=True):
+    """(gw [N, K], gb [N] or None) in float32 of a linear layer y = x w^T + b from grad = gy [..., N] and the 8-bit checkpoint of x
+    [..., K]: gw = sum over rows gy[:, n] x8[:, k], gb = sum over rows gy."""
+    _tensor(grad, "weight_grad8: grad")
+    if not isinstance(packed, Packed8):
+        raise RuntimeError("weight_grad8: packed must be a Packed8 (scp_amd.vit_ops.pack8)")
+    _check_packed(packed, "weight_grad8: packed")
+    if grad.dim() < 1 or grad.shape[:-1] != packed.shape[:-1] or grad.shape[-1] < 1 or packed.shape[-1] < 1:
+        raise RuntimeError("weight_grad8: grad %s does not go with a packed input %s" % (tuple(grad.shape), tuple(packed.shape)))
+    n, k = grad.shape[-1], packed.shape[-1]
+    rows = grad.numel() // n
+    gw = torch.empty(n, k, dtype=torch.float32, device=grad.device)
+    gb = torch.empty(n, dtype=torch.float32, device=grad.device) if bias else None
+    if rows == 0:
+        return gw.zero_(), None if gb is None else gb.zero_()
+    grad = grad.detach().contiguous()
+    L = capi.lib()
+    dt = capi.DTYPES[grad.dtype]
+    nbytes = L.scp_weight_grad8_workspace(rows, n, k, dt)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device) if nbytes else None
+    capi.check(L.scp_weight_grad8(_ptr(grad), _ptr(packed.codes), _ptr(packed.exps), rows, n, k, dt, _ptr(gw), _ptr(gb), _ptr(ws), nbytes,
+                                  capi.current_stream()), "scp_weight_grad8")
+    return gw, gb
+
+
+class _Linear8(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        p = pack8(x) if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else None
+        ctx.save_for_backward(weight, None if p is None else p.codes, None if p is None else p.exps)
+        ctx.x_dtype = x.dtype
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return torch.nn.functional.linear(x, weight, bias)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        weight, codes, exps = ctx.saved_tensors
+        gx = gy.matmul(weight) if ctx.needs_input_grad[0] else None
+        gw = gb = None
+        if codes is not None:
+            gw, gb = weight_grad8(gy, Packed8(codes, exps, ctx.x_dtype), bias=ctx.needs_input_grad[2])
+            gw = gw.to(weight.dtype) if ctx.needs_input_grad[1] else None
+            gb = None if gb is None else gb.to(ctx.bias_dtype)
+        return gx, gw, gb
+
+
+def linear8(x, weight, bias=None):
+    """x [..., K] @ weight [N, K]^T + bias, with x kept for the weight gradient in 8 bits (weight_grad8).  One type for all three.  The
+    forward product and the input's gradient are plain library products at full precision; nothing else is saved."""
+    _check_rows(x, "linear8: x")
+    _tensor(weight, "linear8: weight", (x.dtype,))
+    if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] < 1:
+        raise RuntimeError("linear8: weight %s does not go with x %s" % (tuple(weight.shape), tuple(x.shape)))
+    if bias is not None:
+        _tensor(bias, "linear8: bias", (x.dtype,))
+        if bias.dim() != 1 or bias.shape[0] != weight.shape[0]:
+            raise RuntimeError("linear8: bias must have %d entries" % weight.shape[0])
+    if _wants_grad(x, weight, bias):
+        return _Linear8.apply(x, weight, bias)
+    return torch.nn.functional.linear(x, weight, bias)
