@@ -1,0 +1,681 @@
+// self-corr-pose_amd/csrc/attn_core.h -- matrix-core kernels of csrc/cross_attn.hip, shared by its fp32 and bf16 instantiations.
+//
+// One skeleton serves forward, query gradient and key / value gradient: a wavefront keeps 32 columns (queries, or keys) STATIONARY in
+// registers, lane l31 = lane & 31 owning column l31, and streams 32-row blocks of the other side through LDS.
+//   a dot product block   D[row][col] = X[row][:] . F[col][:]  comes out with the rows in the accumulator registers
+//     (row = (reg & 3) + 8 (reg >> 2) + 4 half, half = lane >> 5), so softmax statistics of a column are lane-local;
+//   a product over rows   Acc[d][col] += X[row][d] P[row][col]  takes P from exactly those registers: its row order inside a matrix
+//     instruction is the order in which the accumulators already hold the rows, and X comes transposed out of LDS in that order
+//     (bf16: ds_read_b64_tr_b16, fp32: 32 consecutive floats per half-wavefront).
+// forward:           stationary Q,     streamed K, V;   Acc = o^T  += V^T p
+// query gradient:    stationary Q, gO, streamed K, V;   Acc = gq^T += K^T gs
+// key/value gradient: stationary K, V, streamed Q, gO;  Acc = gk^T += Q^T gs,  Acc2 = gv^T += gO^T p
+// bf16 runs on v_mfma_f32_32x32x16_bf16 (p and gs rounded to bf16 for their product: one operand of it has to be bf16, and the result is
+// rounded to bf16 anyway), fp32 on v_mfma_f32_32x32x2_f32.
+//
+// LDS tiles are filled by buffer loads that write LDS directly, 16 bytes per lane.  A lane whose row is masked, past the end, or whose
+// channel is past head_dim gets an out-of-range offset: the hardware writes zeros, so nothing stored there can reach a product.  The
+// tile's image is swizzled through the SOURCE address (16-byte chunk `slot ^ f(row)`), such that both reads of it -- 16 consecutive rows at
+// one chunk, 4 consecutive rows at two -- touch each bank once.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "scp_common.h"
+
+namespace scp_attn {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct Args {
+    const void *q, *k, *v, *go;
+    const unsigned char* mask;
+    const void* o_in;
+    void *o, *gq, *gk, *gv;
+    float *lse, *delta;
+    float *part_o, *part_ml;              // split over the keys: [split][bh][R][D], [split][bh][R][2]
+    long qs[3], ks[3], vs[3], gs[3];      // strides in elements: batch, token, head
+    int BH, Nq, Nk, Hk, G, D;
+    int nsplit, keys_per_split;           // keys_per_split: a multiple of the tile
+    float scale;
+};
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float RESCALE_THR = 8.f;        // the accumulator is rescaled only when the maximum grows by more than 2^8
+constexpr unsigned OUT_OF_RANGE = 0x80000000u;
+
+__device__ __forceinline__ int acc_row(int reg, int half) { return (reg & 3) + 8 * (reg >> 2) + 4 * half; }
+__device__ __forceinline__ float other_half(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return (threadIdx.x & 32) ? __uint_as_float(r[0]) : __uint_as_float(r[1]);
+}
+
+// rows of a [32 n][DP] tile in LDS, 16-byte chunks
+template <typename T, int DP> struct Tile {
+    static constexpr int CH = 16 / sizeof(T);          // elements per chunk
+    static constexpr int CPR = DP / CH;                // chunks per row
+    static __device__ __forceinline__ int swizzle(int chunk, int row) {
+        if constexpr (sizeof(T) == 2) {
+            if constexpr (CPR == 4) return chunk ^ ((row >> 2) & 3);
+            else if constexpr (CPR == 8) return chunk ^ ((row & 2) | (row & 4) | ((row >> 3) & 1));
+            else if constexpr (CPR == 12) { const int s = chunk + ((row >> 2) & 3); return s >= 12 ? s - 12 : s; }
+            else return chunk ^ (((row & 7) << 1) | ((row >> 3) & 1));
+        } else {
+            if constexpr (CPR == 16 || CPR == 32) return chunk ^ (row & 15);
+            else return chunk ^ ((row >> 1) & 7);
+        }
+    }
+    static __device__ __forceinline__ int unswizzle(int slot, int row) {
+        if constexpr (sizeof(T) == 2 && CPR == 12) { const int s = slot - ((row >> 2) & 3); return s < 0 ? s + 12 : s; }
+        else return swizzle(slot, row);
+    }
+    static __device__ __forceinline__ int at(int row, int chunk) { return (row * CPR + swizzle(chunk, row)) * CH; }
+};
+
+template <typename T, int DP> struct Mma;
+
+template <int DP> struct Mma<__bf16, DP> {
+    typedef __bf16 T;
+    typedef Tile<T, DP> L;
+    static constexpr int DB = DP / 32;
+    struct Frag { bf16x8 f[DP / 16]; };
+    static __device__ __forceinline__ void load(Frag& x, const T* row, bool valid, int D, float sign) {
+        const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++) {
+            bf16x8 v = {};
+            if (valid && 16 * i + 8 * half < D) v = *reinterpret_cast<const bf16x8*>(row + 16 * i + 8 * half);
+            x.f[i] = sign < 0.f ? -v : v;
+        }
+    }
+    // rows r0 .. r0+31 of `t` times the stationary columns
+    static __device__ __forceinline__ f32x16 dot(const T* t, int r0, const Frag& x) {
+        const int half = (threadIdx.x >> 5) & 1, row = r0 + (threadIdx.x & 31);
+        f32x16 acc = {};
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++) {
+            const bf16x8 a = *reinterpret_cast<const bf16x8*>(t + L::at(row, 2 * i + half));
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, x.f[i], acc, 0, 0, 0);
+        }
+        return acc;
+    }
+    // a[db][d][col] += sum_row t[r0 + row][32 db + d] p[row][col]
+    static __device__ __forceinline__ void add(f32x16 (&a)[DB], const T* t, int r0, const f32x16& p) {
+        const int lane = threadIdx.x & 63, i = lane & 15, half = lane >> 5, cg = (lane >> 4) & 1;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            bf16x8 b;
+#pragma unroll
+            for (int j = 0; j < 8; j++) b[j] = (__bf16)p[8 * s + j];
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                bf16x4 h[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int row = r0 + 16 * s + 8 * u + 4 * half + (i >> 2);
+                    const T* at = t + L::at(row, 4 * db + 2 * cg + ((i & 3) >> 1)) + 4 * (i & 1);
+                    h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)at);
+                }
+                const bf16x8 w = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+                a[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, b, a[db], 0, 0, 0);
+            }
+        }
+    }
+    static __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+        const bf16x4 v = {(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
+        *reinterpret_cast<bf16x4*>(p) = v;
+    }
+};
+
+template <int DP> struct Mma<float, DP> {
+    typedef float T;
+    typedef Tile<T, DP> L;
+    static constexpr int DB = DP / 32;
+    struct Frag { f32x4 f[DP / 8]; };
+    static __device__ __forceinline__ void load(Frag& x, const T* row, bool valid, int D, float sign) {
+        const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+        for (int i = 0; i < DP / 8; i++) {
+            f32x4 v = {};
+            if (valid && 8 * i + 4 * half < D) v = *reinterpret_cast<const f32x4*>(row + 8 * i + 4 * half);
+            x.f[i] = sign < 0.f ? -v : v;
+        }
+    }
+    static __device__ __forceinline__ f32x16 dot(const T* t, int r0, const Frag& x) {
+        const int half = (threadIdx.x >> 5) & 1, row = r0 + (threadIdx.x & 31);
+        f32x16 acc = {};
+#pragma unroll
+        for (int i = 0; i < DP / 8; i++) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(t + L::at(row, 2 * i + half));
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[c], x.f[i][c], acc, 0, 0, 0);
+        }
+        return acc;
+    }
+    static __device__ __forceinline__ void add(f32x16 (&a)[DB], const T* t, int r0, const f32x16& p) {
+        const int half = (threadIdx.x >> 5) & 1, l31 = threadIdx.x & 31;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const int row = r0 + acc_row(r, half);
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                const int d = 32 * db + l31;
+                a[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(t[L::at(row, d >> 2) + (d & 3)], p[r], a[db], 0, 0, 0);
+            }
+        }
+    }
+    static __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+        const f32x4 v = {a, b, c, d};
+        *reinterpret_cast<f32x4*>(p) = v;
+    }
+};
+
+// rows of one head in global memory: row r is token r / G (of stride ts) and head r % G (of stride hs) behind `base`
+struct Rows {
+    const char* base;
+    long ts, hs;          // bytes
+    int G;
+    __device__ __forceinline__ const char* row(int r) const {
+        if (G == 1) return base + r * ts;
+        const int n = r / G;
+        return base + n * ts + (r - n * G) * hs;
+    }
+};
+template <typename T> __device__ __forceinline__ Rows rows_of(const void* p, const long* st, int b, int h, int G) {
+    return {reinterpret_cast<const char*>(static_cast<const T*>(p) + b * st[0] + h * st[2]), st[1] * (long)sizeof(T), st[2] * (long)sizeof(T), G};
+}
+
+// rows r0 .. r0+N-1 -> LDS tile; valid(i): whether row r0 + i exists.  The host has checked that a tile spans less than 2^31 bytes.
+template <typename T, int DP, int N, int WAVES, typename V>
+__device__ __forceinline__ void fill_tile(T* lds, const Rows& src, int r0, int D, V valid) {
+    typedef Tile<T, DP> L;
+    constexpr int PIECES = N * L::CPR / 64;
+    static_assert(PIECES % WAVES == 0, "every wavefront moves the same number of pieces");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = src.G == 1 ? r0 : r0 / src.G;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(src.base + n0 * src.ts), 0, (int)OUT_OF_RANGE, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < PIECES / WAVES; i++) {
+        const int piece = wave + WAVES * i, idx = piece * 64 + lane;
+        const int row = idx / L::CPR, chunk = L::unswizzle(idx % L::CPR, row);
+        unsigned off;
+        if (src.G == 1) off = (unsigned)(row * (int)src.ts);
+        else {
+            const int n = (r0 + row) / src.G;
+            off = (unsigned)((n - n0) * (int)src.ts + (r0 + row - n * src.G) * (int)src.hs);
+        }
+        off = valid(row) && chunk * L::CH < D ? off + 16u * chunk : OUT_OF_RANGE;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + piece * 64 * L::CH), 16, (int)off, 0, 0, 0);
+    }
+}
+__device__ __forceinline__ void wait_tiles() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+// which keys of the next 64 tiles of KT keys exist: one bit per key in `words`, and the tiles that hold any as a bit set
+template <int KT, int WAVES> __device__ __forceinline__ unsigned long long key_window(unsigned* words, const unsigned char* mask, int key0, int key_end) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __syncthreads();
+    static_assert(KT % WAVES == 0, "64 tiles of KT keys are KT groups of 64, dealt to the wavefronts");
+    unsigned char byte[KT / WAVES];
+#pragma unroll
+    for (int i = 0; i < KT / WAVES; i++) {                   // all loads first: one wait for the window
+        byte[i] = 1;
+        if (mask) byte[i] = mask[min(key0 + 64 * (wave + WAVES * i) + lane, key_end - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < KT / WAVES; i++) {
+        const int group = wave + WAVES * i;
+        const unsigned long long bits = __ballot(key0 + 64 * group + lane < key_end && byte[i]);
+        if (lane == 0) {
+            words[2 * group] = (unsigned)bits;
+            words[2 * group + 1] = (unsigned)(bits >> 32);
+        }
+    }
+    __syncthreads();
+    unsigned any = 0;
+#pragma unroll
+    for (int i = 0; i < KT / 32; i++) any |= words[lane * (KT / 32) + i];
+    return __ballot(any != 0);
+}
+
+// block index -> (head, block): blocks of one head on one XCD (its K and V then live in that XCD's L2), heads dealt to the 8 XCDs in turn
+__device__ __forceinline__ bool place(int BH, int per_head, int& bh, int& blk) {
+    const int lin = blockIdx.x;
+    if (BH >= 16) {
+        const int slot = lin >> 3;
+        bh = (slot / per_head) * 8 + (lin & 7);
+        blk = slot % per_head;
+        return bh < BH;
+    }
+    bh = lin / per_head;
+    blk = lin % per_head;
+    return true;
+}
+inline unsigned placed_blocks(int BH, int per_head) { return (unsigned)((BH >= 16 ? (BH + 7) / 8 * 8 : BH) * per_head); }
+
+template <typename T, int DP, bool SHARE> struct FwdShape {
+    // SHARE: the wavefronts share one block of 32 rows and split every tile's keys; otherwise each has its own 32 rows
+    static constexpr int WAVES = SHARE && sizeof(T) == 4 && DP > 64 ? 2 : 4;
+    static constexpr int KT = SHARE ? 32 * WAVES : (sizeof(T) == 2 ? 64 : 32);
+    static constexpr int ROWS = SHARE ? 32 : 32 * WAVES;
+    static constexpr int OCC = SHARE || DP > 64 ? 1 : 2;
+};
+
+template <typename T, int DP, bool SHARE>
+__global__ __launch_bounds__((FwdShape<T, DP, SHARE>::WAVES * 64), (FwdShape<T, DP, SHARE>::OCC)) void forward_kernel(const Args a) {
+    typedef FwdShape<T, DP, SHARE> S;
+    typedef Mma<T, DP> M;
+    constexpr int WAVES = S::WAVES, KT = S::KT, DB = M::DB, NKB = SHARE ? 1 : KT / 32;
+    __shared__ __attribute__((aligned(16))) T kbuf[2][KT * DP];
+    __shared__ __attribute__((aligned(16))) T vbuf[2][KT * DP];
+    __shared__ unsigned words[2 * KT];
+
+    const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int R = a.Nq * a.G, row_blocks = (R + S::ROWS - 1) / S::ROWS;
+    int bh, blk;
+    if (!place(a.BH, row_blocks * a.nsplit, bh, blk)) return;
+    const int split = blk / row_blocks, rb = blk - split * row_blocks;
+    const int b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int r = rb * S::ROWS + (SHARE ? 0 : 32 * wave) + l31;
+    const Rows qr = rows_of<T>(a.q, a.qs, b, hk * a.G, a.G), kr = rows_of<T>(a.k, a.ks, b, hk, 1), vr = rows_of<T>(a.v, a.vs, b, hk, 1);
+    const unsigned char* mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
+    const int key_beg = split * a.keys_per_split, key_end = min(a.Nk, key_beg + a.keys_per_split);
+    // a negative scale goes into q's sign: the maximum of s is the maximum of c s; c > 0 keeps -inf * c = -inf for masked keys at scale 0
+    const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);
+
+    typename M::Frag q;
+    M::load(q, reinterpret_cast<const T*>(qr.row(r < R ? r : 0)), r < R, a.D, a.scale);
+    f32x16 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; i++) o[i] = f32x16{};
+    float m = -INFINITY, l = 0.f;
+
+    for (int win = key_beg; win < key_end; win += 64 * KT) {
+        unsigned long long active = key_window<KT, WAVES>(words, mask, win, key_end);
+        if (!active) continue;
+        auto issue = [&](int t, int buf) {
+            auto valid = [&](int row) { return (words[t * (KT / 32) + (row >> 5)] >> (row & 31)) & 1; };
+            fill_tile<T, DP, KT, WAVES>(kbuf[buf], kr, win + t * KT, a.D, valid);
+            fill_tile<T, DP, KT, WAVES>(vbuf[buf], vr, win + t * KT, a.D, valid);
+        };
+        int t = __builtin_ctzll(active), buf = 0;
+        active &= active - 1;
+        issue(t, 0);
+        for (;;) {
+            wait_tiles();                                    // this tile is in LDS, and nobody reads the other buffer any more
+            const int tn = active ? __builtin_ctzll(active) : -1;
+            if (tn >= 0) {
+                active &= active - 1;
+                issue(tn, buf ^ 1);
+            }
+            f32x16 s[NKB];
+            float top = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < NKB; kb++) {
+                const int r0 = SHARE ? 32 * wave : 32 * kb;
+                s[kb] = M::dot(kbuf[buf], r0, q);
+                const unsigned on = __builtin_amdgcn_readfirstlane(words[t * (KT / 32) + (r0 >> 5)]);
+                if (on != 0xffffffffu) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (!((on >> acc_row(i, half)) & 1)) s[kb][i] = -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) top = fmaxf(top, s[kb][i]);
+            }
+            top = fmaxf(top, other_half(top)) * c;
+            if (__any(top > m + RESCALE_THR)) {
+                const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - mn);
+                const float keep = mn == -INFINITY ? 1.f : alpha;          // a block of masked keys only (SHARE): nothing to rescale
+                l *= keep;
+                m = mn;
+#pragma unroll
+                for (int i = 0; i < DB; i++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) o[i][j] *= keep;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int kb = 0; kb < NKB; kb++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], c, -base));
+                    l += s[kb][i];
+                }
+                M::add(o, vbuf[buf], SHARE ? 32 * wave : 32 * kb, s[kb]);
+            }
+            if (tn < 0) break;
+            t = tn;
+            buf ^= 1;
+        }
+    }
+    l += other_half(l);
+
+    const int H = a.Hk * a.G;
+    if constexpr (SHARE) {                                   // join the wavefronts' shares of the keys
+        float* jo = reinterpret_cast<float*>(&kbuf[0][0]);   // [WAVES][32 rows][DP]
+        float* jm = reinterpret_cast<float*>(&vbuf[0][0]);   // [WAVES][32 rows][2]
+        static_assert(sizeof(kbuf) >= WAVES * 32 * DP * sizeof(float), "the joined partials fit the key tiles");
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < DB; i++)
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+                *reinterpret_cast<f32x4*>(jo + (wave * 32 + l31) * DP + 32 * i + 8 * g + 4 * half) = f32x4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
+        if (half == 0) {
+            jm[(wave * 32 + l31) * 2] = m;
+            jm[(wave * 32 + l31) * 2 + 1] = l;
+        }
+        __syncthreads();
+        for (int idx = threadIdx.x; idx < 32 * (DP / 4); idx += WAVES * 64) {
+            const int row = idx / (DP / 4), d = 4 * (idx % (DP / 4)), rr = rb * 32 + row;
+            if (rr >= R || d >= a.D) continue;
+            float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) mt = fmaxf(mt, jm[(w * 32 + row) * 2]);
+            f32x4 sum = {};
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                const float mw = jm[(w * 32 + row) * 2], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mt);
+                lt += f * jm[(w * 32 + row) * 2 + 1];
+                if (f != 0.f) sum += f * *reinterpret_cast<const f32x4*>(jo + (w * 32 + row) * DP + d);
+            }
+            if (a.nsplit > 1) {
+                const long at = ((long)split * a.BH + bh) * R + rr;
+                *reinterpret_cast<f32x4*>(a.part_o + at * a.D + d) = sum;
+                if (d == 0) {
+                    a.part_ml[2 * at] = mt;
+                    a.part_ml[2 * at + 1] = lt;
+                }
+            } else {
+                const int n = rr / a.G, h = hk * a.G + rr - n * a.G;
+                const float inv = lt == 0.f ? 0.f : 1.f / lt;
+                M::store4(static_cast<T*>(a.o) + (((long)b * a.Nq + n) * H + h) * a.D + d, sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
+                if (a.lse && d == 0) a.lse[(long)bh * R + rr] = lt == 0.f ? INFINITY : mt + __builtin_amdgcn_logf(lt);
+            }
+        }
+    } else {
+        if (r >= R) return;
+        if (a.nsplit > 1) {
+            const long at = ((long)split * a.BH + bh) * R + r;
+#pragma unroll
+            for (int i = 0; i < DB; i++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const int d = 32 * i + 8 * g + 4 * half;
+                    if (d < a.D) *reinterpret_cast<f32x4*>(a.part_o + at * a.D + d) = f32x4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
+                }
+            if (half == 0) {
+                a.part_ml[2 * at] = m;
+                a.part_ml[2 * at + 1] = l;
+            }
+            return;
+        }
+        const int n = r / a.G, h = hk * a.G + r - n * a.G;
+        T* out = static_cast<T*>(a.o) + (((long)b * a.Nq + n) * H + h) * a.D;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int i = 0; i < DB; i++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int d = 32 * i + 8 * g + 4 * half;
+                if (d < a.D) M::store4(out + d, o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv);
+            }
+        if (a.lse && half == 0) a.lse[(long)bh * R + r] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    }
+}
+
+// joins the splits: a thread per 4 channels of a row
+template <typename T> __global__ __launch_bounds__(256) void join_kernel(const Args a) {
+    const int R = a.Nq * a.G, H = a.Hk * a.G, q4 = a.D / 4;
+    const long idx = (long)blockIdx.x * 256 + threadIdx.x, rows = (long)a.BH * R;
+    const long row = idx / q4;
+    if (row >= rows) return;
+    const int d = 4 * (int)(idx - row * q4);
+    float mt = -INFINITY, lt = 0.f;
+    for (int s = 0; s < a.nsplit; s++) mt = fmaxf(mt, a.part_ml[2 * (s * rows + row)]);
+    f32x4 sum = {};
+    for (int s = 0; s < a.nsplit; s++) {
+        const float ms = a.part_ml[2 * (s * rows + row)], f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - mt);
+        lt += f * a.part_ml[2 * (s * rows + row) + 1];
+        if (f != 0.f) sum += f * *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * a.D + d);
+    }
+    const int bh = (int)(row / R), r = (int)(row - (long)bh * R), b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int n = r / a.G, h = hk * a.G + r - n * a.G;
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    Mma<T, 32>::store4(static_cast<T*>(a.o) + (((long)b * a.Nq + n) * H + h) * a.D + d, sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
+    if (a.lse && d == 0) a.lse[row] = lt == 0.f ? INFINITY : mt + __builtin_amdgcn_logf(lt);
+}
+
+// delta[row] = gO . o : 16 lanes per row, up to 8 channels each
+template <typename T> __global__ __launch_bounds__(256) void delta_kernel(const Args a) {
+    const int R = a.Nq * a.G, H = a.Hk * a.G, l = threadIdx.x & 15;
+    const long row = (long)blockIdx.x * 16 + (threadIdx.x >> 4), rows = (long)a.BH * R;
+    if (row >= rows) return;
+    const int bh = (int)(row / R), r = (int)(row - (long)bh * R), b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int n = r / a.G, h = hk * a.G + r - n * a.G;
+    float s = 0.f;
+    if (8 * l < a.D) {
+        const T* g = reinterpret_cast<const T*>(rows_of<T>(a.go, a.gs, b, h, 1).row(n)) + 8 * l;
+        const T* o = static_cast<const T*>(a.o_in) + (((long)b * a.Nq + n) * H + h) * a.D + 8 * l;
+        typedef T tx8 __attribute__((ext_vector_type(8)));
+        const tx8 x = *reinterpret_cast<const tx8*>(g), y = *reinterpret_cast<const tx8*>(o);
+#pragma unroll
+        for (int i = 0; i < 8; i++) s += (float)x[i] * (float)y[i];
+    }
+#pragma unroll
+    for (int k = 1; k < 16; k <<= 1) s += __shfl_xor(s, k);
+    if (l == 0) a.delta[row] = s;
+}
+
+template <typename T, int DP> struct BwdShape {
+    static constexpr int WAVES = 4, ST = sizeof(T) == 2 ? 64 : 32;         // streamed rows per tile
+    static constexpr int OCC = DP > 64 ? 1 : 2;
+};
+
+// KV: stationary keys, streamed query rows (gk, gv); otherwise stationary query rows, streamed keys (gq)
+template <typename T, int DP, bool KV>
+__global__ __launch_bounds__((BwdShape<T, DP>::WAVES * 64), (BwdShape<T, DP>::OCC)) void backward_kernel(const Args a) {
+    typedef BwdShape<T, DP> S;
+    typedef Mma<T, DP> M;
+    constexpr int WAVES = S::WAVES, ST = S::ST, DB = M::DB, COLS = 32 * WAVES;
+    __shared__ __attribute__((aligned(16))) T buf1[2][ST * DP];
+    __shared__ __attribute__((aligned(16))) T buf2[2][ST * DP];
+    __shared__ __attribute__((aligned(16))) float rowstat[KV ? 2 : 1][2][64];
+    __shared__ unsigned words[KV ? 1 : 2 * ST];
+
+    const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int R = a.Nq * a.G, C = KV ? a.Nk : R;
+    int bh, blk;
+    if (!place(a.BH, (C + COLS - 1) / COLS, bh, blk)) return;
+    const int b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int col = blk * COLS + 32 * wave + l31;
+    const unsigned char* mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
+    const bool valid = col < C && (!KV || !mask || mask[col]);
+    const Rows qr = rows_of<T>(a.q, a.qs, b, hk * a.G, a.G), gr = rows_of<T>(a.go, a.gs, b, hk * a.G, a.G);
+    const Rows kr = rows_of<T>(a.k, a.ks, b, hk, 1), vr = rows_of<T>(a.v, a.vs, b, hk, 1);
+    const float* lse = a.lse + (long)bh * R;
+    const float* delta = a.delta + (long)bh * R;
+    const float c = a.scale * LOG2E;
+
+    f32x16 acc1[DB], acc2[KV ? DB : 1];
+#pragma unroll
+    for (int i = 0; i < DB; i++) acc1[i] = f32x16{};
+#pragma unroll
+    for (int i = 0; i < (KV ? DB : 1); i++) acc2[i] = f32x16{};
+    typename M::Frag f1, f2;
+    {
+        const int at = valid ? col : 0;
+        M::load(f1, reinterpret_cast<const T*>((KV ? kr : qr).row(at)), valid, a.D, 1.f);
+        M::load(f2, reinterpret_cast<const T*>((KV ? vr : gr).row(at)), valid, a.D, 1.f);
+    }
+    const float col_lse = KV ? 0.f : (valid ? lse[col] : INFINITY), col_delta = KV ? 0.f : (valid ? delta[col] : 0.f);
+
+    // one 32-row block: p, gs and the products over its rows; `on`: which rows exist (query gradient only)
+    auto block = [&](int buf, int r0, unsigned on) {
+        f32x16 p = M::dot(buf1[buf], r0, f1), ds = M::dot(buf2[buf], r0, f2);
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            f32x4 ls = {col_lse, col_lse, col_lse, col_lse}, dl = {col_delta, col_delta, col_delta, col_delta};
+            if constexpr (KV) {
+                ls = *reinterpret_cast<const f32x4*>(&rowstat[buf][0][r0 + 8 * g + 4 * half]);
+                dl = *reinterpret_cast<const f32x4*>(&rowstat[buf][1][r0 + 8 * g + 4 * half]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int i = 4 * g + j;
+                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], c, -ls[j]));
+                if (!KV && on != 0xffffffffu && !((on >> acc_row(i, half)) & 1)) p[i] = 0.f;
+                ds[i] = p[i] * (ds[i] - dl[j]);
+            }
+        }
+        if constexpr (KV) M::add(acc2, buf2[buf], r0, p);
+        M::add(acc1, buf1[buf], r0, ds);
+    };
+
+    if constexpr (KV) {
+        if (__syncthreads_or(valid)) {
+            auto issue = [&](int r0, int buf) {
+                auto in = [&](int row) { return r0 + row < R; };
+                fill_tile<T, DP, ST, WAVES>(buf1[buf], qr, r0, a.D, in);
+                fill_tile<T, DP, ST, WAVES>(buf2[buf], gr, r0, a.D, in);
+                if (wave < 2) {                              // statistics of the tile's rows; 0 past the last row, where q and gO are 0
+                    const float* src = (wave ? delta : lse) + r0;
+                    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(src), 0, (int)OUT_OF_RANGE, 0x00020000);
+                    const unsigned off = lane < ST && r0 + lane < R ? 4u * lane : OUT_OF_RANGE;
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)&rowstat[buf][wave][0], 4, (int)off, 0, 0, 0);
+                }
+            };
+            issue(0, 0);
+            int buf = 0;
+            for (int r0 = 0; r0 < R; r0 += ST, buf ^= 1) {
+                wait_tiles();
+                if (r0 + ST < R) issue(r0 + ST, buf ^ 1);
+#pragma unroll
+                for (int kb = 0; kb < ST / 32; kb++) block(buf, 32 * kb, 0xffffffffu);
+            }
+        }
+    } else {
+        for (int win = 0; win < a.Nk; win += 64 * ST) {
+            unsigned long long active = key_window<ST, WAVES>(words, mask, win, a.Nk);
+            if (!active) continue;
+            auto issue = [&](int t, int buf) {
+                auto in = [&](int row) { return (words[t * (ST / 32) + (row >> 5)] >> (row & 31)) & 1; };
+                fill_tile<T, DP, ST, WAVES>(buf1[buf], kr, win + t * ST, a.D, in);
+                fill_tile<T, DP, ST, WAVES>(buf2[buf], vr, win + t * ST, a.D, in);
+            };
+            int t = __builtin_ctzll(active), buf = 0;
+            active &= active - 1;
+            issue(t, 0);
+            for (;;) {
+                wait_tiles();
+                const int tn = active ? __builtin_ctzll(active) : -1;
+                if (tn >= 0) {
+                    active &= active - 1;
+                    issue(tn, buf ^ 1);
+                }
+#pragma unroll
+                for (int kb = 0; kb < ST / 32; kb++) block(buf, 32 * kb, __builtin_amdgcn_readfirstlane(words[t * (ST / 32) + kb]));
+                if (tn < 0) break;
+                t = tn;
+                buf ^= 1;
+            }
+        }
+    }
+    if (col >= C) return;
+    long at;
+    if (KV) at = (((long)b * a.Nk + col) * a.Hk + hk) * a.D;
+    else {
+        const int n = col / a.G;
+        at = (((long)b * a.Nq + n) * (a.Hk * a.G) + hk * a.G + col - n * a.G) * a.D;
+    }
+    T* out1 = static_cast<T*>(KV ? a.gk : a.gq);
+    T* out2 = static_cast<T*>(a.gv);
+    const float f = valid ? a.scale : 0.f;
+#pragma unroll
+    for (int i = 0; i < DB; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int d = 32 * i + 8 * g + 4 * half;
+            if (d >= a.D) continue;
+            // a masked key's column is written as zeros whatever went through it
+            if (out1) M::store4(out1 + at + d, valid ? acc1[i][4 * g] * f : 0.f, valid ? acc1[i][4 * g + 1] * f : 0.f, valid ? acc1[i][4 * g + 2] * f : 0.f,
+                                valid ? acc1[i][4 * g + 3] * f : 0.f);
+            if constexpr (KV)
+                if (out2) M::store4(out2 + at + d, valid ? acc2[i][4 * g] : 0.f, valid ? acc2[i][4 * g + 1] : 0.f, valid ? acc2[i][4 * g + 2] : 0.f,
+                                    valid ? acc2[i][4 * g + 3] : 0.f);
+        }
+}
+
+// ---- launch plan --------------------------------------------------------------------------------------------------------------------
+struct Plan {
+    bool share;
+    int nsplit, keys_per_split, row_blocks, waves;
+};
+// share: 32 rows or fewer per head -- four wavefronts with rows of their own would leave three idle.
+// split: fewer than two workgroups per CU -- the keys are divided until there are, with at least two tiles each.
+template <typename T> Plan forward_plan(const Args& a, int DP) {
+    Plan p;
+    const int R = a.Nq * a.G;
+    p.share = R <= 32;
+    p.waves = p.share && sizeof(T) == 4 && DP > 64 ? 2 : 4;
+    const int KT = p.share ? 32 * p.waves : (sizeof(T) == 2 ? 64 : 32);
+    p.row_blocks = (R + (p.share ? 32 : 128) - 1) / (p.share ? 32 : 128);
+    const int tiles = (a.Nk + KT - 1) / KT;
+    const long blocks = (long)a.BH * p.row_blocks;
+    int want = blocks >= 512 ? 1 : (int)((512 + blocks - 1) / blocks);
+    if (want > tiles / 2) want = tiles / 2 > 0 ? tiles / 2 : 1;
+    const int per = (tiles + want - 1) / want;
+    p.nsplit = (tiles + per - 1) / per;
+    p.keys_per_split = per * KT;
+    return p;
+}
+inline int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
+
+template <typename T, int DP> void launch_forward(Args a, const Plan& p, hipStream_t st) {
+    const unsigned blocks = placed_blocks(a.BH, p.row_blocks * p.nsplit);
+    if (p.share) hipLaunchKernelGGL((forward_kernel<T, DP, true>), dim3(blocks), dim3(FwdShape<T, DP, true>::WAVES * 64), 0, st, a);
+    else hipLaunchKernelGGL((forward_kernel<T, DP, false>), dim3(blocks), dim3(256), 0, st, a);
+    if (p.nsplit > 1) {
+        const long n = (long)a.BH * a.Nq * a.G * (a.D / 4);
+        hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    }
+}
+template <typename T, int DP> void launch_backward(const Args& a, hipStream_t st) {
+    const int R = a.Nq * a.G;
+    hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)(((long)a.BH * R + 15) / 16)), dim3(256), 0, st, a);
+    if (a.gq) hipLaunchKernelGGL((backward_kernel<T, DP, false>), dim3(placed_blocks(a.BH, (R + 127) / 128)), dim3(256), 0, st, a);
+    if (a.gk || a.gv) hipLaunchKernelGGL((backward_kernel<T, DP, true>), dim3(placed_blocks(a.BH, (a.Nk + 127) / 128)), dim3(256), 0, st, a);
+}
+
+// instantiated in csrc/cross_attn_f32.hip and csrc/cross_attn_bf16.hip
+template <typename T> void run_forward(const Args& a, const Plan& p, hipStream_t st);
+template <typename T> void run_backward(const Args& a, hipStream_t st);
+
+#define SCP_ATTN_INSTANTIATE(T)                                                                  \
+    namespace scp_attn {                                                                         \
+    template <> void run_forward<T>(const Args& a, const Plan& p, hipStream_t st) {              \
+        switch (padded_dim(a.D)) {                                                               \
+            case 32: launch_forward<T, 32>(a, p, st); break;                                     \
+            case 64: launch_forward<T, 64>(a, p, st); break;                                     \
+            case 96: launch_forward<T, 96>(a, p, st); break;                                     \
+            default: launch_forward<T, 128>(a, p, st); break;                                    \
+        }                                                                                        \
+    }                                                                                            \
+    template <> void run_backward<T>(const Args& a, hipStream_t st) {                            \
+        switch (padded_dim(a.D)) {                                                               \
+            case 32: launch_backward<T, 32>(a, st); break;                                       \
+            case 64: launch_backward<T, 64>(a, st); break;                                       \
+            case 96: launch_backward<T, 96>(a, st); break;                                       \
+            default: launch_backward<T, 128>(a, st); break;                                      \
+        }                                                                                        \
+    }                                                                                            \
+    }
+
+}  // namespace scp_attn

@@ -5,157 +5,24 @@
 // Query heads that share a key / value head are extra ROWS of it: row r of head hk is query r / G of query head hk G + r % G, so the sums
 // of a shared head's gradient are ordinary sums over rows.  A batch entry whose keys are all masked gives zeros, and zero gradients.
 // Masked keys are never read into a product: an infinity or NaN stored there does not reach any result.
+// The kernels are in csrc/attn_core.h; this file checks the arguments and launches.
 #include <hip/hip_runtime.h>
 
+#include "attn_core.h"
 #include "scp_common.h"
 #include "scp_hip.h"
-#include "vec_io.h"
+
+namespace scp_attn {
+template <> void run_forward<float>(const Args&, const Plan&, hipStream_t);
+template <> void run_forward<__bf16>(const Args&, const Plan&, hipStream_t);
+template <> void run_backward<float>(const Args&, hipStream_t);
+template <> void run_backward<__bf16>(const Args&, hipStream_t);
+}  // namespace scp_attn
 
 namespace {
 
-using scp::VecIO;
-constexpr float LOG2E = 1.4426950408889634f;
-
-struct AttnArgs {
-    const void *q, *k, *v, *go;
-    const unsigned char* mask;
-    const void* o_in;
-    void *o, *gq, *gk, *gv;
-    float *lse, *delta;
-    long qs[3], ks[3], vs[3], gs[3];      // strides in elements: batch, token, head
-    int Nq, Nk, Hk, G, D;
-    float scale;
-};
-
-template <typename T> __device__ __forceinline__ const T* row_of(const void* base, const long* st, int b, int n, int h) {
-    return static_cast<const T*>(base) + b * st[0] + n * st[1] + h * st[2];
-}
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v = fmaxf(v, __shfl_xor(v, m));
-    return v;
-}
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
-    return v;
-}
-template <typename T> __device__ __forceinline__ float dot(const T* a, const T* b, int D) {
-    float s = 0.f;
-    for (int d = 0; d < D; d++) s += VecIO<T>::one(a + d) * VecIO<T>::one(b + d);
-    return s;
-}
-
-// one wavefront per row: scores of 64 keys, a lane each; the products with v lane = channel (two channels per lane)
-template <typename T> __global__ __launch_bounds__(64) void attn_forward_kernel(const AttnArgs a) {
-    const int R = a.Nq * a.G, lane = threadIdx.x;
-    const int r = blockIdx.x % R, bh = blockIdx.x / R, hk = bh % a.Hk, b = bh / a.Hk;
-    const int n = r / a.G, h = hk * a.G + r % a.G, H = a.Hk * a.G;
-    const T* q = row_of<T>(a.q, a.qs, b, n, h);
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int j0 = 0; j0 < a.Nk; j0 += 64) {
-        const int j = j0 + lane;
-        const bool on = j < a.Nk && (!a.mask || a.mask[(long)b * a.Nk + j]);
-        const float s = on ? dot<T>(q, row_of<T>(a.k, a.ks, b, j, hk), a.D) * a.scale * LOG2E : -INFINITY;
-        const float mt = fmaxf(m, wave_max(s));
-        if (!__any(on)) continue;
-        const float alpha = exp2f(m - mt), p = on ? exp2f(s - mt) : 0.f;
-        l = l * alpha + wave_sum(p);
-        o0 *= alpha;
-        o1 *= alpha;
-        m = mt;
-        const unsigned long long bits = __ballot(on);
-        for (int t = 0; t < 64; t++) {
-            const float pt = __shfl(p, t);
-            if (!((bits >> t) & 1)) continue;
-            const T* v = row_of<T>(a.v, a.vs, b, j0 + t, hk);
-            if (lane < a.D) o0 += pt * VecIO<T>::one(v + lane);
-            if (lane + 64 < a.D) o1 += pt * VecIO<T>::one(v + lane + 64);
-        }
-    }
-    T* o = static_cast<T*>(a.o) + (((long)b * a.Nq + n) * H + h) * a.D;
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    if (lane < a.D) VecIO<T>::put(o + lane, o0 * inv);
-    if (lane + 64 < a.D) VecIO<T>::put(o + lane + 64, o1 * inv);
-    if (a.lse && lane == 0) a.lse[(long)bh * R + r] = l == 0.f ? INFINITY : m + log2f(l);
-}
-
-// delta_r = go_r . o_r
-template <typename T> __global__ __launch_bounds__(64) void attn_delta_kernel(const AttnArgs a) {
-    const int R = a.Nq * a.G, lane = threadIdx.x;
-    const int r = blockIdx.x % R, bh = blockIdx.x / R, hk = bh % a.Hk, b = bh / a.Hk;
-    const int n = r / a.G, h = hk * a.G + r % a.G, H = a.Hk * a.G;
-    const T* g = row_of<T>(a.go, a.gs, b, n, h);
-    const T* o = static_cast<const T*>(a.o_in) + (((long)b * a.Nq + n) * H + h) * a.D;
-    float s = 0.f;
-    for (int d = lane; d < a.D; d += 64) s += VecIO<T>::one(g + d) * VecIO<T>::one(o + d);
-    s = wave_sum(s);
-    if (lane == 0) a.delta[(long)bh * R + r] = s;
-}
-
-template <typename T> __global__ __launch_bounds__(64) void attn_gq_kernel(const AttnArgs a) {
-    const int R = a.Nq * a.G, lane = threadIdx.x;
-    const int r = blockIdx.x % R, bh = blockIdx.x / R, hk = bh % a.Hk, b = bh / a.Hk;
-    const int n = r / a.G, h = hk * a.G + r % a.G, H = a.Hk * a.G;
-    const T* q = row_of<T>(a.q, a.qs, b, n, h);
-    const T* g = row_of<T>(a.go, a.gs, b, n, h);
-    const float lse = a.lse[(long)bh * R + r], delta = a.delta[(long)bh * R + r];
-    float g0 = 0.f, g1 = 0.f;
-    for (int j0 = 0; j0 < a.Nk; j0 += 64) {
-        const int j = j0 + lane;
-        const bool on = j < a.Nk && (!a.mask || a.mask[(long)b * a.Nk + j]);
-        float ds = 0.f;
-        if (on) {
-            const float p = exp2f(dot<T>(q, row_of<T>(a.k, a.ks, b, j, hk), a.D) * a.scale * LOG2E - lse);
-            ds = p * (dot<T>(g, row_of<T>(a.v, a.vs, b, j, hk), a.D) - delta) * a.scale;
-        }
-        const unsigned long long bits = __ballot(on);
-        for (int t = 0; t < 64; t++) {
-            const float dt = __shfl(ds, t);
-            if (!((bits >> t) & 1)) continue;
-            const T* k = row_of<T>(a.k, a.ks, b, j0 + t, hk);
-            if (lane < a.D) g0 += dt * VecIO<T>::one(k + lane);
-            if (lane + 64 < a.D) g1 += dt * VecIO<T>::one(k + lane + 64);
-        }
-    }
-    T* o = static_cast<T*>(a.gq) + (((long)b * a.Nq + n) * H + h) * a.D;
-    if (lane < a.D) VecIO<T>::put(o + lane, g0);
-    if (lane + 64 < a.D) VecIO<T>::put(o + lane + 64, g1);
-}
-
-// one wavefront per key
-template <typename T> __global__ __launch_bounds__(64) void attn_gkv_kernel(const AttnArgs a) {
-    const int R = a.Nq * a.G, lane = threadIdx.x;
-    const int j = blockIdx.x % a.Nk, bh = blockIdx.x / a.Nk, hk = bh % a.Hk, b = bh / a.Hk;
-    const bool on = !a.mask || a.mask[(long)b * a.Nk + j];
-    const T* k = row_of<T>(a.k, a.ks, b, j, hk);
-    const T* v = row_of<T>(a.v, a.vs, b, j, hk);
-    float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
-    for (int r0 = 0; on && r0 < R; r0 += 64) {
-        const int r = r0 + lane;
-        float p = 0.f, ds = 0.f;
-        if (r < R) {
-            const int n = r / a.G, h = hk * a.G + r % a.G;
-            p = exp2f(dot<T>(row_of<T>(a.q, a.qs, b, n, h), k, a.D) * a.scale * LOG2E - a.lse[(long)bh * R + r]);
-            ds = p * (dot<T>(row_of<T>(a.go, a.gs, b, n, h), v, a.D) - a.delta[(long)bh * R + r]) * a.scale;
-        }
-        for (int t = 0; t < 64 && r0 + t < R; t++) {
-            const float pt = __shfl(p, t), dt = __shfl(ds, t);
-            const int n = (r0 + t) / a.G, h = hk * a.G + (r0 + t) % a.G;
-            const T* q = row_of<T>(a.q, a.qs, b, n, h);
-            const T* g = row_of<T>(a.go, a.gs, b, n, h);
-            if (lane < a.D) { v0 += pt * VecIO<T>::one(g + lane); k0 += dt * VecIO<T>::one(q + lane); }
-            if (lane + 64 < a.D) { v1 += pt * VecIO<T>::one(g + lane + 64); k1 += dt * VecIO<T>::one(q + lane + 64); }
-        }
-    }
-    const long at = (((long)b * a.Nk + j) * a.Hk + hk) * a.D;
-    T* gk = a.gk ? static_cast<T*>(a.gk) + at : nullptr;
-    T* gv = a.gv ? static_cast<T*>(a.gv) + at : nullptr;
-    if (gk && lane < a.D) VecIO<T>::put(gk + lane, k0);
-    if (gk && lane + 64 < a.D) VecIO<T>::put(gk + lane + 64, k1);
-    if (gv && lane < a.D) VecIO<T>::put(gv + lane, v0);
-    if (gv && lane + 64 < a.D) VecIO<T>::put(gv + lane + 64, v1);
-}
+using scp_attn::Args;
+using scp_attn::Plan;
 
 const char* bad_problem(const scp_cross_attn_params* p) {
     if (!p) return "cross_attention: null parameters";
@@ -172,10 +39,20 @@ const char* bad_problem(const scp_cross_attn_params* p) {
         return "cross_attention: more than 2^31 rows or keys over all heads";
     return nullptr;
 }
+// a tile (64 or 128 rows) is addressed with 31-bit byte offsets behind its first row; the tile's own place is a 64-bit address
+bool tile_too_wide(const scp_cross_attn_params* p, bool backward) {
+    const long long size = p->dtype == SCP_DTYPE_F32 ? 4 : 2, lim = 1ll << 31, G = p->heads / p->kv_heads;
+    for (const long long* st : {p->k_stride, p->v_stride})
+        if (st[1] < 0 || 128 * st[1] * size >= lim) return true;
+    if (backward)
+        for (const long long* st : {p->q_stride, p->g_stride})
+            if (st[1] < 0 || st[2] < 0 || (65 * st[1] + G * st[2]) * size >= lim) return true;
+    return false;
+}
 bool misaligned(const void* p) { return (reinterpret_cast<size_t>(p) & 15) != 0; }
 
-AttnArgs make_args(const scp_cross_attn_params* p) {
-    AttnArgs a{};
+Args make_args(const scp_cross_attn_params* p) {
+    Args a{};
     for (int i = 0; i < 3; i++) { a.qs[i] = p->q_stride[i]; a.ks[i] = p->k_stride[i]; a.vs[i] = p->v_stride[i]; a.gs[i] = p->g_stride[i]; }
     a.Nq = p->queries;
     a.Nk = p->keys;
@@ -183,31 +60,50 @@ AttnArgs make_args(const scp_cross_attn_params* p) {
     a.G = p->heads / p->kv_heads;
     a.D = p->head_dim;
     a.scale = p->scale;
+    a.BH = p->batch * a.Hk;
+    a.nsplit = 1;
     return a;
 }
+Plan plan_of(const Args& a, int dtype) {
+    const int DP = scp_attn::padded_dim(a.D);
+    return dtype == SCP_DTYPE_F32 ? scp_attn::forward_plan<float>(a, DP) : scp_attn::forward_plan<__bf16>(a, DP);
+}
+size_t split_floats(const Args& a, const Plan& p) { return p.nsplit > 1 ? (size_t)p.nsplit * a.BH * a.Nq * a.G * (a.D + 2) : 0; }
 
 }  // namespace
 
-extern "C" size_t scp_cross_attention_forward_workspace(const scp_cross_attn_params* p) { return 0; }
+extern "C" size_t scp_cross_attention_forward_workspace(const scp_cross_attn_params* p) {
+    if (bad_problem(p)) return 0;
+    const Args a = make_args(p);
+    return split_floats(a, plan_of(a, p->dtype)) * sizeof(float);
+}
 
 extern "C" int scp_cross_attention_forward(const void* q, const void* k, const void* v, const unsigned char* key_mask,
                                            const scp_cross_attn_params* p, void* out, float* lse, void* workspace, size_t workspace_bytes,
                                            void* stream) {
     if (const char* why = bad_problem(p)) return scp::fail(hipErrorInvalidValue, why);
     if (!q || !k || !v || !out) return scp::fail(hipErrorInvalidValue, "cross_attention_forward: null argument");
-    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out))
+    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(workspace))
         return scp::fail(hipErrorInvalidValue, "cross_attention_forward: tensors must be 16-byte aligned");
-    AttnArgs a = make_args(p);
+    if (tile_too_wide(p, false)) return scp::fail(hipErrorInvalidValue, "cross_attention_forward: token stride of k or v too large");
+    Args a = make_args(p);
+    const Plan plan = plan_of(a, p->dtype);
+    const size_t need = split_floats(a, plan);
+    if (need && (!workspace || workspace_bytes < need * sizeof(float)))
+        return scp::fail(hipErrorInvalidValue, "cross_attention_forward: workspace too small");
     a.q = q;
     a.k = k;
     a.v = v;
     a.mask = key_mask;
     a.o = out;
     a.lse = lse;
-    const dim3 grid((unsigned)(p->batch * a.Hk * (a.Nq * a.G)));
+    a.nsplit = plan.nsplit;
+    a.keys_per_split = plan.keys_per_split;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + (size_t)plan.nsplit * a.BH * a.Nq * a.G * a.D;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (p->dtype == SCP_DTYPE_F32) hipLaunchKernelGGL(attn_forward_kernel<float>, grid, dim3(64), 0, st, a);
-    else hipLaunchKernelGGL(attn_forward_kernel<__bf16>, grid, dim3(64), 0, st, a);
+    if (p->dtype == SCP_DTYPE_F32) scp_attn::run_forward<float>(a, plan, st);
+    else scp_attn::run_forward<__bf16>(a, plan, st);
     return scp::check_launch("cross_attention_forward");
 }
 
@@ -223,9 +119,10 @@ extern "C" int scp_cross_attention_backward(const void* q, const void* k, const 
     if (!q || !k || !v || !out || !lse || !g_out) return scp::fail(hipErrorInvalidValue, "cross_attention_backward: null argument");
     if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(g_out) || misaligned(g_q) || misaligned(g_k) || misaligned(g_v))
         return scp::fail(hipErrorInvalidValue, "cross_attention_backward: tensors must be 16-byte aligned");
+    if (tile_too_wide(p, true)) return scp::fail(hipErrorInvalidValue, "cross_attention_backward: token or head stride too large");
     if (!workspace || workspace_bytes < scp_cross_attention_backward_workspace(p))
         return scp::fail(hipErrorInvalidValue, "cross_attention_backward: workspace too small");
-    AttnArgs a = make_args(p);
+    Args a = make_args(p);
     a.q = q;
     a.k = k;
     a.v = v;
@@ -238,17 +135,7 @@ extern "C" int scp_cross_attention_backward(const void* q, const void* k, const 
     a.gk = g_k;
     a.gv = g_v;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 rows((unsigned)(p->batch * a.Hk * (a.Nq * a.G))), keys((unsigned)(p->batch * a.Hk * a.Nk));
-    const bool f32 = p->dtype == SCP_DTYPE_F32;
-    if (f32) hipLaunchKernelGGL(attn_delta_kernel<float>, rows, dim3(64), 0, st, a);
-    else hipLaunchKernelGGL(attn_delta_kernel<__bf16>, rows, dim3(64), 0, st, a);
-    if (g_q) {
-        if (f32) hipLaunchKernelGGL(attn_gq_kernel<float>, rows, dim3(64), 0, st, a);
-        else hipLaunchKernelGGL(attn_gq_kernel<__bf16>, rows, dim3(64), 0, st, a);
-    }
-    if (g_k || g_v) {
-        if (f32) hipLaunchKernelGGL(attn_gkv_kernel<float>, keys, dim3(64), 0, st, a);
-        else hipLaunchKernelGGL(attn_gkv_kernel<__bf16>, keys, dim3(64), 0, st, a);
-    }
+    if (p->dtype == SCP_DTYPE_F32) scp_attn::run_backward<float>(a, st);
+    else scp_attn::run_backward<__bf16>(a, st);
     return scp::check_launch("cross_attention_backward");
 }

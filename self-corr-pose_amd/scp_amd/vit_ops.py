@@ -131,9 +131,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-6, residual=None):
 
 # ---- cross attention ---------------------------------------------------------------------------------------------------------------------
 def _addressable(t):
-    """t itself when the kernels can address it (channels contiguous, pointer and strides multiples of 16 bytes), else a contiguous copy"""
-    unit = 16 // t.element_size()
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(s % unit for s in t.stride()[:3]):
+    """t itself when the kernels can address it (channels contiguous, pointer and strides multiples of 16 bytes, 128 tokens of all heads
+    within 2^31 bytes), else a contiguous copy"""
+    size = t.element_size()
+    sb, sn, sh, sd = t.stride()
+    if sd == 1 and not (t.data_ptr() | sb * size | sn * size | sh * size) & 15 and (128 * sn + t.shape[2] * sh) * size < 1 << 31:
         return t
     return t.clone(memory_format=torch.contiguous_format)      # contiguous() would return a misaligned tensor as it is
 

@@ -395,9 +395,9 @@ def test_cross_attention_empty_sides():
 
 @gpu
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
-def test_cross_attention_offsets_past_32_bits(dtype):
-    """a cache whose tokens lie 2^25 elements apart: the last key is over 2^31 elements into the storage"""
-    n, step = 66, 1 << 25
+@pytest.mark.parametrize("n,step", [(1100, 1 << 21), (66, 1 << 25)], ids=["addressed", "copied"])
+def test_cross_attention_offsets_past_32_bits(dtype, n, step):
+    """a cache whose last key is over 2^31 elements into the storage; at 2^25 elements per token a tile spans more than 2^31 bytes"""
     store = torch.empty(n * step, dtype=dtype, device="cuda")
     k = store.view(1, n, step)[:, :, :64].unflatten(2, (1, 64))
     v = store.view(1, n, step)[:, :, 64:128].unflatten(2, (1, 64))
