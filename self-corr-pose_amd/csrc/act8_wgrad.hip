@@ -1,6 +1,18 @@
 // self-corr-pose_amd/csrc/act8_wgrad.hip -- weight and bias gradient of a linear layer from the 8-bit checkpoint of its input.
 //
 //   gw[n][k] = sum_m gy[m][n] x8[m][k],   gb[n] = sum_m gy[m][n],   x8 = code * step (csrc/act8.hip)
+//
+// A matrix product whose reduction runs over the ROWS of both operands, on v_mfma_f32_32x32x16_bf16.  x8 is exact in bf16 and bf16 gy is what
+// it is, so every product is exact and only the fp32 accumulation rounds; fp32 gy is cut into three bf16 parts of 8 bits each
+// (gy = h + m + l exactly) and multiplied part by part: 3 matrix instructions for 1, still 5 times the rate of the fp32 cores.
+//   * a workgroup owns a BN x 128 tile of gw over a range of rows and walks it 32 rows at a time: gy and the codes go global -> registers one
+//     step ahead, are cut / dequantised there (once per tile, not per wavefront) and written to LDS row-major; ds_read_b64_tr_b16 turns
+//     4 rows x 16 columns into operand order, the same row order for both operands, so no transposition is ever stored;
+//   * LDS rows are swizzled in 16-byte chunks so that the 4 rows x 2 chunks of one transposed read touch each bank once;
+//   * a wavefront owns (BN / 2) x 64 of the tile.  BN = 256 for bf16 (12 KiB of LDS reads per 16 matrix instructions), 128 for fp32, where
+//     the three parts share the x8 operand and 2 x 64 KiB of LDS keeps two workgroups on a CU;
+//   * the rows are split so that about two workgroups per CU run; each writes an fp32 partial tile and a second kernel adds the partials in
+//     order (bit-reproducible).  gb falls out of the registers of the workgroups of the first column of tiles.
 #include <hip/hip_runtime.h>
 
 #include "scp_common.h"
@@ -10,51 +22,279 @@
 namespace {
 
 using scp::VecIO;
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4_a1 __attribute__((ext_vector_type(4), aligned(1)));
 
-// a 16 x 16 tile of gw per workgroup, a thread per element; 16 rows of gy and x8 at a time through LDS
-template <typename T> __global__ __launch_bounds__(256) void wgrad8_kernel(const T* gy, const signed char* codes, const unsigned char* exps, long M, int N,
-                                                                          int K, float* gw, float* gb) {
-    __shared__ float a[16][17], b[16][17];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int n0 = blockIdx.y * 16, k0 = blockIdx.x * 16, groups = (K + 31) / 32;
-    float acc = 0.f, bias = 0.f;
-    for (long m0 = 0; m0 < M; m0 += 16) {
-        const long m = m0 + ty;
-        const int n = n0 + tx, k = k0 + tx;
-        a[ty][tx] = m < M && n < N ? VecIO<T>::one(gy + m * N + n) : 0.f;
-        float v = 0.f;
-        if (m < M && k < K) {
-            const unsigned e = exps[m * groups + k / 32];
-            v = (float)codes[m * K + k] * __uint_as_float(e == 255 ? 0x7fc00000u : e << 23);
+constexpr int BK = 128, STEP = 32, THREADS = 256;
+
+struct Wgrad8Args {
+    const void* gy;
+    const signed char* codes;
+    const unsigned char* exps;
+    float *gw, *gb;              // the results, or [splits] partials of them
+    long M;
+    int N, K, tiles_n, tiles_k, splits;
+    long rows_per_split;         // a multiple of STEP
+};
+
+// element offset of (row, 16-byte chunk) in a [32][COLS] bf16 tile
+template <int COLS> __device__ __forceinline__ int lds_at(int row, int chunk) {
+    return row * COLS + 8 * (chunk ^ (((row & 7) << 1) | ((row >> 3) & 1)));
+}
+// columns c0 .. c0+31 (one per lane & 31), rows 16 s + {4 half + 0..3, 8 + 4 half + 0..3}
+template <int COLS> __device__ __forceinline__ bf16x8 operand(const __bf16* t, int s, int c0) {
+    const int lane = threadIdx.x & 63, i = lane & 15, half = lane >> 5, cg = (lane >> 4) & 1;
+    bf16x4 h[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const __bf16* at = t + lds_at<COLS>(16 * s + 8 * u + 4 * half + (i >> 2), c0 / 8 + 2 * cg + ((i & 3) >> 1)) + 4 * (i & 1);
+        h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)at);
+    }
+    return __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ unsigned upper_halves(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+
+// 16 bytes of a row of `len` elements from element c: whole, in part (the rest 0), or nothing
+template <typename T> __device__ __forceinline__ u32x4 load16(const T* row, int c, int len) {
+    constexpr int E = 16 / sizeof(T);
+    u32x4 v = {};
+    if (c + E <= len) {
+        v = *reinterpret_cast<const u32x4_a1*>(row + c);
+    } else if (c < len) {
+        T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+        for (int i = 0; i < E; i++)
+            if (c + i < len) e[i] = row[c + i];
+    }
+    return v;
+}
+
+template <typename T> struct Wgrad8Shape {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int BN = F32 ? 128 : 256, PARTS = F32 ? 3 : 1;
+    static constexpr int E = 16 / sizeof(T);                              // gy elements per 16 bytes
+    static constexpr int CPR = BN / E;                                    // 16-byte pieces of gy per row of the tile: 32 either way
+    static constexpr int PIECES = STEP * CPR / THREADS;                   // 4 per thread
+    static constexpr int NB = BN / 64;                                    // 32-column blocks of n per wavefront
+};
+
+template <typename T> __global__ __launch_bounds__(THREADS, 2) void wgrad8_kernel(const Wgrad8Args a) {
+    typedef Wgrad8Shape<T> S;
+    constexpr int BN = S::BN, PARTS = S::PARTS, NB = S::NB;
+    __shared__ __attribute__((aligned(16))) __bf16 gbuf[2][PARTS][STEP * BN];
+    __shared__ __attribute__((aligned(16))) __bf16 xbuf[2][STEP * BK];
+
+    // tiles of one range of rows next to each other on one XCD: they read the same rows of gy and of the codes
+    const int tiles = a.tiles_n * a.tiles_k, total = tiles * a.splits, per = (total + 7) / 8;
+    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (id >= total || (blockIdx.x >> 3) >= (unsigned)per) return;
+    const int split = id / tiles, tile = id - split * tiles, tn = tile / a.tiles_k, tk = tile - tn * a.tiles_k;
+    const int n0 = tn * BN, k0 = tk * BK;
+    const long m_beg = split * a.rows_per_split, m_end = m_beg + a.rows_per_split < a.M ? m_beg + a.rows_per_split : a.M;
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l31 = lane & 31;
+    const int wn = (wave >> 1) * (BN / 2), wk = (wave & 1) * 64;
+    const int groups = (a.K + 31) / 32;
+
+    // loads: gy piece i of this thread = row tid / 32 + 8 i, elements E (tid % 32); codes = row tid / 8, 16 of them
+    const T* gy = static_cast<const T*>(a.gy);
+    const int g_row = threadIdx.x / S::CPR, g_col = n0 + S::E * (threadIdx.x % S::CPR);
+    const int x_row = threadIdx.x >> 3, x_col = k0 + 16 * (threadIdx.x & 7);
+    u32x4 graw[S::PIECES], xraw;
+    unsigned xexp;
+    auto load = [&](long m) {
+#pragma unroll
+        for (int i = 0; i < S::PIECES; i++) {
+            const long r = m + g_row + (THREADS / S::CPR) * i;
+            graw[i] = u32x4{};
+            if (r < m_end) graw[i] = load16<T>(gy + r * a.N, g_col, a.N);
         }
-        b[ty][tx] = v;
+        const long r = m + x_row;
+        xraw = u32x4{};
+        xexp = 1;
+        if (r < m_end && x_col < a.K) {
+            xraw = load16<signed char>(a.codes + r * a.K, x_col, a.K);
+            xexp = a.exps[r * groups + (x_col >> 5)];
+        }
+    };
+    const bool bias = a.gb && tk == 0;
+    float bsum[S::E];
+#pragma unroll
+    for (int i = 0; i < S::E; i++) bsum[i] = 0.f;
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < S::PIECES; i++) {
+            const int row = g_row + (THREADS / S::CPR) * i, col = S::E * (threadIdx.x % S::CPR);
+            if constexpr (S::F32) {
+                unsigned h[4], m[4], l[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {                            // 8 + 8 + 8 bits: h + m + l = gy exactly
+                    const float x = __uint_as_float(graw[i][e]);
+                    h[e] = graw[i][e] & 0xffff0000u;
+                    const float rest = x - __uint_as_float(h[e]);
+                    m[e] = __float_as_uint(rest) & 0xffff0000u;
+                    l[e] = __float_as_uint(rest - __uint_as_float(m[e]));
+                    if (bias) bsum[e] += x;
+                }
+                const int at = lds_at<BN>(row, col / 8) + (col & 7);
+                *reinterpret_cast<u32x2*>(&gbuf[buf][0][at]) = u32x2{upper_halves(h[0], h[1]), upper_halves(h[2], h[3])};
+                *reinterpret_cast<u32x2*>(&gbuf[buf][1 % PARTS][at]) = u32x2{upper_halves(m[0], m[1]), upper_halves(m[2], m[3])};
+                *reinterpret_cast<u32x2*>(&gbuf[buf][2 % PARTS][at]) = u32x2{upper_halves(l[0], l[1]), upper_halves(l[2], l[3])};
+            } else {
+                *reinterpret_cast<u32x4*>(&gbuf[buf][0][lds_at<BN>(row, col / 8)]) = graw[i];
+                if (bias) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) bsum[e % S::E] += __uint_as_float(e & 1 ? graw[i][e / 2] & 0xffff0000u : graw[i][e / 2] << 16);
+                }
+            }
+        }
+        const float step = __uint_as_float(xexp == 255 ? 0x7fc00000u : xexp << 23);
+        u32x4 x[2];
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = (float)(signed char)(xraw[w] >> (8 * e)) * step;
+            x[w >> 1][2 * (w & 1)] = upper_halves(__float_as_uint(v[0]), __float_as_uint(v[1]));
+            x[w >> 1][2 * (w & 1) + 1] = upper_halves(__float_as_uint(v[2]), __float_as_uint(v[3]));
+        }
+#pragma unroll
+        for (int w = 0; w < 2; w++) *reinterpret_cast<u32x4*>(&xbuf[buf][lds_at<BK>(x_row, 2 * (threadIdx.x & 7) + w)]) = x[w];
+    };
+
+    f32x16 acc[NB][2];
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) acc[i][j] = f32x16{};
+
+    load(m_beg);
+    store(0);
+    int buf = 0;
+    for (long m = m_beg; m < m_end; m += STEP, buf ^= 1) {
+        __syncthreads();
+        const bool more = m + STEP < m_end;
+        if (more) load(m + STEP);
+#pragma unroll
+        for (int s = 0; s < STEP / 16; s++) {
+            bf16x8 x[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) x[j] = operand<BK>(xbuf[buf], s, wk + 32 * j);
+#pragma unroll
+            for (int i = 0; i < NB; i++)
+#pragma unroll
+                for (int p = 0; p < PARTS; p++) {
+                    const bf16x8 g = operand<BN>(gbuf[buf][p], s, wn + 32 * i);
+#pragma unroll
+                    for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(g, x[j], acc[i][j], 0, 0, 0);
+                }
+        }
+        if (more) store(buf ^ 1);
+    }
+
+    // accumulator: column k = lane & 31, row n = (reg & 3) + 8 (reg >> 2) + 4 half
+    float* out = a.gw + (size_t)split * a.N * a.K;
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int k = k0 + wk + 32 * j + l31;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int n = n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
+                if (n < a.N && k < a.K) out[(size_t)n * a.K + k] = acc[i][j][r];
+            }
+        }
+    if (bias) {
+        float* red = reinterpret_cast<float*>(&gbuf[0][0][0]);          // [8 row groups][BN]
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            acc += a[i][ty] * b[i][tx];
-            bias += a[i][ty];
-        }
+        for (int e = 0; e < S::E; e++) red[g_row * BN + S::E * (threadIdx.x % S::CPR) + e] = bsum[e];
         __syncthreads();
+        if (threadIdx.x < BN && n0 + threadIdx.x < a.N) {
+            float s = 0.f;
+#pragma unroll
+            for (int g = 0; g < THREADS / S::CPR; g++) s += red[g * BN + threadIdx.x];
+            a.gb[(size_t)split * a.N + n0 + threadIdx.x] = s;
+        }
     }
-    const int n = n0 + ty, k = k0 + tx;
-    if (n < N && k < K) gw[(size_t)n * K + k] = acc;
-    if (gb && blockIdx.x == 0 && tx == 0 && n < N) gb[n] = bias;
+}
+
+// out[i] = sum over the splits of part[split][i], in order
+__global__ __launch_bounds__(256) void wgrad8_fold_kernel(const float* __restrict__ part, float* __restrict__ out, long n, int splits) {
+    const long i = 4 * ((long)blockIdx.x * 256 + threadIdx.x);
+    if (i + 4 <= n && (n & 3) == 0) {
+        f32x4 s = {};
+#pragma unroll 8
+        for (int p = 0; p < splits; p++) s += *reinterpret_cast<const f32x4*>(part + p * n + i);
+        *reinterpret_cast<f32x4*>(out + i) = s;
+    } else {
+        for (long j = i; j < n && j < i + 4; j++) {
+            float s = 0.f;
+            for (int p = 0; p < splits; p++) s += part[p * n + j];
+            out[j] = s;
+        }
+    }
+}
+
+struct Wgrad8Plan { int tiles_n, tiles_k, splits; long rows_per_split; };
+// about two workgroups per CU, none with fewer than 4 steps of rows (a partial tile costs as much traffic as 2 to 4 steps)
+Wgrad8Plan plan_of(long M, int N, int K, int dtype) {
+    Wgrad8Plan p;
+    const int BN = dtype == SCP_DTYPE_F32 ? 128 : 256;
+    p.tiles_n = (N + BN - 1) / BN;
+    p.tiles_k = (K + BK - 1) / BK;
+    const long tiles = (long)p.tiles_n * p.tiles_k, steps = (M + STEP - 1) / STEP;
+    long want = tiles >= 512 ? 1 : 512 / tiles;
+    if (want > (steps + 3) / 4) want = (steps + 3) / 4;
+    const long per = (steps + want - 1) / want;
+    p.splits = (int)((steps + per - 1) / per);
+    p.rows_per_split = per * STEP;
+    return p;
+}
+const char* bad_problem(long M, int N, int K, int dtype) {
+    if (M <= 0 || N <= 0 || K <= 0) return "weight_grad8: empty problem";
+    if (dtype != SCP_DTYPE_F32 && dtype != SCP_DTYPE_BF16) return "weight_grad8: unknown type";
+    if (N > (1 << 20) || K > (1 << 20) || (long)N * K > (1l << 34)) return "weight_grad8: more than 2^20 columns or 2^34 weights";
+    return nullptr;
 }
 
 }  // namespace
 
-extern "C" size_t scp_weight_grad8_workspace(long M, int N, int K, int dtype) { return 0; }
+extern "C" size_t scp_weight_grad8_workspace(long M, int N, int K, int dtype) {
+    if (bad_problem(M, N, K, dtype)) return 0;
+    const Wgrad8Plan p = plan_of(M, N, K, dtype);
+    return p.splits > 1 ? (size_t)p.splits * ((size_t)N * K + N) * sizeof(float) : 0;
+}
 
 extern "C" int scp_weight_grad8(const void* gy, const signed char* codes, const unsigned char* exps, long M, int N, int K, int dtype, float* gw,
                                 float* gb, void* workspace, size_t workspace_bytes, void* stream) {
-    if (M <= 0 || N <= 0 || K <= 0) return scp::fail(hipErrorInvalidValue, "weight_grad8: empty problem");
-    if (dtype != SCP_DTYPE_F32 && dtype != SCP_DTYPE_BF16) return scp::fail(hipErrorInvalidValue, "weight_grad8: unknown type");
+    if (const char* why = bad_problem(M, N, K, dtype)) return scp::fail(hipErrorInvalidValue, why);
     if (!gy || !codes || !exps || !gw) return scp::fail(hipErrorInvalidValue, "weight_grad8: null argument");
+    const Wgrad8Plan p = plan_of(M, N, K, dtype);
+    const size_t n = (size_t)N * K;
+    if (p.splits > 1 && (!workspace || workspace_bytes < p.splits * (n + N) * sizeof(float) || (reinterpret_cast<size_t>(workspace) & 15)))
+        return scp::fail(hipErrorInvalidValue, "weight_grad8: workspace too small or not 16-byte aligned");
+    if ((reinterpret_cast<size_t>(gw) | reinterpret_cast<size_t>(gb)) & 15)
+        return scp::fail(hipErrorInvalidValue, "weight_grad8: gw and gb must be 16-byte aligned");
+    float* part = static_cast<float*>(workspace);
+    const Wgrad8Args a{gy, codes, exps, p.splits > 1 ? part : gw, !gb ? nullptr : p.splits > 1 ? part + p.splits * n : gb, M, N, K, p.tiles_n, p.tiles_k,
+                       p.splits, p.rows_per_split};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid((K + 15) / 16, (N + 15) / 16);
-    if (dtype == SCP_DTYPE_F32)
-        hipLaunchKernelGGL(wgrad8_kernel<float>, grid, dim3(256), 0, st, static_cast<const float*>(gy), codes, exps, M, N, K, gw, gb);
-    else
-        hipLaunchKernelGGL(wgrad8_kernel<__bf16>, grid, dim3(256), 0, st, static_cast<const __bf16*>(gy), codes, exps, M, N, K, gw, gb);
-    return scp::check_launch("weight_grad8");
+    const long total = (long)p.tiles_n * p.tiles_k * p.splits;
+    const dim3 grid((unsigned)((total + 7) / 8 * 8));
+    if (dtype == SCP_DTYPE_F32) hipLaunchKernelGGL(wgrad8_kernel<float>, grid, dim3(THREADS), 0, st, a);
+    else hipLaunchKernelGGL(wgrad8_kernel<__bf16>, grid, dim3(THREADS), 0, st, a);
+    if (const int e = scp::check_launch("weight_grad8")) return e;
+    if (p.splits > 1) {
+        hipLaunchKernelGGL(wgrad8_fold_kernel, dim3((unsigned)((n / 4 + 256) / 256)), dim3(256), 0, st, part, gw, (long)n, p.splits);
+        if (gb) hipLaunchKernelGGL(wgrad8_fold_kernel, dim3((unsigned)((N / 4 + 256) / 256)), dim3(256), 0, st, part + p.splits * n, gb, (long)N, p.splits);
+        return scp::check_launch("weight_grad8 fold");
+    }
+    return 0;
 }
