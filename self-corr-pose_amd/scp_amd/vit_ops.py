@@ -19,21 +19,38 @@ from torch.autograd.function import once_differentiable
 
 from . import capi
 
-_NULL = ctypes.c_void_p(0)
+_F32_BF16 = (torch.float32, torch.bfloat16)
 
 
-def _tensor(t, name, dtypes=(torch.float32, torch.bfloat16)):
-    if not torch.is_tensor(t) or not t.is_cuda:
+def _tensor(t, name, dtypes=_F32_BF16):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError("%s must be a CUDA tensor (no CPU fallback)" % name)
     if t.dtype not in dtypes:
         raise RuntimeError("%s must be %s, not %s" % (name, " or ".join(str(d)[6:] for d in dtypes), t.dtype))
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != torch._C._cuda_getDevice():
         raise RuntimeError("%s lives on cuda:%d but the current device is cuda:%d (torch.cuda.set_device first)"
                            % (name, t.device.index, torch.cuda.current_device()))
 
 
 def _ptr(t):
-    return _NULL if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
+
+
+def _stream():
+    """capi.current_stream() without the Python stream object (3 us of a call whose kernel may take 4)"""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _first_order(f):
+    """backward(ctx, *grads) that refuses to be differentiated again.  torch's once_differentiable does that for a pass that records a
+    graph (create_graph=True); any other pass skips its bookkeeping.  A backward pass runs on the engine's thread, where every
+    Python step costs two to three times what it does on the caller's, so these functions do little: what can be prepared is
+    prepared in the forward pass."""
+    guarded = once_differentiable(f)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else f(ctx, *grads)
+    return backward
 
 
 def _wants_grad(*ts):
@@ -44,57 +61,64 @@ def _wants_grad(*ts):
 def _norm_forward(x, residual, weight, bias, eps, want_stats):
     c = x.shape[-1]
     rows = x.numel() // c
+    dtype = capi.DTYPES[x.dtype]
+    w = weight if weight is not None else bias
+    wdtype = dtype if w is None else capi.DTYPES[w.dtype]
     y = torch.empty_like(x)
     total = None if residual is None else torch.empty_like(x)
-    stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if want_stats else None
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if want_stats else None
     if rows:
-        w = weight if weight is not None else bias
-        wdtype = capi.DTYPES[x.dtype if w is None else w.dtype]
-        capi.check(capi.lib().scp_layernorm_forward(_ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), eps, rows, c, capi.DTYPES[x.dtype], wdtype,
-                                                    _ptr(total), _ptr(y), _ptr(stats), capi.current_stream()), "scp_layernorm_forward")
-    return total, y, stats
+        code = capi.lib().scp_layernorm_forward(x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), eps, rows, c, dtype, wdtype, _ptr(total),
+                                                y.data_ptr(), _ptr(stats), _stream())
+        if code:
+            capi.check(code, "scp_layernorm_forward")
+    return total, y, stats, (rows, c, dtype, wdtype)
 
 
 class _LayerNorm(Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps):
-        total, y, stats = _norm_forward(x, residual, weight, bias, eps, True)
+        total, y, stats, ctx.sizes = _norm_forward(x, residual, weight, bias, eps, True)
         ctx.save_for_backward(x if total is None else total, weight, stats)
         ctx.bias_dtype = None if bias is None else bias.dtype
-        ctx.has_residual = residual is not None
         ctx.set_materialize_grads(False)
-        return (total, y) if ctx.has_residual else y
+        if residual is None:
+            return y
+        return total, y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, *grads):
-        gsum, gy = grads if ctx.has_residual else (None, grads[0])
         s, weight, stats = ctx.saved_tensors
-        want_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
-        want_w, want_b = ctx.needs_input_grad[2], ctx.needs_input_grad[3]
+        want_x, want_r, want_w, want_b = ctx.needs_input_grad[:4]
+        gsum, gy = grads if len(grads) == 2 else (None, grads[0])
         if gy is None:                                           # only the sum was used
-            gx = gsum if want_x else None
-            return gx, gx if ctx.has_residual else None, None, None, None
-        c = s.shape[-1]
-        rows = s.numel() // c
-        gy = gy.contiguous()
-        gsum = None if gsum is None else gsum.contiguous()
-        gx = torch.empty_like(s) if want_x else None
-        if rows:
-            gw = torch.empty(c, dtype=torch.float32, device=s.device) if want_w else None
-            gb = torch.empty(c, dtype=torch.float32, device=s.device) if want_b else None
-            L = capi.lib()
-            nbytes = L.scp_layernorm_backward_workspace(rows, c) if want_w or want_b else 0
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=s.device) if nbytes else None
-            wdtype = capi.DTYPES[s.dtype if weight is None else weight.dtype]
-            capi.check(L.scp_layernorm_backward(_ptr(s), _ptr(weight), _ptr(gy), _ptr(gsum), _ptr(stats), rows, c, capi.DTYPES[s.dtype], wdtype,
-                                                _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), nbytes, capi.current_stream()), "scp_layernorm_backward")
+            return gsum, gsum if want_r else None, None, None, None
+        rows, c, dtype, wdtype = ctx.sizes
+        dev = s.device
+        gx = torch.empty_like(s) if want_x or want_r else None
+        if rows == 0:
+            zero = torch.zeros(c, dtype=torch.float32, device=dev)
+            gw, gb = zero, zero.clone()
         else:
-            gw = torch.zeros(c, dtype=torch.float32, device=s.device) if want_w else None
-            gb = torch.zeros(c, dtype=torch.float32, device=s.device) if want_b else None
-        gw = None if gw is None else gw.to(weight.dtype)
-        gb = None if gb is None else gb.to(ctx.bias_dtype)
-        return gx, gx if ctx.has_residual else None, gw, gb, None
+            gy = gy.contiguous()
+            if gsum is not None:
+                gsum = gsum.contiguous()
+            gw = torch.empty(c, dtype=torch.float32, device=dev) if want_w else None
+            gb = torch.empty(c, dtype=torch.float32, device=dev) if want_b else None
+            L = capi.lib()
+            ws, nbytes = None, 0
+            if want_w or want_b:
+                nbytes = L.scp_layernorm_backward_workspace(rows, c)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            code = L.scp_layernorm_backward(s.data_ptr(), _ptr(weight), gy.data_ptr(), _ptr(gsum), stats.data_ptr(), rows, c, dtype, wdtype, _ptr(gx),
+                                            _ptr(gw), _ptr(gb), _ptr(ws), nbytes, _stream())
+            if code:
+                capi.check(code, "scp_layernorm_backward")
+        if wdtype:                                               # bf16 weights get bf16 gradients
+            gw = None if not want_w else gw.to(weight.dtype)
+            gb = None if not want_b else gb.to(ctx.bias_dtype)
+        return gx if want_x else None, gx if want_r else None, gw if want_w else None, gb if want_b else None, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-6, residual=None):
@@ -125,7 +149,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-6, residual=None):
     bias = None if bias is None else bias.contiguous()
     if _wants_grad(x, residual, weight, bias):
         return _LayerNorm.apply(x, residual, weight, bias, float(eps))
-    total, y, _ = _norm_forward(x, residual, weight, bias, float(eps), False)
+    total, y, _, _ = _norm_forward(x, residual, weight, bias, float(eps), False)
     return y if residual is None else (total, y)
 
 
@@ -140,56 +164,55 @@ def _addressable(t):
     return t.clone(memory_format=torch.contiguous_format)      # contiguous() would return a misaligned tensor as it is
 
 
-def _attn_params(q, k, v, scale, g=None):
-    p = capi.CrossAttnParams()
-    p.batch, p.queries, p.heads, p.head_dim = q.shape
-    p.keys, p.kv_heads = k.shape[1], k.shape[2]
-    p.dtype, p.scale = capi.DTYPES[q.dtype], scale
-    for f, t in (("q_stride", q), ("k_stride", k), ("v_stride", v), ("g_stride", g)):
-        if t is not None:
-            getattr(p, f)[:] = t.stride()[:3]
-    return p
-
-
-def _attn_forward(q, k, v, mask, scale, want_lse):
+def _attn_forward(q, k, v, mask, scale, keep):
+    """(out, log-sum-exp or None, C parameters); keep: for a backward pass"""
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=q.device) if want_lse else None
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if keep else None
     if out.numel() == 0:
-        return out, lse
+        return out, lse, None
     if k.shape[1] == 0:
-        return out.zero_(), lse
+        return out.zero_(), lse, None
     L = capi.lib()
-    p = _attn_params(q, k, v, scale)
-    nbytes = L.scp_cross_attention_forward_workspace(ctypes.byref(p))
+    p = capi.CrossAttnParams(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], capi.DTYPES[q.dtype], scale, q.stride()[:3],
+                             k.stride()[:3], v.stride()[:3])
+    ref = ctypes.byref(p)
+    nbytes = L.scp_cross_attention_forward_workspace(ref)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    capi.check(L.scp_cross_attention_forward(_ptr(q), _ptr(k), _ptr(v), _ptr(mask), ctypes.byref(p), _ptr(out), _ptr(lse), _ptr(ws), nbytes,
-                                             capi.current_stream()), "scp_cross_attention_forward")
-    return out, lse
+    code = L.scp_cross_attention_forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(mask), ref, out.data_ptr(), _ptr(lse), _ptr(ws), nbytes, _stream())
+    if code:
+        capi.check(code, "scp_cross_attention_forward")
+    return out, lse, p
 
 
 class _CrossAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, scale):
-        out, lse = _attn_forward(q, k, v, mask, scale, True)
+        out, lse, ctx.p = _attn_forward(q, k, v, mask, scale, True)
         ctx.save_for_backward(q, k, v, mask, out, lse)
-        ctx.scale = scale
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, g):
         q, k, v, mask, out, lse = ctx.saved_tensors
-        want = ctx.needs_input_grad[:3]
-        gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((q, k, v), want))
-        if q.numel() == 0 or k.shape[1] == 0:                   # no query or no key: nothing depends on the other side
+        wq, wk, wv = ctx.needs_input_grad[:3]
+        dev, dt = q.device, q.dtype
+        gq = torch.empty(q.shape, dtype=dt, device=dev) if wq else None
+        gk = torch.empty(k.shape, dtype=dt, device=dev) if wk else None
+        gv = torch.empty(k.shape, dtype=dt, device=dev) if wv else None
+        p = ctx.p
+        if p is None:                                            # no query or no key: nothing depends on the other side
             return tuple(None if t is None else t.zero_() for t in (gq, gk, gv)) + (None, None)
         g = _addressable(g)
+        p.g_stride = g.stride()[:3]
         L = capi.lib()
-        p = _attn_params(q, k, v, ctx.scale, g)
-        nbytes = L.scp_cross_attention_backward_workspace(ctypes.byref(p))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        capi.check(L.scp_cross_attention_backward(_ptr(q), _ptr(k), _ptr(v), _ptr(mask), _ptr(out), _ptr(lse), _ptr(g), ctypes.byref(p), _ptr(gq),
-                                                  _ptr(gk), _ptr(gv), _ptr(ws), nbytes, capi.current_stream()), "scp_cross_attention_backward")
+        ref = ctypes.byref(p)
+        nbytes = L.scp_cross_attention_backward_workspace(ref)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        code = L.scp_cross_attention_backward(q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(mask), out.data_ptr(), lse.data_ptr(), g.data_ptr(), ref,
+                                              _ptr(gq), _ptr(gk), _ptr(gv), ws.data_ptr(), nbytes, _stream())
+        if code:
+            capi.check(code, "scp_cross_attention_backward")
         return gq, gk, gv, None, None
 
 
@@ -250,13 +273,13 @@ class Packed8:
         if out.numel():
             c = out.shape[-1]
             capi.check(capi.lib().scp_unpack8(_ptr(self.codes), _ptr(self.exps), out.numel() // c, c, capi.DTYPES[dtype], _ptr(out),
-                                              capi.current_stream()), "scp_unpack8")
+                                              _stream()), "scp_unpack8")
         return out
 
 
 def _packed_like(x):
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    exps = torch.empty(tuple(x.shape[:-1]) + ((x.shape[-1] + 31) // 32,), dtype=torch.uint8, device=x.device)
+    codes = torch.empty_like(x, dtype=torch.int8)
+    exps = torch.empty(x.shape[:-1] + ((x.shape[-1] + 31) // 32,), dtype=torch.uint8, device=x.device)
     return codes, exps
 
 
@@ -283,7 +306,7 @@ def pack8(x):
     codes, exps = _packed_like(x)
     if x.numel():
         c = x.shape[-1]
-        capi.check(capi.lib().scp_pack8(_ptr(x), x.numel() // c, c, capi.DTYPES[x.dtype], _ptr(codes), _ptr(exps), capi.current_stream()), "scp_pack8")
+        capi.check(capi.lib().scp_pack8(_ptr(x), x.numel() // c, c, capi.DTYPES[x.dtype], _ptr(codes), _ptr(exps), _stream()), "scp_pack8")
     return Packed8(codes, exps, x.dtype)
 
 
@@ -293,7 +316,7 @@ def _gelu_forward(x, keep):
     if x.numel():
         c = x.shape[-1]
         capi.check(capi.lib().scp_gelu8_forward(_ptr(x), x.numel() // c, c, capi.DTYPES[x.dtype], _ptr(y), _ptr(codes), _ptr(exps),
-                                                capi.current_stream()), "scp_gelu8_forward")
+                                                _stream()), "scp_gelu8_forward")
     return y, codes, exps
 
 
@@ -302,18 +325,20 @@ class _Gelu8(Function):
     def forward(ctx, x):
         y, codes, exps = _gelu_forward(x, True)
         ctx.save_for_backward(codes, exps)
+        ctx.sizes = x.numel(), x.shape[-1], capi.DTYPES[x.dtype]
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, gy):
         codes, exps = ctx.saved_tensors
+        n, c, dtype = ctx.sizes
         gy = gy.contiguous()
         gx = torch.empty_like(gy)
-        if gy.numel():
-            c = gy.shape[-1]
-            capi.check(capi.lib().scp_gelu8_backward(_ptr(codes), _ptr(exps), _ptr(gy), gy.numel() // c, c, capi.DTYPES[gy.dtype], _ptr(gx),
-                                                     capi.current_stream()), "scp_gelu8_backward")
+        if n:
+            code = capi.lib().scp_gelu8_backward(codes.data_ptr(), exps.data_ptr(), gy.data_ptr(), n // c, c, dtype, gx.data_ptr(), _stream())
+            if code:
+                capi.check(code, "scp_gelu8_backward")
         return gx
 
 
@@ -348,7 +373,7 @@ def weight_grad8(grad, packed, bias=True):
     nbytes = L.scp_weight_grad8_workspace(rows, n, k, dt)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device) if nbytes else None
     capi.check(L.scp_weight_grad8(_ptr(grad), _ptr(packed.codes), _ptr(packed.exps), rows, n, k, dt, _ptr(gw), _ptr(gb), _ptr(ws), nbytes,
-                                  capi.current_stream()), "scp_weight_grad8")
+                                  _stream()), "scp_weight_grad8")
     return gw, gb
 
 
@@ -362,7 +387,7 @@ class _Linear8(Function):
         return torch.nn.functional.linear(x, weight, bias)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, gy):
         weight, codes, exps = ctx.saved_tensors
         gx = gy.matmul(weight) if ctx.needs_input_grad[0] else None

@@ -687,6 +687,38 @@ def test_gradients_against_differences(op):
 
 
 @gpu
+def test_second_derivatives_are_refused():
+    g = gen(51)
+    x = torch.randn(5, 64, generator=g, device="cuda").requires_grad_(True)
+    w = torch.randn(64, 64, generator=g, device="cuda").requires_grad_(True)
+    q = torch.randn(1, 4, 2, 32, generator=g, device="cuda").requires_grad_(True)
+    for y, leaf in ((vit_ops.layer_norm(x), x), (vit_ops.gelu8(x), x), (vit_ops.linear8(x, w), x), (vit_ops.cross_attention(q, q, q), q)):
+        first, = torch.autograd.grad((y * y).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(first.sum(), leaf)
+            pytest.fail("a second derivative was not refused")
+
+
+@gpu
+def test_backward_twice_over_one_forward():
+    g = gen(52)
+    x, gy, w = (torch.randn(40, 64, generator=g, device="cuda") for _ in range(3))
+    q, go = (torch.randn(2, 7, 2, 64, generator=g, device="cuda") for _ in range(2))
+    x, w, q = (t.requires_grad_(True) for t in (x, w, q))
+    for y, leaves, up in ((vit_ops.layer_norm(x), (x,), gy), (vit_ops.gelu8(x), (x,), gy), (vit_ops.linear8(x, w), (x, w), gy[:, :40].contiguous()),
+                          (vit_ops.cross_attention(q, q, q), (q,), go)):
+        a = torch.autograd.grad(y, leaves, up, retain_graph=True)
+        keep = [t.clone() for t in a]
+        torch.autograd.grad(y, leaves, 2 * up, retain_graph=True)
+        b = torch.autograd.grad(y, leaves, up.transpose(0, 1).contiguous().transpose(0, 1))
+        assert all(torch.equal(s, k) for s, k in zip(a, keep))                                    # not written again by the second pass
+        library = len(leaves) == 2                                                                # linear8's gx: a library product, whose kernel goes by the layout
+        if library:                                                                               # two fp32 sums of 40 terms: 2 x 40 roundings of sum|terms|
+            within(b[0], a[0].double(), 80 * U * (up.double().abs() @ w.detach().double().abs()), "gx")
+        assert all(torch.equal(s, t) for s, t in list(zip(a, b))[library:])
+
+
+@gpu
 def test_repeated_calls_give_the_same_bits():
     P, q_tok, enc, mask, go = _decoder_setup(5)
 
