@@ -13,12 +13,19 @@
 // bf16 runs on v_mfma_f32_32x32x16_bf16 (p and gs rounded to bf16 for their product: one operand of it has to be bf16, and the result is
 // rounded to bf16 anyway), fp32 on v_mfma_f32_32x32x2_f32.
 //
+// Two ways to deal the work (Plan): OWN -- each of 4 wavefronts has 32 columns of its own and all read the same tile (64 rows in bf16, 32 in
+// fp32); SHARE -- the wavefronts have the SAME 32 columns, each reads its 32 rows of a 128-row tile, and their partial results are joined
+// through LDS at the end.  SHARE quarters the reuse of a tile and quadruples the number of wavefronts: it is for problems that would leave
+// SIMDs empty otherwise.  Tiles are double-buffered (the next one in flight during the products) where two fit 80 KB.
+//
 // LDS tiles are filled by buffer loads that write LDS directly, 16 bytes per lane.  A lane whose row is masked, past the end, or whose
 // channel is past head_dim gets an out-of-range offset: the hardware writes zeros, so nothing stored there can reach a product.  The
 // tile's image is swizzled through the SOURCE address (16-byte chunk `slot ^ f(row)`), such that both reads of it -- 16 consecutive rows at
 // one chunk, 4 consecutive rows at two -- touch each bank once.
 #pragma once
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "scp_common.h"
 
@@ -39,6 +46,7 @@ struct Args {
     long qs[3], ks[3], vs[3], gs[3];      // strides in elements: batch, token, head
     int BH, Nq, Nk, Hk, G, D;
     int nsplit, keys_per_split;           // keys_per_split: a multiple of the tile
+    bool write_delta;                     // the query-gradient kernel leaves delta behind for the key / value gradient
     float scale;
 };
 
@@ -101,6 +109,14 @@ template <int DP> struct Mma<__bf16, DP> {
         }
         return acc;
     }
+    static __device__ __forceinline__ float dot_lane(const Frag& x, const Frag& y) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) s += (float)x.f[i][j] * (float)y.f[i][j];
+        return s;
+    }
     // a[db][d][col] += sum_row t[r0 + row][32 db + d] p[row][col]
     static __device__ __forceinline__ void add(f32x16 (&a)[DB], const T* t, int r0, const f32x16& p) {
         const int lane = threadIdx.x & 63, i = lane & 15, half = lane >> 5, cg = (lane >> 4) & 1;
@@ -154,16 +170,39 @@ template <int DP> struct Mma<float, DP> {
         }
         return acc;
     }
+    static __device__ __forceinline__ float dot_lane(const Frag& x, const Frag& y) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < DP / 8; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) s += x.f[i][j] * y.f[i][j];
+        return s;
+    }
     static __device__ __forceinline__ void add(f32x16 (&a)[DB], const T* t, int r0, const f32x16& p) {
         const int half = (threadIdx.x >> 5) & 1, l31 = threadIdx.x & 31;
+        if constexpr (L::CPR == 16 || L::CPR == 32) {
+            // the swizzle of row 8 i + 4 half + j is j + 4 half in the low three chunk bits and i & 1 in the fourth, which only trades
+            // neighbouring 32-channel blocks: 4 lane addresses, everything else is a constant
+            const T* base[4];
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int row = r0 + acc_row(r, half);
+            for (int j = 0; j < 4; j++) base[j] = t + (r0 + 4 * half + j) * DP + 4 * ((l31 >> 2) ^ (4 * half + j)) + (l31 & 3);
 #pragma unroll
-            for (int db = 0; db < DB; db++) {
-                const int d = 32 * db + l31;
-                a[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(t[L::at(row, d >> 2) + (d & 3)], p[r], a[db], 0, 0, 0);
-            }
+            for (int r = 0; r < 16; r++)
+#pragma unroll
+                for (int db = 0; db < DB; db++)
+                    a[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(base[r & 3][8 * (r >> 2) * DP + 32 * (db ^ ((r >> 2) & 1))], p[r], a[db], 0, 0, 0);
+        } else {
+            // rows 8 i + 4 half + j swizzle by (j >> 1) + 2 half and, every other i, by 4: 8 lane addresses
+            const T* base[2][4];
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) base[e][j] = t + (r0 + 4 * half + j) * DP + 4 * ((l31 >> 2) ^ ((j >> 1) + 2 * half + 4 * e)) + (l31 & 3);
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+#pragma unroll
+                for (int db = 0; db < DB; db++)
+                    a[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(base[(r >> 2) & 1][r & 3][8 * (r >> 2) * DP + 32 * db], p[r], a[db], 0, 0, 0);
         }
     }
     static __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
@@ -187,29 +226,74 @@ template <typename T> __device__ __forceinline__ Rows rows_of(const void* p, con
     return {reinterpret_cast<const char*>(static_cast<const T*>(p) + b * st[0] + h * st[2]), st[1] * (long)sizeof(T), st[2] * (long)sizeof(T), G};
 }
 
-// rows r0 .. r0+N-1 -> LDS tile; valid(i): whether row r0 + i exists.  The host has checked that a tile spans less than 2^31 bytes.
-template <typename T, int DP, int N, int WAVES, typename V>
-__device__ __forceinline__ void fill_tile(T* lds, const Rows& src, int r0, int D, V valid) {
-    typedef Tile<T, DP> L;
-    constexpr int PIECES = N * L::CPR / 64;
-    static_assert(PIECES % WAVES == 0, "every wavefront moves the same number of pieces");
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n0 = src.G == 1 ? r0 : r0 / src.G;
-    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(src.base + n0 * src.ts), 0, (int)OUT_OF_RANGE, 0x00020000);
-#pragma unroll
-    for (int i = 0; i < PIECES / WAVES; i++) {
-        const int piece = wave + WAVES * i, idx = piece * 64 + lane;
-        const int row = idx / L::CPR, chunk = L::unswizzle(idx % L::CPR, row);
-        unsigned off;
-        if (src.G == 1) off = (unsigned)(row * (int)src.ts);
-        else {
-            const int n = (r0 + row) / src.G;
-            off = (unsigned)((n - n0) * (int)src.ts + (r0 + row - n * src.G) * (int)src.hs);
-        }
-        off = valid(row) && chunk * L::CH < D ? off + 16u * chunk : OUT_OF_RANGE;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + piece * 64 * L::CH), 16, (int)off, 0, 0, 0);
-    }
+__device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) const void*)p; }
+// 16 (4) bytes per lane from rsrc + off to LDS at `lds` + 16 (4) lane.  Inline assembly: the compiler would take every later LDS read for one of
+// the bytes in flight and wait for the NEXT tile before working on this one.  wait_tiles() is the wait.
+__device__ __forceinline__ void to_lds16(unsigned off, __amdgpu_buffer_rsrc_t rsrc, unsigned lds) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(off), "s"(rsrc), "s"(lds) : "memory");
 }
+__device__ __forceinline__ void to_lds4(unsigned off, __amdgpu_buffer_rsrc_t rsrc, unsigned lds) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(off), "s"(rsrc), "s"(lds) : "memory");
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)OUT_OF_RANGE, 0x00020000);
+}
+
+// moves rows r0 .. r0+N-1 of one head into an LDS tile; on[]: one bit per row, a clear one gives a row of zeros.  The lanes' offsets behind
+// the tile's first row are the same for every tile (tokens of one head, or a tile of a whole number of tokens), so they are kept; the
+// tile's own place is a 64-bit address.  The host has checked that a tile spans less than 2^31 bytes.
+template <typename T, int DP, int N, int WAVES> struct Loader {
+    typedef Tile<T, DP> L;
+    static constexpr int PIECES = N * L::CPR / 64, NP = PIECES / WAVES;
+    static_assert(PIECES % WAVES == 0, "every wavefront moves the same number of pieces");
+    Rows src;
+    int D, wave;
+    unsigned off[NP];
+    static __device__ __forceinline__ int row_of(int wave, int i) { return ((wave + WAVES * i) * 64 + (int)(threadIdx.x & 63)) / L::CPR; }
+    __device__ __forceinline__ void place_pieces(int r0) {
+        const int n0 = src.G == 1 ? 0 : r0 / src.G;
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            const int row = row_of(wave, i), chunk = L::unswizzle(((wave + WAVES * i) * 64 + (int)(threadIdx.x & 63)) % L::CPR, row);
+            unsigned o;
+            if (src.G == 1) o = (unsigned)row * (unsigned)src.ts;
+            else {
+                const int n = (r0 + row) / src.G;
+                o = (unsigned)(n - n0) * (unsigned)src.ts + (unsigned)(r0 + row - n * src.G) * (unsigned)src.hs;
+            }
+            off[i] = chunk * L::CH < D ? o + 16u * chunk : OUT_OF_RANGE;
+        }
+    }
+    __device__ __forceinline__ Loader(const Rows& rows, int head_dim) : src(rows), D(head_dim) {
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        place_pieces(0);
+    }
+    __device__ __forceinline__ void issue(T* lds, int r0, const unsigned (&on)[N / 32]) {
+        if (src.G > 1 && N % src.G) place_pieces(r0);
+        const __amdgpu_buffer_rsrc_t rsrc = buffer(src.base + (src.G == 1 ? r0 : r0 / src.G) * src.ts);
+        unsigned all = 0xffffffffu;
+#pragma unroll
+        for (int j = 0; j < N / 32; j++) all &= on[j];
+        const unsigned at = __builtin_amdgcn_readfirstlane(lds_address(lds));
+        if (all == 0xffffffffu) {
+#pragma unroll
+            for (int i = 0; i < NP; i++) to_lds16(off[i], rsrc, at + (wave + WAVES * i) * 1024u);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                const int row = row_of(wave, i);
+                unsigned word = on[0];
+#pragma unroll
+                for (int j = 1; j < N / 32; j++) word = (row >> 5) == j ? on[j] : word;
+                to_lds16((word >> (row & 31)) & 1 ? off[i] : OUT_OF_RANGE, rsrc, at + (wave + WAVES * i) * 1024u);
+            }
+        }
+    }
+};
 __device__ __forceinline__ void wait_tiles() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -257,110 +341,154 @@ __device__ __forceinline__ bool place(int BH, int per_head, int& bh, int& blk) {
 }
 inline unsigned placed_blocks(int BH, int per_head) { return (unsigned)((BH >= 16 ? (BH + 7) / 8 * 8 : BH) * per_head); }
 
-template <typename T, int DP, bool SHARE> struct FwdShape {
-    // SHARE: the wavefronts share one block of 32 rows and split every tile's keys; otherwise each has its own 32 rows
-    static constexpr int WAVES = SHARE && sizeof(T) == 4 && DP > 64 ? 2 : 4;
-    static constexpr int KT = SHARE ? 32 * WAVES : (sizeof(T) == 2 ? 64 : 32);
-    static constexpr int ROWS = SHARE ? 32 : 32 * WAVES;
-    static constexpr int OCC = SHARE || DP > 64 ? 1 : 2;
+enum { FORWARD, GRAD_Q, GRAD_KV };
+// SHARE / OWN, tile rows, buffers
+template <typename T, int DP, bool SHARE> struct Shape {
+    static constexpr int WAVES = 4, THREADS = 256;
+    static constexpr int N = SHARE ? 128 : (sizeof(T) == 2 ? 64 : 32);      // rows per tile
+    static constexpr int COLS = SHARE ? 32 : 128;                           // columns per workgroup
+    static constexpr int BYTES = 2 * N * DP * (int)sizeof(T);               // the two tiles
+    static constexpr int NBUF = 2 * BYTES <= 81920 ? 2 : 1;
 };
+// wavefronts per SIMD that the registers are bounded for
+template <typename T, int DP, bool SHARE, int KIND> constexpr int occupancy() {
+    if (SHARE) return DP > 64 ? 1 : 2;                       // two workgroups' tiles per CU at most
+    if (sizeof(T) == 2) return KIND == FORWARD ? (DP <= 64 ? 4 : 2) : DP == 32 ? 3 : DP == 64 ? 2 : 1;
+    return DP == 32 ? 3 : DP == 64 ? 2 : 1;
+}
+
+// walks the tiles of [key_beg, key_end) that hold a key: move(t, buf, on) starts the loads of the tile at key win + t N, work(buf, on) uses it
+template <typename S, typename Move, typename Work>
+__device__ __forceinline__ void walk_keys(unsigned* words, const unsigned char* mask, int key_beg, int key_end, Move move, Work work) {
+    constexpr int W = S::N / 32;
+    for (int win = key_beg; win < key_end; win += 64 * S::N) {
+        unsigned long long active = key_window<S::N, S::WAVES>(words, mask, win, key_end);
+        unsigned on[W], next[W];
+        auto start = [&](int buf, unsigned (&w)[W]) {
+            const int t = __builtin_ctzll(active);
+            active &= active - 1;
+#pragma unroll
+            for (int j = 0; j < W; j++) w[j] = __builtin_amdgcn_readfirstlane(words[t * W + j]);
+            move(win + t * S::N, buf, w);
+        };
+        if (!active) continue;
+        if constexpr (S::NBUF == 2) {
+            int buf = 0;
+            start(0, on);
+            for (;;) {
+                wait_tiles();                                // this tile is in LDS, and nobody reads the other buffer any more
+                const bool more = active != 0;
+                if (more) start(buf ^ 1, next);
+                work(buf, on);
+                if (!more) break;
+                buf ^= 1;
+#pragma unroll
+                for (int j = 0; j < W; j++) on[j] = next[j];
+            }
+        } else {
+            for (;;) {
+                start(0, on);
+                wait_tiles();
+                work(0, on);
+                if (!active) break;
+                __syncthreads();                             // everybody is done with the tile
+            }
+        }
+    }
+}
 
 template <typename T, int DP, bool SHARE>
-__global__ __launch_bounds__((FwdShape<T, DP, SHARE>::WAVES * 64), (FwdShape<T, DP, SHARE>::OCC)) void forward_kernel(const Args a) {
-    typedef FwdShape<T, DP, SHARE> S;
+__global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, FORWARD>())) void forward_kernel(const Args a) {
+    typedef Shape<T, DP, SHARE> S;
     typedef Mma<T, DP> M;
-    constexpr int WAVES = S::WAVES, KT = S::KT, DB = M::DB, NKB = SHARE ? 1 : KT / 32;
-    __shared__ __attribute__((aligned(16))) T kbuf[2][KT * DP];
-    __shared__ __attribute__((aligned(16))) T vbuf[2][KT * DP];
-    __shared__ unsigned words[2 * KT];
+    constexpr int WAVES = S::WAVES, N = S::N, DB = M::DB, NKB = SHARE ? 1 : N / 32;
+    __shared__ __attribute__((aligned(16))) T tile[S::NBUF][2][N * DP];
+    __shared__ unsigned words[2 * N];
+    __shared__ float jm[SHARE ? WAVES * 32 * 2 : 1];
 
     const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int R = a.Nq * a.G, row_blocks = (R + S::ROWS - 1) / S::ROWS;
+    const int R = a.Nq * a.G, row_blocks = (R + S::COLS - 1) / S::COLS;
     int bh, blk;
     if (!place(a.BH, row_blocks * a.nsplit, bh, blk)) return;
-    const int split = blk / row_blocks, rb = blk - split * row_blocks;
+    const int split = SHARE ? blk / row_blocks : 0, rb = blk - split * row_blocks;
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int r = rb * S::ROWS + (SHARE ? 0 : 32 * wave) + l31;
-    const Rows qr = rows_of<T>(a.q, a.qs, b, hk * a.G, a.G), kr = rows_of<T>(a.k, a.ks, b, hk, 1), vr = rows_of<T>(a.v, a.vs, b, hk, 1);
+    const int r_wave = rb * S::COLS + (SHARE ? 0 : 32 * wave), r = r_wave + l31;
+    const bool idle = r_wave >= R;                           // a wavefront without rows only moves tiles
+    const Rows qr = rows_of<T>(a.q, a.qs, b, hk * a.G, a.G);
     const unsigned char* mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
-    const int key_beg = split * a.keys_per_split, key_end = min(a.Nk, key_beg + a.keys_per_split);
+    const int key_beg = SHARE ? split * a.keys_per_split : 0, key_end = SHARE ? min(a.Nk, key_beg + a.keys_per_split) : a.Nk;
     // a negative scale goes into q's sign: the maximum of s is the maximum of c s; c > 0 keeps -inf * c = -inf for masked keys at scale 0
     const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);
 
     typename M::Frag q;
     M::load(q, reinterpret_cast<const T*>(qr.row(r < R ? r : 0)), r < R, a.D, a.scale);
+    Loader<T, DP, N, WAVES> keys(rows_of<T>(a.k, a.ks, b, hk, 1), a.D), values(rows_of<T>(a.v, a.vs, b, hk, 1), a.D);
     f32x16 o[DB];
 #pragma unroll
     for (int i = 0; i < DB; i++) o[i] = f32x16{};
     float m = -INFINITY, l = 0.f;
 
-    for (int win = key_beg; win < key_end; win += 64 * KT) {
-        unsigned long long active = key_window<KT, WAVES>(words, mask, win, key_end);
-        if (!active) continue;
-        auto issue = [&](int t, int buf) {
-            auto valid = [&](int row) { return (words[t * (KT / 32) + (row >> 5)] >> (row & 31)) & 1; };
-            fill_tile<T, DP, KT, WAVES>(kbuf[buf], kr, win + t * KT, a.D, valid);
-            fill_tile<T, DP, KT, WAVES>(vbuf[buf], vr, win + t * KT, a.D, valid);
-        };
-        int t = __builtin_ctzll(active), buf = 0;
-        active &= active - 1;
-        issue(t, 0);
-        for (;;) {
-            wait_tiles();                                    // this tile is in LDS, and nobody reads the other buffer any more
-            const int tn = active ? __builtin_ctzll(active) : -1;
-            if (tn >= 0) {
-                active &= active - 1;
-                issue(tn, buf ^ 1);
-            }
-            f32x16 s[NKB];
-            float top = -INFINITY;
+    auto products = [&](int buf, const unsigned (&on)[N / 32]) {
+        unsigned mine[NKB], all = 0xffffffffu;
+        f32x16 s[NKB];
 #pragma unroll
-            for (int kb = 0; kb < NKB; kb++) {
-                const int r0 = SHARE ? 32 * wave : 32 * kb;
-                s[kb] = M::dot(kbuf[buf], r0, q);
-                const unsigned on = __builtin_amdgcn_readfirstlane(words[t * (KT / 32) + (r0 >> 5)]);
-                if (on != 0xffffffffu) {
-#pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (!((on >> acc_row(i, half)) & 1)) s[kb][i] = -INFINITY;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; i++) top = fmaxf(top, s[kb][i]);
-            }
-            top = fmaxf(top, other_half(top)) * c;
-            if (__any(top > m + RESCALE_THR)) {
-                const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - mn);
-                const float keep = mn == -INFINITY ? 1.f : alpha;          // a block of masked keys only (SHARE): nothing to rescale
-                l *= keep;
-                m = mn;
-#pragma unroll
-                for (int i = 0; i < DB; i++)
-#pragma unroll
-                    for (int j = 0; j < 16; j++) o[i][j] *= keep;
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int kb = 0; kb < NKB; kb++) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], c, -base));
-                    l += s[kb][i];
-                }
-                M::add(o, vbuf[buf], SHARE ? 32 * wave : 32 * kb, s[kb]);
-            }
-            if (tn < 0) break;
-            t = tn;
-            buf ^= 1;
+        for (int kb = 0; kb < NKB; kb++) {
+            mine[kb] = on[kb];
+            if constexpr (SHARE) mine[0] = wave == 0 ? on[0] : wave == 1 ? on[1] : wave == 2 ? on[2] : on[3];
+            all &= mine[kb];
+            s[kb] = M::dot(tile[buf][0], SHARE ? 32 * wave : 32 * kb, q);
         }
-    }
+        if (all != 0xffffffffu) {
+#pragma unroll
+            for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (!((mine[kb] >> acc_row(i, half)) & 1)) s[kb][i] = -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, s[kb][i]);
+        top = fmaxf(top, other_half(top)) * c;
+        if (__any(top > m + RESCALE_THR)) {
+            const float mn = fmaxf(m, top);
+            const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);        // -inf: only masked keys so far (SHARE)
+            l *= alpha;
+            m = mn;
+#pragma unroll
+            for (int i = 0; i < DB; i++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) o[i][j] *= alpha;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < NKB; kb++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], c, -base));
+                part[i & 3] += s[kb][i];
+            }
+            M::add(o, tile[buf][1], SHARE ? 32 * wave : 32 * kb, s[kb]);
+        }
+        l += (part[0] + part[1]) + (part[2] + part[3]);
+    };
+    walk_keys<S>(words, mask, key_beg, key_end,
+                 [&](int key, int buf, const unsigned (&on)[N / 32]) {
+                     keys.issue(tile[buf][0], key, on);
+                     values.issue(tile[buf][1], key, on);
+                 },
+                 [&](int buf, const unsigned (&on)[N / 32]) {
+                     if (!idle) products(buf, on);
+                 });
     l += other_half(l);
 
     const int H = a.Hk * a.G;
     if constexpr (SHARE) {                                   // join the wavefronts' shares of the keys
-        float* jo = reinterpret_cast<float*>(&kbuf[0][0]);   // [WAVES][32 rows][DP]
-        float* jm = reinterpret_cast<float*>(&vbuf[0][0]);   // [WAVES][32 rows][2]
-        static_assert(sizeof(kbuf) >= WAVES * 32 * DP * sizeof(float), "the joined partials fit the key tiles");
+        float* jo = reinterpret_cast<float*>(&tile[0][0][0]);        // [WAVES][32 rows][DP]
+        static_assert(sizeof(tile) >= WAVES * 32 * DP * sizeof(float), "the joined partials fit the tiles");
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < DB; i++)
@@ -372,7 +500,7 @@ __global__ __launch_bounds__((FwdShape<T, DP, SHARE>::WAVES * 64), (FwdShape<T, 
             jm[(wave * 32 + l31) * 2 + 1] = l;
         }
         __syncthreads();
-        for (int idx = threadIdx.x; idx < 32 * (DP / 4); idx += WAVES * 64) {
+        for (int idx = threadIdx.x; idx < 32 * (DP / 4); idx += 256) {
             const int row = idx / (DP / 4), d = 4 * (idx % (DP / 4)), rr = rb * 32 + row;
             if (rr >= R || d >= a.D) continue;
             float mt = -INFINITY, lt = 0.f;
@@ -401,21 +529,6 @@ __global__ __launch_bounds__((FwdShape<T, DP, SHARE>::WAVES * 64), (FwdShape<T, 
         }
     } else {
         if (r >= R) return;
-        if (a.nsplit > 1) {
-            const long at = ((long)split * a.BH + bh) * R + r;
-#pragma unroll
-            for (int i = 0; i < DB; i++)
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const int d = 32 * i + 8 * g + 4 * half;
-                    if (d < a.D) *reinterpret_cast<f32x4*>(a.part_o + at * a.D + d) = f32x4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
-                }
-            if (half == 0) {
-                a.part_ml[2 * at] = m;
-                a.part_ml[2 * at + 1] = l;
-            }
-            return;
-        }
         const int n = r / a.G, h = hk * a.G + r - n * a.G;
         T* out = static_cast<T*>(a.o) + (((long)b * a.Nq + n) * H + h) * a.D;
         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -473,35 +586,30 @@ template <typename T> __global__ __launch_bounds__(256) void delta_kernel(const 
     if (l == 0) a.delta[row] = s;
 }
 
-template <typename T, int DP> struct BwdShape {
-    static constexpr int WAVES = 4, ST = sizeof(T) == 2 ? 64 : 32;         // streamed rows per tile
-    static constexpr int OCC = DP > 64 ? 1 : 2;
-};
-
-// KV: stationary keys, streamed query rows (gk, gv); otherwise stationary query rows, streamed keys (gq)
-template <typename T, int DP, bool KV>
-__global__ __launch_bounds__((BwdShape<T, DP>::WAVES * 64), (BwdShape<T, DP>::OCC)) void backward_kernel(const Args a) {
-    typedef BwdShape<T, DP> S;
+// KV: stationary keys, streamed query rows (gk, gv); otherwise stationary query rows, streamed keys (gq, and delta on the way)
+template <typename T, int DP, bool KV, bool SHARE>
+__global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, KV ? GRAD_KV : GRAD_Q>())) void backward_kernel(const Args a) {
+    typedef Shape<T, DP, SHARE> S;
     typedef Mma<T, DP> M;
-    constexpr int WAVES = S::WAVES, ST = S::ST, DB = M::DB, COLS = 32 * WAVES;
-    __shared__ __attribute__((aligned(16))) T buf1[2][ST * DP];
-    __shared__ __attribute__((aligned(16))) T buf2[2][ST * DP];
-    __shared__ __attribute__((aligned(16))) float rowstat[KV ? 2 : 1][2][64];
-    __shared__ unsigned words[KV ? 1 : 2 * ST];
+    constexpr int WAVES = S::WAVES, N = S::N, DB = M::DB, NRB = SHARE ? 1 : N / 32, W = N / 32;
+    __shared__ __attribute__((aligned(16))) T tile[S::NBUF][2][N * DP];
+    __shared__ __attribute__((aligned(16))) float rowstat[KV ? S::NBUF : 1][2][KV ? (N < 64 ? 64 : N) : 4];
+    __shared__ unsigned words[KV ? 1 : 2 * N];
 
     const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int R = a.Nq * a.G, C = KV ? a.Nk : R;
     int bh, blk;
-    if (!place(a.BH, (C + COLS - 1) / COLS, bh, blk)) return;
+    if (!place(a.BH, (C + S::COLS - 1) / S::COLS, bh, blk)) return;
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int col = blk * COLS + 32 * wave + l31;
+    const int col_wave = blk * S::COLS + (SHARE ? 0 : 32 * wave), col = col_wave + l31;
     const unsigned char* mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
     const bool valid = col < C && (!KV || !mask || mask[col]);
+    const bool idle = !__any(valid);                         // a wavefront without columns only moves tiles
     const Rows qr = rows_of<T>(a.q, a.qs, b, hk * a.G, a.G), gr = rows_of<T>(a.go, a.gs, b, hk * a.G, a.G);
     const Rows kr = rows_of<T>(a.k, a.ks, b, hk, 1), vr = rows_of<T>(a.v, a.vs, b, hk, 1);
     const float* lse = a.lse + (long)bh * R;
-    const float* delta = a.delta + (long)bh * R;
+    float* delta = a.delta + (long)bh * R;
     const float c = a.scale * LOG2E;
 
     f32x16 acc1[DB], acc2[KV ? DB : 1];
@@ -515,11 +623,24 @@ __global__ __launch_bounds__((BwdShape<T, DP>::WAVES * 64), (BwdShape<T, DP>::OC
         M::load(f1, reinterpret_cast<const T*>((KV ? kr : qr).row(at)), valid, a.D, 1.f);
         M::load(f2, reinterpret_cast<const T*>((KV ? vr : gr).row(at)), valid, a.D, 1.f);
     }
-    const float col_lse = KV ? 0.f : (valid ? lse[col] : INFINITY), col_delta = KV ? 0.f : (valid ? delta[col] : 0.f);
+    float col_lse = 0.f, col_delta = 0.f;
+    long out_at;                                             // of this column's row in gk / gv or gq
+    if constexpr (KV) {
+        out_at = (((long)b * a.Nk + col) * a.Hk + hk) * a.D;
+    } else {                                                 // delta = gO . o: the same channels of o as this lane holds of gO
+        const int n = col / a.G;
+        out_at = (((long)b * a.Nq + n) * (a.Hk * a.G) + hk * a.G + col - n * a.G) * a.D;
+        typename M::Frag fo;
+        M::load(fo, static_cast<const T*>(a.o_in) + (valid ? out_at : 0), valid, a.D, 1.f);
+        col_delta = M::dot_lane(f2, fo);
+        col_delta += other_half(col_delta);
+        col_lse = valid ? lse[col] : INFINITY;
+        if (a.write_delta && valid && half == 0 && (!SHARE || wave == 0)) delta[col] = col_delta;
+    }
 
-    // one 32-row block: p, gs and the products over its rows; `on`: which rows exist (query gradient only)
-    auto block = [&](int buf, int r0, unsigned on) {
-        f32x16 p = M::dot(buf1[buf], r0, f1), ds = M::dot(buf2[buf], r0, f2);
+    // one 32-row block: p, gs and the products over its rows
+    auto block = [&](int buf, int r0, auto masked, unsigned on) {
+        f32x16 p = M::dot(tile[buf][0], r0, f1), ds = M::dot(tile[buf][1], r0, f2);
 #pragma unroll
         for (int g = 0; g < 4; g++) {
             f32x4 ls = {col_lse, col_lse, col_lse, col_lse}, dl = {col_delta, col_delta, col_delta, col_delta};
@@ -531,73 +652,127 @@ __global__ __launch_bounds__((BwdShape<T, DP>::WAVES * 64), (BwdShape<T, DP>::OC
             for (int j = 0; j < 4; j++) {
                 const int i = 4 * g + j;
                 p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], c, -ls[j]));
-                if (!KV && on != 0xffffffffu && !((on >> acc_row(i, half)) & 1)) p[i] = 0.f;
+                if constexpr (masked.value)
+                    if (!((on >> acc_row(i, half)) & 1)) p[i] = 0.f;
                 ds[i] = p[i] * (ds[i] - dl[j]);
             }
         }
-        if constexpr (KV) M::add(acc2, buf2[buf], r0, p);
-        M::add(acc1, buf1[buf], r0, ds);
+        if constexpr (KV) M::add(acc2, tile[buf][1], r0, p);
+        M::add(acc1, tile[buf][0], r0, ds);
     };
 
+    Loader<T, DP, N, WAVES> first(KV ? qr : kr, a.D), second(KV ? gr : vr, a.D);
     if constexpr (KV) {
         if (__syncthreads_or(valid)) {
             auto issue = [&](int r0, int buf) {
-                auto in = [&](int row) { return r0 + row < R; };
-                fill_tile<T, DP, ST, WAVES>(buf1[buf], qr, r0, a.D, in);
-                fill_tile<T, DP, ST, WAVES>(buf2[buf], gr, r0, a.D, in);
-                if (wave < 2) {                              // statistics of the tile's rows; 0 past the last row, where q and gO are 0
-                    const float* src = (wave ? delta : lse) + r0;
-                    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(src), 0, (int)OUT_OF_RANGE, 0x00020000);
-                    const unsigned off = lane < ST && r0 + lane < R ? 4u * lane : OUT_OF_RANGE;
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)&rowstat[buf][wave][0], 4, (int)off, 0, 0, 0);
+                unsigned on[W];
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    const int left = R - r0 - 32 * j;
+                    on[j] = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+                }
+                first.issue(tile[buf][0], r0, on);
+                second.issue(tile[buf][1], r0, on);
+                // statistics of the tile's rows, 64 per instruction; 0 past the last row, where q and gO are 0
+                constexpr int HALVES = N > 64 ? 2 : 1;
+                if (wave < 2 * HALVES) {
+                    const int which = wave & 1, part = 64 * (wave >> 1);
+                    const unsigned off = part + lane < N && r0 + part + lane < R ? 4u * (part + lane) : OUT_OF_RANGE;
+                    to_lds4(off, buffer((which ? delta : lse) + r0), __builtin_amdgcn_readfirstlane(lds_address(&rowstat[buf][which][part])));
                 }
             };
-            issue(0, 0);
-            int buf = 0;
-            for (int r0 = 0; r0 < R; r0 += ST, buf ^= 1) {
-                wait_tiles();
-                if (r0 + ST < R) issue(r0 + ST, buf ^ 1);
+            auto products = [&](int buf) {
+                if (idle) return;
+                if constexpr (SHARE) block(buf, 32 * wave, std::false_type{}, 0u);
+                else {
 #pragma unroll
-                for (int kb = 0; kb < ST / 32; kb++) block(buf, 32 * kb, 0xffffffffu);
+                    for (int rb = 0; rb < NRB; rb++) block(buf, 32 * rb, std::false_type{}, 0u);
+                }
+            };
+            if constexpr (S::NBUF == 2) {
+                issue(0, 0);
+                int buf = 0;
+                for (int r0 = 0; r0 < R; r0 += N, buf ^= 1) {
+                    wait_tiles();
+                    if (r0 + N < R) issue(r0 + N, buf ^ 1);
+                    products(buf);
+                }
+            } else {
+                for (int r0 = 0; r0 < R; r0 += N) {
+                    issue(r0, 0);
+                    wait_tiles();
+                    products(0);
+                    __syncthreads();
+                }
             }
         }
     } else {
-        for (int win = 0; win < a.Nk; win += 64 * ST) {
-            unsigned long long active = key_window<ST, WAVES>(words, mask, win, a.Nk);
-            if (!active) continue;
-            auto issue = [&](int t, int buf) {
-                auto in = [&](int row) { return (words[t * (ST / 32) + (row >> 5)] >> (row & 31)) & 1; };
-                fill_tile<T, DP, ST, WAVES>(buf1[buf], kr, win + t * ST, a.D, in);
-                fill_tile<T, DP, ST, WAVES>(buf2[buf], vr, win + t * ST, a.D, in);
-            };
-            int t = __builtin_ctzll(active), buf = 0;
-            active &= active - 1;
-            issue(t, 0);
-            for (;;) {
-                wait_tiles();
-                const int tn = active ? __builtin_ctzll(active) : -1;
-                if (tn >= 0) {
-                    active &= active - 1;
-                    issue(tn, buf ^ 1);
-                }
+        walk_keys<S>(words, mask, 0, a.Nk,
+                     [&](int key, int buf, const unsigned (&on)[W]) {
+                         first.issue(tile[buf][0], key, on);
+                         second.issue(tile[buf][1], key, on);
+                     },
+                     [&](int buf, const unsigned (&on)[W]) {
+                         if (idle) return;
+                         if constexpr (SHARE) {
+                             const unsigned mine = wave == 0 ? on[0] : wave == 1 ? on[1] : wave == 2 ? on[2] : on[3];
+                             if (mine == 0xffffffffu) block(buf, 32 * wave, std::false_type{}, mine);
+                             else if (mine) block(buf, 32 * wave, std::true_type{}, mine);
+                         } else {
+                             unsigned all = 0xffffffffu;
 #pragma unroll
-                for (int kb = 0; kb < ST / 32; kb++) block(buf, 32 * kb, __builtin_amdgcn_readfirstlane(words[t * (ST / 32) + kb]));
-                if (tn < 0) break;
-                t = tn;
-                buf ^= 1;
-            }
-        }
+                             for (int j = 0; j < W; j++) all &= on[j];
+                             if (all == 0xffffffffu) {
+#pragma unroll
+                                 for (int rb = 0; rb < NRB; rb++) block(buf, 32 * rb, std::false_type{}, 0u);
+                             } else {
+#pragma unroll
+                                 for (int rb = 0; rb < NRB; rb++)
+                                     if (on[rb]) block(buf, 32 * rb, std::true_type{}, on[rb]);
+                             }
+                         }
+                     });
     }
-    if (col >= C) return;
-    long at;
-    if (KV) at = (((long)b * a.Nk + col) * a.Hk + hk) * a.D;
-    else {
-        const int n = col / a.G;
-        at = (((long)b * a.Nq + n) * (a.Hk * a.G) + hk * a.G + col - n * a.G) * a.D;
-    }
+
     T* out1 = static_cast<T*>(KV ? a.gk : a.gq);
     T* out2 = static_cast<T*>(a.gv);
-    const float f = valid ? a.scale : 0.f;
+    if constexpr (SHARE) {                                   // add up the wavefronts' rows, in order
+        float* join = reinterpret_cast<float*>(&tile[0][0][0]);      // [WAVES][32 columns][DP]
+        static_assert(sizeof(tile) >= WAVES * 32 * DP * sizeof(float), "the joined partials fit the tiles");
+#pragma unroll
+        for (int which = 0; which < (KV ? 2 : 1); which++) {
+            T* out = which ? out2 : out1;
+            if (!out) continue;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < DB; i++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const f32x16& x = which ? acc2[KV ? i : 0] : acc1[i];
+                    *reinterpret_cast<f32x4*>(join + (wave * 32 + l31) * DP + 32 * i + 8 * g + 4 * half) = f32x4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
+                }
+            __syncthreads();
+            for (int idx = threadIdx.x; idx < 32 * (DP / 4); idx += 256) {
+                const int row = idx / (DP / 4), d = 4 * (idx % (DP / 4)), cc = blk * 32 + row;
+                if (cc >= C || d >= a.D) continue;
+                f32x4 sum = {};
+#pragma unroll
+                for (int w = 0; w < WAVES; w++) sum += *reinterpret_cast<const f32x4*>(join + (w * 32 + row) * DP + d);
+                const float f = which ? 1.f : a.scale;
+                if (KV && mask && !mask[cc]) sum = f32x4{};
+                long at;
+                if (KV) at = (((long)b * a.Nk + cc) * a.Hk + hk) * a.D;
+                else {
+                    const int n = cc / a.G;
+                    at = (((long)b * a.Nq + n) * (a.Hk * a.G) + hk * a.G + cc - n * a.G) * a.D;
+                }
+                M::store4(out + at + d, sum[0] * f, sum[1] * f, sum[2] * f, sum[3] * f);
+            }
+        }
+        return;
+    }
+    if (col >= C) return;
+    const float f = a.scale;
 #pragma unroll
     for (int i = 0; i < DB; i++)
 #pragma unroll
@@ -605,53 +780,61 @@ __global__ __launch_bounds__((BwdShape<T, DP>::WAVES * 64), (BwdShape<T, DP>::OC
             const int d = 32 * i + 8 * g + 4 * half;
             if (d >= a.D) continue;
             // a masked key's column is written as zeros whatever went through it
-            if (out1) M::store4(out1 + at + d, valid ? acc1[i][4 * g] * f : 0.f, valid ? acc1[i][4 * g + 1] * f : 0.f, valid ? acc1[i][4 * g + 2] * f : 0.f,
+            if (out1) M::store4(out1 + out_at + d, valid ? acc1[i][4 * g] * f : 0.f, valid ? acc1[i][4 * g + 1] * f : 0.f, valid ? acc1[i][4 * g + 2] * f : 0.f,
                                 valid ? acc1[i][4 * g + 3] * f : 0.f);
             if constexpr (KV)
-                if (out2) M::store4(out2 + at + d, valid ? acc2[i][4 * g] : 0.f, valid ? acc2[i][4 * g + 1] : 0.f, valid ? acc2[i][4 * g + 2] : 0.f,
+                if (out2) M::store4(out2 + out_at + d, valid ? acc2[i][4 * g] : 0.f, valid ? acc2[i][4 * g + 1] : 0.f, valid ? acc2[i][4 * g + 2] : 0.f,
                                     valid ? acc2[i][4 * g + 3] : 0.f);
         }
 }
 
 // ---- launch plan --------------------------------------------------------------------------------------------------------------------
-struct Plan {
-    bool share;
-    int nsplit, keys_per_split, row_blocks, waves;
-};
-// share: 32 rows or fewer per head -- four wavefronts with rows of their own would leave three idle.
-// split: fewer than two workgroups per CU -- the keys are divided until there are, with at least two tiles each.
-template <typename T> Plan forward_plan(const Args& a, int DP) {
+struct Plan { bool share; int nsplit, keys_per_split, row_blocks; };
+constexpr long SHARE_BELOW = 1024;                           // wavefronts of 32 columns; fewer leave SIMDs empty (256 CUs x 4)
+inline bool share_columns(const Args& a, int columns) { return (long)a.BH * ((columns + 31) / 32) < SHARE_BELOW; }
+// split: where even SHARE has too few workgroups, the keys are divided as long as each part keeps two tiles
+inline Plan forward_plan(const Args& a) {
     Plan p;
     const int R = a.Nq * a.G;
-    p.share = R <= 32;
-    p.waves = p.share && sizeof(T) == 4 && DP > 64 ? 2 : 4;
-    const int KT = p.share ? 32 * p.waves : (sizeof(T) == 2 ? 64 : 32);
+    p.share = share_columns(a, R);
+    p.nsplit = 1;
+    p.keys_per_split = a.Nk;
     p.row_blocks = (R + (p.share ? 32 : 128) - 1) / (p.share ? 32 : 128);
-    const int tiles = (a.Nk + KT - 1) / KT;
-    const long blocks = (long)a.BH * p.row_blocks;
-    int want = blocks >= 512 ? 1 : (int)((512 + blocks - 1) / blocks);
-    if (want > tiles / 2) want = tiles / 2 > 0 ? tiles / 2 : 1;
-    const int per = (tiles + want - 1) / want;
-    p.nsplit = (tiles + per - 1) / per;
-    p.keys_per_split = per * KT;
+    if (p.share) {
+        const int tiles = (a.Nk + 127) / 128;
+        const long blocks = (long)a.BH * p.row_blocks;
+        int want = blocks >= 512 ? 1 : (int)(512 / blocks);
+        if (want > tiles / 2) want = tiles / 2 > 0 ? tiles / 2 : 1;
+        const int per = (tiles + want - 1) / want;
+        p.nsplit = (tiles + per - 1) / per;
+        p.keys_per_split = per * 128;
+    }
     return p;
 }
 inline int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 
-template <typename T, int DP> void launch_forward(Args a, const Plan& p, hipStream_t st) {
-    const unsigned blocks = placed_blocks(a.BH, p.row_blocks * p.nsplit);
-    if (p.share) hipLaunchKernelGGL((forward_kernel<T, DP, true>), dim3(blocks), dim3(FwdShape<T, DP, true>::WAVES * 64), 0, st, a);
-    else hipLaunchKernelGGL((forward_kernel<T, DP, false>), dim3(blocks), dim3(256), 0, st, a);
+template <typename T, int DP> void launch_forward(const Args& a, const Plan& p, hipStream_t st) {
+    const dim3 grid(placed_blocks(a.BH, p.row_blocks * p.nsplit));
+    if (p.share) hipLaunchKernelGGL((forward_kernel<T, DP, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((forward_kernel<T, DP, false>), grid, dim3(256), 0, st, a);
     if (p.nsplit > 1) {
         const long n = (long)a.BH * a.Nq * a.G * (a.D / 4);
         hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
     }
 }
-template <typename T, int DP> void launch_backward(const Args& a, hipStream_t st) {
+template <typename T, int DP, bool KV> void launch_gradient(const Args& a, int columns, hipStream_t st) {
+    if (share_columns(a, columns))
+        hipLaunchKernelGGL((backward_kernel<T, DP, KV, true>), dim3(placed_blocks(a.BH, (columns + 31) / 32)), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((backward_kernel<T, DP, KV, false>), dim3(placed_blocks(a.BH, (columns + 127) / 128)), dim3(256), 0, st, a);
+}
+template <typename T, int DP> void launch_backward(Args a, hipStream_t st) {
     const int R = a.Nq * a.G;
-    hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)(((long)a.BH * R + 15) / 16)), dim3(256), 0, st, a);
-    if (a.gq) hipLaunchKernelGGL((backward_kernel<T, DP, false>), dim3(placed_blocks(a.BH, (R + 127) / 128)), dim3(256), 0, st, a);
-    if (a.gk || a.gv) hipLaunchKernelGGL((backward_kernel<T, DP, true>), dim3(placed_blocks(a.BH, (a.Nk + 127) / 128)), dim3(256), 0, st, a);
+    const bool kv = a.gk || a.gv;
+    a.write_delta = kv;
+    if (a.gq) launch_gradient<T, DP, false>(a, R, st);
+    else if (kv) hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)(((long)a.BH * R + 15) / 16)), dim3(256), 0, st, a);
+    if (kv) launch_gradient<T, DP, true>(a, a.Nk, st);
 }
 
 // instantiated in csrc/cross_attn_f32.hip and csrc/cross_attn_bf16.hip

@@ -39,14 +39,14 @@ const char* bad_problem(const scp_cross_attn_params* p) {
         return "cross_attention: more than 2^31 rows or keys over all heads";
     return nullptr;
 }
-// a tile (64 or 128 rows) is addressed with 31-bit byte offsets behind its first row; the tile's own place is a 64-bit address
+// a tile (at most 128 rows) is addressed with 31-bit byte offsets behind its first row; the tile's own place is a 64-bit address
 bool tile_too_wide(const scp_cross_attn_params* p, bool backward) {
     const long long size = p->dtype == SCP_DTYPE_F32 ? 4 : 2, lim = 1ll << 31, G = p->heads / p->kv_heads;
     for (const long long* st : {p->k_stride, p->v_stride})
         if (st[1] < 0 || 128 * st[1] * size >= lim) return true;
     if (backward)
         for (const long long* st : {p->q_stride, p->g_stride})
-            if (st[1] < 0 || st[2] < 0 || (65 * st[1] + G * st[2]) * size >= lim) return true;
+            if (st[1] < 0 || st[2] < 0 || (129 * st[1] + G * st[2]) * size >= lim) return true;
     return false;
 }
 bool misaligned(const void* p) { return (reinterpret_cast<size_t>(p) & 15) != 0; }
@@ -64,10 +64,6 @@ Args make_args(const scp_cross_attn_params* p) {
     a.nsplit = 1;
     return a;
 }
-Plan plan_of(const Args& a, int dtype) {
-    const int DP = scp_attn::padded_dim(a.D);
-    return dtype == SCP_DTYPE_F32 ? scp_attn::forward_plan<float>(a, DP) : scp_attn::forward_plan<__bf16>(a, DP);
-}
 size_t split_floats(const Args& a, const Plan& p) { return p.nsplit > 1 ? (size_t)p.nsplit * a.BH * a.Nq * a.G * (a.D + 2) : 0; }
 
 }  // namespace
@@ -75,7 +71,7 @@ size_t split_floats(const Args& a, const Plan& p) { return p.nsplit > 1 ? (size_
 extern "C" size_t scp_cross_attention_forward_workspace(const scp_cross_attn_params* p) {
     if (bad_problem(p)) return 0;
     const Args a = make_args(p);
-    return split_floats(a, plan_of(a, p->dtype)) * sizeof(float);
+    return split_floats(a, scp_attn::forward_plan(a)) * sizeof(float);
 }
 
 extern "C" int scp_cross_attention_forward(const void* q, const void* k, const void* v, const unsigned char* key_mask,
@@ -87,7 +83,7 @@ extern "C" int scp_cross_attention_forward(const void* q, const void* k, const v
         return scp::fail(hipErrorInvalidValue, "cross_attention_forward: tensors must be 16-byte aligned");
     if (tile_too_wide(p, false)) return scp::fail(hipErrorInvalidValue, "cross_attention_forward: token stride of k or v too large");
     Args a = make_args(p);
-    const Plan plan = plan_of(a, p->dtype);
+    const Plan plan = scp_attn::forward_plan(a);
     const size_t need = split_floats(a, plan);
     if (need && (!workspace || workspace_bytes < need * sizeof(float)))
         return scp::fail(hipErrorInvalidValue, "cross_attention_forward: workspace too small");
