@@ -46,7 +46,6 @@ struct Args {
     long qs[3], ks[3], vs[3], gs[3];      // strides in elements: batch, token, head
     int BH, Nq, Nk, Hk, G, D;
     int nsplit, keys_per_split;           // keys_per_split: a multiple of the tile
-    bool write_delta;                     // the query-gradient kernel leaves delta behind for the key / value gradient
     float scale;
 };
 
@@ -98,33 +97,28 @@ template <int DP> struct Mma<__bf16, DP> {
             x.f[i] = sign < 0.f ? -v : v;
         }
     }
-    // rows r0 .. r0+31 of `t` times the stationary columns
-    static __device__ __forceinline__ f32x16 dot(const T* t, int r0, const Frag& x) {
+    // acc[c] = rows r0 .. r0+31 of `t` times the stationary columns of block c
+    template <int CB> static __device__ __forceinline__ void dots(f32x16 (&acc)[CB], const T* t, int r0, const Frag (&x)[CB]) {
         const int half = (threadIdx.x >> 5) & 1, row = r0 + (threadIdx.x & 31);
-        f32x16 acc = {};
+#pragma unroll
+        for (int c = 0; c < CB; c++) acc[c] = f32x16{};
 #pragma unroll
         for (int i = 0; i < DP / 16; i++) {
             const bf16x8 a = *reinterpret_cast<const bf16x8*>(t + L::at(row, 2 * i + half));
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, x.f[i], acc, 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < CB; c++) acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, x[c].f[i], acc[c], 0, 0, 0);
         }
-        return acc;
     }
-    static __device__ __forceinline__ float dot_lane(const Frag& x, const Frag& y) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < DP / 16; i++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) s += (float)x.f[i][j] * (float)y.f[i][j];
-        return s;
-    }
-    // a[db][d][col] += sum_row t[r0 + row][32 db + d] p[row][col]
-    static __device__ __forceinline__ void add(f32x16 (&a)[DB], const T* t, int r0, const f32x16& p) {
+    // a[c][db][d][col] += sum_row t[r0 + row][32 db + d] p[c][row][col]
+    template <int CB> static __device__ __forceinline__ void adds(f32x16 (&a)[CB][DB], const T* t, int r0, const f32x16 (&p)[CB]) {
         const int lane = threadIdx.x & 63, i = lane & 15, half = lane >> 5, cg = (lane >> 4) & 1;
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            bf16x8 b;
+            bf16x8 b[CB];
 #pragma unroll
-            for (int j = 0; j < 8; j++) b[j] = (__bf16)p[8 * s + j];
+            for (int c = 0; c < CB; c++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) b[c][j] = (__bf16)p[c][8 * s + j];
 #pragma unroll
             for (int db = 0; db < DB; db++) {
                 bf16x4 h[2];
@@ -135,7 +129,8 @@ template <int DP> struct Mma<__bf16, DP> {
                     h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)at);
                 }
                 const bf16x8 w = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
-                a[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, b, a[db], 0, 0, 0);
+#pragma unroll
+                for (int c = 0; c < CB; c++) a[c][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, b[c], a[c][db], 0, 0, 0);
             }
         }
     }
@@ -159,26 +154,20 @@ template <int DP> struct Mma<float, DP> {
             x.f[i] = sign < 0.f ? -v : v;
         }
     }
-    static __device__ __forceinline__ f32x16 dot(const T* t, int r0, const Frag& x) {
+    template <int CB> static __device__ __forceinline__ void dots(f32x16 (&acc)[CB], const T* t, int r0, const Frag (&x)[CB]) {
         const int half = (threadIdx.x >> 5) & 1, row = r0 + (threadIdx.x & 31);
-        f32x16 acc = {};
+#pragma unroll
+        for (int c = 0; c < CB; c++) acc[c] = f32x16{};
 #pragma unroll
         for (int i = 0; i < DP / 8; i++) {
             const f32x4 a = *reinterpret_cast<const f32x4*>(t + L::at(row, 2 * i + half));
 #pragma unroll
-            for (int c = 0; c < 4; c++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[c], x.f[i][c], acc, 0, 0, 0);
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int c = 0; c < CB; c++) acc[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], x[c].f[i][j], acc[c], 0, 0, 0);
         }
-        return acc;
     }
-    static __device__ __forceinline__ float dot_lane(const Frag& x, const Frag& y) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < DP / 8; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) s += x.f[i][j] * y.f[i][j];
-        return s;
-    }
-    static __device__ __forceinline__ void add(f32x16 (&a)[DB], const T* t, int r0, const f32x16& p) {
+    template <int CB> static __device__ __forceinline__ void adds(f32x16 (&a)[CB][DB], const T* t, int r0, const f32x16 (&p)[CB]) {
         const int half = (threadIdx.x >> 5) & 1, l31 = threadIdx.x & 31;
         if constexpr (L::CPR == 16 || L::CPR == 32) {
             // the swizzle of row 8 i + 4 half + j is j + 4 half in the low three chunk bits and i & 1 in the fourth, which only trades
@@ -189,8 +178,11 @@ template <int DP> struct Mma<float, DP> {
 #pragma unroll
             for (int r = 0; r < 16; r++)
 #pragma unroll
-                for (int db = 0; db < DB; db++)
-                    a[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(base[r & 3][8 * (r >> 2) * DP + 32 * (db ^ ((r >> 2) & 1))], p[r], a[db], 0, 0, 0);
+                for (int db = 0; db < DB; db++) {
+                    const float w = base[r & 3][8 * (r >> 2) * DP + 32 * (db ^ ((r >> 2) & 1))];
+#pragma unroll
+                    for (int c = 0; c < CB; c++) a[c][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(w, p[c][r], a[c][db], 0, 0, 0);
+                }
         } else {
             // rows 8 i + 4 half + j swizzle by (j >> 1) + 2 half and, every other i, by 4: 8 lane addresses
             const T* base[2][4];
@@ -201,8 +193,11 @@ template <int DP> struct Mma<float, DP> {
 #pragma unroll
             for (int r = 0; r < 16; r++)
 #pragma unroll
-                for (int db = 0; db < DB; db++)
-                    a[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(base[(r >> 2) & 1][r & 3][8 * (r >> 2) * DP + 32 * db], p[r], a[db], 0, 0, 0);
+                for (int db = 0; db < DB; db++) {
+                    const float w = base[(r >> 2) & 1][r & 3][8 * (r >> 2) * DP + 32 * db];
+#pragma unroll
+                    for (int c = 0; c < CB; c++) a[c][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(w, p[c][r], a[c][db], 0, 0, 0);
+                }
         }
     }
     static __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
@@ -294,8 +289,12 @@ template <typename T, int DP, int N, int WAVES> struct Loader {
         }
     }
 };
+// every load of this wavefront has arrived (vmcnt 0; the builtin, so that the compiler knows it too and does not wait again later for
+// registers it loaded before the loop), then everybody's
 __device__ __forceinline__ void wait_tiles() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("" ::: "memory");
     __syncthreads();
 }
 
@@ -341,21 +340,20 @@ __device__ __forceinline__ bool place(int BH, int per_head, int& bh, int& blk) {
 }
 inline unsigned placed_blocks(int BH, int per_head) { return (unsigned)((BH >= 16 ? (BH + 7) / 8 * 8 : BH) * per_head); }
 
-enum { FORWARD, GRAD_Q, GRAD_KV };
 // SHARE / OWN, tile rows, buffers
 template <typename T, int DP, bool SHARE> struct Shape {
     static constexpr int WAVES = 4, THREADS = 256;
     static constexpr int N = SHARE ? 128 : (sizeof(T) == 2 ? 64 : 32);      // rows per tile
-    static constexpr int COLS = SHARE ? 32 : 128;                           // columns per workgroup
+    static constexpr int COLS = SHARE ? 32 : 128;                           // columns per workgroup (of one block per wavefront)
     static constexpr int BYTES = 2 * N * DP * (int)sizeof(T);               // the two tiles
     static constexpr int NBUF = 2 * BYTES <= 81920 ? 2 : 1;
+    // column blocks of a wavefront in the forward pass.  Two: every LDS read feeds two matrix instructions, and the products of one block run
+    // beside the exponentials of the other (bf16, 64 channels: 173 -> 160 us for 7686 x 4097 x 16 heads); more would not fit the registers.
+    static constexpr int CB = !SHARE && sizeof(T) == 2 && DP <= 64 ? 2 : 1;
+    // wavefronts per SIMD that the registers are bounded for
+    static constexpr int FWD_OCC = SHARE ? (DP > 64 ? 1 : 2) : sizeof(T) == 2 ? 2 : DP == 32 ? 3 : DP == 64 ? 2 : 1;
+    static constexpr int GRAD_OCC = DP > 64 ? 1 : 2;
 };
-// wavefronts per SIMD that the registers are bounded for
-template <typename T, int DP, bool SHARE, int KIND> constexpr int occupancy() {
-    if (SHARE) return DP > 64 ? 1 : 2;                       // two workgroups' tiles per CU at most
-    if (sizeof(T) == 2) return KIND == FORWARD ? (DP <= 64 ? 4 : 2) : DP == 32 ? 3 : DP == 64 ? 2 : 1;
-    return DP == 32 ? 3 : DP == 64 ? 2 : 1;
-}
 
 // walks the tiles of [key_beg, key_end) that hold a key: move(t, buf, on) starts the loads of the tile at key win + t N, work(buf, on) uses it
 template <typename S, typename Move, typename Work>
@@ -398,22 +396,22 @@ __device__ __forceinline__ void walk_keys(unsigned* words, const unsigned char* 
 }
 
 template <typename T, int DP, bool SHARE>
-__global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, FORWARD>())) void forward_kernel(const Args a) {
+__global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_kernel(const Args a) {
     typedef Shape<T, DP, SHARE> S;
     typedef Mma<T, DP> M;
-    constexpr int WAVES = S::WAVES, N = S::N, DB = M::DB, NKB = SHARE ? 1 : N / 32;
+    constexpr int WAVES = S::WAVES, N = S::N, DB = M::DB, CB = S::CB, COLS = S::COLS * CB;
     __shared__ __attribute__((aligned(16))) T tile[S::NBUF][2][N * DP];
     __shared__ unsigned words[2 * N];
     __shared__ float jm[SHARE ? WAVES * 32 * 2 : 1];
 
     const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int R = a.Nq * a.G, row_blocks = (R + S::COLS - 1) / S::COLS;
+    const int R = a.Nq * a.G, row_blocks = (R + COLS - 1) / COLS;
     int bh, blk;
     if (!place(a.BH, row_blocks * a.nsplit, bh, blk)) return;
     const int split = SHARE ? blk / row_blocks : 0, rb = blk - split * row_blocks;
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int r_wave = rb * S::COLS + (SHARE ? 0 : 32 * wave), r = r_wave + l31;
+    const int r_wave = rb * COLS + (SHARE ? 0 : 32 * CB * wave);
     const bool idle = r_wave >= R;                           // a wavefront without rows only moves tiles
     const Rows qr = rows_of<T>(a.q, a.qs, b, hk * a.G, a.G);
     const unsigned char* mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
@@ -421,59 +419,80 @@ __global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, FORWARD>())) void for
     // a negative scale goes into q's sign: the maximum of s is the maximum of c s; c > 0 keeps -inf * c = -inf for masked keys at scale 0
     const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);
 
-    typename M::Frag q;
-    M::load(q, reinterpret_cast<const T*>(qr.row(r < R ? r : 0)), r < R, a.D, a.scale);
-    Loader<T, DP, N, WAVES> keys(rows_of<T>(a.k, a.ks, b, hk, 1), a.D), values(rows_of<T>(a.v, a.vs, b, hk, 1), a.D);
-    f32x16 o[DB];
+    typename M::Frag q[CB];
+    f32x16 o[CB][DB];
+    float m[CB], l[CB];
 #pragma unroll
-    for (int i = 0; i < DB; i++) o[i] = f32x16{};
-    float m = -INFINITY, l = 0.f;
+    for (int x = 0; x < CB; x++) {
+        const int r = r_wave + 32 * x + l31;
+        M::load(q[x], reinterpret_cast<const T*>(qr.row(r < R ? r : 0)), r < R, a.D, a.scale);
+#pragma unroll
+        for (int i = 0; i < DB; i++) o[x][i] = f32x16{};
+        m[x] = -INFINITY;
+        l[x] = 0.f;
+    }
+    Loader<T, DP, N, WAVES> keys(rows_of<T>(a.k, a.ks, b, hk, 1), a.D), values(rows_of<T>(a.v, a.vs, b, hk, 1), a.D);
 
-    auto products = [&](int buf, const unsigned (&on)[N / 32]) {
-        unsigned mine[NKB], all = 0xffffffffu;
-        f32x16 s[NKB];
+    // `blocks` 32-key blocks from row r0 of the tile
+    auto products = [&](auto blocks, int buf, int r0, const unsigned* on) {
+        constexpr int NKB = decltype(blocks)::value;
+        f32x16 s[NKB][CB];
+        unsigned all = 0xffffffffu;
 #pragma unroll
         for (int kb = 0; kb < NKB; kb++) {
-            mine[kb] = on[kb];
-            if constexpr (SHARE) mine[0] = wave == 0 ? on[0] : wave == 1 ? on[1] : wave == 2 ? on[2] : on[3];
-            all &= mine[kb];
-            s[kb] = M::dot(tile[buf][0], SHARE ? 32 * wave : 32 * kb, q);
+            M::template dots<CB>(s[kb], tile[buf][0], r0 + 32 * kb, q);
+            all &= on[kb];
         }
         if (all != 0xffffffffu) {
 #pragma unroll
             for (int kb = 0; kb < NKB; kb++)
 #pragma unroll
                 for (int i = 0; i < 16; i++)
-                    if (!((mine[kb] >> acc_row(i, half)) & 1)) s[kb][i] = -INFINITY;
+                    if (!((on[kb] >> acc_row(i, half)) & 1)) {
+#pragma unroll
+                        for (int x = 0; x < CB; x++) s[kb][x][i] = -INFINITY;
+                    }
         }
-        float top = s[0][0];
+        float top[CB];
+        bool grow = false;
 #pragma unroll
-        for (int kb = 0; kb < NKB; kb++)
+        for (int x = 0; x < CB; x++) {
+            top[x] = s[0][x][0];
 #pragma unroll
-            for (int i = 0; i < 16; i++) top = fmaxf(top, s[kb][i]);
-        top = fmaxf(top, other_half(top)) * c;
-        if (__any(top > m + RESCALE_THR)) {
-            const float mn = fmaxf(m, top);
-            const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);        // -inf: only masked keys so far (SHARE)
-            l *= alpha;
-            m = mn;
+            for (int kb = 0; kb < NKB; kb++)
 #pragma unroll
-            for (int i = 0; i < DB; i++)
-#pragma unroll
-                for (int j = 0; j < 16; j++) o[i][j] *= alpha;
+                for (int i = 0; i < 16; i++) top[x] = fmaxf(top[x], s[kb][x][i]);
+            top[x] = fmaxf(top[x], other_half(top[x])) * c;
+            grow |= top[x] > m[x] + RESCALE_THR;
         }
-        const float base = m == -INFINITY ? 0.f : m;
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        if (__any(grow)) {
+#pragma unroll
+            for (int x = 0; x < CB; x++) {
+                const float mn = fmaxf(m[x], top[x]);
+                const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[x] - mn);
+                l[x] *= alpha;
+                m[x] = mn;
+#pragma unroll
+                for (int i = 0; i < DB; i++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) o[x][i][j] *= alpha;
+            }
+        }
 #pragma unroll
         for (int kb = 0; kb < NKB; kb++) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], c, -base));
-                part[i & 3] += s[kb][i];
+            for (int x = 0; x < CB; x++) {
+                const float base = m[x] == -INFINITY ? 0.f : m[x];
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    s[kb][x][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][x][i], c, -base));
+                    part[i & 3] += s[kb][x][i];
+                }
+                l[x] += (part[0] + part[1]) + (part[2] + part[3]);
             }
-            M::add(o, tile[buf][1], SHARE ? 32 * wave : 32 * kb, s[kb]);
+            M::template adds<CB>(o, tile[buf][1], r0 + 32 * kb, s[kb]);
         }
-        l += (part[0] + part[1]) + (part[2] + part[3]);
     };
     walk_keys<S>(words, mask, key_beg, key_end,
                  [&](int key, int buf, const unsigned (&on)[N / 32]) {
@@ -481,9 +500,16 @@ __global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, FORWARD>())) void for
                      values.issue(tile[buf][1], key, on);
                  },
                  [&](int buf, const unsigned (&on)[N / 32]) {
-                     if (!idle) products(buf, on);
+                     if (idle) return;
+                     if constexpr (SHARE) {
+                         const unsigned mine = wave == 0 ? on[0] : wave == 1 ? on[1] : wave == 2 ? on[2] : on[3];
+                         if (mine) products(std::integral_constant<int, 1>{}, buf, 32 * wave, &mine);
+                     } else {
+                         products(std::integral_constant<int, N / 32>{}, buf, 0, on);
+                     }
                  });
-    l += other_half(l);
+#pragma unroll
+    for (int x = 0; x < CB; x++) l[x] += other_half(l[x]);
 
     const int H = a.Hk * a.G;
     if constexpr (SHARE) {                                   // join the wavefronts' shares of the keys
@@ -494,10 +520,11 @@ __global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, FORWARD>())) void for
         for (int i = 0; i < DB; i++)
 #pragma unroll
             for (int g = 0; g < 4; g++)
-                *reinterpret_cast<f32x4*>(jo + (wave * 32 + l31) * DP + 32 * i + 8 * g + 4 * half) = f32x4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
+                *reinterpret_cast<f32x4*>(jo + (wave * 32 + l31) * DP + 32 * i + 8 * g + 4 * half) =
+                    f32x4{o[0][i][4 * g], o[0][i][4 * g + 1], o[0][i][4 * g + 2], o[0][i][4 * g + 3]};
         if (half == 0) {
-            jm[(wave * 32 + l31) * 2] = m;
-            jm[(wave * 32 + l31) * 2 + 1] = l;
+            jm[(wave * 32 + l31) * 2] = m[0];
+            jm[(wave * 32 + l31) * 2 + 1] = l[0];
         }
         __syncthreads();
         for (int idx = threadIdx.x; idx < 32 * (DP / 4); idx += 256) {
@@ -528,18 +555,22 @@ __global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, FORWARD>())) void for
             }
         }
     } else {
-        if (r >= R) return;
-        const int n = r / a.G, h = hk * a.G + r - n * a.G;
-        T* out = static_cast<T*>(a.o) + (((long)b * a.Nq + n) * H + h) * a.D;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-        for (int i = 0; i < DB; i++)
+        for (int x = 0; x < CB; x++) {
+            const int r = r_wave + 32 * x + l31;
+            if (r >= R) continue;
+            const int n = r / a.G, h = hk * a.G + r - n * a.G;
+            T* out = static_cast<T*>(a.o) + (((long)b * a.Nq + n) * H + h) * a.D;
+            const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int d = 32 * i + 8 * g + 4 * half;
-                if (d < a.D) M::store4(out + d, o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv);
-            }
-        if (a.lse && half == 0) a.lse[(long)bh * R + r] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+            for (int i = 0; i < DB; i++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const int d = 32 * i + 8 * g + 4 * half;
+                    if (d < a.D) M::store4(out + d, o[x][i][4 * g] * inv, o[x][i][4 * g + 1] * inv, o[x][i][4 * g + 2] * inv, o[x][i][4 * g + 3] * inv);
+                }
+            if (a.lse && half == 0) a.lse[(long)bh * R + r] = l[x] == 0.f ? INFINITY : m[x] + __builtin_amdgcn_logf(l[x]);
+        }
     }
 }
 
@@ -586,21 +617,25 @@ template <typename T> __global__ __launch_bounds__(256) void delta_kernel(const 
     if (l == 0) a.delta[row] = s;
 }
 
-// KV: stationary keys, streamed query rows (gk, gv); otherwise stationary query rows, streamed keys (gq, and delta on the way)
+template <typename T, int DP, bool SHARE> struct GradLds {
+    typedef Shape<T, DP, SHARE> S;
+    T tile[S::NBUF][2][S::N * DP];
+    float rowstat[S::NBUF][2][S::N < 64 ? 64 : S::N];        // log-sum-exp and delta of the streamed rows
+    unsigned words[2 * S::N];
+};
+
+// KV: stationary keys, streamed query rows (gk, gv); otherwise stationary query rows, streamed keys (gq)
 template <typename T, int DP, bool KV, bool SHARE>
-__global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, KV ? GRAD_KV : GRAD_Q>())) void backward_kernel(const Args a) {
+__device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, SHARE>& lds, int bh, int blk) {
     typedef Shape<T, DP, SHARE> S;
     typedef Mma<T, DP> M;
     constexpr int WAVES = S::WAVES, N = S::N, DB = M::DB, NRB = SHARE ? 1 : N / 32, W = N / 32;
-    __shared__ __attribute__((aligned(16))) T tile[S::NBUF][2][N * DP];
-    __shared__ __attribute__((aligned(16))) float rowstat[KV ? S::NBUF : 1][2][KV ? (N < 64 ? 64 : N) : 4];
-    __shared__ unsigned words[KV ? 1 : 2 * N];
+    auto& tile = lds.tile;
+    auto& rowstat = lds.rowstat;
 
     const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int R = a.Nq * a.G, C = KV ? a.Nk : R;
-    int bh, blk;
-    if (!place(a.BH, (C + S::COLS - 1) / S::COLS, bh, blk)) return;
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
     const int col_wave = blk * S::COLS + (SHARE ? 0 : 32 * wave), col = col_wave + l31;
     const unsigned char* mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
@@ -609,38 +644,26 @@ __global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, KV ? GRAD_KV : GRAD_Q
     const Rows qr = rows_of<T>(a.q, a.qs, b, hk * a.G, a.G), gr = rows_of<T>(a.go, a.gs, b, hk * a.G, a.G);
     const Rows kr = rows_of<T>(a.k, a.ks, b, hk, 1), vr = rows_of<T>(a.v, a.vs, b, hk, 1);
     const float* lse = a.lse + (long)bh * R;
-    float* delta = a.delta + (long)bh * R;
+    const float* delta = a.delta + (long)bh * R;
     const float c = a.scale * LOG2E;
 
-    f32x16 acc1[DB], acc2[KV ? DB : 1];
+    f32x16 acc1[1][DB], acc2[1][DB];
 #pragma unroll
-    for (int i = 0; i < DB; i++) acc1[i] = f32x16{};
-#pragma unroll
-    for (int i = 0; i < (KV ? DB : 1); i++) acc2[i] = f32x16{};
-    typename M::Frag f1, f2;
+    for (int i = 0; i < DB; i++) acc1[0][i] = acc2[0][i] = f32x16{};
+    typename M::Frag f1[1], f2[1];
     {
         const int at = valid ? col : 0;
-        M::load(f1, reinterpret_cast<const T*>((KV ? kr : qr).row(at)), valid, a.D, 1.f);
-        M::load(f2, reinterpret_cast<const T*>((KV ? vr : gr).row(at)), valid, a.D, 1.f);
+        M::load(f1[0], reinterpret_cast<const T*>((KV ? kr : qr).row(at)), valid, a.D, 1.f);
+        M::load(f2[0], reinterpret_cast<const T*>((KV ? vr : gr).row(at)), valid, a.D, 1.f);
     }
-    float col_lse = 0.f, col_delta = 0.f;
-    long out_at;                                             // of this column's row in gk / gv or gq
-    if constexpr (KV) {
-        out_at = (((long)b * a.Nk + col) * a.Hk + hk) * a.D;
-    } else {                                                 // delta = gO . o: the same channels of o as this lane holds of gO
-        const int n = col / a.G;
-        out_at = (((long)b * a.Nq + n) * (a.Hk * a.G) + hk * a.G + col - n * a.G) * a.D;
-        typename M::Frag fo;
-        M::load(fo, static_cast<const T*>(a.o_in) + (valid ? out_at : 0), valid, a.D, 1.f);
-        col_delta = M::dot_lane(f2, fo);
-        col_delta += other_half(col_delta);
-        col_lse = valid ? lse[col] : INFINITY;
-        if (a.write_delta && valid && half == 0 && (!SHARE || wave == 0)) delta[col] = col_delta;
-    }
+    const float col_lse = !KV && valid ? lse[col] : INFINITY, col_delta = !KV && valid ? delta[col] : 0.f;
 
     // one 32-row block: p, gs and the products over its rows
     auto block = [&](int buf, int r0, auto masked, unsigned on) {
-        f32x16 p = M::dot(tile[buf][0], r0, f1), ds = M::dot(tile[buf][1], r0, f2);
+        f32x16 pp[1], dd[1];
+        M::template dots<1>(pp, tile[buf][0], r0, f1);
+        M::template dots<1>(dd, tile[buf][1], r0, f2);
+        f32x16 &p = pp[0], &ds = dd[0];
 #pragma unroll
         for (int g = 0; g < 4; g++) {
             f32x4 ls = {col_lse, col_lse, col_lse, col_lse}, dl = {col_delta, col_delta, col_delta, col_delta};
@@ -657,8 +680,8 @@ __global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, KV ? GRAD_KV : GRAD_Q
                 ds[i] = p[i] * (ds[i] - dl[j]);
             }
         }
-        if constexpr (KV) M::add(acc2, tile[buf][1], r0, p);
-        M::add(acc1, tile[buf][0], r0, ds);
+        if constexpr (KV) M::template adds<1>(acc2, tile[buf][1], r0, pp);
+        M::template adds<1>(acc1, tile[buf][0], r0, dd);
     };
 
     Loader<T, DP, N, WAVES> first(KV ? qr : kr, a.D), second(KV ? gr : vr, a.D);
@@ -681,12 +704,15 @@ __global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, KV ? GRAD_KV : GRAD_Q
                     to_lds4(off, buffer((which ? delta : lse) + r0), __builtin_amdgcn_readfirstlane(lds_address(&rowstat[buf][which][part])));
                 }
             };
-            auto products = [&](int buf) {
+            auto products = [&](int buf, int r0) {
                 if (idle) return;
-                if constexpr (SHARE) block(buf, 32 * wave, std::false_type{}, 0u);
-                else {
+                if constexpr (SHARE) {
+                    if (r0 + 32 * wave < R) block(buf, 32 * wave, std::false_type{}, 0u);
+                } else if (NRB == 1 || r0 + N - 32 < R) {
 #pragma unroll
                     for (int rb = 0; rb < NRB; rb++) block(buf, 32 * rb, std::false_type{}, 0u);
+                } else {                                     // the rows end in the tile's first half
+                    block(buf, 0, std::false_type{}, 0u);
                 }
             };
             if constexpr (S::NBUF == 2) {
@@ -695,19 +721,19 @@ __global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, KV ? GRAD_KV : GRAD_Q
                 for (int r0 = 0; r0 < R; r0 += N, buf ^= 1) {
                     wait_tiles();
                     if (r0 + N < R) issue(r0 + N, buf ^ 1);
-                    products(buf);
+                    products(buf, r0);
                 }
             } else {
                 for (int r0 = 0; r0 < R; r0 += N) {
                     issue(r0, 0);
                     wait_tiles();
-                    products(0);
+                    products(0, r0);
                     __syncthreads();
                 }
             }
         }
     } else {
-        walk_keys<S>(words, mask, 0, a.Nk,
+        walk_keys<S>(lds.words, mask, 0, a.Nk,
                      [&](int key, int buf, const unsigned (&on)[W]) {
                          first.issue(tile[buf][0], key, on);
                          second.issue(tile[buf][1], key, on);
@@ -738,7 +764,7 @@ __global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, KV ? GRAD_KV : GRAD_Q
     T* out2 = static_cast<T*>(a.gv);
     if constexpr (SHARE) {                                   // add up the wavefronts' rows, in order
         float* join = reinterpret_cast<float*>(&tile[0][0][0]);      // [WAVES][32 columns][DP]
-        static_assert(sizeof(tile) >= WAVES * 32 * DP * sizeof(float), "the joined partials fit the tiles");
+        static_assert(sizeof(lds.tile) >= WAVES * 32 * DP * sizeof(float), "the joined partials fit the tiles");
 #pragma unroll
         for (int which = 0; which < (KV ? 2 : 1); which++) {
             T* out = which ? out2 : out1;
@@ -748,7 +774,7 @@ __global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, KV ? GRAD_KV : GRAD_Q
             for (int i = 0; i < DB; i++)
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
-                    const f32x16& x = which ? acc2[KV ? i : 0] : acc1[i];
+                    const f32x16& x = which ? acc2[0][i] : acc1[0][i];
                     *reinterpret_cast<f32x4*>(join + (wave * 32 + l31) * DP + 32 * i + 8 * g + 4 * half) = f32x4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
                 }
             __syncthreads();
@@ -772,34 +798,56 @@ __global__ __launch_bounds__(256, (occupancy<T, DP, SHARE, KV ? GRAD_KV : GRAD_Q
         return;
     }
     if (col >= C) return;
-    const float f = a.scale;
+    long at;
+    if (KV) at = (((long)b * a.Nk + col) * a.Hk + hk) * a.D;
+    else {
+        const int n = col / a.G;
+        at = (((long)b * a.Nq + n) * (a.Hk * a.G) + hk * a.G + col - n * a.G) * a.D;
+    }
 #pragma unroll
-    for (int i = 0; i < DB; i++)
+    for (int which = 0; which < (KV ? 2 : 1); which++) {
+        T* out = which ? out2 : out1;
+        if (!out) continue;
+        const float f = which ? 1.f : a.scale;
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const int d = 32 * i + 8 * g + 4 * half;
-            if (d >= a.D) continue;
-            // a masked key's column is written as zeros whatever went through it
-            if (out1) M::store4(out1 + out_at + d, valid ? acc1[i][4 * g] * f : 0.f, valid ? acc1[i][4 * g + 1] * f : 0.f, valid ? acc1[i][4 * g + 2] * f : 0.f,
-                                valid ? acc1[i][4 * g + 3] * f : 0.f);
-            if constexpr (KV)
-                if (out2) M::store4(out2 + out_at + d, valid ? acc2[i][4 * g] : 0.f, valid ? acc2[i][4 * g + 1] : 0.f, valid ? acc2[i][4 * g + 2] : 0.f,
-                                    valid ? acc2[i][4 * g + 3] : 0.f);
-        }
+        for (int i = 0; i < DB; i++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int d = 32 * i + 8 * g + 4 * half;
+                const f32x16& x = which ? acc2[0][i] : acc1[0][i];
+                // a masked key's column is written as zeros whatever went through it
+                if (d < a.D) M::store4(out + at + d, valid ? x[4 * g] * f : 0.f, valid ? x[4 * g + 1] * f : 0.f, valid ? x[4 * g + 2] * f : 0.f, valid ? x[4 * g + 3] * f : 0.f);
+            }
+    }
+}
+
+// Both gradients in one launch: the two kinds of workgroups of a head run next to each other, and the last, partly filled round of
+// workgroups is paid once (32 x 6 heads of 642 x 1025, bf16: two launches 142 us).
+template <typename T, int DP, bool SHARE>
+__global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::GRAD_OCC)) void backward_kernel(const Args a) {
+    typedef Shape<T, DP, SHARE> S;
+    __shared__ __attribute__((aligned(16))) GradLds<T, DP, SHARE> lds;
+    const int nkv = a.gk || a.gv ? (a.Nk + S::COLS - 1) / S::COLS : 0, nq = a.gq ? (a.Nq * a.G + S::COLS - 1) / S::COLS : 0;
+    int bh, blk;
+    if (!place(a.BH, nkv + nq, bh, blk)) return;
+    if (blk < nkv) gradient_columns<T, DP, true, SHARE>(a, lds, bh, blk);
+    else gradient_columns<T, DP, false, SHARE>(a, lds, bh, blk - nkv);
 }
 
 // ---- launch plan --------------------------------------------------------------------------------------------------------------------
 struct Plan { bool share; int nsplit, keys_per_split, row_blocks; };
 constexpr long SHARE_BELOW = 1024;                           // wavefronts of 32 columns; fewer leave SIMDs empty (256 CUs x 4)
-inline bool share_columns(const Args& a, int columns) { return (long)a.BH * ((columns + 31) / 32) < SHARE_BELOW; }
+inline long wavefronts(const Args& a, int columns) { return (long)a.BH * ((columns + 31) / 32); }
+// two_blocks: a wavefront of the OWN kernel takes 64 columns (Shape::CB).
 // split: where even SHARE has too few workgroups, the keys are divided as long as each part keeps two tiles
-inline Plan forward_plan(const Args& a) {
+inline Plan forward_plan(const Args& a, bool two_blocks) {
     Plan p;
     const int R = a.Nq * a.G;
-    p.share = share_columns(a, R);
+    p.share = wavefronts(a, R) < SHARE_BELOW;
     p.nsplit = 1;
     p.keys_per_split = a.Nk;
-    p.row_blocks = (R + (p.share ? 32 : 128) - 1) / (p.share ? 32 : 128);
+    const int cols = p.share ? 32 : two_blocks ? 256 : 128;
+    p.row_blocks = (R + cols - 1) / cols;
     if (p.share) {
         const int tiles = (a.Nk + 127) / 128;
         const long blocks = (long)a.BH * p.row_blocks;
@@ -822,19 +870,15 @@ template <typename T, int DP> void launch_forward(const Args& a, const Plan& p, 
         hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
     }
 }
-template <typename T, int DP, bool KV> void launch_gradient(const Args& a, int columns, hipStream_t st) {
-    if (share_columns(a, columns))
-        hipLaunchKernelGGL((backward_kernel<T, DP, KV, true>), dim3(placed_blocks(a.BH, (columns + 31) / 32)), dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL((backward_kernel<T, DP, KV, false>), dim3(placed_blocks(a.BH, (columns + 127) / 128)), dim3(256), 0, st, a);
-}
-template <typename T, int DP> void launch_backward(Args a, hipStream_t st) {
+template <typename T, int DP> void launch_backward(const Args& a, hipStream_t st) {
     const int R = a.Nq * a.G;
-    const bool kv = a.gk || a.gv;
-    a.write_delta = kv;
-    if (a.gq) launch_gradient<T, DP, false>(a, R, st);
-    else if (kv) hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)(((long)a.BH * R + 15) / 16)), dim3(256), 0, st, a);
-    if (kv) launch_gradient<T, DP, true>(a, a.Nk, st);
+    hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)(((long)a.BH * R + 15) / 16)), dim3(256), 0, st, a);
+    const int rows = a.gq ? R : 0, keys = a.gk || a.gv ? a.Nk : 0;
+    const bool share = wavefronts(a, rows) + wavefronts(a, keys) < 2 * SHARE_BELOW;
+    const int cols = share ? 32 : 128;
+    const dim3 grid(placed_blocks(a.BH, (rows + cols - 1) / cols + (keys + cols - 1) / cols));
+    if (share) hipLaunchKernelGGL((backward_kernel<T, DP, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((backward_kernel<T, DP, false>), grid, dim3(256), 0, st, a);
 }
 
 // instantiated in csrc/cross_attn_f32.hip and csrc/cross_attn_bf16.hip

@@ -64,6 +64,7 @@ Args make_args(const scp_cross_attn_params* p) {
     a.nsplit = 1;
     return a;
 }
+Plan plan_of(const Args& a, int dtype) { return scp_attn::forward_plan(a, dtype == SCP_DTYPE_BF16 && a.D <= 64); }
 size_t split_floats(const Args& a, const Plan& p) { return p.nsplit > 1 ? (size_t)p.nsplit * a.BH * a.Nq * a.G * (a.D + 2) : 0; }
 
 }  // namespace
@@ -71,7 +72,7 @@ size_t split_floats(const Args& a, const Plan& p) { return p.nsplit > 1 ? (size_
 extern "C" size_t scp_cross_attention_forward_workspace(const scp_cross_attn_params* p) {
     if (bad_problem(p)) return 0;
     const Args a = make_args(p);
-    return split_floats(a, scp_attn::forward_plan(a)) * sizeof(float);
+    return split_floats(a, plan_of(a, p->dtype)) * sizeof(float);
 }
 
 extern "C" int scp_cross_attention_forward(const void* q, const void* k, const void* v, const unsigned char* key_mask,
@@ -83,7 +84,7 @@ extern "C" int scp_cross_attention_forward(const void* q, const void* k, const v
         return scp::fail(hipErrorInvalidValue, "cross_attention_forward: tensors must be 16-byte aligned");
     if (tile_too_wide(p, false)) return scp::fail(hipErrorInvalidValue, "cross_attention_forward: token stride of k or v too large");
     Args a = make_args(p);
-    const Plan plan = scp_attn::forward_plan(a);
+    const Plan plan = plan_of(a, p->dtype);
     const size_t need = split_floats(a, plan);
     if (need && (!workspace || workspace_bytes < need * sizeof(float)))
         return scp::fail(hipErrorInvalidValue, "cross_attention_forward: workspace too small");
@@ -116,6 +117,7 @@ extern "C" int scp_cross_attention_backward(const void* q, const void* k, const 
     if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(g_out) || misaligned(g_q) || misaligned(g_k) || misaligned(g_v))
         return scp::fail(hipErrorInvalidValue, "cross_attention_backward: tensors must be 16-byte aligned");
     if (tile_too_wide(p, true)) return scp::fail(hipErrorInvalidValue, "cross_attention_backward: token or head stride too large");
+    if (!g_q && !g_k && !g_v) return 0;
     if (!workspace || workspace_bytes < scp_cross_attention_backward_workspace(p))
         return scp::fail(hipErrorInvalidValue, "cross_attention_backward: workspace too small");
     Args a = make_args(p);
