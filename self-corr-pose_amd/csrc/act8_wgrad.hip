@@ -59,19 +59,15 @@ template <int COLS> __device__ __forceinline__ bf16x8 operand(const __bf16* t, i
 }
 __device__ __forceinline__ unsigned upper_halves(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
 
-// 16 bytes of a row of `len` elements from element c: whole, in part (the rest 0), or nothing
-template <typename T> __device__ __forceinline__ u32x4 load16(const T* row, int c, int len) {
-    constexpr int E = 16 / sizeof(T);
-    u32x4 v = {};
-    if (c + E <= len) {
-        v = *reinterpret_cast<const u32x4_a1*>(row + c);
-    } else if (c < len) {
-        T* e = reinterpret_cast<T*>(&v);
+// the 16 bytes of x from byte `shift` on (what follows them is of no account)
+__device__ __forceinline__ u32x4 from_byte(u32x4 x, int shift) {
+    const bool two = shift & 8, one = shift & 4;
+    u32x4 y = {two ? x[2] : x[0], two ? x[3] : x[1], x[2], x[3]};
+    u32x4 z = {one ? y[1] : y[0], one ? y[2] : y[1], one ? y[3] : y[2], y[3]};
 #pragma unroll
-        for (int i = 0; i < E; i++)
-            if (c + i < len) e[i] = row[c + i];
-    }
-    return v;
+    for (int i = 0; i < 3; i++) z[i] = __builtin_amdgcn_alignbyte(z[i + 1], z[i], shift & 3);
+    z[3] >>= 8 * (shift & 3);
+    return z;
 }
 
 template <typename T> struct Wgrad8Shape {
@@ -83,7 +79,8 @@ template <typename T> struct Wgrad8Shape {
     static constexpr int NB = BN / 64;                                    // 32-column blocks of n per wavefront
 };
 
-template <typename T> __global__ __launch_bounds__(THREADS, 2) void wgrad8_kernel(const Wgrad8Args a) {
+// RAGGED: rows of gy or of the codes are no whole number of 16-byte pieces, or not aligned to them
+template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 2) void wgrad8_kernel(const Wgrad8Args a) {
     typedef Wgrad8Shape<T> S;
     constexpr int BN = S::BN, PARTS = S::PARTS, NB = S::NB;
     __shared__ __attribute__((aligned(16))) __bf16 gbuf[2][PARTS][STEP * BN];
@@ -101,32 +98,53 @@ template <typename T> __global__ __launch_bounds__(THREADS, 2) void wgrad8_kerne
     const int wn = (wave >> 1) * (BN / 2), wk = (wave & 1) * 64;
     const int groups = (a.K + 31) / 32;
 
-    // loads: gy piece i of this thread = row tid / 32 + 8 i, elements E (tid % 32); codes = row tid / 8, 16 of them
-    const T* gy = static_cast<const T*>(a.gy);
+    // loads: gy piece i of this thread = row tid / 32 + 8 i, elements E (tid % 32); codes = row tid / 8, 16 of them.  Pieces past a row's end
+    // are read from its end instead and moved into place (RAGGED); what stands behind them, and in pieces past the matrix, goes into
+    // products that nobody stores.  Rows past the range are read from its last row and stored as zeros.
+    const char* gy = static_cast<const char*>(a.gy);
     const int g_row = threadIdx.x / S::CPR, g_col = n0 + S::E * (threadIdx.x % S::CPR);
     const int x_row = threadIdx.x >> 3, x_col = k0 + 16 * (threadIdx.x & 7);
+    const int g_at = min(g_col, a.N - S::E), x_at = min(x_col, a.K - 16);
+    const int g_shift = min(g_col - g_at, S::E - 1) * (int)sizeof(T), x_shift = min(x_col - x_at, 15);
+    const int e_at = min(x_col >> 5, groups - 1);
     u32x4 graw[S::PIECES], xraw;
     unsigned xexp;
     auto load = [&](long m) {
+        const int last = m_end - m < STEP ? (int)(m_end - m) - 1 : STEP - 1;
+        const char* gbase = gy + m * a.N * (long)sizeof(T);
+        const char* xbase = reinterpret_cast<const char*>(a.codes) + m * a.K;
+        const char* ebase = reinterpret_cast<const char*>(a.exps) + m * groups;
 #pragma unroll
         for (int i = 0; i < S::PIECES; i++) {
-            const long r = m + g_row + (THREADS / S::CPR) * i;
-            graw[i] = u32x4{};
-            if (r < m_end) graw[i] = load16<T>(gy + r * a.N, g_col, a.N);
+            const unsigned off = (unsigned)(min(g_row + (THREADS / S::CPR) * i, last) * a.N + g_at) * (unsigned)sizeof(T);
+            if constexpr (RAGGED) graw[i] = *reinterpret_cast<const u32x4_a1*>(gbase + off);
+            else graw[i] = *reinterpret_cast<const u32x4*>(gbase + off);
         }
-        const long r = m + x_row;
-        xraw = u32x4{};
-        xexp = 1;
-        if (r < m_end && x_col < a.K) {
-            xraw = load16<signed char>(a.codes + r * a.K, x_col, a.K);
-            xexp = a.exps[r * groups + (x_col >> 5)];
-        }
+        const int r = min(x_row, last);
+        if constexpr (RAGGED) xraw = *reinterpret_cast<const u32x4_a1*>(xbase + (unsigned)(r * a.K + x_at));
+        else xraw = *reinterpret_cast<const u32x4*>(xbase + (unsigned)(r * a.K + x_at));
+        xexp = *reinterpret_cast<const unsigned char*>(ebase + (unsigned)(r * groups + e_at));
     };
     const bool bias = a.gb && tk == 0;
     float bsum[S::E];
 #pragma unroll
     for (int i = 0; i < S::E; i++) bsum[i] = 0.f;
-    auto store = [&](int buf) {
+    auto store = [&](int buf, long m) {
+        if constexpr (RAGGED) {
+#pragma unroll
+            for (int i = 0; i < S::PIECES; i++) graw[i] = from_byte(graw[i], g_shift);
+            xraw = from_byte(xraw, x_shift);
+        }
+        if (m + STEP > m_end) {
+            const int rows = (int)(m_end - m);
+#pragma unroll
+            for (int i = 0; i < S::PIECES; i++)
+                if (g_row + (THREADS / S::CPR) * i >= rows) graw[i] = u32x4{};
+            if (x_row >= rows) {
+                xraw = u32x4{};
+                xexp = 1;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < S::PIECES; i++) {
             const int row = g_row + (THREADS / S::CPR) * i, col = S::E * (threadIdx.x % S::CPR);
@@ -174,7 +192,7 @@ template <typename T> __global__ __launch_bounds__(THREADS, 2) void wgrad8_kerne
         for (int j = 0; j < 2; j++) acc[i][j] = f32x16{};
 
     load(m_beg);
-    store(0);
+    store(0, m_beg);
     int buf = 0;
     for (long m = m_beg; m < m_end; m += STEP, buf ^= 1) {
         __syncthreads();
@@ -194,7 +212,7 @@ template <typename T> __global__ __launch_bounds__(THREADS, 2) void wgrad8_kerne
                     for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(g, x[j], acc[i][j], 0, 0, 0);
                 }
         }
-        if (more) store(buf ^ 1);
+        if (more) store(buf ^ 1, m + STEP);
     }
 
     // accumulator: column k = lane & 31, row n = (reg & 3) + 8 (reg >> 2) + 4 half
@@ -225,20 +243,28 @@ template <typename T> __global__ __launch_bounds__(THREADS, 2) void wgrad8_kerne
     }
 }
 
-// out[i] = sum over the splits of part[split][i], in order
-__global__ __launch_bounds__(256) void wgrad8_fold_kernel(const float* __restrict__ part, float* __restrict__ out, long n, int splits) {
-    const long i = 4 * ((long)blockIdx.x * 256 + threadIdx.x);
-    if (i + 4 <= n && (n & 3) == 0) {
+// gw[i] = sum over the splits of part[split][i], in order; gb the same from part_b: a thread per 4 values
+__global__ __launch_bounds__(256) void wgrad8_fold_kernel(const float* __restrict__ part_w, const float* __restrict__ part_b, float* gw, float* gb, long n, int nb,
+                                                         int splits, int blocks_w) {
+    const bool second = blockIdx.x >= (unsigned)blocks_w;
+    const long len = second ? nb : n, i = 4 * ((long)(blockIdx.x - (second ? blocks_w : 0)) * 256 + threadIdx.x);
+    const float* part = second ? part_b : part_w;
+    float* out = second ? gb : gw;
+    if (i + 4 <= len && (len & 3) == 0) {
         f32x4 s = {};
 #pragma unroll 8
-        for (int p = 0; p < splits; p++) s += *reinterpret_cast<const f32x4*>(part + p * n + i);
+        for (int p = 0; p < splits; p++) s += *reinterpret_cast<const f32x4*>(part + p * len + i);
         *reinterpret_cast<f32x4*>(out + i) = s;
     } else {
-        for (long j = i; j < n && j < i + 4; j++) {
-            float s = 0.f;
-            for (int p = 0; p < splits; p++) s += part[p * n + j];
-            out[j] = s;
-        }
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int p = 0; p < splits; p++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (i + j < len) s[j] += part[p * len + i + j];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (i + j < len) out[i + j] = s[j];
     }
 }
 
@@ -260,6 +286,7 @@ Wgrad8Plan plan_of(long M, int N, int K, int dtype) {
 const char* bad_problem(long M, int N, int K, int dtype) {
     if (M <= 0 || N <= 0 || K <= 0) return "weight_grad8: empty problem";
     if (dtype != SCP_DTYPE_F32 && dtype != SCP_DTYPE_BF16) return "weight_grad8: unknown type";
+    if (N < (dtype == SCP_DTYPE_F32 ? 4 : 8) || K < 16) return "weight_grad8: fewer than 16 bytes in a row of gy or of the codes";
     if (N > (1 << 20) || K > (1 << 20) || (long)N * K > (1l << 34)) return "weight_grad8: more than 2^20 columns or 2^34 weights";
     return nullptr;
 }
@@ -288,12 +315,19 @@ extern "C" int scp_weight_grad8(const void* gy, const signed char* codes, const 
     hipStream_t st = static_cast<hipStream_t>(stream);
     const long total = (long)p.tiles_n * p.tiles_k * p.splits;
     const dim3 grid((unsigned)((total + 7) / 8 * 8));
-    if (dtype == SCP_DTYPE_F32) hipLaunchKernelGGL(wgrad8_kernel<float>, grid, dim3(THREADS), 0, st, a);
-    else hipLaunchKernelGGL(wgrad8_kernel<__bf16>, grid, dim3(THREADS), 0, st, a);
+    const size_t size = dtype == SCP_DTYPE_F32 ? 4 : 2;
+    const bool ragged = ((reinterpret_cast<size_t>(gy) | reinterpret_cast<size_t>(codes) | N * size | K) & 15) != 0;
+    if (dtype == SCP_DTYPE_F32) {
+        if (ragged) hipLaunchKernelGGL((wgrad8_kernel<float, true>), grid, dim3(THREADS), 0, st, a);
+        else hipLaunchKernelGGL((wgrad8_kernel<float, false>), grid, dim3(THREADS), 0, st, a);
+    } else {
+        if (ragged) hipLaunchKernelGGL((wgrad8_kernel<__bf16, true>), grid, dim3(THREADS), 0, st, a);
+        else hipLaunchKernelGGL((wgrad8_kernel<__bf16, false>), grid, dim3(THREADS), 0, st, a);
+    }
     if (const int e = scp::check_launch("weight_grad8")) return e;
     if (p.splits > 1) {
-        hipLaunchKernelGGL(wgrad8_fold_kernel, dim3((unsigned)((n / 4 + 256) / 256)), dim3(256), 0, st, part, gw, (long)n, p.splits);
-        if (gb) hipLaunchKernelGGL(wgrad8_fold_kernel, dim3((unsigned)((N / 4 + 256) / 256)), dim3(256), 0, st, part + p.splits * n, gb, (long)N, p.splits);
+        const unsigned blocks_w = (unsigned)((n / 4 + 256) / 256), blocks_b = gb ? (unsigned)((N / 4 + 256) / 256) : 0;
+        hipLaunchKernelGGL(wgrad8_fold_kernel, dim3(blocks_w + blocks_b), dim3(256), 0, st, part, part + p.splits * n, gw, gb, (long)n, N, p.splits, (int)blocks_w);
         return scp::check_launch("weight_grad8 fold");
     }
     return 0;

@@ -35,6 +35,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 struct Args {
     const void *q, *k, *v, *go;
@@ -92,9 +93,9 @@ template <int DP> struct Mma<__bf16, DP> {
         const int half = (threadIdx.x >> 5) & 1;
 #pragma unroll
         for (int i = 0; i < DP / 16; i++) {
-            bf16x8 v = {};
-            if (valid && 16 * i + 8 * half < D) v = *reinterpret_cast<const bf16x8*>(row + 16 * i + 8 * half);
-            x.f[i] = sign < 0.f ? -v : v;
+            u32x4 v = {};
+            if (valid && 16 * i + 8 * half < D) v = *reinterpret_cast<const u32x4*>(row + 16 * i + 8 * half);
+            x.f[i] = __builtin_bit_cast(bf16x8, v ^ (sign < 0.f ? 0x80008000u : 0u));
         }
     }
     // acc[c] = rows r0 .. r0+31 of `t` times the stationary columns of block c
@@ -149,9 +150,9 @@ template <int DP> struct Mma<float, DP> {
         const int half = (threadIdx.x >> 5) & 1;
 #pragma unroll
         for (int i = 0; i < DP / 8; i++) {
-            f32x4 v = {};
-            if (valid && 8 * i + 4 * half < D) v = *reinterpret_cast<const f32x4*>(row + 8 * i + 4 * half);
-            x.f[i] = sign < 0.f ? -v : v;
+            u32x4 v = {};
+            if (valid && 8 * i + 4 * half < D) v = *reinterpret_cast<const u32x4*>(row + 8 * i + 4 * half);
+            x.f[i] = __builtin_bit_cast(f32x4, v ^ (sign < 0.f ? 0x80000000u : 0u));
         }
     }
     template <int CB> static __device__ __forceinline__ void dots(f32x16 (&acc)[CB], const T* t, int r0, const Frag (&x)[CB]) {
@@ -303,25 +304,33 @@ template <int KT, int WAVES> __device__ __forceinline__ unsigned long long key_w
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     __syncthreads();
     static_assert(KT % WAVES == 0, "64 tiles of KT keys are KT groups of 64, dealt to the wavefronts");
-    unsigned char byte[KT / WAVES];
+    const int groups = min(KT, (key_end - key0 + 63) >> 6);  // groups that hold a key; the words of the others are not read
+    if (mask) {
+        constexpr int BATCH = 4;                             // loads in flight per lane
+        for (int g0 = wave; g0 < groups; g0 += BATCH * WAVES) {
+            unsigned char byte[BATCH];
 #pragma unroll
-    for (int i = 0; i < KT / WAVES; i++) {                   // all loads first: one wait for the window
-        byte[i] = 1;
-        if (mask) byte[i] = mask[min(key0 + 64 * (wave + WAVES * i) + lane, key_end - 1)];
-    }
+            for (int i = 0; i < BATCH; i++) byte[i] = mask[min(key0 + 64 * (g0 + WAVES * i) + lane, key_end - 1)];
 #pragma unroll
-    for (int i = 0; i < KT / WAVES; i++) {
-        const int group = wave + WAVES * i;
-        const unsigned long long bits = __ballot(key0 + 64 * group + lane < key_end && byte[i]);
-        if (lane == 0) {
-            words[2 * group] = (unsigned)bits;
-            words[2 * group + 1] = (unsigned)(bits >> 32);
+            for (int i = 0; i < BATCH; i++) {
+                const int g = g0 + WAVES * i;
+                const unsigned long long bits = __ballot(key0 + 64 * g + lane < key_end && byte[i]);
+                if (g < groups && lane < 2) words[2 * g + lane] = (unsigned)(bits >> (32 * lane));
+            }
+        }
+    } else {
+        for (int w = threadIdx.x; w < 2 * groups; w += 64 * WAVES) {
+            const int left = key_end - key0 - 32 * w;
+            words[w] = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
         }
     }
     __syncthreads();
     unsigned any = 0;
+    if (lane * KT < 64 * groups) {
 #pragma unroll
-    for (int i = 0; i < KT / 32; i++) any |= words[lane * (KT / 32) + i];
+        for (int i = 0; i < KT / 32; i++)
+            if (lane * (KT / 32) + i < 2 * groups) any |= words[lane * (KT / 32) + i];
+    }
     return __ballot(any != 0);
 }
 
@@ -366,7 +375,7 @@ __device__ __forceinline__ void walk_keys(unsigned* words, const unsigned char* 
             const int t = __builtin_ctzll(active);
             active &= active - 1;
 #pragma unroll
-            for (int j = 0; j < W; j++) w[j] = __builtin_amdgcn_readfirstlane(words[t * W + j]);
+            for (int j = 0; j < W; j++) w[j] = win + t * S::N + 32 * j < key_end ? __builtin_amdgcn_readfirstlane(words[t * W + j]) : 0u;
             move(win + t * S::N, buf, w);
         };
         if (!active) continue;
@@ -596,17 +605,17 @@ template <typename T> __global__ __launch_bounds__(256) void join_kernel(const A
     if (a.lse && d == 0) a.lse[row] = lt == 0.f ? INFINITY : mt + __builtin_amdgcn_logf(lt);
 }
 
-// delta[row] = gO . o : 16 lanes per row, up to 8 channels each
-template <typename T> __global__ __launch_bounds__(256) void delta_kernel(const Args a) {
-    const int R = a.Nq * a.G, H = a.Hk * a.G, l = threadIdx.x & 15;
-    const long row = (long)blockIdx.x * 16 + (threadIdx.x >> 4), rows = (long)a.BH * R;
-    if (row >= rows) return;
-    const int bh = (int)(row / R), r = (int)(row - (long)bh * R), b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int n = r / a.G, h = hk * a.G + r - n * a.G;
+// delta[row] = gO . o : 16 lanes per row, up to 8 channels each; rows in the order of o (a batch entry's tokens, then heads)
+template <typename T> __global__ __launch_bounds__(256) void delta_kernel(const Args a, int blocks_per_batch) {
+    const int H = a.Hk * a.G, R = a.Nq * a.G, l = threadIdx.x & 15;
+    const int b = blockIdx.x / blocks_per_batch;
+    const unsigned row = (blockIdx.x - b * blocks_per_batch) * 16 + (threadIdx.x >> 4);
+    if (row >= (unsigned)(a.Nq * H)) return;
+    const unsigned n = row / (unsigned)H, h = row - n * H;
     float s = 0.f;
     if (8 * l < a.D) {
-        const T* g = reinterpret_cast<const T*>(rows_of<T>(a.go, a.gs, b, h, 1).row(n)) + 8 * l;
-        const T* o = static_cast<const T*>(a.o_in) + (((long)b * a.Nq + n) * H + h) * a.D + 8 * l;
+        const T* g = static_cast<const T*>(a.go) + b * a.gs[0] + n * a.gs[1] + h * a.gs[2] + 8 * l;
+        const T* o = static_cast<const T*>(a.o_in) + ((long)b * a.Nq * H + row) * a.D + 8 * l;
         typedef T tx8 __attribute__((ext_vector_type(8)));
         const tx8 x = *reinterpret_cast<const tx8*>(g), y = *reinterpret_cast<const tx8*>(o);
 #pragma unroll
@@ -614,7 +623,10 @@ template <typename T> __global__ __launch_bounds__(256) void delta_kernel(const 
     }
 #pragma unroll
     for (int k = 1; k < 16; k <<= 1) s += __shfl_xor(s, k);
-    if (l == 0) a.delta[row] = s;
+    if (l == 0) {
+        const unsigned hk = h / (unsigned)a.G;
+        a.delta[((long)b * a.Hk + hk) * R + n * a.G + (h - hk * a.G)] = s;
+    }
 }
 
 template <typename T, int DP, bool SHARE> struct GradLds {
@@ -815,8 +827,9 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
             for (int g = 0; g < 4; g++) {
                 const int d = 32 * i + 8 * g + 4 * half;
                 const f32x16& x = which ? acc2[0][i] : acc1[0][i];
-                // a masked key's column is written as zeros whatever went through it
-                if (d < a.D) M::store4(out + at + d, valid ? x[4 * g] * f : 0.f, valid ? x[4 * g + 1] * f : 0.f, valid ? x[4 * g + 2] * f : 0.f, valid ? x[4 * g + 3] * f : 0.f);
+                if (d >= a.D) continue;
+                if (valid) M::store4(out + at + d, x[4 * g] * f, x[4 * g + 1] * f, x[4 * g + 2] * f, x[4 * g + 3] * f);
+                else M::store4(out + at + d, 0.f, 0.f, 0.f, 0.f);           // a masked key, whatever went through its column
             }
     }
 }
@@ -872,7 +885,8 @@ template <typename T, int DP> void launch_forward(const Args& a, const Plan& p, 
 }
 template <typename T, int DP> void launch_backward(const Args& a, hipStream_t st) {
     const int R = a.Nq * a.G;
-    hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)(((long)a.BH * R + 15) / 16)), dim3(256), 0, st, a);
+    const int per_batch = (a.Nq * a.Hk * a.G + 15) / 16;
+    hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)(per_batch * (a.BH / a.Hk))), dim3(256), 0, st, a, per_batch);
     const int rows = a.gq ? R : 0, keys = a.gk || a.gv ? a.Nk : 0;
     const bool share = wavefronts(a, rows) + wavefronts(a, keys) < 2 * SHARE_BELOW;
     const int cols = share ? 32 : 128;

@@ -363,17 +363,27 @@ def weight_grad8(grad, packed, bias=True):
         raise RuntimeError("weight_grad8: grad %s does not go with a packed input %s" % (tuple(grad.shape), tuple(packed.shape)))
     n, k = grad.shape[-1], packed.shape[-1]
     rows = grad.numel() // n
-    gw = torch.empty(n, k, dtype=torch.float32, device=grad.device)
-    gb = torch.empty(n, dtype=torch.float32, device=grad.device) if bias else None
     if rows == 0:
-        return gw.zero_(), None if gb is None else gb.zero_()
-    grad = grad.detach().contiguous()
+        return torch.zeros(n, k, dtype=torch.float32, device=grad.device), torch.zeros(n, dtype=torch.float32, device=grad.device) if bias else None
+    grad, codes, exps = grad.detach().contiguous(), packed.codes, packed.exps
+    # the kernel reads 16 bytes of a row at a time: narrower rows are widened with zeros
+    pad_n, pad_k = max(0, 16 // grad.element_size() - n), max(0, 16 - k)
+    if pad_n:
+        grad = torch.nn.functional.pad(grad, (0, pad_n))
+    if pad_k:
+        codes = torch.nn.functional.pad(codes, (0, pad_k))
+    gw = torch.empty(n + pad_n, k + pad_k, dtype=torch.float32, device=grad.device)
+    gb = torch.empty(n + pad_n, dtype=torch.float32, device=grad.device) if bias else None
     L = capi.lib()
     dt = capi.DTYPES[grad.dtype]
-    nbytes = L.scp_weight_grad8_workspace(rows, n, k, dt)
+    nbytes = L.scp_weight_grad8_workspace(rows, n + pad_n, k + pad_k, dt)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device) if nbytes else None
-    capi.check(L.scp_weight_grad8(_ptr(grad), _ptr(packed.codes), _ptr(packed.exps), rows, n, k, dt, _ptr(gw), _ptr(gb), _ptr(ws), nbytes,
-                                  _stream()), "scp_weight_grad8")
+    code = L.scp_weight_grad8(grad.data_ptr(), codes.data_ptr(), exps.data_ptr(), rows, n + pad_n, k + pad_k, dt, gw.data_ptr(), _ptr(gb), _ptr(ws),
+                              nbytes, _stream())
+    if code:
+        capi.check(code, "scp_weight_grad8")
+    if pad_n or pad_k:
+        gw, gb = gw[:n, :k].contiguous(), None if gb is None else gb[:n].contiguous()
     return gw, gb
 
 
