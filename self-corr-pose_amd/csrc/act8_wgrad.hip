@@ -8,7 +8,7 @@
 //   * a workgroup owns a BN x 128 tile of gw over a range of rows and walks it 32 rows at a time: gy and the codes go global -> registers one
 //     step ahead, are cut / dequantised there (once per tile, not per wavefront) and written to LDS row-major; ds_read_b64_tr_b16 turns
 //     4 rows x 16 columns into operand order, the same row order for both operands, so no transposition is ever stored;
-//   * LDS rows are swizzled in 16-byte chunks so that the 4 rows x 2 chunks of one transposed read touch each bank once;
+//   * LDS rows are swizzled in 16-byte chunks so that the 4 rows x 4 chunks of half a transposed read touch each bank once;
 //   * a wavefront owns (BN / 2) x 64 of the tile.  BN = 256 for bf16 (12 KiB of LDS reads per 16 matrix instructions), 128 for fp32, where
 //     the three parts share the x8 operand and 2 x 64 KiB of LDS keeps two workgroups on a CU;
 //   * the rows are split so that about two workgroups per CU run; each writes an fp32 partial tile and a second kernel adds the partials in
@@ -44,7 +44,7 @@ struct Wgrad8Args {
 
 // element offset of (row, 16-byte chunk) in a [32][COLS] bf16 tile
 template <int COLS> __device__ __forceinline__ int lds_at(int row, int chunk) {
-    return row * COLS + 8 * (chunk ^ (((row & 7) << 1) | ((row >> 3) & 1)));
+    return row * COLS + 8 * (chunk ^ (((row & 3) << 2) | ((row >> 2) & 3)));
 }
 // columns c0 .. c0+31 (one per lane & 31), rows 16 s + {4 half + 0..3, 8 + 4 half + 0..3}
 template <int COLS> __device__ __forceinline__ bf16x8 operand(const __bf16* t, int s, int c0) {

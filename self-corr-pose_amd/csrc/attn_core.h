@@ -21,7 +21,7 @@
 // LDS tiles are filled by buffer loads that write LDS directly, 16 bytes per lane.  A lane whose row is masked, past the end, or whose
 // channel is past head_dim gets an out-of-range offset: the hardware writes zeros, so nothing stored there can reach a product.  The
 // tile's image is swizzled through the SOURCE address (16-byte chunk `slot ^ f(row)`), such that both reads of it -- 16 consecutive rows at
-// one chunk, 4 consecutive rows at two -- touch each bank once.
+// one chunk, 4 consecutive rows at four -- touch each bank once.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -67,9 +67,9 @@ template <typename T, int DP> struct Tile {
     static __device__ __forceinline__ int swizzle(int chunk, int row) {
         if constexpr (sizeof(T) == 2) {
             if constexpr (CPR == 4) return chunk ^ ((row >> 2) & 3);
-            else if constexpr (CPR == 8) return chunk ^ ((row & 2) | (row & 4) | ((row >> 3) & 1));
+            else if constexpr (CPR == 8) return chunk ^ (((row & 2) << 1) | ((row & 4) >> 1) | ((row >> 3) & 1));
             else if constexpr (CPR == 12) { const int s = chunk + ((row >> 2) & 3); return s >= 12 ? s - 12 : s; }
-            else return chunk ^ (((row & 7) << 1) | ((row >> 3) & 1));
+            else return chunk ^ (((row & 3) << 2) | ((row >> 2) & 3));
         } else {
             if constexpr (CPR == 16 || CPR == 32) return chunk ^ (row & 15);
             else return chunk ^ ((row >> 1) & 7);
