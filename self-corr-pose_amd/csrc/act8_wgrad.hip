@@ -10,8 +10,10 @@
 //     4 rows x 16 columns into operand order, the same row order for both operands, so no transposition is ever stored;
 //   * LDS rows are swizzled in 16-byte chunks so that the 4 rows x 4 chunks of half a transposed read touch each bank once;
 //   * a wavefront owns (BN / 2) x 64 of the tile.  BN = 256 for bf16 (12 KiB of LDS reads per 16 matrix instructions), 128 for fp32, where
-//     the three parts share the x8 operand and 2 x 64 KiB of LDS keeps two workgroups on a CU;
-//   * the rows are split so that about two workgroups per CU run; each writes an fp32 partial tile and a second kernel adds the partials in
+//     the three parts share the x8 operand;
+//   * a workgroup has two teams of four wavefronts, which take alternate steps of its rows and join their tiles through LDS at the end: two
+//     wavefronts per SIMD at half the partial tiles that two workgroups per CU would write (33 MB for 1536 x 384, not 66);
+//   * the rows are split so that about one workgroup per CU runs; each writes an fp32 partial tile and a second kernel adds the partials in
 //     order (bit-reproducible).  gb falls out of the registers of the workgroups of the first column of tiles.
 #include <hip/hip_runtime.h>
 
@@ -30,7 +32,7 @@ typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4_a1 __attribute__((ext_vector_type(4), aligned(1)));
 
-constexpr int BK = 128, STEP = 32, THREADS = 256;
+constexpr int BK = 128, STEP = 32, TEAM = 256, TEAMS = 2, THREADS = TEAM * TEAMS;
 
 struct Wgrad8Args {
     const void* gy;
@@ -75,7 +77,7 @@ template <typename T> struct Wgrad8Shape {
     static constexpr int BN = F32 ? 128 : 256, PARTS = F32 ? 3 : 1;
     static constexpr int E = 16 / sizeof(T);                              // gy elements per 16 bytes
     static constexpr int CPR = BN / E;                                    // 16-byte pieces of gy per row of the tile: 32 either way
-    static constexpr int PIECES = STEP * CPR / THREADS;                   // 4 per thread
+    static constexpr int PIECES = STEP * CPR / TEAM;                   // 4 per thread
     static constexpr int NB = BN / 64;                                    // 32-column blocks of n per wavefront
 };
 
@@ -83,8 +85,8 @@ template <typename T> struct Wgrad8Shape {
 template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 2) void wgrad8_kernel(const Wgrad8Args a) {
     typedef Wgrad8Shape<T> S;
     constexpr int BN = S::BN, PARTS = S::PARTS, NB = S::NB;
-    __shared__ __attribute__((aligned(16))) __bf16 gbuf[2][PARTS][STEP * BN];
-    __shared__ __attribute__((aligned(16))) __bf16 xbuf[2][STEP * BK];
+    struct Stage { __bf16 g[2][PARTS][STEP * BN], x[2][STEP * BK]; };
+    __shared__ __attribute__((aligned(16))) Stage stage[TEAMS];
 
     // tiles of one range of rows next to each other on one XCD: they read the same rows of gy and of the codes
     const int tiles = a.tiles_n * a.tiles_k, total = tiles * a.splits, per = (total + 7) / 8;
@@ -94,16 +96,19 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 2) void
     const int n0 = tn * BN, k0 = tk * BK;
     const long m_beg = split * a.rows_per_split, m_end = m_beg + a.rows_per_split < a.M ? m_beg + a.rows_per_split : a.M;
 
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l31 = lane & 31;
+    const int tid = threadIdx.x & (TEAM - 1), team = __builtin_amdgcn_readfirstlane(threadIdx.x / TEAM);
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
     const int wn = (wave >> 1) * (BN / 2), wk = (wave & 1) * 64;
+    auto& gbuf = stage[team].g;
+    auto& xbuf = stage[team].x;
     const int groups = (a.K + 31) / 32;
 
     // loads: gy piece i of this thread = row tid / 32 + 8 i, elements E (tid % 32); codes = row tid / 8, 16 of them.  Pieces past a row's end
     // are read from its end instead and moved into place (RAGGED); what stands behind them, and in pieces past the matrix, goes into
     // products that nobody stores.  Rows past the range are read from its last row and stored as zeros.
     const char* gy = static_cast<const char*>(a.gy);
-    const int g_row = threadIdx.x / S::CPR, g_col = n0 + S::E * (threadIdx.x % S::CPR);
-    const int x_row = threadIdx.x >> 3, x_col = k0 + 16 * (threadIdx.x & 7);
+    const int g_row = tid / S::CPR, g_col = n0 + S::E * (tid % S::CPR);
+    const int x_row = tid >> 3, x_col = k0 + 16 * (tid & 7);
     const int g_at = min(g_col, a.N - S::E), x_at = min(x_col, a.K - 16);
     const int g_shift = min(g_col - g_at, S::E - 1) * (int)sizeof(T), x_shift = min(x_col - x_at, 15);
     const int e_at = min(x_col >> 5, groups - 1);
@@ -116,7 +121,7 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 2) void
         const char* ebase = reinterpret_cast<const char*>(a.exps) + m * groups;
 #pragma unroll
         for (int i = 0; i < S::PIECES; i++) {
-            const unsigned off = (unsigned)(min(g_row + (THREADS / S::CPR) * i, last) * a.N + g_at) * (unsigned)sizeof(T);
+            const unsigned off = (unsigned)(min(g_row + (TEAM / S::CPR) * i, last) * a.N + g_at) * (unsigned)sizeof(T);
             if constexpr (RAGGED) graw[i] = *reinterpret_cast<const u32x4_a1*>(gbase + off);
             else graw[i] = *reinterpret_cast<const u32x4*>(gbase + off);
         }
@@ -139,7 +144,7 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 2) void
             const int rows = (int)(m_end - m);
 #pragma unroll
             for (int i = 0; i < S::PIECES; i++)
-                if (g_row + (THREADS / S::CPR) * i >= rows) graw[i] = u32x4{};
+                if (g_row + (TEAM / S::CPR) * i >= rows) graw[i] = u32x4{};
             if (x_row >= rows) {
                 xraw = u32x4{};
                 xexp = 1;
@@ -147,7 +152,7 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 2) void
         }
 #pragma unroll
         for (int i = 0; i < S::PIECES; i++) {
-            const int row = g_row + (THREADS / S::CPR) * i, col = S::E * (threadIdx.x % S::CPR);
+            const int row = g_row + (TEAM / S::CPR) * i, col = S::E * (tid % S::CPR);
             if constexpr (S::F32) {
                 unsigned h[4], m[4], l[4];
 #pragma unroll
@@ -182,7 +187,7 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 2) void
             x[w >> 1][2 * (w & 1) + 1] = upper_halves(__float_as_uint(v[2]), __float_as_uint(v[3]));
         }
 #pragma unroll
-        for (int w = 0; w < 2; w++) *reinterpret_cast<u32x4*>(&xbuf[buf][lds_at<BK>(x_row, 2 * (threadIdx.x & 7) + w)]) = x[w];
+        for (int w = 0; w < 2; w++) *reinterpret_cast<u32x4*>(&xbuf[buf][lds_at<BK>(x_row, 2 * (tid & 7) + w)]) = x[w];
     };
 
     f32x16 acc[NB][2];
@@ -191,53 +196,87 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 2) void
 #pragma unroll
         for (int j = 0; j < 2; j++) acc[i][j] = f32x16{};
 
-    load(m_beg);
-    store(0, m_beg);
-    int buf = 0;
-    for (long m = m_beg; m < m_end; m += STEP, buf ^= 1) {
-        __syncthreads();
-        const bool more = m + STEP < m_end;
-        if (more) load(m + STEP);
-#pragma unroll
-        for (int s = 0; s < STEP / 16; s++) {
-            bf16x8 x[2];
-#pragma unroll
-            for (int j = 0; j < 2; j++) x[j] = operand<BK>(xbuf[buf], s, wk + 32 * j);
-#pragma unroll
-            for (int i = 0; i < NB; i++)
-#pragma unroll
-                for (int p = 0; p < PARTS; p++) {
-                    const bf16x8 g = operand<BN>(gbuf[buf][p], s, wn + 32 * i);
-#pragma unroll
-                    for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(g, x[j], acc[i][j], 0, 0, 0);
-                }
-        }
-        if (more) store(buf ^ 1, m + STEP);
+    // the teams' steps alternate; both pass every barrier, a team without a step left does nothing between them
+    const int steps = (int)((m_end - m_beg + STEP - 1) / STEP);
+    auto at = [&](int i) { return m_beg + (long)i * STEP; };
+    if (team < steps) {
+        load(at(team));
+        store(0, at(team));
     }
-
-    // accumulator: column k = lane & 31, row n = (reg & 3) + 8 (reg >> 2) + 4 half
-    float* out = a.gw + (size_t)split * a.N * a.K;
+    int buf = 0;
+    for (int i0 = 0; i0 < steps; i0 += TEAMS, buf ^= 1) {
+        const int i = i0 + team;
+        __syncthreads();
+        const bool more = i + TEAMS < steps;
+        if (more) load(at(i + TEAMS));
+        if (i < steps) {
 #pragma unroll
-    for (int i = 0; i < NB; i++)
+            for (int s = 0; s < STEP / 16; s++) {
+                bf16x8 x[2];
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int k = k0 + wk + 32 * j + l31;
+                for (int j = 0; j < 2; j++) x[j] = operand<BK>(xbuf[buf], s, wk + 32 * j);
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int n = n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
-                if (n < a.N && k < a.K) out[(size_t)n * a.K + k] = acc[i][j][r];
+                for (int n = 0; n < NB; n++)
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++) {
+                        const bf16x8 g = operand<BN>(gbuf[buf][p], s, wn + 32 * n);
+#pragma unroll
+                        for (int j = 0; j < 2; j++) acc[n][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(g, x[j], acc[n][j], 0, 0, 0);
+                    }
             }
         }
+        if (more) store(buf ^ 1, at(i + TEAMS));
+    }
+
+    // join: the second team's tile through LDS to the first, two 32-row blocks at a time; the bias sums of all rows with it
+    float* join = reinterpret_cast<float*>(&stage[0]);
+    static_assert(sizeof(stage) >= 2 * 2 * 16 * TEAM * sizeof(float), "two blocks of a team's tile fit the stages");
+#pragma unroll
+    for (int n0b = 0; n0b < NB; n0b += 2) {
+        __syncthreads();
+        if (team == 1) {
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) join[((n * 2 + j) * 16 + r) * TEAM + tid] = acc[n0b + n][j][r];
+        }
+        __syncthreads();
+        if (team == 0) {
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[n0b + n][j][r] += join[((n * 2 + j) * 16 + r) * TEAM + tid];
+        }
+    }
+    // accumulator: column k = lane & 31, row n = (reg & 3) + 8 (reg >> 2) + 4 half
+    if (team == 0) {
+        float* out = a.gw + (size_t)split * a.N * a.K;
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int k = k0 + wk + 32 * j + l31;
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int n = n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
+                    if (n < a.N && k < a.K) out[(size_t)n * a.K + k] = acc[i][j][r];
+                }
+            }
+    }
     if (bias) {
-        float* red = reinterpret_cast<float*>(&gbuf[0][0][0]);          // [8 row groups][BN]
+        constexpr int GROUPS = TEAM / S::CPR;                           // rows that a team loads side by side
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < S::E; e++) red[g_row * BN + S::E * (threadIdx.x % S::CPR) + e] = bsum[e];
+        for (int e = 0; e < S::E; e++) join[(team * GROUPS + g_row) * BN + S::E * (tid % S::CPR) + e] = bsum[e];
         __syncthreads();
         if (threadIdx.x < BN && n0 + threadIdx.x < a.N) {
             float s = 0.f;
 #pragma unroll
-            for (int g = 0; g < THREADS / S::CPR; g++) s += red[g * BN + threadIdx.x];
+            for (int g = 0; g < TEAMS * GROUPS; g++) s += join[g * BN + threadIdx.x];
             a.gb[(size_t)split * a.N + n0 + threadIdx.x] = s;
         }
     }
@@ -269,14 +308,14 @@ __global__ __launch_bounds__(256) void wgrad8_fold_kernel(const float* __restric
 }
 
 struct Wgrad8Plan { int tiles_n, tiles_k, splits; long rows_per_split; };
-// about two workgroups per CU, none with fewer than 4 steps of rows (a partial tile costs as much traffic as 2 to 4 steps)
+// about one workgroup per CU, none with fewer than 4 steps of rows (a partial tile costs as much traffic as 2 to 4 steps)
 Wgrad8Plan plan_of(long M, int N, int K, int dtype) {
     Wgrad8Plan p;
     const int BN = dtype == SCP_DTYPE_F32 ? 128 : 256;
     p.tiles_n = (N + BN - 1) / BN;
     p.tiles_k = (K + BK - 1) / BK;
     const long tiles = (long)p.tiles_n * p.tiles_k, steps = (M + STEP - 1) / STEP;
-    long want = tiles >= 512 ? 1 : 512 / tiles;
+    long want = tiles >= 256 ? 1 : 256 / tiles;
     if (want > (steps + 3) / 4) want = (steps + 3) / 4;
     const long per = (steps + want - 1) / want;
     p.splits = (int)((steps + per - 1) / per);
