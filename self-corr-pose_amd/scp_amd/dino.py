@@ -398,6 +398,26 @@ class _Block(nn.Module):
         x, y = add_layernorm(x, self.attn(y), self.norm2)
         return x, self.mlp(y)
 
+    def forward_grad(self, x, pending=None, act8=True):
+        """the same block with gradients for every parameter and for x: x [b, n, dim], pending as in forward() -> (x, pending').
+        LayerNorm, attention and GELU are the operators of scp_amd.vit_ops; act8: the inputs of the four linear layers and of the GELU
+        are kept for the backward pass in 8 bits (about 1 of the 4 bytes per value that would be kept otherwise; the weight gradients are
+        those of the rounded inputs), else as they are.  Under MIXED_BF16 the products and the residual stream are bf16."""
+        from . import vit_ops
+        a, m = self.attn, self.mlp
+        lin = (lambda layer, t: vit_ops.linear8(t, layer.weight.to(t.dtype), layer.bias.to(t.dtype))) if act8 else \
+              (lambda layer, t: F.linear(t, layer.weight.to(t.dtype), layer.bias.to(t.dtype)))
+        if pending is None:
+            y = vit_ops.layer_norm(x, self.norm1.weight, self.norm1.bias, self.norm1.eps)
+        else:
+            x, y = vit_ops.layer_norm(x, self.norm1.weight, self.norm1.bias, self.norm1.eps, residual=pending)
+        b, n, c = y.shape
+        q, k, v = lin(a.qkv, y).view(b, n, 3, a.num_heads, c // a.num_heads).unbind(2)
+        y = lin(a.proj, vit_ops.cross_attention(q, k, v, scale=a.scale).view(b, n, c))
+        x, y = vit_ops.layer_norm(x, self.norm2.weight, self.norm2.bias, self.norm2.eps, residual=y)
+        y = lin(m.fc1, y)
+        return x, lin(m.fc2, vit_ops.gelu8(y) if act8 else F.gelu(y))
+
     # ---- fused path (fp32, GPU): four GEMM launches + two row-statistics launches + attention per block -------------
     def _folded(self):
         """(gamma1 o Wqkv, s, t), (gamma2 o W1, s, t), rebuilt when any of the frozen tensors changes (load_state_dict);
@@ -647,6 +667,22 @@ class VisionTransformer(nn.Module):
         tok, y = add_layernorm(tok, pending, blk.norm1)
         k = blk.attn.keys(y)                                   # b,h,n,d
         return k.permute(0, 2, 1, 3).reshape(k.shape[0], k.shape[2], -1)
+
+    def key_tokens_grad(self, x, layer=9, act8=True):
+        """key_tokens() for fine-tuning: the keys of block `layer`, [b, tokens, heads * d], with gradients for the parameters of every
+        block up to it, the patch embedding and the class token (the positional embedding is interpolated once per size and stays
+        as it is).  GPU only; `act8` as in _Block.forward_grad."""
+        from . import vit_ops
+        tok, pending = self.prepare_tokens(x).contiguous(), None
+        if MIXED_BF16:
+            tok = tok.to(torch.bfloat16)
+        for blk in self.blocks[:layer]:
+            tok, pending = blk.forward_grad(tok, pending, act8)
+        blk, c = self.blocks[layer], tok.shape[-1]
+        y = vit_ops.layer_norm(tok, blk.norm1.weight, blk.norm1.bias, blk.norm1.eps, residual=pending)
+        y = y if pending is None else y[1]
+        w, bias = blk.attn.qkv.weight[c:2 * c].to(y.dtype), blk.attn.qkv.bias[c:2 * c].to(y.dtype)
+        return vit_ops.linear8(y, w, bias) if act8 else F.linear(y, w, bias)
 
     @torch.no_grad()
     def forward(self, x):

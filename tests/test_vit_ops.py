@@ -593,29 +593,30 @@ def _decoder_step(q_tok, enc, mask, P, dtype):
     return s + vit_ops.linear8(vit_ops.gelu8(vit_ops.linear8(y, P["w1"], P["b1"])), P["w2"], P["b2"])
 
 
+class Keep8(torch.autograd.Function):                                                        # gelu whose slope is taken at the 8-bit value
+    @staticmethod
+    def forward(ctx, x):
+        ctx.save_for_backward(round8_reference(x.reshape(-1, x.shape[-1]).float())[0].to(x.device).view_as(x))
+        return gelu64(x)
+
+    @staticmethod
+    def backward(ctx, g):
+        return g * gelu_slope64(ctx.saved_tensors[0])
+
+class Lin8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w):
+        ctx.save_for_backward(round8_reference(x.reshape(-1, x.shape[-1]).float())[0].to(x.device).view_as(x), w)
+        return x @ w.t()
+
+    @staticmethod
+    def backward(ctx, g):
+        x8, w = ctx.saved_tensors
+        return g @ w, g.reshape(-1, g.shape[-1]).t() @ x8.reshape(-1, x8.shape[-1])
+
+
 def _decoder_reference(q_tok, enc, mask, P):
     """the same in float64 with straight-through 8-bit checkpoints"""
-    class Keep8(torch.autograd.Function):                                                        # gelu whose slope is taken at the 8-bit value
-        @staticmethod
-        def forward(ctx, x):
-            ctx.save_for_backward(round8_reference(x.reshape(-1, x.shape[-1]).float())[0].to(x.device).view_as(x))
-            return gelu64(x)
-
-        @staticmethod
-        def backward(ctx, g):
-            return g * gelu_slope64(ctx.saved_tensors[0])
-
-    class Lin8(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, x, w):
-            ctx.save_for_backward(round8_reference(x.reshape(-1, x.shape[-1]).float())[0].to(x.device).view_as(x), w)
-            return x @ w.t()
-
-        @staticmethod
-        def backward(ctx, g):
-            x8, w = ctx.saved_tensors
-            return g @ w, g.reshape(-1, g.shape[-1]).t() @ x8.reshape(-1, x8.shape[-1])
-
     ln = lambda t, w, b: torch.nn.functional.layer_norm(t, t.shape[-1:], w, b, 1e-6)
     s = q_tok + P["pos"]
     y = ln(s, P["n1w"], P["n1b"])
@@ -657,6 +658,85 @@ def test_a_decoder_block_of_them_together():
     assert (out.detach().double() - ref.detach()).norm() <= 1e-5 * ref.detach().norm()
     for n, a, b in zip(names, grads, refs):
         assert (a.double() - b).norm() <= 1e-3 * b.norm(), n
+
+
+def _small_vit():
+    from scp_amd import dino
+    torch.manual_seed(3)
+    vit = dino.VisionTransformer(patch_size=8, embed_dim=128, depth=3, num_heads=2)
+    for p in vit.parameters():                                                                    # trunc_normal(0.02) weights would make every block a near-identity
+        if p.dim() == 2:
+            torch.nn.init.normal_(p, std=0.08)
+    return vit
+
+
+def _vit_reference(vit, img, layer, act8):
+    """key_tokens_grad in float64"""
+    lin = (lambda m, t: Lin8.apply(t, m.weight) + m.bias) if act8 else (lambda m, t: torch.nn.functional.linear(t, m.weight, m.bias))
+    act = Keep8.apply if act8 else gelu64
+    x = vit.prepare_tokens(img)
+    ln = lambda m, t: torch.nn.functional.layer_norm(t, t.shape[-1:], m.weight, m.bias, m.eps)
+    for blk in vit.blocks[:layer]:
+        b, n, c = x.shape
+        q, k, v = (t.transpose(1, 2) for t in lin(blk.attn.qkv, ln(blk.norm1, x)).view(b, n, 3, blk.attn.num_heads, -1).unbind(2))
+        y = ((q @ k.transpose(2, 3) * blk.attn.scale).softmax(3) @ v).transpose(1, 2).reshape(b, n, c)
+        x = x + lin(blk.attn.proj, y)
+        x = x + lin(blk.mlp.fc2, act(lin(blk.mlp.fc1, ln(blk.norm2, x))))
+    c, blk = x.shape[2], vit.blocks[layer]
+    y = ln(blk.norm1, x)
+    w, bias = blk.attn.qkv.weight[c:2 * c], blk.attn.qkv.bias[c:2 * c]
+    return (Lin8.apply(y, w) if act8 else y @ w.t()) + bias
+
+
+@gpu
+@pytest.mark.parametrize("act8", [True, False], ids=["act8", "plain"])
+def test_vit_fine_tuning_path(act8):
+    """VisionTransformer.key_tokens_grad: keys as the frozen path computes them, gradients against float64 (2 blocks deep; products of
+    fp32 library kernels, ~10^3 roundings of 6e-8 in norm: 1e-4; with 8-bit checkpoints 2e-3 for the codes that fall on the other side
+    of a rounding border, as in the decoder test, through two blocks)"""
+    import copy
+    vit = _small_vit()
+    img = torch.rand(2, 3, 40, 40)
+    ref = copy.deepcopy(vit).double()
+    out64 = _vit_reference(ref, img.double(), 2, act8)
+    go = torch.randn(out64.shape)
+    out64.backward(go.double())
+    vit = vit.cuda()
+    out = vit.key_tokens_grad(img.cuda(), layer=2, act8=act8)
+    out.backward(go.cuda())
+    assert (out.detach().double().cpu() - out64.detach()).norm() <= 1e-5 * out64.detach().norm()
+    with torch.no_grad():
+        frozen = vit.key_tokens(img.cuda(), layer=2)
+    assert (frozen.double().cpu() - out64.detach()).norm() <= 1e-5 * out64.detach().norm()
+    checked = 0
+    for (name, p), (_, q) in zip(vit.named_parameters(), ref.named_parameters()):
+        if q.grad is None:
+            assert p.grad is None, name
+            continue
+        checked += 1
+        assert (p.grad.double().cpu() - q.grad).norm() <= (2e-3 if act8 else 1e-4) * q.grad.norm() + 1e-12, name
+    assert checked == 2 * 12 + 4 + 3                                                              # two blocks, norm1 + qkv of the third, patch embedding + class token
+
+
+@gpu
+def test_vit_fine_tuning_path_in_bf16():
+    """MIXED_BF16: the same keys and gradients to bf16's accuracy (every value passes some 30 roundings of 2^-8 of itself: 5 % in norm)"""
+    from scp_amd import dino
+    vit = _small_vit().cuda()
+    img = torch.rand(2, 3, 40, 40, device="cuda")
+    want = vit.key_tokens_grad(img, layer=2, act8=False)
+    go = torch.randn_like(want)
+    want_g = torch.autograd.grad(want, [vit.blocks[0].attn.qkv.weight, vit.blocks[1].mlp.fc1.weight], go)
+    dino.MIXED_BF16 = True
+    try:
+        got = vit.key_tokens_grad(img, layer=2)
+        got_g = torch.autograd.grad(got, [vit.blocks[0].attn.qkv.weight, vit.blocks[1].mlp.fc1.weight], go.bfloat16())
+    finally:
+        dino.MIXED_BF16 = False
+    assert got.dtype == BF16
+    assert (got.detach().float() - want.detach()).norm() <= 0.05 * want.detach().norm()
+    for a, b in zip(got_g, want_g):
+        assert a.dtype == FP32 and (a - b).norm() <= 0.05 * b.norm()
 
 
 @gpu
