@@ -37,7 +37,30 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, float* lds)
     return v;
 }
 
-template <typename W> __device__ __forceinline__ float weight_at(const void* w, int c) { return (float)static_cast<const W*>(w)[c]; }
+// VEC weights from column c0 (NULL: all `fill`); columns past the end repeat the last one
+template <typename W, int VEC> __device__ __forceinline__ void load_weights(const void* w, int c0, int C, float fill, float (&v)[VEC]) {
+    constexpr int WV = VecIO<W>::VEC;
+    const W* p = static_cast<const W*>(w);
+    if (!p) {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) v[i] = fill;
+    } else if (c0 + VEC <= C) {
+        if constexpr (WV == VEC) {
+            VecIO<W>::load(p + c0, v);
+        } else {
+#pragma unroll
+            for (int h = 0; h < VEC / WV; h++) {
+                float x[WV];
+                VecIO<W>::load(p + c0 + h * WV, x);
+#pragma unroll
+                for (int i = 0; i < WV; i++) v[h * WV + i] = x[i];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) v[i] = VecIO<W>::one(p + (c0 + i < C ? c0 + i : C - 1));
+    }
+}
 
 struct NormArgs {
     const void *x, *resid, *gamma, *beta;
@@ -93,13 +116,11 @@ template <typename T, typename W, int TPR, int NCH> __global__ __launch_bounds__
     T* yr = static_cast<T*>(a.y) + (size_t)row * C;
 #pragma unroll
     for (int j = 0; j < NCH; j++) {
-        const int c0 = (lane + TPR * j) * VEC;
+        float g[VEC], b[VEC];
+        load_weights<W, VEC>(a.gamma, (lane + TPR * j) * VEC, C, 1.f, g);
+        load_weights<W, VEC>(a.beta, (lane + TPR * j) * VEC, C, 0.f, b);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const int c = c0 + i < C ? c0 + i : C - 1;
-            const float g = a.gamma ? weight_at<W>(a.gamma, c) : 1.f, b = a.beta ? weight_at<W>(a.beta, c) : 0.f;
-            v[j][i] = (v[j][i] - mean) * rstd * g + b;
-        }
+        for (int i = 0; i < VEC; i++) v[j][i] = (v[j][i] - mean) * rstd * g[i] + b[i];
         scp::store_chunk<T>(yr, lane + TPR * j, C, v[j]);
     }
 }
@@ -108,7 +129,8 @@ struct NormGradArgs {
     const void *s, *gamma, *gy, *gsum;
     const float* stats;
     void* gx;            // may be NULL
-    float* partial;      // [blocks][2][C]; NULL: no weight gradients wanted
+    float *part_w, *part_b;      // column sums of each workgroup, `part_stride` floats apart (one workgroup: the results); NULL: not wanted
+    long part_stride;
     long rows;
     int C;
 };
@@ -122,26 +144,39 @@ template <typename T, typename W, int TPR, int NCH> __global__ __launch_bounds__
     const int C = a.C;
     float w[NCH][VEC], gw[NCH][VEC], gb[NCH][VEC];
 #pragma unroll
-    for (int j = 0; j < NCH; j++)
+    for (int j = 0; j < NCH; j++) {
+        load_weights<W, VEC>(a.gamma, (lane + TPR * j) * VEC, C, 1.f, w[j]);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const int c = (lane + TPR * j) * VEC + i;
-            w[j][i] = a.gamma ? weight_at<W>(a.gamma, c < C ? c : C - 1) : 1.f;
-            gw[j][i] = gb[j][i] = 0.f;
-        }
+        for (int i = 0; i < VEC; i++) gw[j][i] = gb[j][i] = 0.f;
+    }
+    // the next row's x and gy are on their way while this one is worked on (a row past the end reads the last one again)
     const long stride = (long)gridDim.x * GROUPS;
+    const T *sp = static_cast<const T*>(a.s), *gp = static_cast<const T*>(a.gy);
+    float nx[NCH][VEC], ng[NCH][VEC], nmean, nrstd;
+    auto fetch = [&](long row) {
+        row = row < a.rows ? row : a.rows - 1;
+#pragma unroll
+        for (int j = 0; j < NCH; j++) {
+            scp::load_chunk<T>(sp + (size_t)row * C, lane + TPR * j, C, nx[j]);
+            scp::load_chunk<T>(gp + (size_t)row * C, lane + TPR * j, C, ng[j]);
+        }
+        nmean = a.stats[2 * row];
+        nrstd = a.stats[2 * row + 1];
+    };
+    fetch((long)blockIdx.x * GROUPS + group);
     for (long row0 = (long)blockIdx.x * GROUPS; row0 < a.rows; row0 += stride) {
         const long row = row0 + group;
         if (TPR < 256 && row >= a.rows) break;                     // the last row group(s) of the last stride; no barrier below for TPR < 256
-        const T* sr = static_cast<const T*>(a.s) + (size_t)row * C;
-        const T* gr = static_cast<const T*>(a.gy) + (size_t)row * C;
         float x[NCH][VEC], g[NCH][VEC];
 #pragma unroll
-        for (int j = 0; j < NCH; j++) {
-            scp::load_chunk<T>(sr, lane + TPR * j, C, x[j]);
-            scp::load_chunk<T>(gr, lane + TPR * j, C, g[j]);
-        }
-        const float mean = a.stats[2 * row], rstd = a.stats[2 * row + 1];
+        for (int j = 0; j < NCH; j++)
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                x[j][i] = nx[j][i];
+                g[j][i] = ng[j][i];
+            }
+        const float mean = nmean, rstd = nrstd;
+        fetch(row + stride);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NCH; j++)
@@ -172,8 +207,7 @@ template <typename T, typename W, int TPR, int NCH> __global__ __launch_bounds__
             }
         }
     }
-    if (!a.partial) return;
-    float* out = a.partial + (size_t)blockIdx.x * 2 * C;
+    if (!a.part_w && !a.part_b) return;
     if constexpr (TPR == 16) {
 #pragma unroll
         for (int j = 0; j < NCH; j++)
@@ -189,6 +223,9 @@ template <typename T, typename W, int TPR, int NCH> __global__ __launch_bounds__
     const bool mine = TPR != 16 || (threadIdx.x & 63) < 16;
 #pragma unroll
     for (int which = 0; which < 2; which++) {
+        float* out = which ? a.part_b : a.part_w;
+        if (!out) continue;
+        out += blockIdx.x * a.part_stride;
         for (int f = 1; f < FOLD; f++) {                            // partial 0 += 1, 2, ...: a fixed order
             __syncthreads();
             if (folder == f && mine) {
@@ -211,34 +248,39 @@ template <typename T, typename W, int TPR, int NCH> __global__ __launch_bounds__
 #pragma unroll
                 for (int i = 0; i < VEC; i++) {
                     const int c = (lane + TPR * j) * VEC + i;
-                    if (c < C) out[(size_t)which * C + c] = which ? gb[j][i] : gw[j][i];
+                    if (c < C) out[c] = which ? gb[j][i] : gw[j][i];
                 }
         }
     }
 }
 
-// gw[c] = sum_b partial[b][0][c], gb[c] = sum_b partial[b][1][c]: 64 columns x 4 slices of the blocks per workgroup
-__global__ __launch_bounds__(THREADS) void layernorm_fold_kernel(const float* __restrict__ partial, int blocks, int C, float* gw, float* gb) {
-    __shared__ float lds[4][64];
-    const int col = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
+// gw[c] = sum_b partial[b][0][c], gb[c] = sum_b partial[b][1][c]: 64 columns x 16 slices of the blocks per workgroup
+constexpr int SLICES = 16;
+__global__ __launch_bounds__(64 * SLICES) void layernorm_fold_kernel(const float* __restrict__ partial, int blocks, int C, float* gw, float* gb) {
+    __shared__ float lds[SLICES][64];
+    const int t = threadIdx.x & 63, col = blockIdx.x * 64 + t, slice = threadIdx.x >> 6;
     const int n = 2 * C;
     float s = 0.f;
     if (col < n) {
-        const int per = (blocks + 3) / 4, b0 = slice * per, b1 = min(blocks, b0 + per);
+        const int per = (blocks + SLICES - 1) / SLICES, b0 = slice * per, b1 = min(blocks, b0 + per);
 #pragma unroll 8
         for (int b = b0; b < b1; b++) s += partial[(size_t)b * n + col];
     }
-    lds[slice][threadIdx.x & 63] = s;
+    lds[slice][t] = s;
     __syncthreads();
     if (slice == 0 && col < n) {
-        const int t = threadIdx.x;
-        const float r = (lds[0][t] + lds[1][t]) + (lds[2][t] + lds[3][t]);
+        float r = 0.f;
+#pragma unroll
+        for (int i = 0; i < SLICES; i++) r += lds[i][t];
         if (col < C) { if (gw) gw[col] = r; } else { if (gb) gb[col - C] = r; }
     }
 }
 
-int backward_blocks(long rows, int tpr) {
+// One workgroup for up to 2^15 elements: it needs no partials and no second launch, which cost a caller more than the ~8 us that one
+// compute unit takes to stream them.
+int backward_blocks(long rows, int C, int tpr) {
     const long groups = THREADS / tpr, need = (rows + groups - 1) / groups;
+    if (rows * C <= 1 << 15) return 1;
     return (int)(need < BWD_MAX_BLOCKS ? need : BWD_MAX_BLOCKS);
 }
 int lanes_per_row(int C) { return C <= 512 ? 16 : C <= 2048 ? 64 : 256; }
@@ -249,7 +291,7 @@ template <typename T, typename W, int TPR, int NCH> struct Launch {
         hipLaunchKernelGGL((layernorm_forward_kernel<T, W, TPR, NCH>), dim3(blocks), dim3(THREADS), 0, st, a);
     }
     static void backward(const NormGradArgs& a, hipStream_t st) {
-        hipLaunchKernelGGL((layernorm_backward_kernel<T, W, TPR, NCH>), dim3(backward_blocks(a.rows, TPR)), dim3(THREADS), 0, st, a);
+        hipLaunchKernelGGL((layernorm_backward_kernel<T, W, TPR, NCH>), dim3(backward_blocks(a.rows, a.C, TPR)), dim3(THREADS), 0, st, a);
     }
 };
 
@@ -308,7 +350,8 @@ extern "C" int scp_layernorm_forward(const void* x, const void* resid, const voi
 
 extern "C" size_t scp_layernorm_backward_workspace(long rows, int C) {
     if (rows <= 0 || C <= 0 || C > MAX_C) return 0;
-    return (size_t)backward_blocks(rows, lanes_per_row(C)) * 2 * C * sizeof(float);
+    const int blocks = backward_blocks(rows, C, lanes_per_row(C));
+    return blocks > 1 ? (size_t)blocks * 2 * C * sizeof(float) : 0;
 }
 
 extern "C" int scp_layernorm_backward(const void* s, const void* gamma, const void* gy, const void* gsum, const float* stats, long rows,
@@ -316,17 +359,18 @@ extern "C" int scp_layernorm_backward(const void* s, const void* gamma, const vo
                                       size_t workspace_bytes, void* stream) {
     if (const char* why = bad_problem(rows, C, dtype, wdtype)) return scp::fail(hipErrorInvalidValue, why);
     if (!s || !gy || !stats) return scp::fail(hipErrorInvalidValue, "layernorm_backward: null argument");
-    const bool wgrad = g_gamma || g_beta;
-    if (!gx && !wgrad) return 0;
-    if (wgrad && (!workspace || workspace_bytes < scp_layernorm_backward_workspace(rows, C)))
+    if (!gx && !g_gamma && !g_beta) return 0;
+    const int blocks = backward_blocks(rows, C, lanes_per_row(C));
+    const bool fold = blocks > 1 && (g_gamma || g_beta);
+    if (fold && (!workspace || workspace_bytes < scp_layernorm_backward_workspace(rows, C)))
         return scp::fail(hipErrorInvalidValue, "layernorm_backward: workspace too small");
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const NormGradArgs a{s, gamma, gy, gsum, stats, gx, wgrad ? static_cast<float*>(workspace) : nullptr, rows, C};
+    float* part = static_cast<float*>(workspace);
+    const NormGradArgs a{s, gamma, gy, gsum, stats, gx, fold ? part : g_gamma, fold ? part + C : g_beta, fold ? 2l * C : 0, rows, C};
     by_type(dtype, wdtype, C, a, st);
     if (const int e = scp::check_launch("layernorm_backward")) return e;
-    if (wgrad) {
-        hipLaunchKernelGGL(layernorm_fold_kernel, dim3((2 * C + 63) / 64), dim3(THREADS), 0, st, static_cast<const float*>(workspace),
-                           backward_blocks(rows, lanes_per_row(C)), C, g_gamma, g_beta);
+    if (fold) {
+        hipLaunchKernelGGL(layernorm_fold_kernel, dim3((2 * C + 63) / 64), dim3(64 * SLICES), 0, st, part, blocks, C, g_gamma, g_beta);
         return scp::check_launch("layernorm_backward fold");
     }
     return 0;

@@ -110,7 +110,8 @@ class _LayerNorm(Function):
             ws, nbytes = None, 0
             if want_w or want_b:
                 nbytes = L.scp_layernorm_backward_workspace(rows, c)
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+                if nbytes:
+                    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             code = L.scp_layernorm_backward(s.data_ptr(), _ptr(weight), gy.data_ptr(), _ptr(gsum), stats.data_ptr(), rows, c, dtype, wdtype, _ptr(gx),
                                             _ptr(gw), _ptr(gb), _ptr(ws), nbytes, _stream())
             if code:

@@ -88,7 +88,7 @@ def test_c_entries_refuse_bad_problems_before_any_launch():
     assert "8192" in L.scp_last_error().decode()
     assert L.scp_layernorm_forward(one, one, None, None, 1e-6, 4, 64, 0, 0, None, one, None, None) != 0
     assert L.scp_layernorm_forward(one, None, one, None, 1e-6, 4, 64, 0, 1, None, one, None, None) != 0
-    assert L.scp_layernorm_backward(one, None, one, None, one, 4, 64, 0, 0, one, one, one, None, 0, None) != 0
+    assert L.scp_layernorm_backward(one, None, one, None, one, 400, 640, 0, 0, one, one, one, None, 0, None) != 0
     assert "workspace" in L.scp_last_error().decode()
     assert L.scp_pack8(one, 0, 64, 0, one, one, None) != 0 and L.scp_pack8(one, 1, 64, 2, one, one, None) != 0
     assert L.scp_gelu8_forward(one, 1, 64, 0, one, one, None, None) != 0
