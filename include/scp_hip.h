@@ -668,7 +668,7 @@ int scp_cross_attention_backward(const void* q, const void* k, const void* v, co
  * channels share the step 2^(exps - 127), value = code * step; exps = 255: the group held an infinity or a NaN (every value reads as NaN).
  *   gelu8: y = erf GELU of x, with the checkpoint of x written in the same pass (codes and exps NULL: none); backward: gx = gy gelu'(value).
  *   weight_grad8 (csrc/act8_wgrad.hip): gw [N,K] = sum over rows of gy[:,n] value[:,k], gb [N] (may be NULL) = sum over rows of gy; fp32.
- *     N >= 4 (fp32) or 8 (bf16), K >= 16: a row holds at least 16 bytes. */
+ *     N >= 4 (fp32) or 8 (bf16), K >= 8. */
 int scp_pack8(const void* x, long rows, int C, int dtype, signed char* codes, unsigned char* exps, void* stream);
 int scp_unpack8(const signed char* codes, const unsigned char* exps, long rows, int C, int dtype, void* x, void* stream);
 int scp_gelu8_forward(const void* x, long rows, int C, int dtype, void* y, signed char* codes, unsigned char* exps, void* stream);

@@ -367,8 +367,8 @@ def weight_grad8(grad, packed, bias=True):
     if rows == 0:
         return torch.zeros(n, k, dtype=torch.float32, device=grad.device), torch.zeros(n, dtype=torch.float32, device=grad.device) if bias else None
     grad, codes, exps = grad.detach().contiguous(), packed.codes, packed.exps
-    # the kernel reads 16 bytes of a row at a time: narrower rows are widened with zeros
-    pad_n, pad_k = max(0, 16 // grad.element_size() - n), max(0, 16 - k)
+    # the kernel reads 16 bytes of grad and 8 codes of a row at a time: narrower rows are widened with zeros
+    pad_n, pad_k = max(0, 16 // grad.element_size() - n), max(0, 8 - k)
     if pad_n:
         grad = torch.nn.functional.pad(grad, (0, pad_n))
     if pad_k:

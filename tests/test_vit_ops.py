@@ -94,7 +94,7 @@ def test_c_entries_refuse_bad_problems_before_any_launch():
     assert L.scp_gelu8_forward(one, 1, 64, 0, one, one, None, None) != 0
     assert L.scp_weight_grad8(one, one, one, 4, 0, 64, 0, one, None, None, 0, None) != 0
     assert L.scp_weight_grad8(one, one, None, 4, 8, 64, 0, one, None, None, 0, None) != 0
-    assert L.scp_weight_grad8(one, one, one, 4, 7, 64, 1, one, None, None, 0, None) != 0 and L.scp_weight_grad8(one, one, one, 4, 8, 15, 0, one, None, None, 0, None) != 0
+    assert L.scp_weight_grad8(one, one, one, 4, 7, 64, 1, one, None, None, 0, None) != 0 and L.scp_weight_grad8(one, one, one, 4, 8, 7, 0, one, None, None, 0, None) != 0
 
 
 @gpu
@@ -510,7 +510,7 @@ def test_gelu8_matches_definition(shape, dtype):
 
 
 WGRAD_SHAPES = [(1, 1, 1), (1, 8, 16), (3, 7, 5), (33, 64, 64), (100, 65, 96), (257, 128, 128), (1025, 40, 48), (70, 384, 384), (130, 333, 384), (2100, 130, 72), (64, 16, 1001),
-                (515, 136, 160), (31, 17, 33), (32, 129, 131), (65, 257, 17), (200, 4, 16), (200, 8, 15), (97, 261, 16), (1000, 255, 143)]
+                (515, 136, 160), (31, 17, 33), (32, 129, 131), (65, 257, 17), (200, 4, 16), (200, 8, 15), (200, 7, 7), (97, 261, 16), (1000, 255, 143)]
 
 
 def wgrad_reference(gy, x8):
