@@ -11,7 +11,11 @@
 // query gradient:    stationary Q, gO, streamed K, V;   Acc = gq^T += K^T gs
 // key/value gradient: stationary K, V, streamed Q, gO;  Acc = gk^T += Q^T gs,  Acc2 = gv^T += gO^T p
 // bf16 runs on v_mfma_f32_32x32x16_bf16 (p and gs rounded to bf16 for their product: one operand of it has to be bf16, and the result is
-// rounded to bf16 anyway), fp32 on v_mfma_f32_32x32x2_f32.
+// rounded to bf16 anyway), fp32 on v_mfma_f32_32x32x2_f32.  What that rounding does to gs = p (gO . v - delta) where a few keys hold most of
+// the softmax, and gO . v and delta cancel: the denominator is the sum of the ROUNDED p (v_dot2_f32_bf16, as fast as the 16 additions
+// that it replaces), so o is a weighted mean of v whatever the rounding did and its error in delta is of the size of gs's own rounding; and
+// what o is rounded by is kept for the backward pass (o_low), so delta sees o to 16 bits (4 us of 181 for 32 x 6 heads of 642 x 1025).
+// Error of gq, 300 queries x 300 keys with a softmax on 2 to 3 keys: 5.7e-3 without the two, 3.0e-3 with them.
 //
 // Two ways to deal the work (Plan): OWN -- each of 4 wavefronts has 32 columns of its own and all read the same tile (64 rows in bf16, 32 in
 // fp32); SHARE -- the wavefronts have the SAME 32 columns, each reads its 32 rows of a 128-row tile, and their partial results are joined
@@ -32,6 +36,7 @@
 namespace scp_attn {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -40,8 +45,8 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 struct Args {
     const void *q, *k, *v, *go;
     const unsigned char* mask;
-    const void* o_in;
-    void *o, *gq, *gk, *gv;
+    const void *o_in, *o_low_in;
+    void *o, *o_low, *gq, *gk, *gv;
     float *lse, *delta;
     float *part_o, *part_ml;              // split over the keys: [split][bh][R][D], [split][bh][R][2]
     long qs[3], ks[3], vs[3], gs[3];      // strides in elements: batch, token, head
@@ -110,8 +115,8 @@ template <int DP> struct Mma<__bf16, DP> {
             for (int c = 0; c < CB; c++) acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, x[c].f[i], acc[c], 0, 0, 0);
         }
     }
-    // a[c][db][d][col] += sum_row t[r0 + row][32 db + d] p[c][row][col]
-    template <int CB> static __device__ __forceinline__ void adds(f32x16 (&a)[CB][DB], const T* t, int r0, const f32x16 (&p)[CB]) {
+    // a[c][db][d][col] += sum_row t[r0 + row][32 db + d] p[c][row][col];  sums[c] (where given) += the p that were multiplied, half a column each
+    template <int CB> static __device__ __forceinline__ void adds(f32x16 (&a)[CB][DB], const T* t, int r0, const f32x16 (&p)[CB], float* sums = nullptr) {
         const int lane = threadIdx.x & 63, i = lane & 15, half = lane >> 5, cg = (lane >> 4) & 1;
 #pragma unroll
         for (int s = 0; s < 2; s++) {
@@ -120,6 +125,13 @@ template <int DP> struct Mma<__bf16, DP> {
             for (int c = 0; c < CB; c++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) b[c][j] = (__bf16)p[c][8 * s + j];
+            if (sums) {
+                const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+                for (int c = 0; c < CB; c++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) sums[c] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{b[c][2 * j], b[c][2 * j + 1]}, one, sums[c], false);
+            }
 #pragma unroll
             for (int db = 0; db < DB; db++) {
                 bf16x4 h[2];
@@ -138,6 +150,10 @@ template <int DP> struct Mma<__bf16, DP> {
     static __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
         const bf16x4 v = {(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
         *reinterpret_cast<bf16x4*>(p) = v;
+    }
+    // what store4 rounds away
+    static __device__ __forceinline__ void store_low(T* p, float a, float b, float c, float d) {
+        store4(p, a - (float)(__bf16)a, b - (float)(__bf16)b, c - (float)(__bf16)c, d - (float)(__bf16)d);
     }
 };
 
@@ -168,7 +184,7 @@ template <int DP> struct Mma<float, DP> {
                 for (int c = 0; c < CB; c++) acc[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], x[c].f[i][j], acc[c], 0, 0, 0);
         }
     }
-    template <int CB> static __device__ __forceinline__ void adds(f32x16 (&a)[CB][DB], const T* t, int r0, const f32x16 (&p)[CB]) {
+    template <int CB> static __device__ __forceinline__ void adds(f32x16 (&a)[CB][DB], const T* t, int r0, const f32x16 (&p)[CB], float* = nullptr) {
         const int half = (threadIdx.x >> 5) & 1, l31 = threadIdx.x & 31;
         if constexpr (L::CPR == 16 || L::CPR == 32) {
             // the swizzle of row 8 i + 4 half + j is j + 4 half in the low three chunk bits and i & 1 in the fourth, which only trades
@@ -205,6 +221,7 @@ template <int DP> struct Mma<float, DP> {
         const f32x4 v = {a, b, c, d};
         *reinterpret_cast<f32x4*>(p) = v;
     }
+    static __device__ __forceinline__ void store_low(T*, float, float, float, float) {}
 };
 
 // rows of one head in global memory: row r is token r / G (of stride ts) and head r % G (of stride hs) behind `base`
@@ -430,7 +447,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_k
 
     typename M::Frag q[CB];
     f32x16 o[CB][DB];
-    float m[CB], l[CB];
+    float m[CB], l[CB];                                      // maximum, sum of p as they are multiplied
 #pragma unroll
     for (int x = 0; x < CB; x++) {
         const int r = r_wave + 32 * x + l31;
@@ -496,11 +513,11 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_k
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     s[kb][x][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][x][i], c, -base));
-                    part[i & 3] += s[kb][x][i];
+                    if (sizeof(T) == 4) part[i & 3] += s[kb][x][i];
                 }
-                l[x] += (part[0] + part[1]) + (part[2] + part[3]);
+                if (sizeof(T) == 4) l[x] += (part[0] + part[1]) + (part[2] + part[3]);
             }
-            M::template adds<CB>(o, tile[buf][1], r0 + 32 * kb, s[kb]);
+            M::template adds<CB>(o, tile[buf][1], r0 + 32 * kb, s[kb], l);
         }
     };
     walk_keys<S>(words, mask, key_beg, key_end,
@@ -541,13 +558,14 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_k
             if (rr >= R || d >= a.D) continue;
             float mt = -INFINITY, lt = 0.f;
 #pragma unroll
-            for (int w = 0; w < WAVES; w++) mt = fmaxf(mt, jm[(w * 32 + row) * 2]);
+            for (int i = 0; i < WAVES; i++) mt = fmaxf(mt, jm[(i * 32 + row) * 2]);
             f32x4 sum = {};
 #pragma unroll
-            for (int w = 0; w < WAVES; w++) {
-                const float mw = jm[(w * 32 + row) * 2], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mt);
-                lt += f * jm[(w * 32 + row) * 2 + 1];
-                if (f != 0.f) sum += f * *reinterpret_cast<const f32x4*>(jo + (w * 32 + row) * DP + d);
+            for (int i = 0; i < WAVES; i++) {
+                const float* his = jm + (i * 32 + row) * 2;
+                const float f = his[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(his[0] - mt);
+                lt += f * his[1];
+                if (f != 0.f) sum += f * *reinterpret_cast<const f32x4*>(jo + (i * 32 + row) * DP + d);
             }
             if (a.nsplit > 1) {
                 const long at = ((long)split * a.BH + bh) * R + rr;
@@ -558,8 +576,10 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_k
                 }
             } else {
                 const int n = rr / a.G, h = hk * a.G + rr - n * a.G;
-                const float inv = lt == 0.f ? 0.f : 1.f / lt;
-                M::store4(static_cast<T*>(a.o) + (((long)b * a.Nq + n) * H + h) * a.D + d, sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
+                sum *= lt == 0.f ? 0.f : 1.f / lt;
+                const long at = (((long)b * a.Nq + n) * H + h) * a.D + d;
+                M::store4(static_cast<T*>(a.o) + at, sum[0], sum[1], sum[2], sum[3]);
+                if (a.o_low) M::store_low(static_cast<T*>(a.o_low) + at, sum[0], sum[1], sum[2], sum[3]);
                 if (a.lse && d == 0) a.lse[(long)bh * R + rr] = lt == 0.f ? INFINITY : mt + __builtin_amdgcn_logf(lt);
             }
         }
@@ -569,14 +589,17 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_k
             const int r = r_wave + 32 * x + l31;
             if (r >= R) continue;
             const int n = r / a.G, h = hk * a.G + r - n * a.G;
-            T* out = static_cast<T*>(a.o) + (((long)b * a.Nq + n) * H + h) * a.D;
+            const long at = (((long)b * a.Nq + n) * H + h) * a.D;
             const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
 #pragma unroll
             for (int i = 0; i < DB; i++)
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
                     const int d = 32 * i + 8 * g + 4 * half;
-                    if (d < a.D) M::store4(out + d, o[x][i][4 * g] * inv, o[x][i][4 * g + 1] * inv, o[x][i][4 * g + 2] * inv, o[x][i][4 * g + 3] * inv);
+                    if (d >= a.D) continue;
+                    const f32x4 v = {o[x][i][4 * g] * inv, o[x][i][4 * g + 1] * inv, o[x][i][4 * g + 2] * inv, o[x][i][4 * g + 3] * inv};
+                    M::store4(static_cast<T*>(a.o) + at + d, v[0], v[1], v[2], v[3]);
+                    if (a.o_low) M::store_low(static_cast<T*>(a.o_low) + at + d, v[0], v[1], v[2], v[3]);
                 }
             if (a.lse && half == 0) a.lse[(long)bh * R + r] = l[x] == 0.f ? INFINITY : m[x] + __builtin_amdgcn_logf(l[x]);
         }
@@ -594,38 +617,56 @@ template <typename T> __global__ __launch_bounds__(256) void join_kernel(const A
     for (int s = 0; s < a.nsplit; s++) mt = fmaxf(mt, a.part_ml[2 * (s * rows + row)]);
     f32x4 sum = {};
     for (int s = 0; s < a.nsplit; s++) {
-        const float ms = a.part_ml[2 * (s * rows + row)], f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - mt);
-        lt += f * a.part_ml[2 * (s * rows + row) + 1];
+        const float* ml = a.part_ml + 2 * (s * rows + row);
+        const float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - mt);
+        lt += f * ml[1];
         if (f != 0.f) sum += f * *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * a.D + d);
     }
     const int bh = (int)(row / R), r = (int)(row - (long)bh * R), b = bh / a.Hk, hk = bh - b * a.Hk;
     const int n = r / a.G, h = hk * a.G + r - n * a.G;
-    const float inv = lt == 0.f ? 0.f : 1.f / lt;
-    Mma<T, 32>::store4(static_cast<T*>(a.o) + (((long)b * a.Nq + n) * H + h) * a.D + d, sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
+    sum *= lt == 0.f ? 0.f : 1.f / lt;
+    const long at = (((long)b * a.Nq + n) * H + h) * a.D + d;
+    Mma<T, 32>::store4(static_cast<T*>(a.o) + at, sum[0], sum[1], sum[2], sum[3]);
+    if (a.o_low) Mma<T, 32>::store_low(static_cast<T*>(a.o_low) + at, sum[0], sum[1], sum[2], sum[3]);
     if (a.lse && d == 0) a.lse[row] = lt == 0.f ? INFINITY : mt + __builtin_amdgcn_logf(lt);
 }
 
-// delta[row] = gO . o : 16 lanes per row, up to 8 channels each; rows in the order of o (a batch entry's tokens, then heads)
-template <typename T> __global__ __launch_bounds__(256) void delta_kernel(const Args a, int blocks_per_batch) {
-    const int H = a.Hk * a.G, R = a.Nq * a.G, l = threadIdx.x & 15;
+// delta[row] = gO . o: DP / 8 lanes per row (rounded up to a power of two), 8 channels each, DELTA_ROWS rows per group of lanes with all their
+// loads in flight at once (32 x 642 rows of 6 x 64, bf16: 16 lanes and one row each 10 us); rows in the order of o (a batch entry's tokens, then heads)
+constexpr int DELTA_ROWS = 4;
+constexpr int delta_lanes(int DP) { return DP <= 32 ? 4 : DP <= 64 ? 8 : 16; }
+template <typename T, int DP> __global__ __launch_bounds__(256) void delta_kernel(const Args a, int blocks_per_batch) {
+    constexpr int LANES = delta_lanes(DP), GROUPS = 256 / LANES;
+    typedef T tx8 __attribute__((ext_vector_type(8)));
+    const int H = a.Hk * a.G, R = a.Nq * a.G, l = threadIdx.x % LANES;
     const int b = blockIdx.x / blocks_per_batch;
-    const unsigned row = (blockIdx.x - b * blocks_per_batch) * 16 + (threadIdx.x >> 4);
-    if (row >= (unsigned)(a.Nq * H)) return;
-    const unsigned n = row / (unsigned)H, h = row - n * H;
-    float s = 0.f;
-    if (8 * l < a.D) {
-        const T* g = static_cast<const T*>(a.go) + b * a.gs[0] + n * a.gs[1] + h * a.gs[2] + 8 * l;
-        const T* o = static_cast<const T*>(a.o_in) + ((long)b * a.Nq * H + row) * a.D + 8 * l;
-        typedef T tx8 __attribute__((ext_vector_type(8)));
-        const tx8 x = *reinterpret_cast<const tx8*>(g), y = *reinterpret_cast<const tx8*>(o);
+    const unsigned first = (blockIdx.x - b * blocks_per_batch) * (GROUPS * DELTA_ROWS) + threadIdx.x / LANES, rows = a.Nq * H;
+    const int d = 8 * l < a.D ? 8 * l : 0;                   // a lane past the last channel reads the first ones and leaves them out
+    unsigned n[DELTA_ROWS], h[DELTA_ROWS];
+    tx8 x[DELTA_ROWS], y[DELTA_ROWS], z[DELTA_ROWS];
 #pragma unroll
-        for (int i = 0; i < 8; i++) s += (float)x[i] * (float)y[i];
+    for (int i = 0; i < DELTA_ROWS; i++) {
+        const unsigned row = min(first + GROUPS * i, rows - 1);
+        n[i] = row / (unsigned)H;
+        h[i] = row - n[i] * H;
+        x[i] = *reinterpret_cast<const tx8*>(static_cast<const T*>(a.go) + b * a.gs[0] + n[i] * a.gs[1] + h[i] * a.gs[2] + d);
+        const long at = ((long)b * rows + row) * a.D + d;
+        y[i] = *reinterpret_cast<const tx8*>(static_cast<const T*>(a.o_in) + at);
+        z[i] = tx8{};
+        if (sizeof(T) == 2 && a.o_low_in) z[i] = *reinterpret_cast<const tx8*>(static_cast<const T*>(a.o_low_in) + at);
     }
 #pragma unroll
-    for (int k = 1; k < 16; k <<= 1) s += __shfl_xor(s, k);
-    if (l == 0) {
-        const unsigned hk = h / (unsigned)a.G;
-        a.delta[((long)b * a.Hk + hk) * R + n * a.G + (h - hk * a.G)] = s;
+    for (int i = 0; i < DELTA_ROWS; i++) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) s += (float)x[i][e] * ((float)y[i][e] + (float)z[i][e]);
+        if (8 * l >= a.D) s = 0.f;
+#pragma unroll
+        for (int k = 1; k < LANES; k <<= 1) s += __shfl_xor(s, k);
+        if (l == 0 && first + GROUPS * i < rows) {
+            const unsigned hk = h[i] / (unsigned)a.G;
+            a.delta[((long)b * a.Hk + hk) * R + n[i] * a.G + (h[i] - hk * a.G)] = s;
+        }
     }
 }
 
@@ -885,8 +926,9 @@ template <typename T, int DP> void launch_forward(const Args& a, const Plan& p, 
 }
 template <typename T, int DP> void launch_backward(const Args& a, hipStream_t st) {
     const int R = a.Nq * a.G;
-    const int per_batch = (a.Nq * a.Hk * a.G + 15) / 16;
-    hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)(per_batch * (a.BH / a.Hk))), dim3(256), 0, st, a, per_batch);
+    constexpr int PER = 256 / delta_lanes(DP) * DELTA_ROWS;
+    const int per_batch = (a.Nq * a.Hk * a.G + PER - 1) / PER;
+    hipLaunchKernelGGL((delta_kernel<T, DP>), dim3((unsigned)(per_batch * (a.BH / a.Hk))), dim3(256), 0, st, a, per_batch);
     const int rows = a.gq ? R : 0, keys = a.gk || a.gv ? a.Nk : 0;
     const bool share = wavefronts(a, rows) + wavefronts(a, keys) < 2 * SHARE_BELOW;
     const int cols = share ? 32 : 128;

@@ -76,11 +76,11 @@ extern "C" size_t scp_cross_attention_forward_workspace(const scp_cross_attn_par
 }
 
 extern "C" int scp_cross_attention_forward(const void* q, const void* k, const void* v, const unsigned char* key_mask,
-                                           const scp_cross_attn_params* p, void* out, float* lse, void* workspace, size_t workspace_bytes,
-                                           void* stream) {
+                                           const scp_cross_attn_params* p, void* out, void* out_low, float* lse, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
     if (const char* why = bad_problem(p)) return scp::fail(hipErrorInvalidValue, why);
     if (!q || !k || !v || !out) return scp::fail(hipErrorInvalidValue, "cross_attention_forward: null argument");
-    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(workspace))
+    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(out_low) || misaligned(workspace))
         return scp::fail(hipErrorInvalidValue, "cross_attention_forward: tensors must be 16-byte aligned");
     if (tile_too_wide(p, false)) return scp::fail(hipErrorInvalidValue, "cross_attention_forward: token stride of k or v too large");
     Args a = make_args(p);
@@ -93,6 +93,7 @@ extern "C" int scp_cross_attention_forward(const void* q, const void* k, const v
     a.v = v;
     a.mask = key_mask;
     a.o = out;
+    a.o_low = p->dtype == SCP_DTYPE_F32 ? nullptr : out_low;
     a.lse = lse;
     a.nsplit = plan.nsplit;
     a.keys_per_split = plan.keys_per_split;
@@ -110,11 +111,11 @@ extern "C" size_t scp_cross_attention_backward_workspace(const scp_cross_attn_pa
 }
 
 extern "C" int scp_cross_attention_backward(const void* q, const void* k, const void* v, const unsigned char* key_mask, const void* out,
-                                            const float* lse, const void* g_out, const scp_cross_attn_params* p, void* g_q, void* g_k,
+                                            const void* out_low, const float* lse, const void* g_out, const scp_cross_attn_params* p, void* g_q, void* g_k,
                                             void* g_v, void* workspace, size_t workspace_bytes, void* stream) {
     if (const char* why = bad_problem(p)) return scp::fail(hipErrorInvalidValue, why);
     if (!q || !k || !v || !out || !lse || !g_out) return scp::fail(hipErrorInvalidValue, "cross_attention_backward: null argument");
-    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(g_out) || misaligned(g_q) || misaligned(g_k) || misaligned(g_v))
+    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(out_low) || misaligned(g_out) || misaligned(g_q) || misaligned(g_k) || misaligned(g_v))
         return scp::fail(hipErrorInvalidValue, "cross_attention_backward: tensors must be 16-byte aligned");
     if (tile_too_wide(p, true)) return scp::fail(hipErrorInvalidValue, "cross_attention_backward: token or head stride too large");
     if (!g_q && !g_k && !g_v) return 0;
@@ -126,6 +127,7 @@ extern "C" int scp_cross_attention_backward(const void* q, const void* k, const 
     a.v = v;
     a.mask = key_mask;
     a.o_in = out;
+    a.o_low_in = out_low;
     a.lse = const_cast<float*>(lse);
     a.go = g_out;
     a.delta = static_cast<float*>(workspace);

@@ -178,9 +178,9 @@ SYMBOLS = {
     "scp_layernorm_backward_workspace": (ctypes.c_size_t, [ctypes.c_long, _I]),
     "scp_layernorm_backward": (ctypes.c_int, [_P] * 5 + [ctypes.c_long, _I, _I, _I] + [_P] * 4 + [ctypes.c_size_t, _P]),
     "scp_cross_attention_forward_workspace": (ctypes.c_size_t, [ctypes.POINTER(CrossAttnParams)]),
-    "scp_cross_attention_forward": (ctypes.c_int, [_P] * 4 + [ctypes.POINTER(CrossAttnParams)] + [_P] * 3 + [ctypes.c_size_t, _P]),
+    "scp_cross_attention_forward": (ctypes.c_int, [_P] * 4 + [ctypes.POINTER(CrossAttnParams)] + [_P] * 4 + [ctypes.c_size_t, _P]),
     "scp_cross_attention_backward_workspace": (ctypes.c_size_t, [ctypes.POINTER(CrossAttnParams)]),
-    "scp_cross_attention_backward": (ctypes.c_int, [_P] * 7 + [ctypes.POINTER(CrossAttnParams)] + [_P] * 4 + [ctypes.c_size_t, _P]),
+    "scp_cross_attention_backward": (ctypes.c_int, [_P] * 8 + [ctypes.POINTER(CrossAttnParams)] + [_P] * 4 + [ctypes.c_size_t, _P]),
     "scp_pack8": (ctypes.c_int, [_P, ctypes.c_long, _I, _I, _P, _P, _P]),
     "scp_unpack8": (ctypes.c_int, [_P, _P, ctypes.c_long, _I, _I, _P, _P]),
     "scp_gelu8_forward": (ctypes.c_int, [_P, ctypes.c_long, _I, _I] + [_P] * 4),

@@ -166,36 +166,38 @@ def _addressable(t):
 
 
 def _attn_forward(q, k, v, mask, scale, keep):
-    """(out, log-sum-exp or None, C parameters); keep: for a backward pass"""
+    """(out, what its rounding to bfloat16 left or None, log-sum-exp or None, C parameters); keep: for a backward pass"""
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if keep else None
     if out.numel() == 0:
-        return out, lse, None
+        return out, None, lse, None
     if k.shape[1] == 0:
-        return out.zero_(), lse, None
+        return out.zero_(), None, lse, None
+    low = torch.empty_like(out) if keep and out.dtype == torch.bfloat16 else None
     L = capi.lib()
     p = capi.CrossAttnParams(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], capi.DTYPES[q.dtype], scale, q.stride()[:3],
                              k.stride()[:3], v.stride()[:3])
     ref = ctypes.byref(p)
     nbytes = L.scp_cross_attention_forward_workspace(ref)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    code = L.scp_cross_attention_forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(mask), ref, out.data_ptr(), _ptr(lse), _ptr(ws), nbytes, _stream())
+    code = L.scp_cross_attention_forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(mask), ref, out.data_ptr(), _ptr(low), _ptr(lse),
+                                         _ptr(ws), nbytes, _stream())
     if code:
         capi.check(code, "scp_cross_attention_forward")
-    return out, lse, p
+    return out, low, lse, p
 
 
 class _CrossAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, scale):
-        out, lse, ctx.p = _attn_forward(q, k, v, mask, scale, True)
-        ctx.save_for_backward(q, k, v, mask, out, lse)
+        out, low, lse, ctx.p = _attn_forward(q, k, v, mask, scale, True)
+        ctx.save_for_backward(q, k, v, mask, out, low, lse)
         return out
 
     @staticmethod
     @_first_order
     def backward(ctx, g):
-        q, k, v, mask, out, lse = ctx.saved_tensors
+        q, k, v, mask, out, low, lse = ctx.saved_tensors
         wq, wk, wv = ctx.needs_input_grad[:3]
         dev, dt = q.device, q.dtype
         gq = torch.empty(q.shape, dtype=dt, device=dev) if wq else None
@@ -210,8 +212,8 @@ class _CrossAttention(Function):
         ref = ctypes.byref(p)
         nbytes = L.scp_cross_attention_backward_workspace(ref)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        code = L.scp_cross_attention_backward(q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(mask), out.data_ptr(), lse.data_ptr(), g.data_ptr(), ref,
-                                              _ptr(gq), _ptr(gk), _ptr(gv), ws.data_ptr(), nbytes, _stream())
+        code = L.scp_cross_attention_backward(q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(mask), out.data_ptr(), _ptr(low), lse.data_ptr(),
+                                              g.data_ptr(), ref, _ptr(gq), _ptr(gk), _ptr(gv), ws.data_ptr(), nbytes, _stream())
         if code:
             capi.check(code, "scp_cross_attention_backward")
         return gq, gk, gv, None, None
