@@ -151,6 +151,39 @@ template <int DP> struct Mma<__bf16, DP> {
         const bf16x4 v = {(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
         *reinterpret_cast<bf16x4*>(p) = v;
     }
+    // channels 32 db .. 32 db + 31 of this lane's column, in accumulator order, to `row` where ok; `low` (or null): what that rounds away.
+    // The halves of the wavefront trade accumulators, so that each lane stores 8 channels in a row.
+    static __device__ __forceinline__ void store_column(T* row, T* low, int db, int D, bool ok, const f32x16& v) {
+        const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int d = 32 * db + 16 * k + 8 * half;
+            u32x4 hi = {}, lo = {};
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                unsigned h[2], l[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const float x = v[8 * k + 4 * u + 2 * w], y = v[8 * k + 4 * u + 2 * w + 1];
+                    const bf16x2 top = {(__bf16)x, (__bf16)y}, rest = {(__bf16)(x - (float)top[0]), (__bf16)(y - (float)top[1])};
+                    h[u] = __builtin_bit_cast(unsigned, top);
+                    l[u] = __builtin_bit_cast(unsigned, rest);
+                }
+                const auto a = __builtin_amdgcn_permlane32_swap(h[0], h[1], false, false);
+                hi[w] = a[0];
+                hi[2 + w] = a[1];
+                if (low) {
+                    const auto c = __builtin_amdgcn_permlane32_swap(l[0], l[1], false, false);
+                    lo[w] = c[0];
+                    lo[2 + w] = c[1];
+                }
+            }
+            if (ok && d < D) {
+                *reinterpret_cast<u32x4*>(row + d) = hi;
+                if (low) *reinterpret_cast<u32x4*>(low + d) = lo;
+            }
+        }
+    }
     // what store4 rounds away
     static __device__ __forceinline__ void store_low(T* p, float a, float b, float c, float d) {
         store4(p, a - (float)(__bf16)a, b - (float)(__bf16)b, c - (float)(__bf16)c, d - (float)(__bf16)d);
@@ -220,6 +253,14 @@ template <int DP> struct Mma<float, DP> {
     static __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
         const f32x4 v = {a, b, c, d};
         *reinterpret_cast<f32x4*>(p) = v;
+    }
+    static __device__ __forceinline__ void store_column(T* row, T*, int db, int D, bool ok, const f32x16& v) {
+        const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int d = 32 * db + 8 * g + 4 * half;
+            if (ok && d < D) store4(row + d, v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+        }
     }
     static __device__ __forceinline__ void store_low(T*, float, float, float, float) {}
 };
@@ -586,22 +627,13 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_k
     } else {
 #pragma unroll
         for (int x = 0; x < CB; x++) {
-            const int r = r_wave + 32 * x + l31;
-            if (r >= R) continue;
-            const int n = r / a.G, h = hk * a.G + r - n * a.G;
+            const int r = r_wave + 32 * x + l31, n = r / a.G, h = hk * a.G + r - n * a.G;
             const long at = (((long)b * a.Nq + n) * H + h) * a.D;
             const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
+            T* low = a.o_low ? static_cast<T*>(a.o_low) + at : nullptr;
 #pragma unroll
-            for (int i = 0; i < DB; i++)
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const int d = 32 * i + 8 * g + 4 * half;
-                    if (d >= a.D) continue;
-                    const f32x4 v = {o[x][i][4 * g] * inv, o[x][i][4 * g + 1] * inv, o[x][i][4 * g + 2] * inv, o[x][i][4 * g + 3] * inv};
-                    M::store4(static_cast<T*>(a.o) + at + d, v[0], v[1], v[2], v[3]);
-                    if (a.o_low) M::store_low(static_cast<T*>(a.o_low) + at + d, v[0], v[1], v[2], v[3]);
-                }
-            if (a.lse && half == 0) a.lse[(long)bh * R + r] = l[x] == 0.f ? INFINITY : m[x] + __builtin_amdgcn_logf(l[x]);
+            for (int i = 0; i < DB; i++) M::store_column(static_cast<T*>(a.o) + at, low, i, a.D, r < R, o[x][i] * inv);
+            if (a.lse && half == 0 && r < R) a.lse[(long)bh * R + r] = l[x] == 0.f ? INFINITY : m[x] + __builtin_amdgcn_logf(l[x]);
         }
     }
 }
@@ -850,7 +882,6 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
         }
         return;
     }
-    if (col >= C) return;
     long at;
     if (KV) at = (((long)b * a.Nk + col) * a.Hk + hk) * a.D;
     else {
@@ -863,15 +894,8 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
         if (!out) continue;
         const float f = which ? 1.f : a.scale;
 #pragma unroll
-        for (int i = 0; i < DB; i++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int d = 32 * i + 8 * g + 4 * half;
-                const f32x16& x = which ? acc2[0][i] : acc1[0][i];
-                if (d >= a.D) continue;
-                if (valid) M::store4(out + at + d, x[4 * g] * f, x[4 * g + 1] * f, x[4 * g + 2] * f, x[4 * g + 3] * f);
-                else M::store4(out + at + d, 0.f, 0.f, 0.f, 0.f);           // a masked key, whatever went through its column
-            }
+        for (int i = 0; i < DB; i++)                         // a masked key gets zeros, whatever went through its column
+            M::store_column(out + at, nullptr, i, a.D, col < C, valid ? (which ? acc2[0][i] : acc1[0][i]) * f : f32x16{});
     }
 }
 
