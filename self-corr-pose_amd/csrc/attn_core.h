@@ -462,6 +462,46 @@ __device__ __forceinline__ void walk_keys(unsigned* words, const unsigned char* 
     }
 }
 
+// factor of a partial softmax with maximum m and sum l in one with maximum `top`.  m is -inf where there was no key (l is 0: nothing to add) or
+// where every score was NaN (l is NaN, and so is the result).
+__device__ __forceinline__ float share_of(float m, float l, float top) { return m == -INFINITY ? l : __builtin_amdgcn_exp2f(m - top); }
+
+// joins the 4 wavefronts' partials jo [4][ROWS][DP], jm [4][ROWS][maximum, sum] of rows row0 .. into the result, or into this split's partial
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void join_waves(const Args& a, const float* jo, const float* jm, int row0, int split, int bh) {
+    const int R = a.Nq * a.G, H = a.Hk * a.G, b = bh / a.Hk, hk = bh - b * a.Hk;
+    for (int idx = threadIdx.x; idx < ROWS * (DP / 4); idx += 256) {
+        const int row = idx / (DP / 4), d = 4 * (idx % (DP / 4)), rr = row0 + row;
+        if (rr >= R || d >= a.D) continue;
+        float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) mt = fmaxf(mt, jm[(i * ROWS + row) * 2]);
+        f32x4 sum = {};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float* his = jm + (i * ROWS + row) * 2;
+            const float f = share_of(his[0], his[1], mt);
+            lt += f * his[1];
+            if (f != 0.f) sum += f * *reinterpret_cast<const f32x4*>(jo + (i * ROWS + row) * DP + d);
+        }
+        if (a.nsplit > 1) {
+            const long at = ((long)split * a.BH + bh) * R + rr;
+            *reinterpret_cast<f32x4*>(a.part_o + at * a.D + d) = sum;
+            if (d == 0) {
+                a.part_ml[2 * at] = mt;
+                a.part_ml[2 * at + 1] = lt;
+            }
+        } else {
+            const int n = rr / a.G, h = hk * a.G + rr - n * a.G;
+            sum *= lt == 0.f ? 0.f : 1.f / lt;
+            const long at = (((long)b * a.Nq + n) * H + h) * a.D + d;
+            Mma<T, DP>::store4(static_cast<T*>(a.o) + at, sum[0], sum[1], sum[2], sum[3]);
+            if (a.o_low) Mma<T, DP>::store_low(static_cast<T*>(a.o_low) + at, sum[0], sum[1], sum[2], sum[3]);
+            if (a.lse && d == 0) a.lse[(long)bh * R + rr] = lt == 0.f ? INFINITY : mt + __builtin_amdgcn_logf(lt);
+        }
+    }
+}
+
 template <typename T, int DP, bool SHARE>
 __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_kernel(const Args a) {
     typedef Shape<T, DP, SHARE> S;
@@ -594,36 +634,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_k
             jm[(wave * 32 + l31) * 2 + 1] = l[0];
         }
         __syncthreads();
-        for (int idx = threadIdx.x; idx < 32 * (DP / 4); idx += 256) {
-            const int row = idx / (DP / 4), d = 4 * (idx % (DP / 4)), rr = rb * 32 + row;
-            if (rr >= R || d >= a.D) continue;
-            float mt = -INFINITY, lt = 0.f;
-#pragma unroll
-            for (int i = 0; i < WAVES; i++) mt = fmaxf(mt, jm[(i * 32 + row) * 2]);
-            f32x4 sum = {};
-#pragma unroll
-            for (int i = 0; i < WAVES; i++) {
-                const float* his = jm + (i * 32 + row) * 2;
-                const float f = his[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(his[0] - mt);
-                lt += f * his[1];
-                if (f != 0.f) sum += f * *reinterpret_cast<const f32x4*>(jo + (i * 32 + row) * DP + d);
-            }
-            if (a.nsplit > 1) {
-                const long at = ((long)split * a.BH + bh) * R + rr;
-                *reinterpret_cast<f32x4*>(a.part_o + at * a.D + d) = sum;
-                if (d == 0) {
-                    a.part_ml[2 * at] = mt;
-                    a.part_ml[2 * at + 1] = lt;
-                }
-            } else {
-                const int n = rr / a.G, h = hk * a.G + rr - n * a.G;
-                sum *= lt == 0.f ? 0.f : 1.f / lt;
-                const long at = (((long)b * a.Nq + n) * H + h) * a.D + d;
-                M::store4(static_cast<T*>(a.o) + at, sum[0], sum[1], sum[2], sum[3]);
-                if (a.o_low) M::store_low(static_cast<T*>(a.o_low) + at, sum[0], sum[1], sum[2], sum[3]);
-                if (a.lse && d == 0) a.lse[(long)bh * R + rr] = lt == 0.f ? INFINITY : mt + __builtin_amdgcn_logf(lt);
-            }
-        }
+        join_waves<T, DP, 32>(a, jo, jm, rb * 32, split, bh);
     } else {
 #pragma unroll
         for (int x = 0; x < CB; x++) {
@@ -650,7 +661,7 @@ template <typename T> __global__ __launch_bounds__(256) void join_kernel(const A
     f32x4 sum = {};
     for (int s = 0; s < a.nsplit; s++) {
         const float* ml = a.part_ml + 2 * (s * rows + row);
-        const float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - mt);
+        const float f = share_of(ml[0], ml[1], mt);
         lt += f * ml[1];
         if (f != 0.f) sum += f * *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * a.D + d);
     }

@@ -370,6 +370,23 @@ def test_cross_attention_peaked_and_scaled(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("nq", [1, 3, 40, 2500])
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+def test_cross_attention_shows_nan(dtype, nq):
+    """a NaN in a query, or at a key that is not masked, is in the rows it belongs to and in no other; in every form of the forward pass"""
+    q, k, v, go, _ = attn_inputs(2, nq, 700, 2, 2, 64, dtype, 31)
+    q[0, nq - 1, 1, 5] = math.nan
+    o = vit_ops.cross_attention(q, k, v)
+    assert o[0, nq - 1, 1].isnan().all() and o.isnan().sum() == 64
+    k[1, 650, 0, 7] = math.nan
+    o = vit_ops.cross_attention(q, k, v)
+    assert o[1, :, 0].isnan().all() and o.isnan().sum() == 64 + 64 * nq
+    mask = torch.ones(2, 700, dtype=torch.bool, device="cuda")
+    mask[1, 650] = False
+    assert vit_ops.cross_attention(q, k, v, key_mask=mask).isnan().sum() == 64
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
 def test_cross_attention_layouts(dtype):
     g = gen(8)
