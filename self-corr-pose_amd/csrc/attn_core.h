@@ -649,6 +649,152 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_k
     }
 }
 
+// ---- few rows (single queries) -------------------------------------------------------------------------------------------------------
+// With few rows per key / value head nothing is reused: the time is that of reading K and V once, and what counts is how much of them
+// is in flight.  No LDS tiles: a group of LPR = DP / 8 lanes holds a key, 8 channels per lane; a wavefront loads UNROLL x 64 / LPR keys and
+// their values straight into registers, all loads in flight together, and each group keeps its own softmax of the keys it has seen (fp32
+// products and weights); groups, wavefronts and splits are joined at the end.
+template <typename T, int DP> struct Few {
+    static constexpr int LPR = DP <= 32 ? 4 : DP <= 64 ? 8 : 16, GROUPS = 64 / LPR;
+    static constexpr int UNROLL = sizeof(T) == 2 ? 8 : 4, KEYS = UNROLL * GROUPS;       // keys of a wavefront at a time
+    static constexpr int NV = 8 * sizeof(T) / 16;                                       // 16-byte pieces of 8 channels
+};
+template <int CTRL> __device__ __forceinline__ float dpp(float x) {
+    return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+// sum over the LPR neighbouring lanes: lane ^ 1, lane ^ 2, the other quad of 8, the other half of 16
+template <int LPR> __device__ __forceinline__ float group_sum(float x) {
+    x += dpp<0xB1>(x);
+    x += dpp<0x4E>(x);
+    if constexpr (LPR >= 8) x += dpp<0x141>(x);
+    if constexpr (LPR >= 16) x += dpp<0x140>(x);
+    return x;
+}
+__device__ __forceinline__ float channel(const u32x4 (&x)[1], int i) { return __uint_as_float(i & 1 ? x[0][i / 2] & 0xffff0000u : x[0][i / 2] << 16); }
+__device__ __forceinline__ float channel(const u32x4 (&x)[2], int i) { return __uint_as_float(x[i / 4][i & 3]); }
+__device__ __forceinline__ float dot8(const u32x4 (&x)[1], const u32x4 (&y)[1]) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const unsigned u = x[0][i], v = y[0][i];             // (bit_cast of the subscript itself takes element 0 every time)
+        s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u), __builtin_bit_cast(bf16x2, v), s, false);
+    }
+    return s;
+}
+__device__ __forceinline__ float dot8(const u32x4 (&x)[2], const u32x4 (&y)[2]) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) s = __builtin_fmaf(channel(x, i), channel(y, i), s);
+    return s;
+}
+template <typename T, int DP, int ROWS> __global__ __launch_bounds__(256, 2) void few_rows_kernel(const Args a) {
+    typedef Few<T, DP> S;
+    constexpr int UNROLL = S::UNROLL, GROUPS = S::GROUPS, LPR = S::LPR, NV = S::NV;
+    __shared__ __attribute__((aligned(16))) float jo[4 * ROWS * DP];
+    __shared__ float jm[4 * ROWS * 2];
+    int bh, split;
+    if (!place(a.BH, a.nsplit, bh, split)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane / LPR, d = 8 * (lane % LPR);
+    const int R = a.Nq * a.G, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const bool has = d < a.D;
+    const Rows qr = rows_of<T>(a.q, a.qs, b, hk * a.G, a.G), kr = rows_of<T>(a.k, a.ks, b, hk, 1), vr = rows_of<T>(a.v, a.vs, b, hk, 1);
+    const unsigned char* mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
+    const int key_beg = split * a.keys_per_split, key_end = min(a.Nk, key_beg + a.keys_per_split);
+    const float c = a.scale * LOG2E;
+
+    u32x4 q[ROWS][NV];
+    float m[ROWS], l[ROWS], acc[ROWS][8];
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            q[r][i] = u32x4{};
+            if (r < R && has) q[r][i] = *reinterpret_cast<const u32x4*>(qr.row(r) + d * sizeof(T) + 16 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) acc[r][i] = 0.f;
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+    }
+    for (int key0 = key_beg + wave * S::KEYS; key0 < key_end; key0 += 4 * S::KEYS) {
+        bool on[UNROLL];
+        unsigned char byte[UNROLL];
+        if (mask) {
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) byte[u] = mask[min(key0 + GROUPS * u + g, key_end - 1)];
+        }
+        bool any = false;
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            on[u] = key0 + GROUPS * u + g < key_end && (!mask || byte[u]);
+            any |= on[u];
+        }
+        if (!__any(any)) continue;
+        const __amdgpu_buffer_rsrc_t kb = buffer(kr.base + key0 * kr.ts), vb = buffer(vr.base + key0 * vr.ts);
+        u32x4 kx[UNROLL][NV], vx[UNROLL][NV];
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const unsigned off = on[u] && has ? (unsigned)(GROUPS * u + g) * (unsigned)kr.ts + d * sizeof(T) : OUT_OF_RANGE;
+#pragma unroll
+            for (int i = 0; i < NV; i++) kx[u][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kb, off + 16 * i, 0, 0));
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const unsigned off = on[u] && has ? (unsigned)(GROUPS * u + g) * (unsigned)vr.ts + d * sizeof(T) : OUT_OF_RANGE;
+#pragma unroll
+            for (int i = 0; i < NV; i++) vx[u][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vb, off + 16 * i, 0, 0));
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            float s[UNROLL], top = m[r];
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) {
+                s[u] = on[u] ? c * group_sum<LPR>(dot8(q[r], kx[u])) : -INFINITY;
+                top = fmaxf(top, s[u]);
+            }
+            const float base = top == -INFINITY ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m[r] - base);
+            m[r] = top;
+            l[r] *= alpha;
+#pragma unroll
+            for (int i = 0; i < 8; i++) acc[r][i] *= alpha;
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) {
+                const float p = __builtin_amdgcn_exp2f(s[u] - base);
+                l[r] += p;
+#pragma unroll
+                for (int i = 0; i < 8; i++) acc[r][i] = __builtin_fmaf(p, channel(vx[u], i), acc[r][i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {                         // join the groups of the wavefront
+        float top = m[r];
+#pragma unroll
+        for (int x = LPR; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+        const float f = share_of(m[r], l[r], top);
+        l[r] *= f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) acc[r][i] *= f;
+#pragma unroll
+        for (int x = LPR; x < 64; x <<= 1) {
+            l[r] += __shfl_xor(l[r], x);
+#pragma unroll
+            for (int i = 0; i < 8; i++) acc[r][i] += __shfl_xor(acc[r][i], x);
+        }
+        if (g == 0 && d < DP) {
+            float* to = jo + (wave * ROWS + r) * DP + d;
+            *reinterpret_cast<f32x4*>(to) = f32x4{acc[r][0], acc[r][1], acc[r][2], acc[r][3]};
+            *reinterpret_cast<f32x4*>(to + 4) = f32x4{acc[r][4], acc[r][5], acc[r][6], acc[r][7]};
+        }
+        if (lane == 0) {
+            jm[(wave * ROWS + r) * 2] = top;
+            jm[(wave * ROWS + r) * 2 + 1] = l[r];
+        }
+    }
+    __syncthreads();
+    join_waves<T, DP, ROWS>(a, jo, jm, 0, split, bh);
+}
+
 // joins the splits: a thread per 4 channels of a row
 template <typename T> __global__ __launch_bounds__(256) void join_kernel(const Args a) {
     const int R = a.Nq * a.G, H = a.Hk * a.G, q4 = a.D / 4;
@@ -924,14 +1070,30 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::GRAD_OCC)) void backward
 }
 
 // ---- launch plan --------------------------------------------------------------------------------------------------------------------
-struct Plan { bool share; int nsplit, keys_per_split, row_blocks; };
+struct Plan { bool share, few; int nsplit, keys_per_split, row_blocks; };
+// Rows that few_rows_kernel takes (one query, or the heads that share its keys).  fp32, where a 32-row product on the matrix cores costs 16
+// times a bf16 one: 64 x 6 heads of 64 x 4097 keys, 1 / 4 rows: 147 / 154 us against SHARE's 186; 32 x 8 heads of 128 x 1025 keys: 48 against
+// 91.  bf16: 1 row 76 against 74, 128 channels 29 against 41, 32 x 6 x 1025 keys 15.7 against 18.5 with the join; 2 / 4 rows 80 / 93
+// against 74 / 75, so only one.
+constexpr int few_rows(int size) { return size == 4 ? 4 : 1; }
+constexpr int FEW_BLOCKS = 512;                              // workgroups to split the keys for: 1024 and more only make the join longer (32 x 6 x 1025 fp32 24.4 us, 512: 22.7)
 constexpr long SHARE_BELOW = 1024;                           // wavefronts of 32 columns; fewer leave SIMDs empty (256 CUs x 4)
 inline long wavefronts(const Args& a, int columns) { return (long)a.BH * ((columns + 31) / 32); }
 // two_blocks: a wavefront of the OWN kernel takes 64 columns (Shape::CB).
 // split: where even SHARE has too few workgroups, the keys are divided as long as each part keeps two tiles
-inline Plan forward_plan(const Args& a, bool two_blocks) {
+inline Plan forward_plan(const Args& a, bool two_blocks, int max_few, int few_keys) {
     Plan p;
     const int R = a.Nq * a.G;
+    p.few = R <= max_few;
+    if (p.few) {
+        p.share = false;
+        p.row_blocks = 1;
+        long want = (FEW_BLOCKS - 1 + a.BH) / a.BH, most = (a.Nk + 4 * few_keys - 1) / (4 * few_keys);
+        if (want > most) want = most;
+        p.keys_per_split = ((a.Nk + (int)want - 1) / (int)want + 15) / 16 * 16;
+        p.nsplit = (a.Nk + p.keys_per_split - 1) / p.keys_per_split;
+        return p;
+    }
     p.share = wavefronts(a, R) < SHARE_BELOW;
     p.nsplit = 1;
     p.keys_per_split = a.Nk;
@@ -952,7 +1114,16 @@ inline int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96
 
 template <typename T, int DP> void launch_forward(const Args& a, const Plan& p, hipStream_t st) {
     const dim3 grid(placed_blocks(a.BH, p.row_blocks * p.nsplit));
-    if (p.share) hipLaunchKernelGGL((forward_kernel<T, DP, true>), grid, dim3(256), 0, st, a);
+    if (p.few) {
+        constexpr int DF = DP == 96 ? 128 : DP;              // lanes per key: a power of two
+        const int R = a.Nq * a.G;
+        if (R == 1) {
+            hipLaunchKernelGGL((few_rows_kernel<T, DF, 1>), grid, dim3(256), 0, st, a);
+        } else if constexpr (few_rows(sizeof(T)) > 1) {
+            if (R == 2) hipLaunchKernelGGL((few_rows_kernel<T, DF, 2>), grid, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((few_rows_kernel<T, DF, 4>), grid, dim3(256), 0, st, a);
+        }
+    } else if (p.share) hipLaunchKernelGGL((forward_kernel<T, DP, true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((forward_kernel<T, DP, false>), grid, dim3(256), 0, st, a);
     if (p.nsplit > 1) {
         const long n = (long)a.BH * a.Nq * a.G * (a.D / 4);
