@@ -43,13 +43,14 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 struct Args {
-    const void *q, *k, *v, *go;
+    const void *q, *k, *v, *go;           // what the matrix products read: the tensors (bf16), or their parts (fp32: Parts)
+    const void* dgo;                      // g_out itself, for delta
     const unsigned char* mask;
     const void *o_in, *o_low_in;
     void *o, *o_low, *gq, *gk, *gv;
     float *lse, *delta;
     float *part_o, *part_ml;              // split over the keys: [split][bh][R][D], [split][bh][R][2]
-    long qs[3], ks[3], vs[3], gs[3];      // strides in elements: batch, token, head
+    long qs[3], ks[3], vs[3], gs[3], dgs[3];      // strides in elements: batch, token, head
     int BH, Nq, Nk, Hk, G, D;
     int nsplit, keys_per_split;           // keys_per_split: a multiple of the tile
     float scale;
@@ -65,88 +66,40 @@ __device__ __forceinline__ float other_half(float x) {
     return (threadIdx.x & 32) ? __uint_as_float(r[0]) : __uint_as_float(r[1]);
 }
 
-// rows of a [32 n][DP] tile in LDS, 16-byte chunks
-template <typename T, int DP> struct Tile {
-    static constexpr int CH = 16 / sizeof(T);          // elements per chunk
+// what a tensor's element becomes for the matrix cores: bf16 itself, or three bf16 parts of 8 bits each of an fp32 number
+template <typename T> constexpr int PARTS = sizeof(T) == 4 ? 3 : 1;
+
+// rows of a [32 n][DP] bf16 tile in LDS, 16-byte chunks
+template <int DP> struct Tile {
+    static constexpr int CH = 8;                       // elements per chunk
     static constexpr int CPR = DP / CH;                // chunks per row
     static __device__ __forceinline__ int swizzle(int chunk, int row) {
-        if constexpr (sizeof(T) == 2) {
-            if constexpr (CPR == 4) return chunk ^ ((row >> 2) & 3);
-            else if constexpr (CPR == 8) return chunk ^ (((row & 2) << 1) | ((row & 4) >> 1) | ((row >> 3) & 1));
-            else if constexpr (CPR == 12) { const int s = chunk + ((row >> 2) & 3); return s >= 12 ? s - 12 : s; }
-            else return chunk ^ (((row & 3) << 2) | ((row >> 2) & 3));
-        } else {
-            if constexpr (CPR == 16 || CPR == 32) return chunk ^ (row & 15);
-            else return chunk ^ ((row >> 1) & 7);
-        }
+        if constexpr (CPR == 4) return chunk ^ ((row >> 2) & 3);
+        else if constexpr (CPR == 8) return chunk ^ (((row & 2) << 1) | ((row & 4) >> 1) | ((row >> 3) & 1));
+        else if constexpr (CPR == 12) { const int s = chunk + ((row >> 2) & 3); return s >= 12 ? s - 12 : s; }
+        else return chunk ^ (((row & 3) << 2) | ((row >> 2) & 3));
     }
     static __device__ __forceinline__ int unswizzle(int slot, int row) {
-        if constexpr (sizeof(T) == 2 && CPR == 12) { const int s = slot - ((row >> 2) & 3); return s < 0 ? s + 12 : s; }
+        if constexpr (CPR == 12) { const int s = slot - ((row >> 2) & 3); return s < 0 ? s + 12 : s; }
         else return swizzle(slot, row);
     }
     static __device__ __forceinline__ int at(int row, int chunk) { return (row * CPR + swizzle(chunk, row)) * CH; }
 };
 
-template <typename T, int DP> struct Mma;
+// an fp32 number as h + m + l, each of 8 bits; the parts of two numbers packed
+__device__ __forceinline__ unsigned upper_halves(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+__device__ __forceinline__ void three_parts(float x, float y, unsigned (&out)[3]) {
+    const unsigned xh = __float_as_uint(x) & 0xffff0000u, yh = __float_as_uint(y) & 0xffff0000u;
+    const float xr = x - __uint_as_float(xh), yr = y - __uint_as_float(yh);
+    const unsigned xm = __float_as_uint(xr) & 0xffff0000u, ym = __float_as_uint(yr) & 0xffff0000u;
+    out[0] = upper_halves(xh, yh);
+    out[1] = upper_halves(xm, ym);
+    out[2] = upper_halves(__float_as_uint(xr - __uint_as_float(xm)), __float_as_uint(yr - __uint_as_float(ym)));
+}
 
-template <int DP> struct Mma<__bf16, DP> {
+template <typename T> struct Out;
+template <> struct Out<__bf16> {
     typedef __bf16 T;
-    typedef Tile<T, DP> L;
-    static constexpr int DB = DP / 32;
-    struct Frag { bf16x8 f[DP / 16]; };
-    static __device__ __forceinline__ void load(Frag& x, const T* row, bool valid, int D, float sign) {
-        const int half = (threadIdx.x >> 5) & 1;
-#pragma unroll
-        for (int i = 0; i < DP / 16; i++) {
-            u32x4 v = {};
-            if (valid && 16 * i + 8 * half < D) v = *reinterpret_cast<const u32x4*>(row + 16 * i + 8 * half);
-            x.f[i] = __builtin_bit_cast(bf16x8, v ^ (sign < 0.f ? 0x80008000u : 0u));
-        }
-    }
-    // acc[c] = rows r0 .. r0+31 of `t` times the stationary columns of block c
-    template <int CB> static __device__ __forceinline__ void dots(f32x16 (&acc)[CB], const T* t, int r0, const Frag (&x)[CB]) {
-        const int half = (threadIdx.x >> 5) & 1, row = r0 + (threadIdx.x & 31);
-#pragma unroll
-        for (int c = 0; c < CB; c++) acc[c] = f32x16{};
-#pragma unroll
-        for (int i = 0; i < DP / 16; i++) {
-            const bf16x8 a = *reinterpret_cast<const bf16x8*>(t + L::at(row, 2 * i + half));
-#pragma unroll
-            for (int c = 0; c < CB; c++) acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, x[c].f[i], acc[c], 0, 0, 0);
-        }
-    }
-    // a[c][db][d][col] += sum_row t[r0 + row][32 db + d] p[c][row][col];  sums[c] (where given) += the p that were multiplied, half a column each
-    template <int CB> static __device__ __forceinline__ void adds(f32x16 (&a)[CB][DB], const T* t, int r0, const f32x16 (&p)[CB], float* sums = nullptr) {
-        const int lane = threadIdx.x & 63, i = lane & 15, half = lane >> 5, cg = (lane >> 4) & 1;
-#pragma unroll
-        for (int s = 0; s < 2; s++) {
-            bf16x8 b[CB];
-#pragma unroll
-            for (int c = 0; c < CB; c++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) b[c][j] = (__bf16)p[c][8 * s + j];
-            if (sums) {
-                const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
-#pragma unroll
-                for (int c = 0; c < CB; c++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) sums[c] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{b[c][2 * j], b[c][2 * j + 1]}, one, sums[c], false);
-            }
-#pragma unroll
-            for (int db = 0; db < DB; db++) {
-                bf16x4 h[2];
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const int row = r0 + 16 * s + 8 * u + 4 * half + (i >> 2);
-                    const T* at = t + L::at(row, 4 * db + 2 * cg + ((i & 3) >> 1)) + 4 * (i & 1);
-                    h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)at);
-                }
-                const bf16x8 w = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                for (int c = 0; c < CB; c++) a[c][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, b[c], a[c][db], 0, 0, 0);
-            }
-        }
-    }
     static __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
         const bf16x4 v = {(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
         *reinterpret_cast<bf16x4*>(p) = v;
@@ -189,67 +142,8 @@ template <int DP> struct Mma<__bf16, DP> {
         store4(p, a - (float)(__bf16)a, b - (float)(__bf16)b, c - (float)(__bf16)c, d - (float)(__bf16)d);
     }
 };
-
-template <int DP> struct Mma<float, DP> {
+template <> struct Out<float> {
     typedef float T;
-    typedef Tile<T, DP> L;
-    static constexpr int DB = DP / 32;
-    struct Frag { f32x4 f[DP / 8]; };
-    static __device__ __forceinline__ void load(Frag& x, const T* row, bool valid, int D, float sign) {
-        const int half = (threadIdx.x >> 5) & 1;
-#pragma unroll
-        for (int i = 0; i < DP / 8; i++) {
-            u32x4 v = {};
-            if (valid && 8 * i + 4 * half < D) v = *reinterpret_cast<const u32x4*>(row + 8 * i + 4 * half);
-            x.f[i] = __builtin_bit_cast(f32x4, v ^ (sign < 0.f ? 0x80000000u : 0u));
-        }
-    }
-    template <int CB> static __device__ __forceinline__ void dots(f32x16 (&acc)[CB], const T* t, int r0, const Frag (&x)[CB]) {
-        const int half = (threadIdx.x >> 5) & 1, row = r0 + (threadIdx.x & 31);
-#pragma unroll
-        for (int c = 0; c < CB; c++) acc[c] = f32x16{};
-#pragma unroll
-        for (int i = 0; i < DP / 8; i++) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(t + L::at(row, 2 * i + half));
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-                for (int c = 0; c < CB; c++) acc[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], x[c].f[i][j], acc[c], 0, 0, 0);
-        }
-    }
-    template <int CB> static __device__ __forceinline__ void adds(f32x16 (&a)[CB][DB], const T* t, int r0, const f32x16 (&p)[CB], float* = nullptr) {
-        const int half = (threadIdx.x >> 5) & 1, l31 = threadIdx.x & 31;
-        if constexpr (L::CPR == 16 || L::CPR == 32) {
-            // the swizzle of row 8 i + 4 half + j is j + 4 half in the low three chunk bits and i & 1 in the fourth, which only trades
-            // neighbouring 32-channel blocks: 4 lane addresses, everything else is a constant
-            const T* base[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) base[j] = t + (r0 + 4 * half + j) * DP + 4 * ((l31 >> 2) ^ (4 * half + j)) + (l31 & 3);
-#pragma unroll
-            for (int r = 0; r < 16; r++)
-#pragma unroll
-                for (int db = 0; db < DB; db++) {
-                    const float w = base[r & 3][8 * (r >> 2) * DP + 32 * (db ^ ((r >> 2) & 1))];
-#pragma unroll
-                    for (int c = 0; c < CB; c++) a[c][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(w, p[c][r], a[c][db], 0, 0, 0);
-                }
-        } else {
-            // rows 8 i + 4 half + j swizzle by (j >> 1) + 2 half and, every other i, by 4: 8 lane addresses
-            const T* base[2][4];
-#pragma unroll
-            for (int e = 0; e < 2; e++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) base[e][j] = t + (r0 + 4 * half + j) * DP + 4 * ((l31 >> 2) ^ ((j >> 1) + 2 * half + 4 * e)) + (l31 & 3);
-#pragma unroll
-            for (int r = 0; r < 16; r++)
-#pragma unroll
-                for (int db = 0; db < DB; db++) {
-                    const float w = base[(r >> 2) & 1][r & 3][8 * (r >> 2) * DP + 32 * db];
-#pragma unroll
-                    for (int c = 0; c < CB; c++) a[c][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(w, p[c][r], a[c][db], 0, 0, 0);
-                }
-        }
-    }
     static __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
         const f32x4 v = {a, b, c, d};
         *reinterpret_cast<f32x4*>(p) = v;
@@ -263,6 +157,96 @@ template <int DP> struct Mma<float, DP> {
         }
     }
     static __device__ __forceinline__ void store_low(T*, float, float, float, float) {}
+};
+
+// PS: elements between the planes of a tile (its parts, one [rows][DP] image each)
+template <typename T, int DP, int PS> struct Mma {
+    typedef Tile<DP> L;
+    static constexpr int DB = DP / 32, NP = PARTS<T>;
+    struct Frag { bf16x8 f[NP][DP / 16]; };
+    // the parts' products that count, the small ones first: (part of x, part of y)
+    static constexpr int PAIRS = NP == 1 ? 1 : 6;
+    static constexpr int PX[6] = {NP == 1 ? 0 : 2, 1, 0, 1, 0, 0}, PY[6] = {0, 1, 2, 0, 1, 0};
+    static __device__ __forceinline__ void load(Frag& x, const __bf16* row, bool valid, int D, float sign) {
+        const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+        for (int p = 0; p < NP; p++)
+#pragma unroll
+            for (int i = 0; i < DP / 16; i++) {
+                u32x4 v = {};
+                if (valid && 16 * i + 8 * half < D) v = *reinterpret_cast<const u32x4*>(row + p * D + 16 * i + 8 * half);
+                x.f[p][i] = __builtin_bit_cast(bf16x8, v ^ (sign < 0.f ? 0x80008000u : 0u));
+            }
+    }
+    // acc[c] = rows r0 .. r0+31 of `t` times the stationary columns of block c
+    template <int CB> static __device__ __forceinline__ void dots(f32x16 (&acc)[CB], const __bf16* t, int r0, const Frag (&x)[CB]) {
+        const int half = (threadIdx.x >> 5) & 1, row = r0 + (threadIdx.x & 31);
+#pragma unroll
+        for (int c = 0; c < CB; c++) acc[c] = f32x16{};
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++) {
+            bf16x8 a[NP];
+#pragma unroll
+            for (int p = 0; p < NP; p++) a[p] = *reinterpret_cast<const bf16x8*>(t + p * PS + L::at(row, 2 * i + half));
+#pragma unroll
+            for (int y = 0; y < PAIRS; y++)
+#pragma unroll
+                for (int c = 0; c < CB; c++) acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[PX[y]], x[c].f[PY[y]][i], acc[c], 0, 0, 0);
+        }
+    }
+    // a[c][db][d][col] += sum_row t[r0 + row][32 db + d] p[c][row][col];  bf16: sums[c] (where given) += the p that were multiplied, half a
+    // column each
+    template <int CB> static __device__ __forceinline__ void adds(f32x16 (&a)[CB][DB], const __bf16* t, int r0, const f32x16 (&p)[CB], float* sums = nullptr) {
+        const int lane = threadIdx.x & 63, i = lane & 15, half = lane >> 5, cg = (lane >> 4) & 1;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            bf16x8 b[CB][NP];
+#pragma unroll
+            for (int c = 0; c < CB; c++) {
+                if constexpr (NP == 1) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) b[c][0][j] = (__bf16)p[c][8 * s + j];
+                } else {
+                    u32x4 parts[3];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        unsigned w[3];
+                        three_parts(p[c][8 * s + 2 * j], p[c][8 * s + 2 * j + 1], w);
+#pragma unroll
+                        for (int k = 0; k < 3; k++) parts[k][j] = w[k];
+                    }
+#pragma unroll
+                    for (int k = 0; k < NP; k++) b[c][k] = __builtin_bit_cast(bf16x8, parts[k]);
+                }
+            }
+            if (NP == 1 && sums) {
+                const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+                for (int c = 0; c < CB; c++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) sums[c] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{b[c][0][2 * j], b[c][0][2 * j + 1]}, one, sums[c], false);
+            }
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                bf16x8 w[NP];
+#pragma unroll
+                for (int k = 0; k < NP; k++) {
+                    bf16x4 h[2];
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const int row = r0 + 16 * s + 8 * u + 4 * half + (i >> 2);
+                        const __bf16* at = t + k * PS + L::at(row, 4 * db + 2 * cg + ((i & 3) >> 1)) + 4 * (i & 1);
+                        h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)at);
+                    }
+                    w[k] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+#pragma unroll
+                for (int y = 0; y < PAIRS; y++)
+#pragma unroll
+                    for (int c = 0; c < CB; c++) a[c][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[PX[y]], b[c][PY[y]], a[c][db], 0, 0, 0);
+            }
+        }
+    }
 };
 
 // rows of one head in global memory: row r is token r / G (of stride ts) and head r % G (of stride hs) behind `base`
@@ -300,10 +284,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p) {
 // moves rows r0 .. r0+N-1 of one head into an LDS tile; on[]: one bit per row, a clear one gives a row of zeros.  The lanes' offsets behind
 // the tile's first row are the same for every tile (tokens of one head, or a tile of a whole number of tokens), so they are kept; the
 // tile's own place is a 64-bit address.  The host has checked that a tile spans less than 2^31 bytes.
-template <typename T, int DP, int N, int WAVES> struct Loader {
-    typedef Tile<T, DP> L;
-    static constexpr int PIECES = N * L::CPR / 64, NP = PIECES / WAVES;
-    static_assert(PIECES % WAVES == 0, "every wavefront moves the same number of pieces");
+template <int DP, int N, int WAVES, int NPARTS> struct Loader {
+    typedef Tile<DP> L;
+    static constexpr int PIECES = N * L::CPR / 64, NP = (PIECES + WAVES - 1) / WAVES;
     Rows src;
     int D, wave;
     unsigned off[NP];
@@ -326,7 +309,7 @@ template <typename T, int DP, int N, int WAVES> struct Loader {
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         place_pieces(0);
     }
-    __device__ __forceinline__ void issue(T* lds, int r0, const unsigned (&on)[N / 32]) {
+    __device__ __forceinline__ void issue(__bf16* lds, int r0, const unsigned (&on)[N / 32]) {
         if (src.G > 1 && N % src.G) place_pieces(r0);
         const __amdgpu_buffer_rsrc_t rsrc = buffer(src.base + (src.G == 1 ? r0 : r0 / src.G) * src.ts);
         unsigned all = 0xffffffffu;
@@ -335,7 +318,10 @@ template <typename T, int DP, int N, int WAVES> struct Loader {
         const unsigned at = __builtin_amdgcn_readfirstlane(lds_address(lds));
         if (all == 0xffffffffu) {
 #pragma unroll
-            for (int i = 0; i < NP; i++) to_lds16(off[i], rsrc, at + (wave + WAVES * i) * 1024u);
+            for (int p = 0; p < NPARTS; p++)
+#pragma unroll
+                for (int i = 0; i < NP; i++)
+                    if (wave + WAVES * i < PIECES) to_lds16(off[i] + 2u * p * D, rsrc, at + 2u * p * N * DP + (wave + WAVES * i) * 1024u);
         } else {
 #pragma unroll
             for (int i = 0; i < NP; i++) {
@@ -343,7 +329,10 @@ template <typename T, int DP, int N, int WAVES> struct Loader {
                 unsigned word = on[0];
 #pragma unroll
                 for (int j = 1; j < N / 32; j++) word = (row >> 5) == j ? on[j] : word;
-                to_lds16((word >> (row & 31)) & 1 ? off[i] : OUT_OF_RANGE, rsrc, at + (wave + WAVES * i) * 1024u);
+                const unsigned o = (word >> (row & 31)) & 1 ? off[i] : OUT_OF_RANGE;
+#pragma unroll
+                for (int p = 0; p < NPARTS; p++)
+                    if (wave + WAVES * i < PIECES) to_lds16(o + 2u * p * D, rsrc, at + 2u * p * N * DP + (wave + WAVES * i) * 1024u);
             }
         }
     }
@@ -407,20 +396,21 @@ __device__ __forceinline__ bool place(int BH, int per_head, int& bh, int& blk) {
 }
 inline unsigned placed_blocks(int BH, int per_head) { return (unsigned)((BH >= 16 ? (BH + 7) / 8 * 8 : BH) * per_head); }
 
-// SHARE / OWN, tile rows, buffers
-template <typename T, int DP, bool SHARE> struct Shape {
-    static constexpr int WAVES = 4, THREADS = 256;
-    static constexpr int N = SHARE ? 128 : (sizeof(T) == 2 ? 64 : 32);      // rows per tile
-    static constexpr int COLS = SHARE ? 32 : 128;                           // columns per workgroup (of one block per wavefront)
-    static constexpr int BYTES = 2 * N * DP * (int)sizeof(T);               // the two tiles
+// SH: wavefronts that share their columns (1: OWN); tile rows, buffers
+template <typename T, int DP, int SH> struct Shape {
+    static constexpr int WAVES = 4, THREADS = 256, NP = PARTS<T>;
+    static constexpr int N = SH > 1 ? 32 * SH : NP == 1 ? 64 : 32;          // rows per tile
+    static constexpr int COLS = 128 / SH;                                   // columns per workgroup (of one block per wavefront)
+    static constexpr int BYTES = 2 * NP * N * DP * 2;                       // the two tiles
     static constexpr int NBUF = 2 * BYTES <= 81920 ? 2 : 1;
     // column blocks of a wavefront in the forward pass.  Two: every LDS read feeds two matrix instructions, and the products of one block run
     // beside the exponentials of the other (bf16, 64 channels: 173 -> 160 us for 7686 x 4097 x 16 heads); more would not fit the registers.
-    static constexpr int CB = !SHARE && sizeof(T) == 2 && DP <= 64 ? 2 : 1;
+    static constexpr int CB = SH == 1 && NP == 1 && DP <= 64 ? 2 : 1;
     // wavefronts per SIMD that the registers are bounded for
-    static constexpr int FWD_OCC = SHARE ? (DP > 64 ? 1 : 2) : sizeof(T) == 2 ? 2 : DP == 32 ? 3 : DP == 64 ? 2 : 1;
+    static constexpr int FWD_OCC = NP == 1 && SH == 1 ? 2 : DP > 64 ? 1 : 2;
     static constexpr int GRAD_OCC = DP > 64 ? 1 : 2;
 };
+template <typename T> constexpr int SHARED = PARTS<T> == 1 ? 4 : 2;         // SH where the columns are too few for OWN
 
 // walks the tiles of [key_beg, key_end) that hold a key: move(t, buf, on) starts the loads of the tile at key win + t N, work(buf, on) uses it
 template <typename S, typename Move, typename Work>
@@ -462,12 +452,17 @@ __device__ __forceinline__ void walk_keys(unsigned* words, const unsigned char* 
     }
 }
 
+// (a loop over on[] would keep it in memory)
+template <int SH> __device__ __forceinline__ unsigned one_of(const unsigned* on, int i) {
+    if constexpr (SH == 2) return i == 0 ? on[0] : on[1];
+    else return i == 0 ? on[0] : i == 1 ? on[1] : i == 2 ? on[2] : on[3];
+}
 // factor of a partial softmax with maximum m and sum l in one with maximum `top`.  m is -inf where there was no key (l is 0: nothing to add) or
 // where every score was NaN (l is NaN, and so is the result).
 __device__ __forceinline__ float share_of(float m, float l, float top) { return m == -INFINITY ? l : __builtin_amdgcn_exp2f(m - top); }
 
-// joins the 4 wavefronts' partials jo [4][ROWS][DP], jm [4][ROWS][maximum, sum] of rows row0 .. into the result, or into this split's partial
-template <typename T, int DP, int ROWS>
+// joins SHARES wavefronts' partials jo [SHARES][ROWS][DP], jm [SHARES][ROWS][maximum, sum] of rows row0 .. into the result, or into this split's partial
+template <typename T, int DP, int ROWS, int SHARES>
 __device__ __forceinline__ void join_waves(const Args& a, const float* jo, const float* jm, int row0, int split, int bh) {
     const int R = a.Nq * a.G, H = a.Hk * a.G, b = bh / a.Hk, hk = bh - b * a.Hk;
     for (int idx = threadIdx.x; idx < ROWS * (DP / 4); idx += 256) {
@@ -475,10 +470,10 @@ __device__ __forceinline__ void join_waves(const Args& a, const float* jo, const
         if (rr >= R || d >= a.D) continue;
         float mt = -INFINITY, lt = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) mt = fmaxf(mt, jm[(i * ROWS + row) * 2]);
+        for (int i = 0; i < SHARES; i++) mt = fmaxf(mt, jm[(i * ROWS + row) * 2]);
         f32x4 sum = {};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < SHARES; i++) {
             const float* his = jm + (i * ROWS + row) * 2;
             const float f = share_of(his[0], his[1], mt);
             lt += f * his[1];
@@ -495,21 +490,22 @@ __device__ __forceinline__ void join_waves(const Args& a, const float* jo, const
             const int n = rr / a.G, h = hk * a.G + rr - n * a.G;
             sum *= lt == 0.f ? 0.f : 1.f / lt;
             const long at = (((long)b * a.Nq + n) * H + h) * a.D + d;
-            Mma<T, DP>::store4(static_cast<T*>(a.o) + at, sum[0], sum[1], sum[2], sum[3]);
-            if (a.o_low) Mma<T, DP>::store_low(static_cast<T*>(a.o_low) + at, sum[0], sum[1], sum[2], sum[3]);
+            Out<T>::store4(static_cast<T*>(a.o) + at, sum[0], sum[1], sum[2], sum[3]);
+            if (a.o_low) Out<T>::store_low(static_cast<T*>(a.o_low) + at, sum[0], sum[1], sum[2], sum[3]);
             if (a.lse && d == 0) a.lse[(long)bh * R + rr] = lt == 0.f ? INFINITY : mt + __builtin_amdgcn_logf(lt);
         }
     }
 }
 
-template <typename T, int DP, bool SHARE>
-__global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_kernel(const Args a) {
-    typedef Shape<T, DP, SHARE> S;
-    typedef Mma<T, DP> M;
+template <typename T, int DP, int SH>
+__global__ __launch_bounds__(256, (Shape<T, DP, SH>::FWD_OCC)) void forward_kernel(const Args a) {
+    typedef Shape<T, DP, SH> S;
+    typedef Mma<T, DP, S::N * DP> M;
+    constexpr bool SHARE = SH > 1;
     constexpr int WAVES = S::WAVES, N = S::N, DB = M::DB, CB = S::CB, COLS = S::COLS * CB;
-    __shared__ __attribute__((aligned(16))) T tile[S::NBUF][2][N * DP];
+    __shared__ __attribute__((aligned(16))) __bf16 tile[S::NBUF][2][S::NP * N * DP];
     __shared__ unsigned words[2 * N];
-    __shared__ float jm[SHARE ? WAVES * 32 * 2 : 1];
+    __shared__ float jm[SHARE ? 2 * SH * COLS : 1];
 
     const int lane = threadIdx.x & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -518,9 +514,9 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_k
     if (!place(a.BH, row_blocks * a.nsplit, bh, blk)) return;
     const int split = SHARE ? blk / row_blocks : 0, rb = blk - split * row_blocks;
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int r_wave = rb * COLS + (SHARE ? 0 : 32 * CB * wave);
+    const int r_wave = rb * COLS + 32 * CB * (wave / SH);
     const bool idle = r_wave >= R;                           // a wavefront without rows only moves tiles
-    const Rows qr = rows_of<T>(a.q, a.qs, b, hk * a.G, a.G);
+    const Rows qr = rows_of<__bf16>(a.q, a.qs, b, hk * a.G, a.G);
     const unsigned char* mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
     const int key_beg = SHARE ? split * a.keys_per_split : 0, key_end = SHARE ? min(a.Nk, key_beg + a.keys_per_split) : a.Nk;
     // a negative scale goes into q's sign: the maximum of s is the maximum of c s; c > 0 keeps -inf * c = -inf for masked keys at scale 0
@@ -532,13 +528,13 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_k
 #pragma unroll
     for (int x = 0; x < CB; x++) {
         const int r = r_wave + 32 * x + l31;
-        M::load(q[x], reinterpret_cast<const T*>(qr.row(r < R ? r : 0)), r < R, a.D, a.scale);
+        M::load(q[x], reinterpret_cast<const __bf16*>(qr.row(r < R ? r : 0)), r < R, a.D, a.scale);
 #pragma unroll
         for (int i = 0; i < DB; i++) o[x][i] = f32x16{};
         m[x] = -INFINITY;
         l[x] = 0.f;
     }
-    Loader<T, DP, N, WAVES> keys(rows_of<T>(a.k, a.ks, b, hk, 1), a.D), values(rows_of<T>(a.v, a.vs, b, hk, 1), a.D);
+    Loader<DP, N, WAVES, S::NP> keys(rows_of<__bf16>(a.k, a.ks, b, hk, 1), a.D), values(rows_of<__bf16>(a.v, a.vs, b, hk, 1), a.D);
 
     // `blocks` 32-key blocks from row r0 of the tile
     auto products = [&](auto blocks, int buf, int r0, const unsigned* on) {
@@ -609,8 +605,8 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_k
                  [&](int buf, const unsigned (&on)[N / 32]) {
                      if (idle) return;
                      if constexpr (SHARE) {
-                         const unsigned mine = wave == 0 ? on[0] : wave == 1 ? on[1] : wave == 2 ? on[2] : on[3];
-                         if (mine) products(std::integral_constant<int, 1>{}, buf, 32 * wave, &mine);
+                         const unsigned mine = one_of<SH>(on, wave % SH);
+                         if (mine) products(std::integral_constant<int, 1>{}, buf, 32 * (wave % SH), &mine);
                      } else {
                          products(std::integral_constant<int, N / 32>{}, buf, 0, on);
                      }
@@ -620,21 +616,22 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_k
 
     const int H = a.Hk * a.G;
     if constexpr (SHARE) {                                   // join the wavefronts' shares of the keys
-        float* jo = reinterpret_cast<float*>(&tile[0][0][0]);        // [WAVES][32 rows][DP]
-        static_assert(sizeof(tile) >= WAVES * 32 * DP * sizeof(float), "the joined partials fit the tiles");
+        float* jo = reinterpret_cast<float*>(&tile[0][0][0]);        // [SH][COLS rows][DP]
+        const int share = wave % SH, mine = 32 * (wave / SH) + l31;
+        static_assert(sizeof(tile) >= SH * COLS * DP * sizeof(float), "the joined partials fit the tiles");
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < DB; i++)
 #pragma unroll
             for (int g = 0; g < 4; g++)
-                *reinterpret_cast<f32x4*>(jo + (wave * 32 + l31) * DP + 32 * i + 8 * g + 4 * half) =
+                *reinterpret_cast<f32x4*>(jo + (share * COLS + mine) * DP + 32 * i + 8 * g + 4 * half) =
                     f32x4{o[0][i][4 * g], o[0][i][4 * g + 1], o[0][i][4 * g + 2], o[0][i][4 * g + 3]};
         if (half == 0) {
-            jm[(wave * 32 + l31) * 2] = m[0];
-            jm[(wave * 32 + l31) * 2 + 1] = l[0];
+            jm[(share * COLS + mine) * 2] = m[0];
+            jm[(share * COLS + mine) * 2 + 1] = l[0];
         }
         __syncthreads();
-        join_waves<T, DP, 32>(a, jo, jm, rb * 32, split, bh);
+        join_waves<T, DP, COLS, SH>(a, jo, jm, rb * COLS, split, bh);
     } else {
 #pragma unroll
         for (int x = 0; x < CB; x++) {
@@ -643,7 +640,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::FWD_OCC)) void forward_k
             const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
             T* low = a.o_low ? static_cast<T*>(a.o_low) + at : nullptr;
 #pragma unroll
-            for (int i = 0; i < DB; i++) M::store_column(static_cast<T*>(a.o) + at, low, i, a.D, r < R, o[x][i] * inv);
+            for (int i = 0; i < DB; i++) Out<T>::store_column(static_cast<T*>(a.o) + at, low, i, a.D, r < R, o[x][i] * inv);
             if (a.lse && half == 0 && r < R) a.lse[(long)bh * R + r] = l[x] == 0.f ? INFINITY : m[x] + __builtin_amdgcn_logf(l[x]);
         }
     }
@@ -792,7 +789,7 @@ template <typename T, int DP, int ROWS> __global__ __launch_bounds__(256, 2) voi
         }
     }
     __syncthreads();
-    join_waves<T, DP, ROWS>(a, jo, jm, 0, split, bh);
+    join_waves<T, DP, ROWS, 4>(a, jo, jm, 0, split, bh);
 }
 
 // joins the splits: a thread per 4 channels of a row
@@ -815,8 +812,8 @@ template <typename T> __global__ __launch_bounds__(256) void join_kernel(const A
     const int n = r / a.G, h = hk * a.G + r - n * a.G;
     sum *= lt == 0.f ? 0.f : 1.f / lt;
     const long at = (((long)b * a.Nq + n) * H + h) * a.D + d;
-    Mma<T, 32>::store4(static_cast<T*>(a.o) + at, sum[0], sum[1], sum[2], sum[3]);
-    if (a.o_low) Mma<T, 32>::store_low(static_cast<T*>(a.o_low) + at, sum[0], sum[1], sum[2], sum[3]);
+    Out<T>::store4(static_cast<T*>(a.o) + at, sum[0], sum[1], sum[2], sum[3]);
+    if (a.o_low) Out<T>::store_low(static_cast<T*>(a.o_low) + at, sum[0], sum[1], sum[2], sum[3]);
     if (a.lse && d == 0) a.lse[row] = lt == 0.f ? INFINITY : mt + __builtin_amdgcn_logf(lt);
 }
 
@@ -838,7 +835,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void delta_kerne
         const unsigned row = min(first + GROUPS * i, rows - 1);
         n[i] = row / (unsigned)H;
         h[i] = row - n[i] * H;
-        x[i] = *reinterpret_cast<const tx8*>(static_cast<const T*>(a.go) + b * a.gs[0] + n[i] * a.gs[1] + h[i] * a.gs[2] + d);
+        x[i] = *reinterpret_cast<const tx8*>(static_cast<const T*>(a.dgo) + b * a.dgs[0] + n[i] * a.dgs[1] + h[i] * a.dgs[2] + d);
         const long at = ((long)b * rows + row) * a.D + d;
         y[i] = *reinterpret_cast<const tx8*>(static_cast<const T*>(a.o_in) + at);
         z[i] = tx8{};
@@ -859,18 +856,19 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void delta_kerne
     }
 }
 
-template <typename T, int DP, bool SHARE> struct GradLds {
-    typedef Shape<T, DP, SHARE> S;
-    T tile[S::NBUF][2][S::N * DP];
+template <typename T, int DP, int SH> struct GradLds {
+    typedef Shape<T, DP, SH> S;
+    __bf16 tile[S::NBUF][2][S::NP * S::N * DP];
     float rowstat[S::NBUF][2][S::N < 64 ? 64 : S::N];        // log-sum-exp and delta of the streamed rows
     unsigned words[2 * S::N];
 };
 
 // KV: stationary keys, streamed query rows (gk, gv); otherwise stationary query rows, streamed keys (gq)
-template <typename T, int DP, bool KV, bool SHARE>
-__device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, SHARE>& lds, int bh, int blk) {
-    typedef Shape<T, DP, SHARE> S;
-    typedef Mma<T, DP> M;
+template <typename T, int DP, bool KV, int SH>
+__device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, SH>& lds, int bh, int blk) {
+    typedef Shape<T, DP, SH> S;
+    typedef Mma<T, DP, S::N * DP> M;
+    constexpr bool SHARE = SH > 1;
     constexpr int WAVES = S::WAVES, N = S::N, DB = M::DB, NRB = SHARE ? 1 : N / 32, W = N / 32;
     auto& tile = lds.tile;
     auto& rowstat = lds.rowstat;
@@ -879,12 +877,12 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int R = a.Nq * a.G, C = KV ? a.Nk : R;
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int col_wave = blk * S::COLS + (SHARE ? 0 : 32 * wave), col = col_wave + l31;
+    const int col_wave = blk * S::COLS + 32 * (wave / SH), col = col_wave + l31;
     const unsigned char* mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
     const bool valid = col < C && (!KV || !mask || mask[col]);
     const bool idle = !__any(valid);                         // a wavefront without columns only moves tiles
-    const Rows qr = rows_of<T>(a.q, a.qs, b, hk * a.G, a.G), gr = rows_of<T>(a.go, a.gs, b, hk * a.G, a.G);
-    const Rows kr = rows_of<T>(a.k, a.ks, b, hk, 1), vr = rows_of<T>(a.v, a.vs, b, hk, 1);
+    const Rows qr = rows_of<__bf16>(a.q, a.qs, b, hk * a.G, a.G), gr = rows_of<__bf16>(a.go, a.gs, b, hk * a.G, a.G);
+    const Rows kr = rows_of<__bf16>(a.k, a.ks, b, hk, 1), vr = rows_of<__bf16>(a.v, a.vs, b, hk, 1);
     const float* lse = a.lse + (long)bh * R;
     const float* delta = a.delta + (long)bh * R;
     const float c = a.scale * LOG2E;
@@ -895,8 +893,8 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
     typename M::Frag f1[1], f2[1];
     {
         const int at = valid ? col : 0;
-        M::load(f1[0], reinterpret_cast<const T*>((KV ? kr : qr).row(at)), valid, a.D, 1.f);
-        M::load(f2[0], reinterpret_cast<const T*>((KV ? vr : gr).row(at)), valid, a.D, 1.f);
+        M::load(f1[0], reinterpret_cast<const __bf16*>((KV ? kr : qr).row(at)), valid, a.D, 1.f);
+        M::load(f2[0], reinterpret_cast<const __bf16*>((KV ? vr : gr).row(at)), valid, a.D, 1.f);
     }
     const float col_lse = !KV && valid ? lse[col] : INFINITY, col_delta = !KV && valid ? delta[col] : 0.f;
 
@@ -926,7 +924,7 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
         M::template adds<1>(acc1, tile[buf][0], r0, dd);
     };
 
-    Loader<T, DP, N, WAVES> first(KV ? qr : kr, a.D), second(KV ? gr : vr, a.D);
+    Loader<DP, N, WAVES, S::NP> first(KV ? qr : kr, a.D), second(KV ? gr : vr, a.D);
     if constexpr (KV) {
         if (__syncthreads_or(valid)) {
             auto issue = [&](int r0, int buf) {
@@ -949,7 +947,7 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
             auto products = [&](int buf, int r0) {
                 if (idle) return;
                 if constexpr (SHARE) {
-                    if (r0 + 32 * wave < R) block(buf, 32 * wave, std::false_type{}, 0u);
+                    if (r0 + 32 * (wave % SH) < R) block(buf, 32 * (wave % SH), std::false_type{}, 0u);
                 } else if (NRB == 1 || r0 + N - 32 < R) {
 #pragma unroll
                     for (int rb = 0; rb < NRB; rb++) block(buf, 32 * rb, std::false_type{}, 0u);
@@ -983,9 +981,9 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
                      [&](int buf, const unsigned (&on)[W]) {
                          if (idle) return;
                          if constexpr (SHARE) {
-                             const unsigned mine = wave == 0 ? on[0] : wave == 1 ? on[1] : wave == 2 ? on[2] : on[3];
-                             if (mine == 0xffffffffu) block(buf, 32 * wave, std::false_type{}, mine);
-                             else if (mine) block(buf, 32 * wave, std::true_type{}, mine);
+                             const unsigned mine = one_of<SH>(on, wave % SH);
+                             if (mine == 0xffffffffu) block(buf, 32 * (wave % SH), std::false_type{}, mine);
+                             else if (mine) block(buf, 32 * (wave % SH), std::true_type{}, mine);
                          } else {
                              unsigned all = 0xffffffffu;
 #pragma unroll
@@ -1005,8 +1003,10 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
     T* out1 = static_cast<T*>(KV ? a.gk : a.gq);
     T* out2 = static_cast<T*>(a.gv);
     if constexpr (SHARE) {                                   // add up the wavefronts' rows, in order
-        float* join = reinterpret_cast<float*>(&tile[0][0][0]);      // [WAVES][32 columns][DP]
-        static_assert(sizeof(lds.tile) >= WAVES * 32 * DP * sizeof(float), "the joined partials fit the tiles");
+        float* join = reinterpret_cast<float*>(&tile[0][0][0]);      // [SH][COLS columns][DP]
+        constexpr int COLS = S::COLS;
+        const int share = wave % SH, at_col = 32 * (wave / SH) + l31;
+        static_assert(sizeof(lds.tile) >= SH * COLS * DP * sizeof(float), "the joined partials fit the tiles");
 #pragma unroll
         for (int which = 0; which < (KV ? 2 : 1); which++) {
             T* out = which ? out2 : out1;
@@ -1017,15 +1017,15 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
                     const f32x16& x = which ? acc2[0][i] : acc1[0][i];
-                    *reinterpret_cast<f32x4*>(join + (wave * 32 + l31) * DP + 32 * i + 8 * g + 4 * half) = f32x4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
+                    *reinterpret_cast<f32x4*>(join + (share * COLS + at_col) * DP + 32 * i + 8 * g + 4 * half) = f32x4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
                 }
             __syncthreads();
-            for (int idx = threadIdx.x; idx < 32 * (DP / 4); idx += 256) {
-                const int row = idx / (DP / 4), d = 4 * (idx % (DP / 4)), cc = blk * 32 + row;
+            for (int idx = threadIdx.x; idx < COLS * (DP / 4); idx += 256) {
+                const int row = idx / (DP / 4), d = 4 * (idx % (DP / 4)), cc = blk * COLS + row;
                 if (cc >= C || d >= a.D) continue;
                 f32x4 sum = {};
 #pragma unroll
-                for (int w = 0; w < WAVES; w++) sum += *reinterpret_cast<const f32x4*>(join + (w * 32 + row) * DP + d);
+                for (int w = 0; w < SH; w++) sum += *reinterpret_cast<const f32x4*>(join + (w * COLS + row) * DP + d);
                 const float f = which ? 1.f : a.scale;
                 if (KV && mask && !mask[cc]) sum = f32x4{};
                 long at;
@@ -1034,7 +1034,7 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
                     const int n = cc / a.G;
                     at = (((long)b * a.Nq + n) * (a.Hk * a.G) + hk * a.G + cc - n * a.G) * a.D;
                 }
-                M::store4(out + at + d, sum[0] * f, sum[1] * f, sum[2] * f, sum[3] * f);
+                Out<T>::store4(out + at + d, sum[0] * f, sum[1] * f, sum[2] * f, sum[3] * f);
             }
         }
         return;
@@ -1052,21 +1052,21 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
         const float f = which ? 1.f : a.scale;
 #pragma unroll
         for (int i = 0; i < DB; i++)                         // a masked key gets zeros, whatever went through its column
-            M::store_column(out + at, nullptr, i, a.D, col < C, valid ? (which ? acc2[0][i] : acc1[0][i]) * f : f32x16{});
+            Out<T>::store_column(out + at, nullptr, i, a.D, col < C, valid ? (which ? acc2[0][i] : acc1[0][i]) * f : f32x16{});
     }
 }
 
 // Both gradients in one launch: the two kinds of workgroups of a head run next to each other, and the last, partly filled round of
 // workgroups is paid once (32 x 6 heads of 642 x 1025, bf16: two launches 142 us).
-template <typename T, int DP, bool SHARE>
-__global__ __launch_bounds__(256, (Shape<T, DP, SHARE>::GRAD_OCC)) void backward_kernel(const Args a) {
-    typedef Shape<T, DP, SHARE> S;
-    __shared__ __attribute__((aligned(16))) GradLds<T, DP, SHARE> lds;
+template <typename T, int DP, int SH>
+__global__ __launch_bounds__(256, (Shape<T, DP, SH>::GRAD_OCC)) void backward_kernel(const Args a) {
+    typedef Shape<T, DP, SH> S;
+    __shared__ __attribute__((aligned(16))) GradLds<T, DP, SH> lds;
     const int nkv = a.gk || a.gv ? (a.Nk + S::COLS - 1) / S::COLS : 0, nq = a.gq ? (a.Nq * a.G + S::COLS - 1) / S::COLS : 0;
     int bh, blk;
     if (!place(a.BH, nkv + nq, bh, blk)) return;
-    if (blk < nkv) gradient_columns<T, DP, true, SHARE>(a, lds, bh, blk);
-    else gradient_columns<T, DP, false, SHARE>(a, lds, bh, blk - nkv);
+    if (blk < nkv) gradient_columns<T, DP, true, SH>(a, lds, bh, blk);
+    else gradient_columns<T, DP, false, SH>(a, lds, bh, blk - nkv);
 }
 
 // ---- launch plan --------------------------------------------------------------------------------------------------------------------
@@ -1079,9 +1079,9 @@ constexpr int few_rows(int size) { return size == 4 ? 4 : 1; }
 constexpr int FEW_BLOCKS = 512;                              // workgroups to split the keys for: 1024 and more only make the join longer (32 x 6 x 1025 fp32 24.4 us, 512: 22.7)
 constexpr long SHARE_BELOW = 1024;                           // wavefronts of 32 columns; fewer leave SIMDs empty (256 CUs x 4)
 inline long wavefronts(const Args& a, int columns) { return (long)a.BH * ((columns + 31) / 32); }
-// two_blocks: a wavefront of the OWN kernel takes 64 columns (Shape::CB).
+// own_cols: columns of an OWN workgroup; shared: SHARED.
 // split: where even SHARE has too few workgroups, the keys are divided as long as each part keeps two tiles
-inline Plan forward_plan(const Args& a, bool two_blocks, int max_few, int few_keys) {
+inline Plan forward_plan(const Args& a, int own_cols, int shared, int max_few, int few_keys) {
     Plan p;
     const int R = a.Nq * a.G;
     p.few = R <= max_few;
@@ -1097,16 +1097,16 @@ inline Plan forward_plan(const Args& a, bool two_blocks, int max_few, int few_ke
     p.share = wavefronts(a, R) < SHARE_BELOW;
     p.nsplit = 1;
     p.keys_per_split = a.Nk;
-    const int cols = p.share ? 32 : two_blocks ? 256 : 128;
+    const int cols = p.share ? 128 / shared : own_cols, tile = 32 * shared;
     p.row_blocks = (R + cols - 1) / cols;
     if (p.share) {
-        const int tiles = (a.Nk + 127) / 128;
+        const int tiles = (a.Nk + tile - 1) / tile;
         const long blocks = (long)a.BH * p.row_blocks;
         int want = blocks >= 512 ? 1 : (int)(512 / blocks);
         if (want > tiles / 2) want = tiles / 2 > 0 ? tiles / 2 : 1;
         const int per = (tiles + want - 1) / want;
         p.nsplit = (tiles + per - 1) / per;
-        p.keys_per_split = per * 128;
+        p.keys_per_split = per * tile;
     }
     return p;
 }
@@ -1123,8 +1123,8 @@ template <typename T, int DP> void launch_forward(const Args& a, const Plan& p, 
             if (R == 2) hipLaunchKernelGGL((few_rows_kernel<T, DF, 2>), grid, dim3(256), 0, st, a);
             else hipLaunchKernelGGL((few_rows_kernel<T, DF, 4>), grid, dim3(256), 0, st, a);
         }
-    } else if (p.share) hipLaunchKernelGGL((forward_kernel<T, DP, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((forward_kernel<T, DP, false>), grid, dim3(256), 0, st, a);
+    } else if (p.share) hipLaunchKernelGGL((forward_kernel<T, DP, SHARED<T>>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((forward_kernel<T, DP, 1>), grid, dim3(256), 0, st, a);
     if (p.nsplit > 1) {
         const long n = (long)a.BH * a.Nq * a.G * (a.D / 4);
         hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
@@ -1137,10 +1137,10 @@ template <typename T, int DP> void launch_backward(const Args& a, hipStream_t st
     hipLaunchKernelGGL((delta_kernel<T, DP>), dim3((unsigned)(per_batch * (a.BH / a.Hk))), dim3(256), 0, st, a, per_batch);
     const int rows = a.gq ? R : 0, keys = a.gk || a.gv ? a.Nk : 0;
     const bool share = wavefronts(a, rows) + wavefronts(a, keys) < 2 * SHARE_BELOW;
-    const int cols = share ? 32 : 128;
+    const int cols = share ? 128 / SHARED<T> : 128;
     const dim3 grid(placed_blocks(a.BH, (rows + cols - 1) / cols + (keys + cols - 1) / cols));
-    if (share) hipLaunchKernelGGL((backward_kernel<T, DP, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((backward_kernel<T, DP, false>), grid, dim3(256), 0, st, a);
+    if (share) hipLaunchKernelGGL((backward_kernel<T, DP, SHARED<T>>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((backward_kernel<T, DP, 1>), grid, dim3(256), 0, st, a);
 }
 
 // instantiated in csrc/cross_attn_f32.hip and csrc/cross_attn_bf16.hip

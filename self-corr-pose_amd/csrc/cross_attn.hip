@@ -42,6 +42,7 @@ const char* bad_problem(const scp_cross_attn_params* p) {
 // a tile (at most 128 rows) is addressed with 31-bit byte offsets behind its first row; the tile's own place is a 64-bit address
 bool tile_too_wide(const scp_cross_attn_params* p, bool backward) {
     const long long size = p->dtype == SCP_DTYPE_F32 ? 4 : 2, lim = 1ll << 31, G = p->heads / p->kv_heads;
+    if (size == 4 && 130ll * p->heads * p->head_dim * 6 >= lim) return true;                 // a tile of the parts
     for (const long long* st : {p->k_stride, p->v_stride})
         if (st[1] < 0 || 128 * st[1] * size >= lim) return true;
     if (backward)
@@ -67,16 +68,80 @@ Args make_args(const scp_cross_attn_params* p) {
 Plan plan_of(const Args& a, int dtype) {
     const bool bf16 = dtype == SCP_DTYPE_BF16;
     const int few_keys = (bf16 ? 8 : 4) * 64 / (a.D <= 32 ? 4 : a.D <= 64 ? 8 : 16);                          // Few::KEYS
-    return scp_attn::forward_plan(a, bf16 && a.D <= 64, scp_attn::few_rows(bf16 ? 2 : 4), few_keys);
+    return scp_attn::forward_plan(a, bf16 && a.D <= 64 ? 256 : 128, bf16 ? scp_attn::SHARED<__bf16> : scp_attn::SHARED<float>, scp_attn::few_rows(bf16 ? 2 : 4),
+                                  few_keys);
 }
 size_t split_floats(const Args& a, const Plan& p) { return p.nsplit > 1 ? (size_t)p.nsplit * a.BH * a.Nq * a.G * (a.D + 2) : 0; }
+
+
+// fp32 tensors as three bf16 parts: dst [batch][tokens][heads][3][D]; a thread per 8 channels, 256 / lanes rows per workgroup
+struct Parts { const float* src[4]; __bf16* dst[4]; long st[4][3]; int tokens[4], heads[4]; unsigned first[5]; int batch, D; };
+constexpr int parts_rows(int D) { return 256 / (D <= 32 ? 4 : D <= 64 ? 8 : 16); }
+__global__ __launch_bounds__(256) void parts_kernel(const Parts a) {
+    int t = 0;
+#pragma unroll
+    for (int i = 1; i < 4; i++) t += blockIdx.x >= a.first[i];
+    const int lanes = 256 / parts_rows(a.D), d = 8 * (threadIdx.x % lanes);
+    const unsigned heads = a.heads[t], per = (unsigned)a.tokens[t] * heads;
+    const unsigned row = (blockIdx.x - a.first[t]) * (256 / lanes) + threadIdx.x / lanes;
+    if (row >= per * (unsigned)a.batch || d >= a.D) return;
+    const unsigned b = row / per, r = row - b * per, n = r / heads, h = r - n * heads;
+    const float* x = a.src[t] + b * a.st[t][0] + n * a.st[t][1] + h * a.st[t][2] + d;
+    const scp_attn::f32x4 lo = *reinterpret_cast<const scp_attn::f32x4*>(x), hi = *reinterpret_cast<const scp_attn::f32x4*>(x + 4);
+    scp_attn::u32x4 parts[3];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        unsigned w[3];
+        if (j < 2) scp_attn::three_parts(lo[2 * j], lo[2 * j + 1], w);
+        else scp_attn::three_parts(hi[2 * j - 4], hi[2 * j - 3], w);
+#pragma unroll
+        for (int k = 0; k < 3; k++) parts[k][j] = w[k];
+    }
+    __bf16* to = a.dst[t] + (long)row * 3 * a.D + d;
+#pragma unroll
+    for (int k = 0; k < 3; k++) *reinterpret_cast<scp_attn::u32x4*>(to + k * a.D) = parts[k];
+}
+// bytes of the parts of q (and g_out), k and v
+size_t parts_bytes(const scp_cross_attn_params* p, bool backward) {
+    if (p->dtype != SCP_DTYPE_F32) return 0;
+    return (size_t)p->batch * ((size_t)p->queries * p->heads * (backward ? 2 : 1) + 2 * (size_t)p->keys * p->kv_heads) * p->head_dim * 6;
+}
+// makes the parts at `to` and points the matrix kernels at them
+void make_parts(Args& a, const scp_cross_attn_params* p, bool backward, void* to, hipStream_t st) {
+    Parts c{};
+    const void** view[4] = {&a.q, &a.k, &a.v, &a.go};
+    long* strides[4] = {a.qs, a.ks, a.vs, a.gs};
+    __bf16* at = static_cast<__bf16*>(to);
+    c.batch = p->batch;
+    c.D = p->head_dim;
+    unsigned blocks = 0;
+    for (int t = 0; t < 4; t++) {
+        c.first[t] = t < 3 || backward ? blocks : ~0u;
+        if (t == 3 && !backward) break;
+        const bool keys = t == 1 || t == 2;
+        c.tokens[t] = keys ? p->keys : p->queries;
+        c.heads[t] = keys ? p->kv_heads : p->heads;
+        c.src[t] = static_cast<const float*>(*view[t]);
+        c.dst[t] = at;
+        for (int i = 0; i < 3; i++) c.st[t][i] = strides[t][i];
+        const long rows = (long)p->batch * c.tokens[t] * c.heads[t], row = 3l * p->head_dim;
+        blocks += (unsigned)((rows + parts_rows(c.D) - 1) / parts_rows(c.D));
+        *view[t] = at;
+        strides[t][2] = row;
+        strides[t][1] = row * c.heads[t];
+        strides[t][0] = strides[t][1] * c.tokens[t];
+        at += rows * row;
+    }
+    hipLaunchKernelGGL(parts_kernel, dim3(blocks), dim3(256), 0, st, c);
+}
 
 }  // namespace
 
 extern "C" size_t scp_cross_attention_forward_workspace(const scp_cross_attn_params* p) {
     if (bad_problem(p)) return 0;
     const Args a = make_args(p);
-    return split_floats(a, plan_of(a, p->dtype)) * sizeof(float);
+    const Plan plan = plan_of(a, p->dtype);
+    return (plan.few ? 0 : parts_bytes(p, false)) + split_floats(a, plan) * sizeof(float);
 }
 
 extern "C" int scp_cross_attention_forward(const void* q, const void* k, const void* v, const unsigned char* key_mask,
@@ -89,8 +154,8 @@ extern "C" int scp_cross_attention_forward(const void* q, const void* k, const v
     if (tile_too_wide(p, false)) return scp::fail(hipErrorInvalidValue, "cross_attention_forward: token stride of k or v too large");
     Args a = make_args(p);
     const Plan plan = plan_of(a, p->dtype);
-    const size_t need = split_floats(a, plan);
-    if (need && (!workspace || workspace_bytes < need * sizeof(float)))
+    const size_t parts = plan.few ? 0 : parts_bytes(p, false), need = parts + split_floats(a, plan) * sizeof(float);
+    if (need && (!workspace || workspace_bytes < need))
         return scp::fail(hipErrorInvalidValue, "cross_attention_forward: workspace too small");
     a.q = q;
     a.k = k;
@@ -101,9 +166,13 @@ extern "C" int scp_cross_attention_forward(const void* q, const void* k, const v
     a.lse = lse;
     a.nsplit = plan.nsplit;
     a.keys_per_split = plan.keys_per_split;
-    a.part_o = static_cast<float*>(workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + parts);
     a.part_ml = a.part_o + (size_t)plan.nsplit * a.BH * a.Nq * a.G * a.D;
     hipStream_t st = static_cast<hipStream_t>(stream);
+    if (parts) {
+        make_parts(a, p, false, workspace, st);
+        if (const int e = scp::check_launch("cross_attention_forward parts")) return e;
+    }
     if (p->dtype == SCP_DTYPE_F32) scp_attn::run_forward<float>(a, plan, st);
     else scp_attn::run_forward<__bf16>(a, plan, st);
     return scp::check_launch("cross_attention_forward");
@@ -111,7 +180,7 @@ extern "C" int scp_cross_attention_forward(const void* q, const void* k, const v
 
 extern "C" size_t scp_cross_attention_backward_workspace(const scp_cross_attn_params* p) {
     if (bad_problem(p)) return 0;
-    return (size_t)p->batch * p->heads * p->queries * sizeof(float);
+    return parts_bytes(p, true) + (size_t)p->batch * p->heads * p->queries * sizeof(float);
 }
 
 extern "C" int scp_cross_attention_backward(const void* q, const void* k, const void* v, const unsigned char* key_mask, const void* out,
@@ -119,7 +188,7 @@ extern "C" int scp_cross_attention_backward(const void* q, const void* k, const 
                                             void* g_v, void* workspace, size_t workspace_bytes, void* stream) {
     if (const char* why = bad_problem(p)) return scp::fail(hipErrorInvalidValue, why);
     if (!q || !k || !v || !out || !lse || !g_out) return scp::fail(hipErrorInvalidValue, "cross_attention_backward: null argument");
-    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(out_low) || misaligned(g_out) || misaligned(g_q) || misaligned(g_k) || misaligned(g_v))
+    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(out_low) || misaligned(g_out) || misaligned(workspace) || misaligned(g_q) || misaligned(g_k) || misaligned(g_v))
         return scp::fail(hipErrorInvalidValue, "cross_attention_backward: tensors must be 16-byte aligned");
     if (tile_too_wide(p, true)) return scp::fail(hipErrorInvalidValue, "cross_attention_backward: token or head stride too large");
     if (!g_q && !g_k && !g_v) return 0;
@@ -133,12 +202,18 @@ extern "C" int scp_cross_attention_backward(const void* q, const void* k, const 
     a.o_in = out;
     a.o_low_in = out_low;
     a.lse = const_cast<float*>(lse);
-    a.go = g_out;
-    a.delta = static_cast<float*>(workspace);
+    a.go = a.dgo = g_out;
+    for (int i = 0; i < 3; i++) a.dgs[i] = a.gs[i];
+    const size_t parts = parts_bytes(p, true);
+    a.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + parts);
     a.gq = g_q;
     a.gk = g_k;
     a.gv = g_v;
     hipStream_t st = static_cast<hipStream_t>(stream);
+    if (parts) {
+        make_parts(a, p, true, workspace, st);
+        if (const int e = scp::check_launch("cross_attention_backward parts")) return e;
+    }
     if (p->dtype == SCP_DTYPE_F32) scp_attn::run_backward<float>(a, st);
     else scp_attn::run_backward<__bf16>(a, st);
     return scp::check_launch("cross_attention_backward");
