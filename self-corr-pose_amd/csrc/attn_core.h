@@ -6,21 +6,27 @@
 //     (row = (reg & 3) + 8 (reg >> 2) + 4 half, half = lane >> 5), so softmax statistics of a column are lane-local;
 //   a product over rows   Acc[d][col] += X[row][d] P[row][col]  takes P from exactly those registers: its row order inside a matrix
 //     instruction is the order in which the accumulators already hold the rows, and X comes transposed out of LDS in that order
-//     (bf16: ds_read_b64_tr_b16, fp32: 32 consecutive floats per half-wavefront).
+//     (ds_read_b64_tr_b16).
 // forward:           stationary Q,     streamed K, V;   Acc = o^T  += V^T p
 // query gradient:    stationary Q, gO, streamed K, V;   Acc = gq^T += K^T gs
 // key/value gradient: stationary K, V, streamed Q, gO;  Acc = gk^T += Q^T gs,  Acc2 = gv^T += gO^T p
-// bf16 runs on v_mfma_f32_32x32x16_bf16 (p and gs rounded to bf16 for their product: one operand of it has to be bf16, and the result is
-// rounded to bf16 anyway), fp32 on v_mfma_f32_32x32x2_f32.  What that rounding does to gs = p (gO . v - delta) where a few keys hold most of
-// the softmax, and gO . v and delta cancel: the denominator is the sum of the ROUNDED p (v_dot2_f32_bf16, as fast as the 16 additions
-// that it replaces), so o is a weighted mean of v whatever the rounding did and its error in delta is of the size of gs's own rounding; and
-// what o is rounded by is kept for the backward pass (o_low), so delta sees o to 16 bits (4 us of 181 for 32 x 6 heads of 642 x 1025).
-// Error of gq, 300 queries x 300 keys with a softmax on 2 to 3 keys: 5.7e-3 without the two, 3.0e-3 with them.
+// Everything runs on v_mfma_f32_32x32x16_bf16.
+// fp32: every operand is three bf16 parts of 8 bits each (x = h + m + l exactly), q, k, v and g_out cut once into a workspace by csrc/
+// cross_attn.hip, p and gs in registers; a product is the six products of parts that reach 2^-24 of it, the small ones first.  That is 6 matrix
+// instructions for 16 of v_mfma_f32_32x32x2_f32 and the same LDS reads (4 x 6 heads of 642 x 1025: forward + backward 193 -> 144 us).  An
+// infinity that is not masked gives NaN: its parts are inf and NaN.
+// bf16: p and gs are rounded to bf16 for their product: one operand of it has to be bf16, and the result is rounded to bf16 anyway.  What
+// that does to gs = p (gO . v - delta) where a few keys hold most of the softmax, and gO . v and delta cancel: the denominator is the sum of
+// the ROUNDED p (v_dot2_f32_bf16, as fast as the 16 additions that it replaces), so o is a weighted mean of v whatever the rounding did
+// and its error in delta is of the size of gs's own rounding; and what o is rounded by is kept for the backward pass (o_low), so delta sees
+// o to 16 bits (4 us of 179 for 32 x 6 heads of 642 x 1025).  Error of gq, 300 queries x 300 keys with a softmax on 2 to 3 keys: 5.7e-3
+// without the two, 3.0e-3 with them.
 //
-// Two ways to deal the work (Plan): OWN -- each of 4 wavefronts has 32 columns of its own and all read the same tile (64 rows in bf16, 32 in
-// fp32); SHARE -- the wavefronts have the SAME 32 columns, each reads its 32 rows of a 128-row tile, and their partial results are joined
-// through LDS at the end.  SHARE quarters the reuse of a tile and quadruples the number of wavefronts: it is for problems that would leave
-// SIMDs empty otherwise.  Tiles are double-buffered (the next one in flight during the products) where two fit 80 KB.
+// Three ways to deal the work (Plan).  OWN: each of 4 wavefronts has 32 columns of its own and all read the same tile (64 rows in bf16, 32 in
+// fp32).  SHARE: 4 (bf16) or 2 (fp32) wavefronts have the SAME 32 columns, each reads its 32 rows of a tile of 128 or 64, and their partial
+// results are joined through LDS at the end; that divides the reuse of a tile by the number and multiplies the wavefronts by it: it is for
+// problems that would leave SIMDs empty otherwise.  FEW: no tiles, see few_rows_kernel.  Tiles are double-buffered (the next one in flight
+// during the products) where two fit 80 KB.
 //
 // LDS tiles are filled by buffer loads that write LDS directly, 16 bytes per lane.  A lane whose row is masked, past the end, or whose
 // channel is past head_dim gets an out-of-range offset: the hardware writes zeros, so nothing stored there can reach a product.  The
@@ -689,10 +695,12 @@ template <typename T, int DP, int ROWS> __global__ __launch_bounds__(256, 2) voi
     constexpr int UNROLL = S::UNROLL, GROUPS = S::GROUPS, LPR = S::LPR, NV = S::NV;
     __shared__ __attribute__((aligned(16))) float jo[4 * ROWS * DP];
     __shared__ float jm[4 * ROWS * 2];
-    int bh, split;
-    if (!place(a.BH, a.nsplit, bh, split)) return;
+    const int R = a.Nq * a.G, row_groups = (R + ROWS - 1) / ROWS;
+    int bh, blk;
+    if (!place(a.BH, a.nsplit * row_groups, bh, blk)) return;
+    const int split = blk / row_groups, row0 = ROWS * (blk - split * row_groups);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane / LPR, d = 8 * (lane % LPR);
-    const int R = a.Nq * a.G, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int b = bh / a.Hk, hk = bh - b * a.Hk;
     const bool has = d < a.D;
     const Rows qr = rows_of<T>(a.q, a.qs, b, hk * a.G, a.G), kr = rows_of<T>(a.k, a.ks, b, hk, 1), vr = rows_of<T>(a.v, a.vs, b, hk, 1);
     const unsigned char* mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
@@ -706,7 +714,7 @@ template <typename T, int DP, int ROWS> __global__ __launch_bounds__(256, 2) voi
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             q[r][i] = u32x4{};
-            if (r < R && has) q[r][i] = *reinterpret_cast<const u32x4*>(qr.row(r) + d * sizeof(T) + 16 * i);
+            if (row0 + r < R && has) q[r][i] = *reinterpret_cast<const u32x4*>(qr.row(row0 + r) + d * sizeof(T) + 16 * i);
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) acc[r][i] = 0.f;
@@ -789,7 +797,7 @@ template <typename T, int DP, int ROWS> __global__ __launch_bounds__(256, 2) voi
         }
     }
     __syncthreads();
-    join_waves<T, DP, ROWS, 4>(a, jo, jm, 0, split, bh);
+    join_waves<T, DP, ROWS, 4>(a, jo, jm, row0, split, bh);
 }
 
 // joins the splits: a thread per 4 channels of a row
@@ -1071,11 +1079,12 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SH>::GRAD_OCC)) void backward_ke
 
 // ---- launch plan --------------------------------------------------------------------------------------------------------------------
 struct Plan { bool share, few; int nsplit, keys_per_split, row_blocks; };
-// Rows that few_rows_kernel takes (one query, or the heads that share its keys).  fp32, where a 32-row product on the matrix cores costs 16
-// times a bf16 one: 64 x 6 heads of 64 x 4097 keys, 1 / 4 rows: 147 / 154 us against SHARE's 186; 32 x 8 heads of 128 x 1025 keys: 48 against
-// 91.  bf16: 1 row 76 against 74, 128 channels 29 against 41, 32 x 6 x 1025 keys 15.7 against 18.5 with the join; 2 / 4 rows 80 / 93
-// against 74 / 75, so only one.
-constexpr int few_rows(int size) { return size == 4 ? 4 : 1; }
+// Rows per key / value head that few_rows_kernel takes, in groups of up to 8 that each read K and V.
+// fp32, where the matrix kernels first write the tensors' parts (6 bytes an element) and read them again: 64 x 6 heads of 64 x 4097 keys,
+// 1 / 8 / 32 / 64 rows: 144 / 163 / 388 / 742 us against 610 to 619; 32 x 6 x 1025 keys: 23 / 39 / 63 / 110 against 73 to 79.
+// bf16, where they read the tensors: 64 x 6 x 4097 keys, 1 / 2 / 4 rows: 76 / 80 / 93 us against 74 to 75, but 32 x 6 x 1025 keys, 1 row:
+// 15.7 against 18.5, 32 x 8 heads of 128: 29 against 41; so one row only.
+constexpr int few_rows(int size) { return size == 4 ? 32 : 1; }
 constexpr int FEW_BLOCKS = 512;                              // workgroups to split the keys for: 1024 and more only make the join longer (32 x 6 x 1025 fp32 24.4 us, 512: 22.7)
 constexpr long SHARE_BELOW = 1024;                           // wavefronts of 32 columns; fewer leave SIMDs empty (256 CUs x 4)
 inline long wavefronts(const Args& a, int columns) { return (long)a.BH * ((columns + 31) / 32); }
@@ -1087,8 +1096,9 @@ inline Plan forward_plan(const Args& a, int own_cols, int shared, int max_few, i
     p.few = R <= max_few;
     if (p.few) {
         p.share = false;
-        p.row_blocks = 1;
-        long want = (FEW_BLOCKS - 1 + a.BH) / a.BH, most = (a.Nk + 4 * few_keys - 1) / (4 * few_keys);
+        p.row_blocks = R <= 4 ? 1 : (R + 7) / 8;
+        const long blocks = (long)a.BH * p.row_blocks;
+        long want = (FEW_BLOCKS - 1 + blocks) / blocks, most = (a.Nk + 4 * few_keys - 1) / (4 * few_keys);
         if (want > most) want = most;
         p.keys_per_split = ((a.Nk + (int)want - 1) / (int)want + 15) / 16 * 16;
         p.nsplit = (a.Nk + p.keys_per_split - 1) / p.keys_per_split;
@@ -1121,7 +1131,8 @@ template <typename T, int DP> void launch_forward(const Args& a, const Plan& p, 
             hipLaunchKernelGGL((few_rows_kernel<T, DF, 1>), grid, dim3(256), 0, st, a);
         } else if constexpr (few_rows(sizeof(T)) > 1) {
             if (R == 2) hipLaunchKernelGGL((few_rows_kernel<T, DF, 2>), grid, dim3(256), 0, st, a);
-            else hipLaunchKernelGGL((few_rows_kernel<T, DF, 4>), grid, dim3(256), 0, st, a);
+            else if (R <= 4) hipLaunchKernelGGL((few_rows_kernel<T, DF, 4>), grid, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((few_rows_kernel<T, DF, 8>), grid, dim3(256), 0, st, a);
         }
     } else if (p.share) hipLaunchKernelGGL((forward_kernel<T, DP, SHARED<T>>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((forward_kernel<T, DP, 1>), grid, dim3(256), 0, st, a);
