@@ -649,7 +649,7 @@ int scp_layernorm_backward(const void* s, const void* gamma, const void* gy, con
  * strides in ELEMENTS (batch, token, head; a stride may be 0; channels contiguous; strides and pointers multiples of 16 bytes); out, g_q
  * [batch,queries,heads,head_dim], g_k, g_v [batch,keys,kv_heads,head_dim] are contiguous.  key_mask [batch,keys] or NULL.  A batch entry
  * without a key gives zeros and zero gradients; values stored at masked keys, NaN included, never reach a result.
- *   out_low (bf16 only, like out; may be NULL): what out was rounded by.  Given back to the backward pass it keeps the gradients exact where a
+ *   out_low (bf16 only, a byte per element of out; may be NULL): the 8 bits of out that follow its rounding.  Given back to the backward pass it keeps the gradients exact where a
  *     few keys hold most of the softmax; without it gO . out is taken from the rounded out.
  *   lse [batch,kv_heads,queries * heads / kv_heads]: log2 of the softmax denominator per row, kept for the backward pass; may be NULL.
  *   head_dim: a multiple of 8, <= 128.  g_q / g_k / g_v may each be NULL. */
@@ -660,9 +660,9 @@ typedef struct scp_cross_attn_params {
 } scp_cross_attn_params;
 size_t scp_cross_attention_forward_workspace(const scp_cross_attn_params* p);
 int scp_cross_attention_forward(const void* q, const void* k, const void* v, const unsigned char* key_mask, const scp_cross_attn_params* p,
-                                void* out, void* out_low, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+                                void* out, signed char* out_low, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 size_t scp_cross_attention_backward_workspace(const scp_cross_attn_params* p);
-int scp_cross_attention_backward(const void* q, const void* k, const void* v, const unsigned char* key_mask, const void* out, const void* out_low,
+int scp_cross_attention_backward(const void* q, const void* k, const void* v, const unsigned char* key_mask, const void* out, const signed char* out_low,
                                  const float* lse, const void* g_out, const scp_cross_attn_params* p, void* g_q, void* g_k, void* g_v, void* workspace,
                                  size_t workspace_bytes, void* stream);
 

@@ -18,8 +18,8 @@
 // bf16: p and gs are rounded to bf16 for their product: one operand of it has to be bf16, and the result is rounded to bf16 anyway.  What
 // that does to gs = p (gO . v - delta) where a few keys hold most of the softmax, and gO . v and delta cancel: the denominator is the sum of
 // the ROUNDED p (v_dot2_f32_bf16, as fast as the 16 additions that it replaces), so o is a weighted mean of v whatever the rounding did
-// and its error in delta is of the size of gs's own rounding; and what o is rounded by is kept for the backward pass (o_low), so delta sees
-// o to 16 bits (4 us of 179 for 32 x 6 heads of 642 x 1025).  Error of gq, 300 queries x 300 keys with a softmax on 2 to 3 keys: 5.7e-3
+// and its error in delta is of the size of gs's own rounding; and the next 8 bits of o are kept for the backward pass (o_low), so delta sees
+// o to 16 bits.  Error of gq, 300 queries x 300 keys with a softmax on 2 to 3 keys: 5.7e-3
 // without the two, 3.0e-3 with them.
 //
 // Three ways to deal the work (Plan).  OWN: each of 4 wavefronts has 32 columns of its own and all read the same tile (64 rows in bf16, 32 in
@@ -46,14 +46,17 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 struct Args {
     const void *q, *k, *v, *go;           // what the matrix products read: the tensors (bf16), or their parts (fp32: Parts)
     const void* dgo;                      // g_out itself, for delta
     const unsigned char* mask;
-    const void *o_in, *o_low_in;
-    void *o, *o_low, *gq, *gk, *gv;
+    const void* o_in;
+    const signed char* o_low_in;
+    void *o, *gq, *gk, *gv;
+    signed char* o_low;
     float *lse, *delta;
     float *part_o, *part_ml;              // split over the keys: [split][bh][R][D], [split][bh][R][2]
     long qs[3], ks[3], vs[3], gs[3], dgs[3];      // strides in elements: batch, token, head
@@ -110,43 +113,50 @@ template <> struct Out<__bf16> {
         const bf16x4 v = {(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
         *reinterpret_cast<bf16x4*>(p) = v;
     }
-    // channels 32 db .. 32 db + 31 of this lane's column, in accumulator order, to `row` where ok; `low` (or null): what that rounds away.
+    // channels 32 db .. 32 db + 31 of this lane's column, in accumulator order, to `row` where ok; `low` (or null): low_bits of them.
     // The halves of the wavefront trade accumulators, so that each lane stores 8 channels in a row.
-    static __device__ __forceinline__ void store_column(T* row, T* low, int db, int D, bool ok, const f32x16& v) {
+    static __device__ __forceinline__ void store_column(T* row, signed char* low, int db, int D, bool ok, const f32x16& v) {
         const int half = (threadIdx.x >> 5) & 1;
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             const int d = 32 * db + 16 * k + 8 * half;
-            u32x4 hi = {}, lo = {};
+            u32x4 hi = {};
 #pragma unroll
             for (int w = 0; w < 2; w++) {
-                unsigned h[2], l[2];
+                unsigned h[2];
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const float x = v[8 * k + 4 * u + 2 * w], y = v[8 * k + 4 * u + 2 * w + 1];
-                    const bf16x2 top = {(__bf16)x, (__bf16)y}, rest = {(__bf16)(x - (float)top[0]), (__bf16)(y - (float)top[1])};
-                    h[u] = __builtin_bit_cast(unsigned, top);
-                    l[u] = __builtin_bit_cast(unsigned, rest);
+                    const bf16x2 pair = {(__bf16)v[8 * k + 4 * u + 2 * w], (__bf16)v[8 * k + 4 * u + 2 * w + 1]};
+                    h[u] = __builtin_bit_cast(unsigned, pair);
                 }
                 const auto a = __builtin_amdgcn_permlane32_swap(h[0], h[1], false, false);
                 hi[w] = a[0];
                 hi[2 + w] = a[1];
-                if (low) {
-                    const auto c = __builtin_amdgcn_permlane32_swap(l[0], l[1], false, false);
-                    lo[w] = c[0];
-                    lo[2 + w] = c[1];
-                }
             }
-            if (ok && d < D) {
-                *reinterpret_cast<u32x4*>(row + d) = hi;
-                if (low) *reinterpret_cast<u32x4*>(low + d) = lo;
+            if (ok && d < D) *reinterpret_cast<u32x4*>(row + d) = hi;
+            if (low) {
+                unsigned l[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) l[u] = low_bits(v[8 * k + 4 * u], v[8 * k + 4 * u + 1], v[8 * k + 4 * u + 2], v[8 * k + 4 * u + 3]);
+                const auto a = __builtin_amdgcn_permlane32_swap(l[0], l[1], false, false);
+                if (ok && d < D) *reinterpret_cast<u32x2*>(low + d) = u32x2{a[0], a[1]};
             }
         }
     }
-    // what store4 rounds away
-    static __device__ __forceinline__ void store_low(T* p, float a, float b, float c, float d) {
-        store4(p, a - (float)(__bf16)a, b - (float)(__bf16)b, c - (float)(__bf16)c, d - (float)(__bf16)d);
+    // The 8 bits of a number that follow its bf16 rounding, signed: (bits - rounded bits) >> 8, whole numbers both, is in -128 .. 127; with
+    // half a step of it added the number comes back to 2^-16 of itself.
+    static __device__ __forceinline__ unsigned low_bits(float a, float b, float c, float d) {
+        const float x[4] = {a, b, c, d};
+        unsigned out = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float top = (float)(__bf16)x[i];
+            out |= (((__float_as_uint(x[i]) - __float_as_uint(top)) >> 8) & 0xffu) << (8 * i);
+        }
+        return out;
     }
+    static __device__ __forceinline__ float with_low(float top, int code) { return __uint_as_float(__float_as_uint(top) + (unsigned)(code * 256 + 128)); }
+    static __device__ __forceinline__ void store_low(signed char* p, float a, float b, float c, float d) { *reinterpret_cast<unsigned*>(p) = low_bits(a, b, c, d); }
 };
 template <> struct Out<float> {
     typedef float T;
@@ -154,7 +164,7 @@ template <> struct Out<float> {
         const f32x4 v = {a, b, c, d};
         *reinterpret_cast<f32x4*>(p) = v;
     }
-    static __device__ __forceinline__ void store_column(T* row, T*, int db, int D, bool ok, const f32x16& v) {
+    static __device__ __forceinline__ void store_column(T* row, signed char*, int db, int D, bool ok, const f32x16& v) {
         const int half = (threadIdx.x >> 5) & 1;
 #pragma unroll
         for (int g = 0; g < 4; g++) {
@@ -162,7 +172,8 @@ template <> struct Out<float> {
             if (ok && d < D) store4(row + d, v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
         }
     }
-    static __device__ __forceinline__ void store_low(T*, float, float, float, float) {}
+    static __device__ __forceinline__ void store_low(signed char*, float, float, float, float) {}
+    static __device__ __forceinline__ float with_low(float top, int) { return top; }
 };
 
 // PS: elements between the planes of a tile (its parts, one [rows][DP] image each)
@@ -497,7 +508,7 @@ __device__ __forceinline__ void join_waves(const Args& a, const float* jo, const
             sum *= lt == 0.f ? 0.f : 1.f / lt;
             const long at = (((long)b * a.Nq + n) * H + h) * a.D + d;
             Out<T>::store4(static_cast<T*>(a.o) + at, sum[0], sum[1], sum[2], sum[3]);
-            if (a.o_low) Out<T>::store_low(static_cast<T*>(a.o_low) + at, sum[0], sum[1], sum[2], sum[3]);
+            if (a.o_low) Out<T>::store_low(a.o_low + at, sum[0], sum[1], sum[2], sum[3]);
             if (a.lse && d == 0) a.lse[(long)bh * R + rr] = lt == 0.f ? INFINITY : mt + __builtin_amdgcn_logf(lt);
         }
     }
@@ -644,7 +655,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SH>::FWD_OCC)) void forward_kern
             const int r = r_wave + 32 * x + l31, n = r / a.G, h = hk * a.G + r - n * a.G;
             const long at = (((long)b * a.Nq + n) * H + h) * a.D;
             const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
-            T* low = a.o_low ? static_cast<T*>(a.o_low) + at : nullptr;
+            signed char* low = a.o_low ? a.o_low + at : nullptr;
 #pragma unroll
             for (int i = 0; i < DB; i++) Out<T>::store_column(static_cast<T*>(a.o) + at, low, i, a.D, r < R, o[x][i] * inv);
             if (a.lse && half == 0 && r < R) a.lse[(long)bh * R + r] = l[x] == 0.f ? INFINITY : m[x] + __builtin_amdgcn_logf(l[x]);
@@ -821,7 +832,7 @@ template <typename T> __global__ __launch_bounds__(256) void join_kernel(const A
     sum *= lt == 0.f ? 0.f : 1.f / lt;
     const long at = (((long)b * a.Nq + n) * H + h) * a.D + d;
     Out<T>::store4(static_cast<T*>(a.o) + at, sum[0], sum[1], sum[2], sum[3]);
-    if (a.o_low) Out<T>::store_low(static_cast<T*>(a.o_low) + at, sum[0], sum[1], sum[2], sum[3]);
+    if (a.o_low) Out<T>::store_low(a.o_low + at, sum[0], sum[1], sum[2], sum[3]);
     if (a.lse && d == 0) a.lse[row] = lt == 0.f ? INFINITY : mt + __builtin_amdgcn_logf(lt);
 }
 
@@ -837,7 +848,10 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void delta_kerne
     const unsigned first = (blockIdx.x - b * blocks_per_batch) * (GROUPS * DELTA_ROWS) + threadIdx.x / LANES, rows = a.Nq * H;
     const int d = 8 * l < a.D ? 8 * l : 0;                   // a lane past the last channel reads the first ones and leaves them out
     unsigned n[DELTA_ROWS], h[DELTA_ROWS];
-    tx8 x[DELTA_ROWS], y[DELTA_ROWS], z[DELTA_ROWS];
+    typedef signed char cx8 __attribute__((ext_vector_type(8)));
+    tx8 x[DELTA_ROWS], y[DELTA_ROWS];
+    cx8 z[DELTA_ROWS];
+    const bool low = sizeof(T) == 2 && a.o_low_in;
 #pragma unroll
     for (int i = 0; i < DELTA_ROWS; i++) {
         const unsigned row = min(first + GROUPS * i, rows - 1);
@@ -846,14 +860,13 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void delta_kerne
         x[i] = *reinterpret_cast<const tx8*>(static_cast<const T*>(a.dgo) + b * a.dgs[0] + n[i] * a.dgs[1] + h[i] * a.dgs[2] + d);
         const long at = ((long)b * rows + row) * a.D + d;
         y[i] = *reinterpret_cast<const tx8*>(static_cast<const T*>(a.o_in) + at);
-        z[i] = tx8{};
-        if (sizeof(T) == 2 && a.o_low_in) z[i] = *reinterpret_cast<const tx8*>(static_cast<const T*>(a.o_low_in) + at);
+        if (low) z[i] = *reinterpret_cast<const cx8*>(a.o_low_in + at);
     }
 #pragma unroll
     for (int i = 0; i < DELTA_ROWS; i++) {
         float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) s += (float)x[i][e] * ((float)y[i][e] + (float)z[i][e]);
+        for (int e = 0; e < 8; e++) s += (float)x[i][e] * (low ? Out<T>::with_low((float)y[i][e], z[i][e]) : (float)y[i][e]);
         if (8 * l >= a.D) s = 0.f;
 #pragma unroll
         for (int k = 1; k < LANES; k <<= 1) s += __shfl_xor(s, k);

@@ -145,7 +145,7 @@ extern "C" size_t scp_cross_attention_forward_workspace(const scp_cross_attn_par
 }
 
 extern "C" int scp_cross_attention_forward(const void* q, const void* k, const void* v, const unsigned char* key_mask,
-                                           const scp_cross_attn_params* p, void* out, void* out_low, float* lse, void* workspace,
+                                           const scp_cross_attn_params* p, void* out, signed char* out_low, float* lse, void* workspace,
                                            size_t workspace_bytes, void* stream) {
     if (const char* why = bad_problem(p)) return scp::fail(hipErrorInvalidValue, why);
     if (!q || !k || !v || !out) return scp::fail(hipErrorInvalidValue, "cross_attention_forward: null argument");
@@ -184,7 +184,7 @@ extern "C" size_t scp_cross_attention_backward_workspace(const scp_cross_attn_pa
 }
 
 extern "C" int scp_cross_attention_backward(const void* q, const void* k, const void* v, const unsigned char* key_mask, const void* out,
-                                            const void* out_low, const float* lse, const void* g_out, const scp_cross_attn_params* p, void* g_q, void* g_k,
+                                            const signed char* out_low, const float* lse, const void* g_out, const scp_cross_attn_params* p, void* g_q, void* g_k,
                                             void* g_v, void* workspace, size_t workspace_bytes, void* stream) {
     if (const char* why = bad_problem(p)) return scp::fail(hipErrorInvalidValue, why);
     if (!q || !k || !v || !out || !lse || !g_out) return scp::fail(hipErrorInvalidValue, "cross_attention_backward: null argument");

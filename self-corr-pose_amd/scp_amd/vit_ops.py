@@ -166,14 +166,14 @@ def _addressable(t):
 
 
 def _attn_forward(q, k, v, mask, scale, keep):
-    """(out, what its rounding to bfloat16 left or None, log-sum-exp or None, C parameters); keep: for a backward pass"""
+    """(out, the bits after its rounding to bfloat16 or None, log-sum-exp or None, C parameters); keep: for a backward pass"""
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if keep else None
     if out.numel() == 0:
         return out, None, lse, None
     if k.shape[1] == 0:
         return out.zero_(), None, lse, None
-    low = torch.empty_like(out) if keep and out.dtype == torch.bfloat16 else None
+    low = torch.empty_like(out, dtype=torch.int8) if keep and out.dtype == torch.bfloat16 else None
     L = capi.lib()
     p = capi.CrossAttnParams(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], capi.DTYPES[q.dtype], scale, q.stride()[:3],
                              k.stride()[:3], v.stride()[:3])
