@@ -649,8 +649,9 @@ int scp_layernorm_backward(const void* s, const void* gamma, const void* gy, con
  * strides in ELEMENTS (batch, token, head; a stride may be 0; channels contiguous; strides and pointers multiples of 16 bytes); out, g_q
  * [batch,queries,heads,head_dim], g_k, g_v [batch,keys,kv_heads,head_dim] are contiguous.  key_mask [batch,keys] or NULL.  A batch entry
  * without a key gives zeros and zero gradients; values stored at masked keys, NaN included, never reach a result.
- *   out_low (bf16 only, a byte per element of out; may be NULL): the 8 bits of out that follow its rounding.  Given back to the backward pass it keeps the gradients exact where a
- *     few keys hold most of the softmax; without it gO . out is taken from the rounded out.
+ *   out_low (bf16 only, a byte per element of out; may be NULL): the 8 bits of out that follow its rounding.  Given back to the backward
+ *     pass it keeps the gradients exact where a few keys hold most of the softmax; without it g_out . out is taken from the rounded out.
+ *   fp32 tensors are multiplied as three exact bf16 parts, which the workspace holds: an infinity that is not masked may come out as NaN.
  *   lse [batch,kv_heads,queries * heads / kv_heads]: log2 of the softmax denominator per row, kept for the backward pass; may be NULL.
  *   head_dim: a multiple of 8, <= 128.  g_q / g_k / g_v may each be NULL. */
 typedef struct scp_cross_attn_params {

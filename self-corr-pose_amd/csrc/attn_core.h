@@ -27,6 +27,8 @@
 // results are joined through LDS at the end; that divides the reuse of a tile by the number and multiplies the wavefronts by it: it is for
 // problems that would leave SIMDs empty otherwise.  FEW: no tiles, see few_rows_kernel.  Tiles are double-buffered (the next one in flight
 // during the products) where two fit 80 KB.
+// Measured: bf16 forward of 2562 x 4097, 8 x 6 heads of 64 on 2, 156 us (830 TFLOP/s); forward + backward of 642 x 1025, 32 x 6 heads, a padded
+// batch, 178 us; what bounds both is matrix and vector instructions, which overlap to about 70 % of their sum.
 //
 // LDS tiles are filled by buffer loads that write LDS directly, 16 bytes per lane.  A lane whose row is masked, past the end, or whose
 // channel is past head_dim gets an out-of-range offset: the hardware writes zeros, so nothing stored there can reach a product.  The
@@ -1099,7 +1101,9 @@ struct Plan { bool share, few; int nsplit, keys_per_split, row_blocks; };
 // 15.7 against 18.5, 32 x 8 heads of 128: 29 against 41; so one row only.
 constexpr int few_rows(int size) { return size == 4 ? 32 : 1; }
 constexpr int FEW_BLOCKS = 512;                              // workgroups to split the keys for: 1024 and more only make the join longer (32 x 6 x 1025 fp32 24.4 us, 512: 22.7)
-constexpr long SHARE_BELOW = 1024;                           // wavefronts of 32 columns; fewer leave SIMDs empty (256 CUs x 4)
+// SHARE below so many wavefronts of 32 columns; fewer leave SIMDs empty (256 CUs x 4).  8 x 6 heads of 642 x 1025, bf16: backward pass OWN 72 us,
+// SHARE 97; fp32: forward OWN 92, SHARE 98, 4 x 6 heads backward OWN 130, SHARE 120; 512 to 4096 are within 10 % of each other there.
+constexpr long SHARE_BELOW = 1024;
 inline long wavefronts(const Args& a, int columns) { return (long)a.BH * ((columns + 31) / 32); }
 // own_cols: columns of an OWN workgroup; shared: SHARED.
 // split: where even SHARE has too few workgroups, the keys are divided as long as each part keeps two tiles

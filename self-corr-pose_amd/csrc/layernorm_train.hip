@@ -11,6 +11,8 @@
 // over the registers in 32 bits (no E[x^2] - E[x]^2 cancellation).
 // Column sums: a workgroup strides over the rows with its gw / gb partials in registers, folds its row groups through LDS in a fixed
 // order and writes one [2][C] partial; a second kernel adds the partials of all workgroups in order.  No atomics: bit-reproducible.
+// Measured: 32800 x 384 fp32 with the residual add, forward 43 us and backward 45 + 4 us for 202 MB each (4.6 TB/s; a copy of that size 5.1);
+// 8209 x 1001 bf16 14 and 22 + 4 us.
 #include <hip/hip_runtime.h>
 
 #include "scp_common.h"

@@ -224,7 +224,8 @@ def cross_attention(q, k, v, scale=None, key_mask=None):
     (contiguous).  H a multiple of Hkv: query head h reads key / value head h // (H // Hkv).  D a multiple of 8, at most 128.  `scale`
     defaults to D ** -0.5.  `key_mask` (bool [B, Nk], True = attend): an image's padding; values stored at masked keys, NaN included,
     reach no result; a batch entry without a key gives zeros, and zero gradients.  Any strides (slices of a fused qkv projection, an
-    expanded batch); gradients for q, k and v."""
+    expanded batch); gradients for q, k and v.  float32 is multiplied as three exact bfloat16 parts: an infinity that is not masked may come
+    out as NaN."""
     _tensor(q, "cross_attention: q")
     for t, name in ((k, "k"), (v, "v")):
         _tensor(t, "cross_attention: " + name, (q.dtype,))
