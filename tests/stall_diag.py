@@ -6,8 +6,7 @@ pytest.ini's timeout) gets a report on stderr and in gpurun_out/stall_<test>.txt
   * every torch stream / event of the process: busy or idle, and which attribute holds it;
   * KFD's view of the process (/sys/class/kfd/kfd/proc/<pid>): queues, per-GPU `cu_occupancy` (waves resident = a kernel that does not end;
     zero = queues evicted / nothing dispatched) and `evicted_ms`, sampled twice one second apart;
-  * rocm-smi use / pids and the kernel log tail where readable;
-  * rocgdb attached to the process: agents, queues, the dispatches in flight with their kernel names, and the first wavefronts with their PCs.
+  * rocm-smi use / pids and the kernel log tail where readable.
 Round 5's GPU suite stalled inside Trainer.train with none of this on record; this file is what makes the next stall a
 diagnosis instead of a timeout.  Test infrastructure only."""
 import faulthandler
@@ -92,8 +91,8 @@ def torch_state():
     return "\n".join(lines) + "\n"
 
 
-def report(what, path=None, gdb=True):
-    """write the report section by section (a section that hangs -- rocgdb on a wedged device -- must not cost the ones before it)"""
+def report(what, path=None):
+    """write the report section by section (a section that hangs must not cost the ones before it)"""
     pid = os.getpid()
     out = sys.__stderr__
     fh = None
@@ -130,14 +129,6 @@ def report(what, path=None, gdb=True):
     emit("---- children\n" + _sh("ps -o pid,ppid,stat,etime,wchan:24,cmd --ppid %d; ps -L -o tid,stat,wchan:28,comm -p %d | head -60" % (pid, pid)))
     emit("---- rocm-smi\n" + _sh("rocm-smi --showuse --showpids --showmemuse 2>&1 | tail -30", 60))
     emit("---- dmesg\n" + _sh("dmesg 2>&1 | tail -40", 20))
-    emit("---- debugfs (best effort)\n" + _sh("mountpoint -q /sys/kernel/debug || mount -t debugfs none /sys/kernel/debug 2>&1; "
-                                              "for f in /sys/kernel/debug/kfd/hqds /sys/kernel/debug/kfd/rls /sys/kernel/debug/dri/*/amdgpu_fence_info; do "
-                                              "echo \"== $f\"; head -c 6000 $f 2>&1; done", 30))
-    if gdb and os.path.exists("/opt/rocm/bin/rocgdb"):
-        cmd = ("timeout -s KILL 80 /opt/rocm/bin/rocgdb -p %d -batch -ex 'set pagination off' -ex 'info agents' -ex 'info queues' -ex 'info dispatches' "
-               "-ex 'info threads' 2>&1 | grep -v '^\\[New\\|^warning: \\|Thread debugging\\|^Reading symbols\\|No such file' | head -260" % pid)
-        emit("---- rocgdb\n")
-        emit(_sh(cmd, 90))
     emit("==== stall_diag: end of report\n")
     if fh is not None:
         fh.close()
