@@ -1,4 +1,5 @@
-"""self-corr-pose_amd/build.py -- compiles csrc/*.hip into the in-tree libscp_hip.so for gfx950.
+"""self-corr-pose_amd/build.py -- compiles csrc/*.hip into the in-tree libscp_hip.so for gfx950, and csrc/vit_ops_binding.cpp (autograd nodes of
+scp_amd/vit_ops.py, host code against torch's headers) into scp_vit_ops.so beside it.
 
     python self-corr-pose_amd/build.py [--force]
 
@@ -50,14 +51,38 @@ def _echo(err):
             print(line, file=sys.stderr)
 
 
+BINDING = os.path.join(HERE, "lib", "scp_vit_ops.so")
+
+
+def start_binding(force=False, verbose=True):
+    """the compilation of BINDING as a running process, or None if it is up to date"""
+    src = os.path.join(CSRC, "vit_ops_binding.cpp")
+    deps = [src, os.path.join(ROOT, "include", "scp_hip.h"), __file__]
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) > max(os.path.getmtime(d) for d in deps):
+        return None
+    import sysconfig
+    import torch
+    t = torch.__path__[0]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-DTORCH_EXTENSION_NAME=scp_vit_ops",
+           "-I" + os.path.join(ROOT, "include"), "-isystem", os.path.join(t, "include"), "-isystem", os.path.join(t, "include", "torch", "csrc", "api", "include"),
+           "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"], src, "-o", BINDING,
+           "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    os.makedirs(os.path.dirname(BINDING), exist_ok=True)
+    return subprocess.Popen(cmd)
+
+
 def sources():
     return sorted(f for f in os.listdir(CSRC) if f.endswith(".hip"))
 
 
 def needs_build():
-    if not os.path.exists(OUT):
+    if not os.path.exists(OUT) or not os.path.exists(BINDING):
         return True
     t = os.path.getmtime(OUT)
+    t = min(t, os.path.getmtime(BINDING))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(ROOT, "include", "scp_hip.h"), __file__]
     return any(os.path.getmtime(d) > t for d in deps)
 
@@ -71,6 +96,7 @@ def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     objs = []
     procs = []
+    binding = start_binding(force, verbose)
     for s in sources():
         o = os.path.join(objdir, s[:-4] + ".o")
         src = os.path.join(CSRC, s)
@@ -89,10 +115,13 @@ def build(force=False, verbose=True):
         _echo(err)
         if p.returncode != 0:
             raise RuntimeError("hipcc failed on " + s)
+    if binding is not None and binding.wait() != 0:
+        raise RuntimeError("the compiler failed on vit_ops_binding.cpp")
     cmd = [hipcc, "-shared", "-fPIC", "--offload-arch=" + ARCH] + objs + ["-o", OUT]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)
+    os.utime(BINDING)
     return OUT
 
 
