@@ -63,6 +63,10 @@ template <int COLS> __device__ __forceinline__ bf16x8 operand(const __bf16* t, i
 }
 __device__ __forceinline__ unsigned upper_halves(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
 
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes > 0 ? bytes : 0, 0x00020000);
+}
+
 // the bytes of x from byte `shift` on (what follows them is of no account)
 __device__ __forceinline__ u32x2 from_byte(u32x2 x, int shift) {
     const u32x2 y = {shift & 4 ? x[1] : x[0], x[1]};
@@ -117,9 +121,8 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 4) void
         for (int i = 0; i < NB; i++)
 #pragma unroll
             for (int j = 0; j < 2; j++) acc[i][j] = f32x16{};
-        for (int i = 0; i < steps; i++) {
+        auto multiply = [&](int buf) {
             __syncthreads();
-            const int buf = i & 1;
 #pragma unroll
             for (int s = 0; s < STEP / 16; s++) {
                 bf16x8 x[2];
@@ -134,7 +137,13 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 4) void
                         for (int j = 0; j < 2; j++) acc[n][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(g, x[j], acc[n][j], 0, 0, 0);
                     }
             }
+        };
+        int i = 0;
+        for (; i + 1 < steps; i += 2) {                                 // the buffers by name: every LDS address is a constant of the loop
+            multiply(0);
+            multiply(1);
         }
+        if (i < steps) multiply(0);
         __syncthreads();                                                // the filling wavefronts' last one
         // accumulator: column k = lane & 31, row n = (reg & 3) + 8 (reg >> 2) + 4 half
         float* out = a.gw + (size_t)split * a.N * a.K;
@@ -160,7 +169,8 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 4) void
 
     // loads: gy piece i of this thread = row tid / 32 + 16 i, elements E (tid % 32); codes = rows tid / 16 and tid / 16 + 32, 8 of each.
     // Pieces past a row's end are read from its end instead and moved into place (RAGGED); what stands behind them, and in pieces past the
-    // matrix, goes into products that nobody stores.  Rows past the range are read from its last row and stored as zeros.
+    // matrix, goes into products that nobody stores.  Rows past the range are read from its last row and stored as zeros (RAGGED), or read
+    // as zeros from behind the end of a buffer: without minima and multiplications per piece, which cost as much as the dequantisation.
     const char* gy = static_cast<const char*>(a.gy);
     const int g_row = tid / S::CPR, g_col = n0 + S::E * (tid % S::CPR);
     const int x_row = tid >> 4, x_col = k0 + 8 * (tid & 15);
@@ -171,23 +181,33 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 4) void
     constexpr int XR = STEP * 16 / FILL;                                 // rows of codes per thread
     struct Raw { u32x4 g[S::PIECES]; u32x2 x[XR]; unsigned exp[XR]; };
     constexpr int XROWS = FILL / 16;
+    const int g_off = (g_row * a.N + g_at) * (int)sizeof(T), g_next = FILL / S::CPR * a.N * (int)sizeof(T);
+    const int x_off = x_row * a.K + x_at, x_next = XROWS * a.K, e_off = x_row * groups + e_at, e_next = XROWS * groups;
     auto load = [&](Raw& raw, long m) {
-        const int last = m_end - m < STEP ? (int)(m_end - m) - 1 : STEP - 1;
+        const int rows = m_end - m < STEP ? (int)(m_end - m) : STEP;
         const char* gbase = gy + m * a.N * (long)sizeof(T);
         const char* xbase = reinterpret_cast<const char*>(a.codes) + m * a.K;
         const char* ebase = reinterpret_cast<const char*>(a.exps) + m * groups;
+        if constexpr (RAGGED) {
 #pragma unroll
-        for (int i = 0; i < S::PIECES; i++) {
-            const unsigned off = (unsigned)(min(g_row + (FILL / S::CPR) * i, last) * a.N + g_at) * (unsigned)sizeof(T);
-            if constexpr (RAGGED) raw.g[i] = *reinterpret_cast<const u32x4_a1*>(gbase + off);
-            else raw.g[i] = *reinterpret_cast<const u32x4*>(gbase + off);
-        }
+            for (int i = 0; i < S::PIECES; i++)
+                raw.g[i] = *reinterpret_cast<const u32x4_a1*>(gbase + (unsigned)(min(g_row + (FILL / S::CPR) * i, rows - 1) * a.N + g_at) * (unsigned)sizeof(T));
 #pragma unroll
-        for (int i = 0; i < XR; i++) {
-            const int r = min(x_row + XROWS * i, last);
-            if constexpr (RAGGED) raw.x[i] = *reinterpret_cast<const u32x2_a1*>(xbase + (unsigned)(r * a.K + x_at));
-            else raw.x[i] = *reinterpret_cast<const u32x2*>(xbase + (unsigned)(r * a.K + x_at));
-            raw.exp[i] = *reinterpret_cast<const unsigned char*>(ebase + (unsigned)(r * groups + e_at));
+            for (int i = 0; i < XR; i++) {
+                const int r = min(x_row + XROWS * i, rows - 1);
+                raw.x[i] = *reinterpret_cast<const u32x2_a1*>(xbase + (unsigned)(r * a.K + x_at));
+                raw.exp[i] = *reinterpret_cast<const unsigned char*>(ebase + (unsigned)(r * groups + e_at));
+            }
+        } else {                                                        // rows past the range are past the buffer's end: zeros
+            const int g_bytes = rows * a.N * (int)sizeof(T), x_bytes = rows * a.K, e_bytes = rows * groups;
+#pragma unroll
+            for (int i = 0; i < S::PIECES; i++)
+                raw.g[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer(gbase + i * g_next, g_bytes - i * g_next), g_off, 0, 0));
+#pragma unroll
+            for (int i = 0; i < XR; i++) {
+                raw.x[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(buffer(xbase + i * x_next, x_bytes - i * x_next), x_off, 0, 0));
+                raw.exp[i] = __builtin_amdgcn_raw_buffer_load_b8(buffer(ebase + i * e_next, e_bytes - i * e_next), e_off, 0, 0);
+            }
         }
     };
     const bool bias = a.gb && tk == 0;
@@ -201,7 +221,7 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 4) void
 #pragma unroll
             for (int i = 0; i < XR; i++) raw.x[i] = from_byte(raw.x[i], x_shift);
         }
-        if (m + STEP > m_end) {
+        if (RAGGED && m + STEP > m_end) {
             const int rows = (int)(m_end - m);
 #pragma unroll
             for (int i = 0; i < S::PIECES; i++)
