@@ -422,9 +422,10 @@ template <typename T, int DP, int SH> struct Shape {
     static constexpr int COLS = 128 / SH;                                   // columns per workgroup (of one block per wavefront)
     static constexpr int BYTES = 2 * NP * N * DP * 2;                       // the two tiles
     static constexpr int NBUF = 2 * BYTES <= 81920 ? 2 : 1;
-    // column blocks of a wavefront in the forward pass.  Two: every LDS read feeds two matrix instructions, and the products of one block run
-    // beside the exponentials of the other (bf16, 64 channels: 173 -> 160 us for 7686 x 4097 x 16 heads); more would not fit the registers.
-    static constexpr int CB = SH == 1 && NP == 1 && DP <= 64 ? 2 : 1;
+    // column blocks that a wavefront can take in the forward pass.  Two: every LDS read feeds two matrix instructions, and the products of one
+    // block run beside the exponentials of the other (bf16, 64 channels: 173 -> 160 us for 7686 x 4097 x 16 heads); more would not fit
+    // the registers.
+    static constexpr int MAX_CB = SH == 1 && NP == 1 && DP <= 64 ? 2 : 1;
     // wavefronts per SIMD that the registers are bounded for
     static constexpr int FWD_OCC = NP == 1 && SH == 1 ? 2 : DP > 64 ? 1 : 2;
     static constexpr int GRAD_OCC = DP > 64 ? 1 : 2;
@@ -516,12 +517,12 @@ __device__ __forceinline__ void join_waves(const Args& a, const float* jo, const
     }
 }
 
-template <typename T, int DP, int SH>
+template <typename T, int DP, int SH, int CB>
 __global__ __launch_bounds__(256, (Shape<T, DP, SH>::FWD_OCC)) void forward_kernel(const Args a) {
     typedef Shape<T, DP, SH> S;
     typedef Mma<T, DP, S::N * DP> M;
     constexpr bool SHARE = SH > 1;
-    constexpr int WAVES = S::WAVES, N = S::N, DB = M::DB, CB = S::CB, COLS = S::COLS * CB;
+    constexpr int WAVES = S::WAVES, N = S::N, DB = M::DB, COLS = S::COLS * CB;
     __shared__ __attribute__((aligned(16))) __bf16 tile[S::NBUF][2][S::NP * N * DP];
     __shared__ unsigned words[2 * N];
     __shared__ float jm[SHARE ? 2 * SH * COLS : 1];
@@ -1093,7 +1094,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SH>::GRAD_OCC)) void backward_ke
 }
 
 // ---- launch plan --------------------------------------------------------------------------------------------------------------------
-struct Plan { bool share, few; int nsplit, keys_per_split, row_blocks; };
+struct Plan { bool share, few, two_blocks; int nsplit, keys_per_split, row_blocks; };
 // Rows per key / value head that few_rows_kernel takes, in groups of up to 8 that each read K and V.
 // fp32, where the matrix kernels first write the tensors' parts (6 bytes an element) and read them again: 64 x 6 heads of 64 x 4097 keys,
 // 1 / 8 / 32 / 64 rows: 144 / 163 / 388 / 742 us against 610 to 619; 32 x 6 x 1025 keys: 23 / 39 / 63 / 110 against 73 to 79.
@@ -1105,11 +1106,15 @@ constexpr int FEW_BLOCKS = 512;                              // workgroups to sp
 // SHARE 97; fp32: forward OWN 92, SHARE 98, 4 x 6 heads backward OWN 130, SHARE 120; 512 to 4096 are within 10 % of each other there.
 constexpr long SHARE_BELOW = 1024;
 inline long wavefronts(const Args& a, int columns) { return (long)a.BH * ((columns + 31) / 32); }
-// own_cols: columns of an OWN workgroup; shared: SHARED.
+// may_two: the OWN kernel can take two column blocks per wavefront (Shape::MAX_CB); shared: SHARED.
+// Two blocks or one: a CU works through its workgroups, so the time goes by the largest number that one CU gets; a workgroup of 128 columns
+// takes 0.54 of one of 256 (1025 keys, 64 channels: 12.2 and 22.5 us).  16 / 24 / 32 / 64 x 6 heads of 642 queries: two blocks 45 / 45 /
+// 74 / 103 us, one 36 / 49 / 64 / 96; 8 x 6 heads of 2562: 67, 51; 7686 rows x 4097 keys x 16: 154, 172.
 // split: where even SHARE has too few workgroups, the keys are divided as long as each part keeps two tiles
-inline Plan forward_plan(const Args& a, int own_cols, int shared, int max_few, int few_keys) {
+inline Plan forward_plan(const Args& a, bool may_two, int shared, int max_few, int few_keys) {
     Plan p;
     const int R = a.Nq * a.G;
+    p.two_blocks = false;
     p.few = R <= max_few;
     if (p.few) {
         p.share = false;
@@ -1124,7 +1129,11 @@ inline Plan forward_plan(const Args& a, int own_cols, int shared, int max_few, i
     p.share = wavefronts(a, R) < SHARE_BELOW;
     p.nsplit = 1;
     p.keys_per_split = a.Nk;
-    const int cols = p.share ? 128 / shared : own_cols, tile = 32 * shared;
+    if (may_two && !p.share) {
+        const long one = ((long)a.BH * ((R + 127) / 128) + 255) / 256, two = ((long)a.BH * ((R + 255) / 256) + 255) / 256;
+        p.two_blocks = 54 * one >= 100 * two;
+    }
+    const int cols = p.share ? 128 / shared : p.two_blocks ? 256 : 128, tile = 32 * shared;
     p.row_blocks = (R + cols - 1) / cols;
     if (p.share) {
         const int tiles = (a.Nk + tile - 1) / tile;
@@ -1151,8 +1160,9 @@ template <typename T, int DP> void launch_forward(const Args& a, const Plan& p, 
             else if (R <= 4) hipLaunchKernelGGL((few_rows_kernel<T, DF, 4>), grid, dim3(256), 0, st, a);
             else hipLaunchKernelGGL((few_rows_kernel<T, DF, 8>), grid, dim3(256), 0, st, a);
         }
-    } else if (p.share) hipLaunchKernelGGL((forward_kernel<T, DP, SHARED<T>>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((forward_kernel<T, DP, 1>), grid, dim3(256), 0, st, a);
+    } else if (p.share) hipLaunchKernelGGL((forward_kernel<T, DP, SHARED<T>, 1>), grid, dim3(256), 0, st, a);
+    else if (Shape<T, DP, 1>::MAX_CB == 1 || !p.two_blocks) hipLaunchKernelGGL((forward_kernel<T, DP, 1, 1>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((forward_kernel<T, DP, 1, Shape<T, DP, 1>::MAX_CB>), grid, dim3(256), 0, st, a);
     if (p.nsplit > 1) {
         const long n = (long)a.BH * a.Nq * a.G * (a.D / 4);
         hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);

@@ -68,7 +68,7 @@ Args make_args(const scp_cross_attn_params* p) {
 Plan plan_of(const Args& a, int dtype) {
     const bool bf16 = dtype == SCP_DTYPE_BF16;
     const int few_keys = (bf16 ? 8 : 4) * 64 / (a.D <= 32 ? 4 : a.D <= 64 ? 8 : 16);                          // Few::KEYS
-    return scp_attn::forward_plan(a, bf16 && a.D <= 64 ? 256 : 128, bf16 ? scp_attn::SHARED<__bf16> : scp_attn::SHARED<float>, scp_attn::few_rows(bf16 ? 2 : 4),
+    return scp_attn::forward_plan(a, bf16 && a.D <= 64, bf16 ? scp_attn::SHARED<__bf16> : scp_attn::SHARED<float>, scp_attn::few_rows(bf16 ? 2 : 4),
                                   few_keys);
 }
 size_t split_floats(const Args& a, const Plan& p) { return p.nsplit > 1 ? (size_t)p.nsplit * a.BH * a.Nq * a.G * (a.D + 2) : 0; }

@@ -319,7 +319,8 @@ ATTN_SHAPES = [  # batch, queries, keys, heads, kv_heads, head_dim
     (1, 1, 1, 1, 1, 64), (2, 1, 77, 6, 6, 64), (1, 3, 64, 4, 1, 64), (2, 33, 65, 2, 2, 64), (1, 128, 128, 3, 1, 64), (2, 129, 31, 6, 2, 64), (1, 200, 1025, 2, 1, 64),
     (1, 70, 97, 2, 2, 32), (1, 45, 130, 2, 1, 96), (2, 40, 100, 2, 1, 128), (1, 37, 50, 3, 3, 8), (1, 65, 70, 2, 1, 40), (1, 50, 66, 1, 1, 120), (9, 5, 257, 2, 1, 64),
     (3, 2, 4, 8, 8, 16), (1, 642, 300, 1, 1, 64), (2, 1, 4097, 4, 2, 64), (1, 9, 2050, 1, 1, 128),
-    (2, 3, 300, 2, 2, 64), (1, 1, 500, 4, 1, 96), (2, 2, 90, 4, 2, 128), (1, 1, 2050, 1, 1, 32), (20, 1, 130, 3, 3, 8), (2, 1, 700, 2, 2, 120), (1, 4, 1500, 1, 1, 40), (3, 20, 400, 2, 2, 40), (1, 17, 1100, 2, 1, 64), (1, 33, 300, 1, 1, 96)]
+    (2, 3, 300, 2, 2, 64), (1, 1, 500, 4, 1, 96), (2, 2, 90, 4, 2, 128), (1, 1, 2050, 1, 1, 32), (20, 1, 130, 3, 3, 8), (2, 1, 700, 2, 2, 120), (1, 4, 1500, 1, 1, 40), (3, 20, 400, 2, 2, 40), (1, 17, 1100, 2, 1, 64), (1, 33, 300, 1, 1, 96),
+    (16, 700, 40, 3, 3, 64), (24, 600, 33, 6, 6, 32)]
 
 
 @gpu
