@@ -356,6 +356,20 @@ def test_cross_attention_masks(dtype, nq):
 
 @gpu
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(24, 642, 161, 6, 6, 32), (48, 66, 300, 8, 2, 64), (40, 130, 193, 8, 8, 64), (33, 320, 140, 4, 4, 40), (24, 257, 129, 6, 3, 128)], ids=str)
+def test_cross_attention_many_columns(shape, dtype):
+    """enough rows and keys for workgroups of 128 of them, with short last ones of 1 to 64, or more, on either side; masked keys among them"""
+    b, nq, nk, h, hk, d = shape
+    q, k, v, go, g = attn_inputs(b, nq, nk, h, hk, d, dtype, 77)
+    mask = torch.rand(b, nk, generator=g, device="cuda") < 0.7
+    mask[0, :128] = False
+    mask[1, 128:] = False
+    k = torch.where(mask[:, :, None, None], k, torch.full_like(k, math.nan))
+    check_attn(q, k, v, go, mask)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
 def test_cross_attention_peaked_and_scaled(dtype):
     """scores of +-hundreds (the running maximum moves late), a negative and a zero scale"""
     q, k, v, go, _ = attn_inputs(1, 70, 260, 2, 1, 64, dtype, 5, spread=6.0)
