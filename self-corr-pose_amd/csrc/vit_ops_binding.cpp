@@ -71,7 +71,7 @@ Tensor tensor(const py::handle& o, const char* name, std::initializer_list<at::S
     if (t.get_device() != device)
         refuse(std::string(name) + " lives on cuda:" + std::to_string(t.get_device()) + " but the current device is cuda:" + std::to_string(device) +
                " (torch.cuda.set_device first)");
-    return t;
+    return t.is_neg() ? t.resolve_neg() : t;
 }
 Tensor operand(const py::handle& o, const char* name) { return tensor(o, name, {at::kFloat, at::kBFloat16}); }
 Tensor operand_like(const py::handle& o, const char* name, const Tensor& like) { return tensor(o, name, {like.scalar_type()}); }
@@ -261,7 +261,8 @@ struct CrossAttention : Function<CrossAttention> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &mask = saved[3], &out = saved[4], &low = saved[5], &lse = saved[6];
+        const Tensor q = addressable(saved[0]), k = addressable(saved[1]), v = addressable(saved[2]);             // a hook may have moved them
+        const Tensor &mask = saved[3], &out = saved[4], &low = saved[5], &lse = saved[6];
         Tensor gq, gk, gv;
         if (ctx->needs_input_grad(0)) gq = at::empty(q.sizes(), q.options());
         if (ctx->needs_input_grad(1)) gk = at::empty(k.sizes(), k.options());
@@ -415,6 +416,9 @@ py::tuple weight_grad8(const py::object& grad_, const py::object& codes_, const 
     return py::make_tuple(r.gw, r.gb.defined() ? py::cast(r.gb) : py::none());
 }
 
+// the library products run in their operands' type under autocast too
+struct OwnType { c10::impl::ExcludeDispatchKeyGuard guard{c10::DispatchKey::AutocastCUDA}; };
+
 struct Linear8 : Function<Linear8> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Maybe& bias_, bool keep) {
         const Tensor bias = plain(bias_);
@@ -432,6 +436,7 @@ struct Linear8 : Function<Linear8> {
         Tensor gx, gw, gb;
         {
             at::NoGradGuard no;
+            const OwnType own_type;
             if (want_x) gx = gy.matmul(weight);
             if (saved[1].defined() && (want_w || want_b)) {
                 WeightGrad r = weight_grad(gy.detach(), saved[1], saved[2], want_b);
@@ -452,6 +457,7 @@ Tensor linear8(const py::object& x_, const py::object& weight_, const py::object
         if (bias.dim() != 1 || bias.size(0) != weight.size(0)) refuse("linear8: bias must have " + std::to_string(weight.size(0)) + " entries");
     }
     py::gil_scoped_release release;
+    const OwnType own_type;
     if (wants_grad({x, weight, bias})) return Linear8::apply(x, weight, maybe(bias), wants_grad({weight, bias}))[0];
     return bias.defined() ? at::linear(x, weight, bias) : at::linear(x, weight);
 }

@@ -847,6 +847,70 @@ def test_backward_twice_over_one_forward():
         assert all(torch.equal(s, t) for s, t in list(zip(a, b))[library:])
 
 
+def _all_operators(seed=41):
+    """outputs and gradients of each operator"""
+    g = gen(seed)
+    new = lambda *s: torch.randn(*s, generator=g, device="cuda").requires_grad_(True)
+    x, r, w, b = new(40, 96), new(40, 96), new(96), new(96)
+    q, kv, lw, lb = new(2, 9, 2, 32), new(2, 70, 2, 2, 32), new(48, 96), new(48)
+    s, y = vit_ops.layer_norm(x, w, b, residual=r)
+    outs = [s, y, vit_ops.cross_attention(q, kv[:, :, 0], kv[:, :, 1]), vit_ops.gelu8(x), vit_ops.linear8(x, lw, lb)]
+    go = [torch.randn(o.shape, generator=g, device="cuda") for o in outs]
+    return outs + list(torch.autograd.grad(outs, (x, r, w, b, q, kv, lw, lb), go))
+
+
+@gpu
+def test_saved_tensors_kept_on_the_host():
+    """what the operators keep for their backward passes can be moved away by saved-tensor hooks; strided views come back contiguous"""
+    plain = _all_operators()
+    with torch.autograd.graph.save_on_cpu():
+        moved = _all_operators()
+    for i, (a, b) in enumerate(zip(plain, moved)):
+        assert torch.equal(a, b), i
+
+
+@gpu
+def test_autocast_leaves_the_types():
+    plain = _all_operators()
+    with torch.autocast("cuda", dtype=BF16):
+        cast = _all_operators()
+    for i, (a, b) in enumerate(zip(plain, cast)):
+        assert a.dtype == b.dtype == FP32 and torch.equal(a, b), i
+
+
+@gpu
+def test_lazily_negated_input():
+    x = torch.randn(5, 64, generator=gen(3), device="cuda")
+    neg = torch._neg_view(x)
+    assert neg.is_neg() and torch.equal(vit_ops.layer_norm(neg), vit_ops.layer_norm(-x)) and torch.equal(vit_ops.gelu8(neg), vit_ops.gelu8(-x))
+
+
+@gpu
+def test_two_threads_at_once():
+    """callers on two threads and streams: each gets the bits it gets alone"""
+    import threading
+    want = [_all_operators(s) for s in (51, 52)]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i] = _all_operators(51 + i)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                                   # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 @gpu
 def test_repeated_calls_give_the_same_bits():
     P, q_tok, enc, mask, go = _decoder_setup(5)
