@@ -214,17 +214,20 @@ template <typename T, int DP, int PS> struct Mma {
         }
     }
     // a[c][db][d][col] += sum_row t[r0 + row][32 db + d] p[c][row][col];  bf16: sums[c] (where given) += the p that were multiplied, half a
-    // column each
-    template <int CB> static __device__ __forceinline__ void adds(f32x16 (&a)[CB][DB], const __bf16* t, int r0, const f32x16 (&p)[CB], float* sums = nullptr) {
+    // column each; LOW: what rounding p to bf16 drops is multiplied too
+    template <int CB, bool LOW = false> static __device__ __forceinline__ void adds(f32x16 (&a)[CB][DB], const __bf16* t, int r0, const f32x16 (&p)[CB], float* sums = nullptr) {
         const int lane = threadIdx.x & 63, i = lane & 15, half = lane >> 5, cg = (lane >> 4) & 1;
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            bf16x8 b[CB][NP];
+            bf16x8 b[CB][NP], low[CB];
 #pragma unroll
             for (int c = 0; c < CB; c++) {
                 if constexpr (NP == 1) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) b[c][0][j] = (__bf16)p[c][8 * s + j];
+                    for (int j = 0; j < 8; j++) {
+                        b[c][0][j] = (__bf16)p[c][8 * s + j];
+                        if constexpr (LOW) low[c][j] = (__bf16)(p[c][8 * s + j] - (float)b[c][0][j]);
+                    }
                 } else {
                     u32x4 parts[3];
 #pragma unroll
@@ -258,6 +261,10 @@ template <typename T, int DP, int PS> struct Mma {
                         h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)at);
                     }
                     w[k] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+                if constexpr (NP == 1 && LOW) {
+#pragma unroll
+                    for (int c = 0; c < CB; c++) a[c][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[0], low[c], a[c][db], 0, 0, 0);
                 }
 #pragma unroll
                 for (int y = 0; y < PAIRS; y++)
@@ -888,7 +895,7 @@ template <typename T, int DP, int SH> struct GradLds {
 };
 
 // KV: stationary keys, streamed query rows (gk, gv); otherwise stationary query rows, streamed keys (gq)
-template <typename T, int DP, bool KV, int SH>
+template <typename T, int DP, bool KV, int SH, bool LOW>
 __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, SH>& lds, int bh, int blk) {
     typedef Shape<T, DP, SH> S;
     typedef Mma<T, DP, S::N * DP> M;
@@ -944,8 +951,8 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
                 ds[i] = p[i] * (ds[i] - dl[j]);
             }
         }
-        if constexpr (KV) M::template adds<1>(acc2, tile[buf][1], r0, pp);
-        M::template adds<1>(acc1, tile[buf][0], r0, dd);
+        if constexpr (KV) M::template adds<1, LOW>(acc2, tile[buf][1], r0, pp);
+        M::template adds<1, LOW>(acc1, tile[buf][0], r0, dd);
     };
 
     Loader<DP, N, WAVES, S::NP> first(KV ? qr : kr, a.D), second(KV ? gr : vr, a.D);
@@ -1082,15 +1089,18 @@ __device__ __forceinline__ void gradient_columns(const Args& a, GradLds<T, DP, S
 
 // Both gradients in one launch: the two kinds of workgroups of a head run next to each other, and the last, partly filled round of
 // workgroups is paid once (32 x 6 heads of 642 x 1025, bf16: two launches 142 us).
-template <typename T, int DP, int SH>
+// LOW (bf16): p and gs enter their products with 16 bits instead of 8, 10 products for 7: where there are few rows to sum over, so that single
+// roundings show (gv of one query: 2.8e-3 off without it, 1.7e-3, the rounding of gv itself, with it).  32 x 6 heads of 1 x 1025: 65 us for
+// 60; 8 x 6 heads of 2562 x 40 would be 112 for 87.
+template <typename T, int DP, int SH, bool LOW>
 __global__ __launch_bounds__(256, (Shape<T, DP, SH>::GRAD_OCC)) void backward_kernel(const Args a) {
     typedef Shape<T, DP, SH> S;
     __shared__ __attribute__((aligned(16))) GradLds<T, DP, SH> lds;
     const int nkv = a.gk || a.gv ? (a.Nk + S::COLS - 1) / S::COLS : 0, nq = a.gq ? (a.Nq * a.G + S::COLS - 1) / S::COLS : 0;
     int bh, blk;
     if (!place(a.BH, nkv + nq, bh, blk)) return;
-    if (blk < nkv) gradient_columns<T, DP, true, SH>(a, lds, bh, blk);
-    else gradient_columns<T, DP, false, SH>(a, lds, bh, blk - nkv);
+    if (blk < nkv) gradient_columns<T, DP, true, SH, LOW>(a, lds, bh, blk);
+    else gradient_columns<T, DP, false, SH, LOW>(a, lds, bh, blk - nkv);
 }
 
 // ---- launch plan --------------------------------------------------------------------------------------------------------------------
@@ -1105,6 +1115,7 @@ constexpr int FEW_BLOCKS = 512;                              // workgroups to sp
 // SHARE below so many wavefronts of 32 columns; fewer leave SIMDs empty (256 CUs x 4).  8 x 6 heads of 642 x 1025, bf16: backward pass OWN 72 us,
 // SHARE 97; fp32: forward OWN 92, SHARE 98, 4 x 6 heads backward OWN 130, SHARE 120; 512 to 4096 are within 10 % of each other there.
 constexpr long SHARE_BELOW = 1024;
+constexpr int LOW_ROWS = 16;
 inline long wavefronts(const Args& a, int columns) { return (long)a.BH * ((columns + 31) / 32); }
 // may_two: the OWN kernel can take two column blocks per wavefront (Shape::MAX_CB); shared: SHARED.
 // Two blocks or one: a CU works through its workgroups, so the time goes by the largest number that one CU gets; a workgroup of 128 columns
@@ -1177,8 +1188,12 @@ template <typename T, int DP> void launch_backward(const Args& a, hipStream_t st
     const bool share = wavefronts(a, rows) + wavefronts(a, keys) < 2 * SHARE_BELOW;
     const int cols = share ? 128 / SHARED<T> : 128;
     const dim3 grid(placed_blocks(a.BH, (rows + cols - 1) / cols + (keys + cols - 1) / cols));
-    if (share) hipLaunchKernelGGL((backward_kernel<T, DP, SHARED<T>>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((backward_kernel<T, DP, 1>), grid, dim3(256), 0, st, a);
+    constexpr bool CAN = PARTS<T> == 1;
+    const bool low = CAN && (R <= LOW_ROWS || a.Nk <= LOW_ROWS);
+    if (share && low) hipLaunchKernelGGL((backward_kernel<T, DP, SHARED<T>, CAN>), grid, dim3(256), 0, st, a);
+    else if (share) hipLaunchKernelGGL((backward_kernel<T, DP, SHARED<T>, false>), grid, dim3(256), 0, st, a);
+    else if (low) hipLaunchKernelGGL((backward_kernel<T, DP, 1, CAN>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((backward_kernel<T, DP, 1, false>), grid, dim3(256), 0, st, a);
 }
 
 // instantiated in csrc/cross_attn_f32.hip and csrc/cross_attn_bf16.hip

@@ -245,7 +245,10 @@ def attn_reference(q, k, v, mask, scale, go, dtype):
     b, nq, h, d = q.shape
     nk, hk = k.shape[1], k.shape[2]
     g = h // hk
-    e = half_step(dtype) if dtype != FP32 else 0.0                               # rounding of a probability / score gradient before a product
+    # rounding of a probability before its product with v (one row: fp32 all the way); and of a probability or a score gradient in the
+    # backward pass, which keeps 16 bits of it where one side has at most 16 rows
+    half = half_step(dtype) if dtype != FP32 else 0.0
+    e, e_back = half if nq * g > 1 else 0.0, half ** 2 if min(nq * g, nk) <= 16 else half
     if mask is not None:                                                         # values at masked keys do not exist
         k = torch.where(mask[:, :, None, None], k, torch.zeros_like(k))
         v = torch.where(mask[:, :, None, None], v, torch.zeros_like(v))
@@ -283,12 +286,12 @@ def attn_reference(q, k, v, mask, scale, go, dtype):
             + (d + 2) * U * (G * o).abs().sum(3, keepdim=True)
         d_p = d_p + e1 * p                                                       # the backward pass divides the unrounded p by the sum of the w
         d_gs = d_p * (gp - delta).abs() + p * (d_delta + (d + 4) * U * (G.abs() @ V.abs().transpose(2, 3)))
-        d_gs = d_gs + (e + 4 * U) * (gs.abs() + d_gs)
+        d_gs = d_gs + (e_back + 4 * U) * (gs.abs() + d_gs)
         n_q, n_r = (nk / 4 + 24) * U, (nq * g + 24) * U
         fold = lambda t: t.reshape(b, hk, g, nk, d).sum(2).permute(0, 2, 1, 3)
         for name, val, err in (("gq", back(scale * gs @ K), back(abs(scale) * (d_gs + n_q * gs.abs()) @ K.abs())),
                                ("gk", fold(scale * gs.transpose(2, 3) @ Q), fold(abs(scale) * (d_gs + n_r * gs.abs()).transpose(2, 3) @ Q.abs())),
-                               ("gv", fold(p.transpose(2, 3) @ G), fold((d_p + (e + n_r) * p).transpose(2, 3) @ G.abs()))):
+                               ("gv", fold(p.transpose(2, 3) @ G), fold((d_p + (e_back + n_r) * p).transpose(2, 3) @ G.abs()))):
             out[name] = (val, err + half_step(dtype) * (val.abs() + err))
     return out
 
