@@ -14,8 +14,9 @@
 //   * the rows are split so that about one workgroup per CU runs; each writes an fp32 partial tile and a second kernel adds the partials in
 //     order (bit-reproducible).  gb falls out of the registers of the filling wavefronts of the first column of tiles.
 // Bound by filling and multiplying together, not by memory: of 77 us for 32800 rows, 384 -> 1536, bf16 (with pack8 9 and the fold 6.5), 62 are
-// left without the products, 55 without the filling, 28 without both; steps of 64 rows instead of 32 halve the barriers: 69 us.  The
-// kernel alone: 58 us, 660 TFLOP/s; 1536 -> 384, fp32 131 us, 3 x 295.
+// left without the products, 55 without the filling, 28 without both; steps of 64 rows instead of 32 halve the barriers (69), addresses that
+// are constants of the loop and rows past the end read as zeros: 67 us.  The kernel alone: 57 us, 680 TFLOP/s; 1536 -> 384, fp32 131 us,
+// 3 x 295.
 #include <hip/hip_runtime.h>
 
 #include "scp_common.h"

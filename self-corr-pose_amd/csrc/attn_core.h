@@ -28,7 +28,7 @@
 // problems that would leave SIMDs empty otherwise.  FEW: no tiles, see few_rows_kernel.  Tiles are double-buffered (the next one in flight
 // during the products) where two fit 80 KB.
 // Measured: bf16 forward of 2562 x 4097, 8 x 6 heads of 64 on 2, 156 us (830 TFLOP/s); forward + backward of 642 x 1025, 32 x 6 heads, a padded
-// batch, 178 us; what bounds both is matrix and vector instructions, which overlap to about 70 % of their sum.
+// batch, 174 us; what bounds both is matrix and vector instructions, which overlap to about 70 % of their sum.
 //
 // LDS tiles are filled by buffer loads that write LDS directly, 16 bytes per lane.  A lane whose row is masked, past the end, or whose
 // channel is past head_dim gets an out-of-range offset: the hardware writes zeros, so nothing stored there can reach a product.  The
