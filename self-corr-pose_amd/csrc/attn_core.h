@@ -1109,9 +1109,11 @@ struct Plan { bool share, few, two_blocks; int nsplit, keys_per_split, row_block
 // fp32, where the matrix kernels first write the tensors' parts (6 bytes an element) and read them again: 64 x 6 heads of 64 x 4097 keys,
 // 1 / 8 / 32 / 64 rows: 144 / 163 / 388 / 742 us against 610 to 619; 32 x 6 x 1025 keys: 23 / 39 / 63 / 110 against 73 to 79.
 // bf16, where they read the tensors: 64 x 6 x 4097 keys, 1 / 2 / 4 rows: 76 / 80 / 93 us against 74 to 75, but 32 x 6 x 1025 keys, 1 row:
-// 15.7 against 18.5, 32 x 8 heads of 128: 29 against 41; so one row only.
+// 13.5 against 18.5, 32 x 8 heads of 128: 27 against 41; so one row only.
 constexpr int few_rows(int size) { return size == 4 ? 32 : 1; }
-constexpr int FEW_BLOCKS = 512;                              // workgroups to split the keys for: 1024 and more only make the join longer (32 x 6 x 1025 fp32 24.4 us, 512: 22.7)
+// workgroups to split the keys for: a second launch for the join costs 3 to 4 us.  192 / 384 / 512: 32 x 6 x 1025 keys fp32 19.7 / 22.0 / 22.4 us,
+// bf16 15.1 / 15.9 / 16.4; 64 x 6 x 257 bf16 7.1 / 7.1 / 10.2; 16 x 6 x 4097 bf16 27.0 / 24.2 / 25.9, fp32 36.2 / 36.9 / 38.6
+constexpr int FEW_BLOCKS = 192;
 // SHARE below so many wavefronts of 32 columns; fewer leave SIMDs empty (256 CUs x 4).  8 x 6 heads of 642 x 1025, bf16: backward pass OWN 72 us,
 // SHARE 97; fp32: forward OWN 92, SHARE 98, 4 x 6 heads backward OWN 130, SHARE 120; 512 to 4096 are within 10 % of each other there.
 constexpr long SHARE_BELOW = 1024;
