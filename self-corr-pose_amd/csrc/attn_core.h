@@ -1151,7 +1151,10 @@ inline Plan forward_plan(const Args& a, bool may_two, int shared, int max_few, i
     if (p.share) {
         const int tiles = (a.Nk + tile - 1) / tile;
         const long blocks = (long)a.BH * p.row_blocks;
-        int want = blocks >= 512 ? 1 : (int)(512 / blocks);
+        // 256 / 512: bf16 4 x 6 heads of 64 x 4097 19 / 22 us, 16 x 6 of 40 x 1025 15 / 18 (the join is a second launch); fp32, whose workgroups take
+        // longer, 16 x 6 of 40 x 1025 52 / 47, 4 x 6 of 64 x 4097 56 / 57
+        const int target = shared == SHARED<__bf16> ? 256 : 512;
+        int want = blocks >= target ? 1 : (int)(target / blocks);
         if (want > tiles / 2) want = tiles / 2 > 0 ? tiles / 2 : 1;
         const int per = (tiles + want - 1) / want;
         p.nsplit = (tiles + per - 1) / per;
