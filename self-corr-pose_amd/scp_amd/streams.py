@@ -42,7 +42,7 @@ def stamp_status():
         return False, "no readable stamp (%s)" % (e,)
     import torch
     if (torch.__version__, str(torch.version.hip)) != (want.get("torch"), want.get("hip")):
-        return False, "scanned torch %s / HIP %s, running torch %s / HIP %s" % (want.get("torch"), want.get("hip"), torch.__version__,
+        return False, "stamped torch %s / HIP %s, running torch %s / HIP %s" % (want.get("torch"), want.get("hip"), torch.__version__,
                                                                                 torch.version.hip)
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     h, n = hashlib.sha256(), 0
@@ -53,12 +53,12 @@ def stamp_status():
                 h.update(("%s:%d;" % (f, os.path.getsize(os.path.join(d, f)))).encode())
                 n += 1
     if (n, h.hexdigest()[:16]) != (want.get("code_objects"), want.get("digest")):
-        return False, "the library GEMM code objects differ from the scanned ones (%d files, digest %s)" % (n, h.hexdigest()[:16])
-    return True, "scan matches torch %s / HIP %s" % (want["torch"], want["hip"])
+        return False, "the library GEMM files differ from the stamped ones (%d files, digest %s)" % (n, h.hexdigest()[:16])
+    return True, "stamp matches torch %s / HIP %s" % (want["torch"], want["hip"])
 
 
 def _default_mode():
-    """`overlap` only for an installation the shipped scan vouches for; anything else gets the one-stream schedule and one line that
+    """`overlap` only for an installation the shipped stamp vouches for; anything else gets the one-stream schedule and one line that
     says why (SCP_STREAMS=overlap overrides: the dynamic screen, tests/test_coresidency_gpu.py, is then the only evidence)"""
     ok, why = stamp_status()
     if ok:
