@@ -79,24 +79,7 @@ class MeshNet(nn.Module):
 
         occ_arg = occ if opts.use_occ else None
         cam = (foc_crop, pp_crop, rotation, translation)
-        # The soft-texture pass and its loss share nothing with the mask / depth / canonical-xyz group but their inputs: with
-        # SCP_TEXTURE_STREAM=1 they run on a side stream of their own (off by default since round 6, streams.overlap_texture()).  Both chains are rasteriser launches (VALU-bound, far from filling the device)
-        # strung together by small latency-bound kernels, forward and -- autograd replays nodes on their forward stream --
-        # backward; side by side they shorten the step's serial middle part.
-        tex_side = opts.train and img.is_cuda and tex is not None and getattr(self, "overlap_texture_pass", streams.overlap_texture())
-        if tex_side:
-            if getattr(self, "_tex_stream", None) is None:
-                self._tex_stream = streams.side_stream(img.device)
-            main = torch.cuda.current_stream(img.device)
-            self._tex_stream.wait_stream(main)
-            with torch.cuda.stream(self._tex_stream):
-                streams.crumb("texture pass: start")
-                texture_loss = wts.tex_wt * self._texture_loss(pred_v, faces, tex, cam, img, mask, occ_arg).mean(0)
-                streams.crumb("texture pass: done")
-            for t in (pred_v, faces, tex, foc_crop, pp_crop, rotation, translation, img, mask) + ((occ_arg,) if occ_arg is not None else ()):
-                t.record_stream(self._tex_stream)
-        else:
-            texture_loss = wts.tex_wt * self._texture_loss(pred_v, faces, tex, cam, img, mask, occ_arg).mean(0)
+        texture_loss = wts.tex_wt * self._texture_loss(pred_v, faces, tex, cam, img, mask, occ_arg).mean(0)
         # fused per-pixel losses (csrc/losses.hip) when they cover the configuration, the torch compositions otherwise
         fused = (getattr(self, "fuse_image_losses", True) and occ_arg is None and opts.use_depth and not opts.depth_loss_chamfer
                  and self.renderer.shares_mask_with_depth() and fused_losses.covers(img, mask, depth, match))
@@ -134,9 +117,6 @@ class MeshNet(nn.Module):
             cycle_loss = self.corr_net.compute_rotation_cycle_loss(img, mask, img_feat, self.encoder,
                                                                    angle=self.rotation_angle)[0] * wts.cycle_loss_wt
 
-        if tex_side:
-            torch.cuda.current_stream(img.device).wait_stream(self._tex_stream)
-            texture_loss.record_stream(torch.cuda.current_stream(img.device))
         total_loss = (mask_loss + symmetry_loss + triangle_loss + deform_loss + pullfar_loss + texture_loss +
                       match_loss + imatch_loss + cycle_loss_pt + cycle_loss)
         if opts.use_depth:

@@ -3,7 +3,7 @@
 SCP_STREAMS=overlap (default): the frozen-DINO ViT and the rotation-cycle branch (second encoder pass) run on side HIP streams of the
 step's own (side_stream below), Trainer.step() starts the NEXT batch's ViT pass during this step's backward (look-ahead) and the gradient
 buckets are all-reduced from inside backward.  ~6 ms per step faster at B = 32 than one stream (29.2-30.5 vs 36.2 ms on one MI355X).
-The soft-texture render pass on a THIRD side stream (-0.4 ms) is opt-in, SCP_TEXTURE_STREAM=1: see overlap_texture() for why.
+The soft-texture render pass stays on the main stream: see the refusal of SCP_TEXTURE_STREAM below.
 SCP_STREAMS=serial: one HIP stream; kernels of the step never run side by side.
 
 Why this was `serial` for half a round, and why it no longer has to be.  Round 4 found kernels returning different results
@@ -78,17 +78,13 @@ def overlap():
     return MODE == "overlap"
 
 
-def overlap_texture():
-    """the soft-texture render pass + its loss on a THIRD side stream?  Off by default since round 6 (SCP_TEXTURE_STREAM=1 switches it on).
-    With three side streams (frozen ViT, rotation-cycle pass, texture pass) the step loop has stream placements at which the device stops
-    -- every stream waiting on an event, no wavefront resident; with ROC_CPU_WAIT_FOR_SIGNAL=1 the host blocks instead -- in 60-100 % of
-    fresh processes: torch pool entries (3,4,5) / (4,5,6) after other users of the pool, the step's own streams as the 5th-7th or 8th-10th
-    stream of the process, with 4 or 16 hardware queues alike (profiles/r06_stall_rates_call4..8.txt, ~600 processes of
-    tools/r06/hang_repro.py; this is what hung round 5's GPU suite).  With the texture pass on the main stream -- two side streams -- 0 of
-    98 processes stalled over 14 placements, pool and own streams (profiles/r06_stall_rates_call10.txt); the cause sits below this code
-    (torch 2.10.0+rocm7.0 / HIP 7.0.51831) and is not understood, so the default is the schedule that has no known stalling placement.
-    Cost: DESIGN 5.4."""
-    return overlap() and os.environ.get("SCP_TEXTURE_STREAM", "0") == "1"
+# A third side stream (SCP_TEXTURE_STREAM=1, the soft-texture render pass; -0.4 ms) is refused.  With three side streams (frozen ViT,
+# rotation-cycle pass, texture pass) the step loop has stream placements at which the device stops -- every stream waiting on an event, no
+# wavefront resident -- in 60-100 % of fresh processes, on pool and own streams, with 4 or 16 hardware queues alike
+# (profiles/r06_stall_rates_call4..8.txt).  With the texture pass on the main stream 0 of 98 processes stalled over 14 placements
+# (profiles/r06_stall_rates_call10.txt); the cause sits below this code (torch 2.10.0+rocm7.0 / HIP 7.0.51831) and is not understood.
+if os.environ.get("SCP_TEXTURE_STREAM", "0") not in ("", "0"):
+    raise RuntimeError("scp_amd.streams: SCP_TEXTURE_STREAM is not supported: with a third side stream the device can stop; unset it")
 
 
 class DeviceStall(RuntimeError):
@@ -171,7 +167,7 @@ def crumb_report(named_streams=None):
 # SCP_SIDE_STREAMS=own (default): a side stream is a HIP stream this build creates for the purpose (scp_stream_create), wrapped as a
 # torch.cuda.ExternalStream -- a fresh stream nobody used before.  SCP_SIDE_STREAMS=pool: torch.cuda.Stream(), i.e. the next entry of
 # torch's round-robin pool of 32 long-lived streams per device, whose earlier users (other libraries, earlier phases of the process) and
-# hardware-queue placement the step knows nothing about.  Round 6: with the three side streams of the step on pool entries
+# hardware-queue placement the step knows nothing about.  With three side streams of the step on pool entries
 # that had been used before, the step loop stalled on the device -- every stream waiting, no wavefront resident -- in 24 of 30 fresh
 # processes at one pool position and in none at any other; the GPU suite hit that position whenever test_coresidency_gpu.py had run first.
 SIDE_STREAMS = os.environ.get("SCP_SIDE_STREAMS", "own")
@@ -191,7 +187,7 @@ def _new_own_stream(index):
 
 
 def side_stream(device):
-    """a stream for one overlapped branch of the step (frozen ViT, rotation-cycle pass, texture pass, gradient all-reduce)"""
+    """a stream for one overlapped branch of the step (frozen ViT, rotation-cycle pass, gradient all-reduce)"""
     import torch
     if SIDE_STREAMS != "own":
         return torch.cuda.Stream(device=device)

@@ -217,9 +217,8 @@ class Trainer:
         # are cached per process; a perturbed search can settle on slower solvers for the whole run).
         serial = (self._steps_done == 0 or not streams.overlap()) and self.device.type == "cuda"
         if serial:
-            saved = tuple(getattr(self.model, k, d) for k, d in (("overlap_dino", streams.overlap()), ("overlap_rotation_cycle", streams.overlap()),
-                                                                 ("overlap_texture_pass", streams.overlap_texture())))
-            self.model.overlap_dino = self.model.overlap_rotation_cycle = self.model.overlap_texture_pass = False
+            saved = tuple(getattr(self.model, k, streams.overlap()) for k in ("overlap_dino", "overlap_rotation_cycle"))
+            self.model.overlap_dino = self.model.overlap_rotation_cycle = False
             next_data = None
         try:
             streams.crumb("step %d: start" % self.iteration)
@@ -231,7 +230,7 @@ class Trainer:
             streams.crumb("step %d: backward done" % self.iteration)
         finally:
             if serial:
-                self.model.overlap_dino, self.model.overlap_rotation_cycle, self.model.overlap_texture_pass = saved
+                self.model.overlap_dino, self.model.overlap_rotation_cycle = saved
         self._steps_done += 1
         grad = self.collect_grad()
         streams.crumb("step %d: clip done" % self.iteration)
@@ -287,7 +286,7 @@ class Trainer:
             return {}
         m = self.model
         out = {"main": torch.cuda.current_stream(self.device),
-               "rotation-cycle side stream": getattr(m, "_cycle_stream", None), "texture-pass side stream": getattr(m, "_tex_stream", None),
+               "rotation-cycle side stream": getattr(m, "_cycle_stream", None),
                "frozen-ViT side stream": getattr(m.pretrain_corr_net, "_side_stream", None),
                "all-reduce stream": getattr(self.grads, "comm_stream", None)}
         return {k: v for k, v in out.items() if v is not None}

@@ -426,29 +426,23 @@ def test_training_reduces_the_loss_on_a_fixed_batch():
 
 
 def test_step_loop_does_not_stall_at_the_known_bad_stream_placements():
-    """Round 5's GPU suite hung in Trainer.train.  Round 6 reproduced it without pytest or DataLoader
-    (tools/r06/hang_repro.py, one trial per fresh process): eight steps of the B = 6 loop with look-ahead stop on the device -- every stream
-    waiting, no wavefront resident -- in 60-100 % of the processes when the step runs THREE side streams and those sit at certain
-    placements (torch pool entries (3,4,5) after 35 or 3 other used streams; own streams after 3), and in 0 of 98 processes over 14
-    placements with the texture pass on the main stream (profiles/r06_stall_rates_call4..10.txt).  The default schedule (two side
-    streams of the step's own) must run through at the placements that stalled, with and without the multi-GPU schedule's communication
-    stream (one-rank RCCL group); the three-stream schedule on pool streams runs once as a control and is REPORTED, not asserted (it
-    stalls on most boxes, which is the point)."""
+    """With three side streams the step loop had stream placements at which the device stopped, every stream waiting and no wavefront
+    resident (profiles/r06_stall_rates_call4..10.txt); the default schedule, two side streams of the step's own and the texture pass on
+    the main stream, did not stop at any of 14.  It must run through at three of those placements, with and without the multi-GPU
+    schedule's communication stream (one-rank RCCL group).  One trial per fresh process (tests/step_trial.py), every wait bounded."""
     import os
     import subprocess
     import sys
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    script = os.path.join(root, "tools", "r06", "hang_repro.py")
+    script = os.path.join(root, "tests", "step_trial.py")
 
     def trial(pre, **env):
-        e = dict(os.environ, SCP_DEVICE_TIMEOUT_S="10", SCP_REPRO_ITERS="8", **env)
-        for k in ("SCP_TEXTURE_STREAM", "SCP_SIDE_STREAMS", "SCP_FORCE_COLLECTIVES"):
+        e = dict(os.environ, SCP_DEVICE_TIMEOUT_S="10", **env)
+        for k in ("SCP_SIDE_STREAMS", "SCP_FORCE_COLLECTIVES"):
             if k not in env:
                 e.pop(k, None)
-        r = subprocess.run([sys.executable, script, str(pre), "steps"], env=e, capture_output=True, text=True, timeout=150)
+        r = subprocess.run([sys.executable, script, str(pre)], env=e, capture_output=True, text=True, timeout=150)
         lines = [l for l in r.stdout.splitlines() if l.startswith(("OK", "HANG"))]
         return lines[-1] if lines else "?? rc=%d %s" % (r.returncode, (r.stdout + r.stderr)[-400:])
     got = [trial(35), trial(3), trial(0), trial(35, SCP_FORCE_COLLECTIVES="1")]
     assert all(g.startswith("OK") for g in got), got
-    control = trial(35, SCP_TEXTURE_STREAM="1", SCP_SIDE_STREAMS="pool")
-    print("control (three side streams on pool entries 3,4,5): %s" % control[:4])

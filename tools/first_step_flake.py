@@ -39,10 +39,10 @@ for i in range(int(sys.argv[3]) if len(sys.argv) > 3 else 3):
     pc.topk_override = ref["topk"].to(device)
     bench.pin_encoder_outputs(tr.model, ref["geometry"], ref["features"])
     if os.environ.get("FLAKE_SERIAL") == "1":
-        tr.model.overlap_dino = tr.model.overlap_rotation_cycle = tr.model.overlap_texture_pass = False
-    only = os.environ.get("FLAKE_ONLY")             # dino | cycle | tex: that side stream alone
+        tr.model.overlap_dino = tr.model.overlap_rotation_cycle = False
+    only = os.environ.get("FLAKE_ONLY")             # dino | cycle: that side stream alone
     if only:
-        tr.model.overlap_dino, tr.model.overlap_rotation_cycle, tr.model.overlap_texture_pass = only == "dino", only == "cycle", only == "tex"
+        tr.model.overlap_dino, tr.model.overlap_rotation_cycle = only == "dino", only == "cycle"
     stub = os.environ.get("FLAKE_STUB")             # vit: no ViT kernels (keys = zeros); nn: no mutual-NN kernel; blocks=<n>: only n ViT blocks
     if stub == "vit":
         kt = pc.net.key_tokens
