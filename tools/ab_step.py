@@ -34,14 +34,3 @@ for attr in sys.argv[1:]:
             for _ in range(3):
                 tr.step(data)
             print("%s=%s: %.2f ms/step" % (attr, val, timed()), flush=True)
-
-if os.environ.get("AB_PRIORITY") == "1":
-    hs = torch.cuda.Stream(priority=-1)
-    hs.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(hs):
-        for val in (True, False, True, False):
-            tr.model.eager_cycle_backward = val
-            for _ in range(3):
-                tr.step(data)
-            print("main stream HIGH priority, eager_cycle_backward=%s: %.2f ms/step" % (val, timed()), flush=True)
-    torch.cuda.current_stream().wait_stream(hs)
