@@ -418,6 +418,21 @@ py::tuple weight_grad8(const py::object& grad_, const py::object& codes_, const 
 
 // the library products run in their operands' type under autocast too
 struct OwnType { c10::impl::ExcludeDispatchKeyGuard guard{c10::DispatchKey::AutocastCUDA}; };
+// t [..., c] as a contiguous matrix.  The library products are two-dimensional: a strided tensor of more dimensions would become a batched
+// product with a transposed view as its right operand, which has faulted the GPU in bf16.
+Tensor as_matrix(const Tensor& t) {
+    const int64_t c = t.size(-1);
+    return t.contiguous().view({t.numel() / c, c});
+}
+std::vector<int64_t> with_last(const Tensor& like, int64_t c) {
+    std::vector<int64_t> s = like.sizes().vec();
+    s.back() = c;
+    return s;
+}
+Tensor linear(const Tensor& x, const Tensor& weight, const Tensor& bias) {
+    const Tensor y = bias.defined() ? at::linear(as_matrix(x), weight, bias) : at::linear(as_matrix(x), weight);
+    return at::_unsafe_view(y, with_last(x, weight.size(0)));                       // not a view of it: a caller may change the result in place
+}
 
 struct Linear8 : Function<Linear8> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Maybe& bias_, bool keep) {
@@ -426,20 +441,21 @@ struct Linear8 : Function<Linear8> {
         if (keep) p = pack(x.contiguous());
         ctx->save_for_backward({weight, p.codes, p.exps});
         ctx->saved_data["present"] = present({x, weight, bias});
-        return {bias.defined() ? at::linear(x, weight, bias) : at::linear(x, weight)};
+        return {linear(x, weight, bias)};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &weight = saved[0], &gy = grads[0];
+        const Tensor &weight = saved[0];
         Wanted wanted{ctx, ctx->saved_data["present"].toInt()};
         const bool want_x = wanted(), want_w = wanted(), want_b = wanted();
         Tensor gx, gw, gb;
         {
             at::NoGradGuard no;
             const OwnType own_type;
-            if (want_x) gx = gy.matmul(weight);
+            const Tensor gy = as_matrix(grads[0]);
+            if (want_x) gx = at::_unsafe_view(gy.mm(weight), with_last(grads[0], weight.size(1)));
             if (saved[1].defined() && (want_w || want_b)) {
-                WeightGrad r = weight_grad(gy.detach(), saved[1], saved[2], want_b);
+                WeightGrad r = weight_grad(gy, saved[1], saved[2], want_b);
                 if (want_w) gw = r.gw.to(weight.scalar_type());
                 if (r.gb.defined()) gb = r.gb.to(weight.scalar_type());
             }
@@ -459,7 +475,7 @@ Tensor linear8(const py::object& x_, const py::object& weight_, const py::object
     py::gil_scoped_release release;
     const OwnType own_type;
     if (wants_grad({x, weight, bias})) return Linear8::apply(x, weight, maybe(bias), wants_grad({weight, bias}))[0];
-    return bias.defined() ? at::linear(x, weight, bias) : at::linear(x, weight);
+    return linear(x, weight, bias);
 }
 
 }  // namespace
