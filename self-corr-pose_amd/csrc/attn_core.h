@@ -145,19 +145,24 @@ template <> struct Out<__bf16> {
             }
         }
     }
-    // The 8 bits of a number that follow its bf16 rounding, signed: (bits - rounded bits) >> 8, whole numbers both, is in -128 .. 127; with
-    // half a step of it added the number comes back to 2^-16 of itself.
+    // The 8 bits of a number that follow its bf16 rounding, signed: (bits - rounded bits) >> 8, whole numbers both, is in -128 .. 128 (a tie
+    // that rounds down to even is +128) and is kept as at most 127; with half a step of it added the number comes back to 2^-16 of itself.
     static __device__ __forceinline__ unsigned low_bits(float a, float b, float c, float d) {
         const float x[4] = {a, b, c, d};
         unsigned out = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float top = (float)(__bf16)x[i];
-            out |= (((__float_as_uint(x[i]) - __float_as_uint(top)) >> 8) & 0xffu) << (8 * i);
+            const int rest = min((int)(__float_as_uint(x[i]) - __float_as_uint(top)), 0x7fff);
+            out |= ((unsigned)(rest >> 8) & 0xffu) << (8 * i);
         }
         return out;
     }
-    static __device__ __forceinline__ float with_low(float top, int code) { return __uint_as_float(__float_as_uint(top) + (unsigned)(code * 256 + 128)); }
+    // (an infinity stays one; a NaN's rest is of no account)
+    static __device__ __forceinline__ float with_low(float top, int code) {
+        const unsigned bits = __float_as_uint(top);
+        return __uint_as_float((bits & 0x7f800000u) == 0x7f800000u ? bits : bits + (unsigned)(code * 256 + 128));
+    }
     static __device__ __forceinline__ void store_low(signed char* p, float a, float b, float c, float d) { *reinterpret_cast<unsigned*>(p) = low_bits(a, b, c, d); }
 };
 template <> struct Out<float> {

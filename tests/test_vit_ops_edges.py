@@ -1,10 +1,93 @@
 """scp_amd.vit_ops at calls that tests/test_vit_ops.py does not make: exact ties, lazily negated gradients, forward-mode derivatives and
 tracing, problems past a launch's limits, infinities, many steps of the pipelines.  Tolerances are bounds per element as there."""
+import ctypes
+
 import pytest
 import torch
 
 from scp_amd import vit_ops
-from test_vit_ops import BF16, FP32, U, gen, gpu, half_step, wgrad_reference, within
+from test_vit_ops import BF16, FP32, U, attn_inputs, attn_reference, gen, gpu, half_step, wgrad_reference, within
+
+
+# ---- cross attention: the bits of the output that its rounding drops ----------------------------------------------------------------------
+TIES = [  # batch, queries, keys, heads, kv_heads, attended keys (None: all); the forms of the forward pass
+    (3, 1, 2, 2, 2, None), (2, 40, 4, 2, 1, None), (24, 250, 4, 6, 6, None), (24, 700, 2, 6, 6, None), (1, 1, 2050, 1, 1, 4), (1, 40, 2050, 2, 2, 2)]
+
+
+def _even_weights(shape, seed):
+    b, nq, nk, h, hk, kept = shape
+    g = gen(seed)
+    new = lambda *s: torch.randn(*s, generator=g, device="cuda").to(BF16)
+    k, v = new(b, nk, hk, 64), new(b, nk, hk, 64)
+    mask = None
+    if kept is not None:
+        mask = torch.zeros(b, nk, dtype=torch.bool, device="cuda")
+        mask[:, torch.linspace(3, nk - 2, kept).long()] = True
+    return torch.zeros(b, nq, h, 64, device="cuda", dtype=BF16), k, v, mask, g
+
+
+@gpu
+@pytest.mark.parametrize("shape", TIES, ids=str)
+def test_attention_output_low_bits_at_ties(shape):
+    """q = 0: the output is the mean of 2 or 4 values of 8 bits, half-way between two bf16 numbers for one element in ten.  The bf16 output
+    and its low byte together are within half a step of the byte, 2^-16 of the value, and 4 roundings of the sum."""
+    from scp_amd import capi
+    b, nq, nk, h, hk, kept = shape
+    q, k, v, mask, _ = _even_weights(shape, sum(shape[:5]))
+    p = capi.CrossAttnParams()
+    p.batch, p.queries, p.keys, p.heads, p.kv_heads, p.head_dim, p.dtype, p.scale = b, nq, nk, h, hk, 64, 1, 1.0
+    for f, t in (("q_stride", q), ("k_stride", k), ("v_stride", v)):
+        getattr(p, f)[:] = t.stride()[:3]
+    lib = capi.lib()
+    ws = torch.empty(lib.scp_cross_attention_forward_workspace(ctypes.byref(p)) + 16, dtype=torch.uint8, device="cuda")
+    out, low = torch.empty_like(q), torch.empty(q.shape, dtype=torch.int8, device="cuda")
+    at = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())
+    m8 = None if mask is None else mask.to(torch.uint8)
+    assert lib.scp_cross_attention_forward(at(q), at(k), at(v), at(m8), ctypes.byref(p), at(out), at(low), None, at(ws), ws.numel(), capi.current_stream()) == 0
+    on = torch.ones(b, nk, dtype=torch.float64, device="cuda") if mask is None else mask.double()
+    wide = v.double().repeat_interleave(h // hk, 2)
+    w = on / on.sum(1, keepdim=True)
+    ref = torch.einsum("bn,bnhd->bhd", w, wide)[:, None].expand(b, nq, h, 64)
+    mean_abs = torch.einsum("bn,bnhd->bhd", w, wide.abs())[:, None].expand(b, nq, h, 64)
+    ties = (ref != ref.to(BF16).double()) & (ref == 0.5 * (ref.to(BF16).double() + (2 * ref - ref.to(BF16).double()).to(BF16).double()))
+    assert ties.double().mean() > 0.03
+    restored = (out.float().view(torch.int32) + low.int() * 256 + 128).view(FP32)
+    within(restored, ref, 2.0 ** -16 * ref.abs() + 4 * U * mean_abs, "output with its low bits")
+
+
+@gpu
+@pytest.mark.parametrize("shape", TIES[:4], ids=str)
+def test_attention_gradient_at_ties(shape):
+    """two values that are each other with neighbouring channels swapped, a gradient that is the same for both of a pair: gO . v = gO . o for
+    every key, gs = 0 and gq = 0.  What may be left: 2^-16 of o in delta, the roundings of two sums of 64 products, of gs, and of gq itself."""
+    b, nq, nk, h, hk, _ = shape
+    q, k, v, _, g = _even_weights((b, nq, 2, h, hk, None), 5 + sum(shape[:5]))
+    v[:, 1] = v[:, 0].unflatten(-1, (32, 2)).flip(-1).flatten(-2)
+    go = torch.randn(b, nq, h, 32, 1, generator=g, device="cuda").expand(-1, -1, -1, -1, 2).flatten(-2).to(BF16)
+    leaf = q.requires_grad_(True)
+    gq, = torch.autograd.grad(vit_ops.cross_attention(leaf, k, v, scale=1.0), leaf, go)
+    G, V, K = go.double(), v.double().repeat_interleave(h // hk, 2), k.double().repeat_interleave(h // hk, 2)
+    o = V.mean(1, keepdim=True)
+    d_delta = (G.abs() * (2.0 ** -16 * o.abs() + 8 * U * V.abs().mean(1, keepdim=True))).sum(-1) + 66 * U * (G * o).abs().sum(-1)
+    d_gp = 66 * U * (G.abs()[:, :, None] * V.abs()[:, None]).sum(-1)                              # b, q, key, head
+    d_gs = 0.5 * (d_gp + d_delta[:, :, None]) * (1 + 2.0 ** -8)
+    bound = (d_gs[..., None] * K.abs()[:, None]).sum(2) * (1 + 2.0 ** -7)
+    within(gq, torch.zeros_like(bound), bound, "gq")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("nq", [1, 40, 700])
+def test_attention_gradients_asked_for_one_by_one(dtype, nq):
+    """any of gq, gk, gv alone or in pairs"""
+    q, k, v, go, _ = attn_inputs(2, nq, 150, 4, 2, 64, dtype, 13)
+    ref = attn_reference(q, k, v, None, 64 ** -0.5, go, dtype)
+    for bits in range(1, 7):
+        ls = [t.detach().requires_grad_(bool(bits >> i & 1)) for i, t in enumerate((q, k, v))]
+        wanted = [t for t in ls if t.requires_grad]
+        got = torch.autograd.grad(vit_ops.cross_attention(*ls), wanted, go)
+        for a, name in zip(got, [f for i, f in enumerate(("gq", "gk", "gv")) if bits >> i & 1]):
+            within(a, *ref[name], "%s of %d" % (name, bits))
 
 
 # ---- linear8 ----------------------------------------------------------------------------------------------------------------------------------------
