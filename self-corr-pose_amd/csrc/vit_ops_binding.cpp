@@ -105,6 +105,8 @@ struct Wanted {                                                      // asked fo
         return is && ctx->needs_input_grad(next++);
     }
 };
+// an incoming gradient as its memory holds it: autograd hands on tensors whose negation is only a bit of theirs
+Tensor resolved(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 // Gradients of a backward pass that is itself recorded (create_graph) cannot be differentiated again: they get a node that says so.
 variable_list first_order(variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -145,7 +147,7 @@ struct LayerNorm : Function<LayerNorm> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         Wanted wanted{ctx, ctx->saved_data["present"].toInt()};
         const bool want_x = wanted(), want_r = wanted(), want_w = wanted(), want_b = wanted();
-        const Tensor gsum = grads.size() == 2 ? grads[0] : Tensor(), gy = grads.back();
+        const Tensor gsum = grads.size() == 2 ? resolved(grads[0]) : Tensor(), gy = resolved(grads.back());
         if (!gy.defined()) return {want_x ? gsum : Tensor(), want_r ? gsum : Tensor(), {}, {}, {}};            // only the sum was used
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &s = saved[0], &weight = saved[1], &stats = saved[2];
@@ -271,7 +273,7 @@ struct CrossAttention : Function<CrossAttention> {
             for (Tensor* g : {&gq, &gk, &gv})
                 if (g->defined()) g->zero_();
         } else {
-            const Tensor g = addressable(grads[0]);
+            const Tensor g = addressable(resolved(grads[0]));
             scp_cross_attn_params p = attention_params(q, k, v, ctx->saved_data["scale"].toDouble());
             strides(g, p.g_stride);
             const size_t bytes = lib.scp_cross_attention_backward_workspace_(&p);
@@ -366,7 +368,7 @@ struct Gelu8 : Function<Gelu8> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor gy = grads[0].contiguous();
+        const Tensor gy = resolved(grads[0]).contiguous();
         Tensor gx = at::empty(gy.sizes(), gy.options());
         if (gy.numel())
             check(lib.scp_gelu8_backward_(ptr<signed char>(saved[0]), ptr<unsigned char>(saved[1]), gy.data_ptr(), gy.numel() / gy.size(-1), (int)gy.size(-1), type_of(gy),
@@ -452,7 +454,7 @@ struct Linear8 : Function<Linear8> {
         {
             at::NoGradGuard no;
             const OwnType own_type;
-            const Tensor gy = as_matrix(grads[0]);
+            const Tensor gy = as_matrix(resolved(grads[0]));
             if (want_x) gx = at::_unsafe_view(gy.mm(weight), with_last(grads[0], weight.size(1)));
             if (saved[1].defined() && (want_w || want_b)) {
                 WeightGrad r = weight_grad(gy, saved[1], saved[2], want_b);

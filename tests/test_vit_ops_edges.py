@@ -90,6 +90,45 @@ def test_attention_gradients_asked_for_one_by_one(dtype, nq):
             within(a, *ref[name], "%s of %d" % (name, bits))
 
 
+# ---- incoming gradients and other kinds of derivatives --------------------------------------------------------------------------------------
+def _calls(seed=71, dtype=FP32):
+    """(name, output, leaves) of every operator with a gradient"""
+    g = gen(seed)
+    new = lambda *s: torch.randn(*s, generator=g, device="cuda").to(dtype).requires_grad_(True)
+    x, r, w, b, q, kv, lw, lb = new(40, 96), new(40, 96), new(96), new(96), new(2, 9, 2, 32), new(2, 70, 2, 2, 32), new(48, 96), new(48)
+    return [("norm", vit_ops.layer_norm(x, w, b), (x, w, b)), ("norm + residual", vit_ops.layer_norm(x, w, b, residual=r), (x, r, w, b)),
+            ("attention", vit_ops.cross_attention(q, kv[:, :, 0], kv[:, :, 1]), (q, kv)), ("gelu8", vit_ops.gelu8(x), (x,)), ("linear8", vit_ops.linear8(x, lw, lb), (x, lw, lb))]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+def test_lazily_negated_gradients(dtype):
+    """autograd hands a gradient with the negative bit on as it is (the imaginary part of a conjugate is one)"""
+    for name, out, leaves in _calls(dtype=dtype):
+        outs = out if isinstance(out, tuple) else (out,)
+        gs = [torch.randn(o.shape, generator=gen(72), device="cuda").to(dtype) for o in outs]
+        want = torch.autograd.grad(outs, leaves, [-t for t in gs], retain_graph=True)
+        neg = [torch._neg_view(t) for t in gs]
+        assert all(t.is_neg() for t in neg)
+        for a, c in zip(torch.autograd.grad(outs, leaves, neg), want):
+            assert torch.equal(a, c), name
+    x = torch.randn(30, 64, generator=gen(73), device="cuda").to(dtype)
+    p = vit_ops.pack8(x)
+    for a, c in zip(vit_ops.weight_grad8(torch._neg_view(x), p), vit_ops.weight_grad8(-x, p)):
+        assert torch.equal(a, c)
+
+
+@gpu
+def test_a_conjugate_brings_a_negated_gradient():
+    """the same through ordinary operations"""
+    x = torch.randn(6, 64, generator=gen(74), device="cuda").requires_grad_(True)
+    up = torch.randn(6, 64, generator=gen(75), device="cuda")
+    through = lambda y: (torch.complex(torch.zeros_like(y), y).conj().imag * up).sum()            # = -(y up).sum()
+    got, = torch.autograd.grad(through(vit_ops.gelu8(x)), x)
+    want, = torch.autograd.grad(vit_ops.gelu8(x), x, -up)
+    assert torch.equal(got, want)
+
+
 # ---- linear8 ----------------------------------------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
