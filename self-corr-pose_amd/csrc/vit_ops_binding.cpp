@@ -9,6 +9,7 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <stdexcept>
@@ -55,7 +56,7 @@ std::string text(at::IntArrayRef s) {
     for (size_t i = 0; i < s.size(); i++) r += (i ? ", " : "") + std::to_string(s[i]);
     return r + ")";
 }
-// the tensor behind a Python object: on the current device and of one of the types
+// the tensor behind a Python object: on the current device, of one of the types, and with nothing attached that would be lost
 Tensor tensor(const py::handle& o, const char* name, std::initializer_list<at::ScalarType> types) {
     if (!THPVariable_Check(o.ptr())) refuse(std::string(name) + " must be a CUDA tensor (no CPU fallback)");
     const Tensor& t = THPVariable_Unpack(o.ptr());
@@ -71,6 +72,9 @@ Tensor tensor(const py::handle& o, const char* name, std::initializer_list<at::S
     if (t.get_device() != device)
         refuse(std::string(name) + " lives on cuda:" + std::to_string(t.get_device()) + " but the current device is cuda:" + std::to_string(device) +
                " (torch.cuda.set_device first)");
+    // autograd's nodes of this file know neither: without the refusal the tangent would be dropped, the traced result kept as a constant
+    if (t._fw_grad(/*level=*/0).defined()) refuse(std::string(name) + " has a forward-mode tangent: the operators of scp_amd.vit_ops have no forward-mode derivative");
+    if (torch::jit::tracer::isTracing()) refuse(std::string(name) + ": the operators of scp_amd.vit_ops cannot be traced (torch.jit.trace)");
     return t.is_neg() ? t.resolve_neg() : t;
 }
 Tensor operand(const py::handle& o, const char* name) { return tensor(o, name, {at::kFloat, at::kBFloat16}); }

@@ -129,6 +129,36 @@ def test_a_conjugate_brings_a_negated_gradient():
     assert torch.equal(got, want)
 
 
+def _entries():
+    x, w, b, r = (torch.randn(*s, device="cuda") for s in ((4, 64), (64,), (64,), (4, 64)))
+    q, k, lw, lb = (torch.randn(*s, device="cuda") for s in ((1, 3, 2, 32), (1, 5, 2, 32), (8, 64), (8,)))
+    p = vit_ops.pack8(x)
+    return [(lambda *a: vit_ops.layer_norm(a[0], a[1], a[2], residual=a[3]), [x, w, b, r]), (lambda *a: vit_ops.cross_attention(*a), [q, k, k.clone()]),
+            (lambda *a: vit_ops.gelu8(*a), [x]), (lambda *a: vit_ops.linear8(*a), [x, lw, lb]), (lambda a: vit_ops.pack8(a).codes, [x]),
+            (lambda a: vit_ops.weight_grad8(a, p)[0], [r])]
+
+
+@gpu
+def test_forward_mode_derivatives_are_refused():
+    """a tangent on any operand: an error, not a result without it"""
+    import torch.autograd.forward_ad as fwd
+    for i, (call, args) in enumerate(_entries()):
+        call(*args)
+        for j in range(len(args)):
+            with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+                call(*[fwd.make_dual(t, torch.ones_like(t)) if n == j else t for n, t in enumerate(args)])
+                pytest.fail("operand %d of call %d was not refused" % (j, i))
+
+
+@gpu
+def test_tracing_is_refused():
+    """torch.jit.trace would keep the result of the traced call as a constant"""
+    for i, (call, args) in enumerate(_entries()):
+        with pytest.raises(RuntimeError, match="trac"):
+            torch.jit.trace(call, tuple(args), check_trace=False)
+            pytest.fail("call %d was traced" % i)
+
+
 # ---- linear8 ----------------------------------------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
