@@ -478,9 +478,12 @@ Tensor linear8(const py::object& x_, const py::object& weight_, const py::object
         bias = operand_like(bias_, "linear8: bias", x);
         if (bias.dim() != 1 || bias.size(0) != weight.size(0)) refuse("linear8: bias must have " + std::to_string(weight.size(0)) + " entries");
     }
+    const bool packs = wants_grad({weight, bias});
+    if (packs && (x.size(-1) > 1 << 20 || weight.size(0) > 1 << 20 || weight.numel() > 1l << 34))
+        refuse("linear8: a gradient of weight " + text(weight.sizes()) + "; at most 2^20 rows and columns and 2^34 entries are possible");
     py::gil_scoped_release release;
     const OwnType own_type;
-    if (wants_grad({x, weight, bias})) return Linear8::apply(x, weight, maybe(bias), wants_grad({weight, bias}))[0];
+    if (packs || wants_grad({x})) return Linear8::apply(x, weight, maybe(bias), packs)[0];
     return linear(x, weight, bias);
 }
 

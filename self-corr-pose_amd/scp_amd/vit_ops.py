@@ -97,7 +97,7 @@ def gelu8(x):
 
 def weight_grad8(grad, packed, bias=True):
     """(gw [N, K], gb [N] or None) in float32 of a linear layer y = x w^T + b from grad = gy [..., N] and the 8-bit checkpoint of x
-    [..., K]: gw = sum over rows gy[:, n] x8[:, k], gb = sum over rows gy."""
+    [..., K]: gw = sum over rows gy[:, n] x8[:, k], gb = sum over rows gy.  N and K at most 2^20, N K at most 2^34; not differentiable."""
     if isinstance(packed, Packed8):
         return (_binding or _load()).weight_grad8(grad, packed.codes, packed.exps, bias)
     if isinstance(grad, torch.Tensor) and not grad.is_cuda:
@@ -107,5 +107,6 @@ def weight_grad8(grad, packed, bias=True):
 
 def linear8(x, weight, bias=None):
     """x [..., K] @ weight [N, K]^T + bias, with x kept for the weight gradient in 8 bits (weight_grad8).  One type for all three.  The
-    forward product and the input's gradient are plain library products at full precision; nothing else is saved."""
+    forward product and the input's gradient are plain library products at full precision; nothing else is saved.  A weight or bias that
+    takes a gradient may have 2^20 rows, 2^20 columns and 2^34 entries."""
     return (_binding or _load()).linear8(x, weight, bias)

@@ -159,6 +159,22 @@ def test_tracing_is_refused():
             pytest.fail("call %d was traced" % i)
 
 
+# ---- sizes ---------------------------------------------------------------------------------------------------------------------------------------
+@gpu
+def test_linear8_refuses_at_once_what_its_backward_pass_cannot_take():
+    c = (1 << 20) + 8
+    x, w = torch.randn(2, c, device="cuda"), torch.randn(1, c, device="cuda")
+    with pytest.raises(RuntimeError, match="2\\^20"):
+        vit_ops.linear8(x, w.clone().requires_grad_(True))
+    with pytest.raises(RuntimeError, match="2\\^20"):
+        vit_ops.linear8(x, w, torch.zeros(1, device="cuda", requires_grad=True))
+    with pytest.raises(RuntimeError, match="2\\^20"):
+        vit_ops.linear8(torch.randn(2, 8, device="cuda"), torch.randn(c, 8, device="cuda").requires_grad_(True))
+    leaf = x.clone().requires_grad_(True)                                        # a frozen weight asks for no weight gradient
+    gx, = torch.autograd.grad(vit_ops.linear8(leaf, w), leaf, torch.ones(2, 1, device="cuda"))
+    assert torch.equal(gx, w.expand(2, c))
+
+
 # ---- linear8 ----------------------------------------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
