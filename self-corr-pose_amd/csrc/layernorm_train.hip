@@ -288,9 +288,20 @@ int backward_blocks(long rows, int C, int tpr) {
 int lanes_per_row(int C) { return C <= 512 ? 16 : C <= 2048 ? 64 : 256; }
 
 template <typename T, typename W, int TPR, int NCH> struct Launch {
+    // a launch has fewer than 2^32 threads: more than 2^23 workgroups go out in several
     static void forward(const NormArgs& a, hipStream_t st) {
-        const unsigned blocks = (unsigned)((a.rows + THREADS / TPR - 1) / (THREADS / TPR));
-        hipLaunchKernelGGL((layernorm_forward_kernel<T, W, TPR, NCH>), dim3(blocks), dim3(THREADS), 0, st, a);
+        constexpr long PER = THREADS / TPR, MOST = PER << 23;
+        for (long row = 0; row < a.rows; row += MOST) {
+            NormArgs part = a;
+            const size_t at = (size_t)row * a.C;
+            part.rows = a.rows - row < MOST ? a.rows - row : MOST;
+            part.x = static_cast<const T*>(a.x) + at;
+            if (a.resid) part.resid = static_cast<const T*>(a.resid) + at;
+            if (a.sum) part.sum = static_cast<T*>(a.sum) + at;
+            part.y = static_cast<T*>(a.y) + at;
+            if (a.stats) part.stats = a.stats + 2 * row;
+            hipLaunchKernelGGL((layernorm_forward_kernel<T, W, TPR, NCH>), dim3((unsigned)((part.rows + PER - 1) / PER)), dim3(THREADS), 0, st, part);
+        }
     }
     static void backward(const NormGradArgs& a, hipStream_t st) {
         hipLaunchKernelGGL((layernorm_backward_kernel<T, W, TPR, NCH>), dim3(backward_blocks(a.rows, a.C, TPR)), dim3(THREADS), 0, st, a);

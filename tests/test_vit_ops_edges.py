@@ -175,6 +175,23 @@ def test_linear8_refuses_at_once_what_its_backward_pass_cannot_take():
     assert torch.equal(gx, w.expand(2, c))
 
 
+@gpu
+def test_layer_norm_of_more_rows_than_one_launch_holds():
+    """2^28 rows and some: 2^24 workgroups of 16 rows would have 2^32 threads.  y of two channels is +-1 scaled; both ends are compared"""
+    from test_vit_ops import norm_reference
+    rows = (1 << 28) + 37
+    x = torch.empty(rows, 2, device="cuda", dtype=BF16).normal_(generator=gen(3))
+    w, b = torch.tensor([1.5, -0.75], device="cuda"), torch.tensor([0.25, 3.0], device="cuda")
+    x.requires_grad_(True)
+    y = vit_ops.layer_norm(x, w, b, eps=1e-2)
+    gx, = torch.autograd.grad(y, x, x.detach())
+    for part in (slice(0, 3000), slice((1 << 27) - 1500, (1 << 27) + 1500), slice((1 << 28) - 1500, (1 << 28) + 37)):
+        xs = x.detach()[part].contiguous()
+        ref = norm_reference(xs, None, w, b, 1e-2, xs, None, BF16)
+        within(y.detach()[part], *ref["y"], "y")
+        within(gx[part], *ref["gx"], "gx")
+
+
 # ---- linear8 ----------------------------------------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
