@@ -19,6 +19,8 @@
 // 3 x 295.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "scp_common.h"
 #include "scp_hip.h"
 #include "vec_io.h"
@@ -99,6 +101,7 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 4) void
     __shared__ __attribute__((aligned(16))) __bf16 gbuf[2][PARTS][STEP * BN];
     __shared__ __attribute__((aligned(16))) __bf16 xbuf[2][STEP * BK];
     __shared__ float bias_sums[FILL / S::CPR][BN];
+    __shared__ int again;
 
     // tiles of one range of rows next to each other on one XCD: they read the same rows of gy and of the codes
     const int tiles = a.tiles_n * a.tiles_k, total = tiles * a.splits, per = (total + 7) / 8;
@@ -114,14 +117,11 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 4) void
     const int steps = (int)((m_end - m_beg + STEP - 1) / STEP);
     auto at = [&](int i) { return m_beg + (long)(i < steps ? i : steps - 1) * STEP; };        // a step past the end repeats the last
 
+    if (threadIdx.x == 0) again = 0;                                    // (read after the barrier that ends the first pass)
     if (!fills) {
         const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
         const int wn = (wave >> 1) * (BN / 4), wk = (wave & 1) * 64;
         f32x16 acc[NB][2];
-#pragma unroll
-        for (int i = 0; i < NB; i++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) acc[i][j] = f32x16{};
         auto multiply = [&](int buf) {
             __syncthreads();
 #pragma unroll
@@ -139,13 +139,30 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 4) void
                     }
             }
         };
-        int i = 0;
-        for (; i + 1 < steps; i += 2) {                                 // the buffers by name: every LDS address is a constant of the loop
-            multiply(0);
-            multiply(1);
+        for (bool first = true;; first = false) {
+#pragma unroll
+            for (int i = 0; i < NB; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) acc[i][j] = f32x16{};
+            int i = 0;
+            for (; i + 1 < steps; i += 2) {                             // the buffers by name: every LDS address is a constant of the loop
+                multiply(0);
+                multiply(1);
+            }
+            if (i < steps) multiply(0);
+            if (S::F32 && first) {                                      // a NaN: a second pass, see below
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < NB; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) sum += acc[i][j][r];
+                if (sum != sum) again = 1;
+            }
+            __syncthreads();                                            // the filling wavefronts' last one of the pass
+            if (!S::F32 || !first || !again) break;
         }
-        if (i < steps) multiply(0);
-        __syncthreads();                                                // the filling wavefronts' last one
         // accumulator: column k = lane & 31, row n = (reg & 3) + 8 (reg >> 2) + 4 half
         float* out = a.gw + (size_t)split * a.N * a.K;
 #pragma unroll
@@ -168,136 +185,150 @@ template <typename T, bool RAGGED> __global__ __launch_bounds__(THREADS, 4) void
         return;
     }
 
-    // loads: gy piece i of this thread = row tid / 32 + 16 i, elements E (tid % 32); codes = rows tid / 16 and tid / 16 + 32, 8 of each.
-    // Pieces past a row's end are read from its end instead and moved into place (RAGGED); what stands behind them, and in pieces past the
-    // matrix, goes into products that nobody stores.  Rows past the range are read from its last row and stored as zeros (RAGGED), or read
-    // as zeros from behind the end of a buffer: without minima and multiplications per piece, which cost as much as the dequantisation.
-    const char* gy = static_cast<const char*>(a.gy);
-    const int g_row = tid / S::CPR, g_col = n0 + S::E * (tid % S::CPR);
-    const int x_row = tid >> 4, x_col = k0 + 8 * (tid & 15);
-    const int g_at = min(g_col, a.N - S::E), x_at = min(x_col, a.K - 8);
-    const int g_shift = min(g_col - g_at, S::E - 1) * (int)sizeof(T), x_shift = min(x_col - x_at, 7);
-    const int e_at = min(x_col >> 5, groups - 1);
-    // (Loads are never conditional: the wait for the older of the two register sets can then leave the younger in flight.)
-    constexpr int XR = STEP * 16 / FILL;                                 // rows of codes per thread
-    struct Raw { u32x4 g[S::PIECES]; u32x2 x[XR]; unsigned exp[XR]; };
-    constexpr int XROWS = FILL / 16;
-    const int g_off = (g_row * a.N + g_at) * (int)sizeof(T), g_next = FILL / S::CPR * a.N * (int)sizeof(T);
-    const int x_off = x_row * a.K + x_at, x_next = XROWS * a.K, e_off = x_row * groups + e_at, e_next = XROWS * groups;
-    auto load = [&](Raw& raw, long m) {
-        const int rows = m_end - m < STEP ? (int)(m_end - m) : STEP;
-        const char* gbase = gy + m * a.N * (long)sizeof(T);
-        const char* xbase = reinterpret_cast<const char*>(a.codes) + m * a.K;
-        const char* ebase = reinterpret_cast<const char*>(a.exps) + m * groups;
-        if constexpr (RAGGED) {
+    auto fill = [&](const int tid, auto infinities) {
+        // loads: gy piece i of this thread = row tid / 32 + 16 i, elements E (tid % 32); codes = rows tid / 16 and tid / 16 + 32, 8 of each.
+        // Pieces past a row's end are read from its end instead and moved into place (RAGGED); what stands behind them, and in pieces past the
+        // matrix, goes into products that nobody stores.  Rows past the range are read from its last row and stored as zeros (RAGGED), or read
+        // as zeros from behind the end of a buffer: without minima and multiplications per piece, which cost as much as the dequantisation.
+        const char* gy = static_cast<const char*>(a.gy);
+        const int g_row = tid / S::CPR, g_col = n0 + S::E * (tid % S::CPR);
+        const int x_row = tid >> 4, x_col = k0 + 8 * (tid & 15);
+        const int g_at = min(g_col, a.N - S::E), x_at = min(x_col, a.K - 8);
+        const int g_shift = min(g_col - g_at, S::E - 1) * (int)sizeof(T), x_shift = min(x_col - x_at, 7);
+        const int e_at = min(x_col >> 5, groups - 1);
+        // (Loads are never conditional: the wait for the older of the two register sets can then leave the younger in flight.)
+        constexpr int XR = STEP * 16 / FILL;                                 // rows of codes per thread
+        struct Raw { u32x4 g[S::PIECES]; u32x2 x[XR]; unsigned exp[XR]; };
+        constexpr int XROWS = FILL / 16;
+        const int g_off = (g_row * a.N + g_at) * (int)sizeof(T), g_next = FILL / S::CPR * a.N * (int)sizeof(T);
+        const int x_off = x_row * a.K + x_at, x_next = XROWS * a.K, e_off = x_row * groups + e_at, e_next = XROWS * groups;
+        auto load = [&](Raw& raw, long m) {
+            const int rows = m_end - m < STEP ? (int)(m_end - m) : STEP;
+            const char* gbase = gy + m * a.N * (long)sizeof(T);
+            const char* xbase = reinterpret_cast<const char*>(a.codes) + m * a.K;
+            const char* ebase = reinterpret_cast<const char*>(a.exps) + m * groups;
+            if constexpr (RAGGED) {
 #pragma unroll
-            for (int i = 0; i < S::PIECES; i++)
-                raw.g[i] = *reinterpret_cast<const u32x4_a1*>(gbase + (unsigned)(min(g_row + (FILL / S::CPR) * i, rows - 1) * a.N + g_at) * (unsigned)sizeof(T));
+                for (int i = 0; i < S::PIECES; i++)
+                    raw.g[i] = *reinterpret_cast<const u32x4_a1*>(gbase + (unsigned)(min(g_row + (FILL / S::CPR) * i, rows - 1) * a.N + g_at) * (unsigned)sizeof(T));
+#pragma unroll
+                for (int i = 0; i < XR; i++) {
+                    const int r = min(x_row + XROWS * i, rows - 1);
+                    raw.x[i] = *reinterpret_cast<const u32x2_a1*>(xbase + (unsigned)(r * a.K + x_at));
+                    raw.exp[i] = *reinterpret_cast<const unsigned char*>(ebase + (unsigned)(r * groups + e_at));
+                }
+            } else {                                                        // rows past the range are past the buffer's end: zeros
+                const int g_bytes = rows * a.N * (int)sizeof(T), x_bytes = rows * a.K, e_bytes = rows * groups;
+#pragma unroll
+                for (int i = 0; i < S::PIECES; i++)
+                    raw.g[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer(gbase + i * g_next, g_bytes - i * g_next), g_off, 0, 0));
+#pragma unroll
+                for (int i = 0; i < XR; i++) {
+                    raw.x[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(buffer(xbase + i * x_next, x_bytes - i * x_next), x_off, 0, 0));
+                    raw.exp[i] = __builtin_amdgcn_raw_buffer_load_b8(buffer(ebase + i * e_next, e_bytes - i * e_next), e_off, 0, 0);
+                }
+            }
+        };
+        const bool bias = a.gb && tk == 0;
+        float bsum[S::E];
+#pragma unroll
+        for (int i = 0; i < S::E; i++) bsum[i] = 0.f;
+        auto store = [&](Raw& raw, int buf, long m, bool counts) {
+            if constexpr (RAGGED) {
+#pragma unroll
+                for (int i = 0; i < S::PIECES; i++) raw.g[i] = from_byte(raw.g[i], g_shift);
+#pragma unroll
+                for (int i = 0; i < XR; i++) raw.x[i] = from_byte(raw.x[i], x_shift);
+            }
+            if (RAGGED && m + STEP > m_end) {
+                const int rows = (int)(m_end - m);
+#pragma unroll
+                for (int i = 0; i < S::PIECES; i++)
+                    if (g_row + (FILL / S::CPR) * i >= rows) raw.g[i] = u32x4{};
+#pragma unroll
+                for (int i = 0; i < XR; i++)
+                    if (x_row + XROWS * i >= rows) {
+                        raw.x[i] = u32x2{};
+                        raw.exp[i] = 1;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < S::PIECES; i++) {
+                const int row = g_row + (FILL / S::CPR) * i, col = S::E * (tid % S::CPR);
+                if constexpr (S::F32) {
+                    unsigned h[4], m[4], l[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {                            // 8 + 8 + 8 bits: h + m + l = gy exactly
+                        const float x = __uint_as_float(raw.g[i][e]);
+                        h[e] = raw.g[i][e] & 0xffff0000u;
+                        float rest = x - __uint_as_float(h[e]);
+                        if constexpr (infinities.value) rest = (raw.g[i][e] & 0x7fffffffu) == 0x7f800000u ? 0.f : rest;
+                        m[e] = __float_as_uint(rest) & 0xffff0000u;
+                        l[e] = __float_as_uint(rest - __uint_as_float(m[e]));
+                        if (bias && counts) bsum[e] += x;
+                    }
+                    const int at = lds_at<BN>(row, col / 8) + (col & 7);
+                    *reinterpret_cast<u32x2*>(&gbuf[buf][0][at]) = u32x2{upper_halves(h[0], h[1]), upper_halves(h[2], h[3])};
+                    *reinterpret_cast<u32x2*>(&gbuf[buf][1 % PARTS][at]) = u32x2{upper_halves(m[0], m[1]), upper_halves(m[2], m[3])};
+                    *reinterpret_cast<u32x2*>(&gbuf[buf][2 % PARTS][at]) = u32x2{upper_halves(l[0], l[1]), upper_halves(l[2], l[3])};
+                } else {
+                    *reinterpret_cast<u32x4*>(&gbuf[buf][0][lds_at<BN>(row, col / 8)]) = raw.g[i];
+                    if (bias && counts) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) bsum[e % S::E] += __uint_as_float(e & 1 ? raw.g[i][e / 2] & 0xffff0000u : raw.g[i][e / 2] << 16);
+                    }
+                }
+            }
 #pragma unroll
             for (int i = 0; i < XR; i++) {
-                const int r = min(x_row + XROWS * i, rows - 1);
-                raw.x[i] = *reinterpret_cast<const u32x2_a1*>(xbase + (unsigned)(r * a.K + x_at));
-                raw.exp[i] = *reinterpret_cast<const unsigned char*>(ebase + (unsigned)(r * groups + e_at));
-            }
-        } else {                                                        // rows past the range are past the buffer's end: zeros
-            const int g_bytes = rows * a.N * (int)sizeof(T), x_bytes = rows * a.K, e_bytes = rows * groups;
+                const float unit = __uint_as_float(raw.exp[i] == 255 ? 0x7fc00000u : raw.exp[i] << 23);
+                u32x4 x;
 #pragma unroll
-            for (int i = 0; i < S::PIECES; i++)
-                raw.g[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer(gbase + i * g_next, g_bytes - i * g_next), g_off, 0, 0));
+                for (int w = 0; w < 2; w++) {
+                    float v[4];
 #pragma unroll
-            for (int i = 0; i < XR; i++) {
-                raw.x[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(buffer(xbase + i * x_next, x_bytes - i * x_next), x_off, 0, 0));
-                raw.exp[i] = __builtin_amdgcn_raw_buffer_load_b8(buffer(ebase + i * e_next, e_bytes - i * e_next), e_off, 0, 0);
-            }
-        }
-    };
-    const bool bias = a.gb && tk == 0;
-    float bsum[S::E];
-#pragma unroll
-    for (int i = 0; i < S::E; i++) bsum[i] = 0.f;
-    auto store = [&](Raw& raw, int buf, long m, bool counts) {
-        if constexpr (RAGGED) {
-#pragma unroll
-            for (int i = 0; i < S::PIECES; i++) raw.g[i] = from_byte(raw.g[i], g_shift);
-#pragma unroll
-            for (int i = 0; i < XR; i++) raw.x[i] = from_byte(raw.x[i], x_shift);
-        }
-        if (RAGGED && m + STEP > m_end) {
-            const int rows = (int)(m_end - m);
-#pragma unroll
-            for (int i = 0; i < S::PIECES; i++)
-                if (g_row + (FILL / S::CPR) * i >= rows) raw.g[i] = u32x4{};
-#pragma unroll
-            for (int i = 0; i < XR; i++)
-                if (x_row + XROWS * i >= rows) {
-                    raw.x[i] = u32x2{};
-                    raw.exp[i] = 1;
+                    for (int e = 0; e < 4; e++) v[e] = (float)(signed char)(raw.x[i][w] >> (8 * e)) * unit;
+                    x[2 * w] = upper_halves(__float_as_uint(v[0]), __float_as_uint(v[1]));
+                    x[2 * w + 1] = upper_halves(__float_as_uint(v[2]), __float_as_uint(v[3]));
                 }
-        }
-#pragma unroll
-        for (int i = 0; i < S::PIECES; i++) {
-            const int row = g_row + (FILL / S::CPR) * i, col = S::E * (tid % S::CPR);
-            if constexpr (S::F32) {
-                unsigned h[4], m[4], l[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {                            // 8 + 8 + 8 bits: h + m + l = gy exactly
-                    const float x = __uint_as_float(raw.g[i][e]);
-                    h[e] = raw.g[i][e] & 0xffff0000u;
-                    const float rest = x - __uint_as_float(h[e]);
-                    m[e] = __float_as_uint(rest) & 0xffff0000u;
-                    l[e] = __float_as_uint(rest - __uint_as_float(m[e]));
-                    if (bias && counts) bsum[e] += x;
-                }
-                const int at = lds_at<BN>(row, col / 8) + (col & 7);
-                *reinterpret_cast<u32x2*>(&gbuf[buf][0][at]) = u32x2{upper_halves(h[0], h[1]), upper_halves(h[2], h[3])};
-                *reinterpret_cast<u32x2*>(&gbuf[buf][1 % PARTS][at]) = u32x2{upper_halves(m[0], m[1]), upper_halves(m[2], m[3])};
-                *reinterpret_cast<u32x2*>(&gbuf[buf][2 % PARTS][at]) = u32x2{upper_halves(l[0], l[1]), upper_halves(l[2], l[3])};
-            } else {
-                *reinterpret_cast<u32x4*>(&gbuf[buf][0][lds_at<BN>(row, col / 8)]) = raw.g[i];
-                if (bias && counts) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) bsum[e % S::E] += __uint_as_float(e & 1 ? raw.g[i][e / 2] & 0xffff0000u : raw.g[i][e / 2] << 16);
-                }
+                *reinterpret_cast<u32x4*>(&xbuf[buf][lds_at<BK>(x_row + XROWS * i, tid & 15)]) = x;
             }
-        }
-#pragma unroll
-        for (int i = 0; i < XR; i++) {
-            const float unit = __uint_as_float(raw.exp[i] == 255 ? 0x7fc00000u : raw.exp[i] << 23);
-            u32x4 x;
-#pragma unroll
-            for (int w = 0; w < 2; w++) {
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = (float)(signed char)(raw.x[i][w] >> (8 * e)) * unit;
-                x[2 * w] = upper_halves(__float_as_uint(v[0]), __float_as_uint(v[1]));
-                x[2 * w + 1] = upper_halves(__float_as_uint(v[2]), __float_as_uint(v[3]));
-            }
-            *reinterpret_cast<u32x4*>(&xbuf[buf][lds_at<BK>(x_row + XROWS * i, tid & 15)]) = x;
-        }
-    };
+        };
 
-    Raw even, odd;
-    load(even, at(0));
-    load(odd, at(1));
-    store(even, 0, at(0), true);
-    load(even, at(2));
-    // step i is being multiplied: step i + 1 goes to the other buffer, the loads of step i + 3 start
-    auto step = [&](int i, int buf, Raw& next) {
-        __syncthreads();
-        store(next, buf ^ 1, at(i + 1), i + 1 < steps);
-        load(next, at(i + 3));
-    };
-    int i = 0;
-    for (; i + 1 < steps; i += 2) {
-        step(i, 0, odd);
-        step(i + 1, 1, even);
-    }
-    if (i < steps) __syncthreads();                                     // the last of an odd number of steps: nothing left to fill
-    if (bias) {
+        Raw even, odd;
+        load(even, at(0));
+        load(odd, at(1));
+        store(even, 0, at(0), true);
+        load(even, at(2));
+        // step i is being multiplied: step i + 1 goes to the other buffer, the loads of step i + 3 start
+        auto step = [&](int i, int buf, Raw& next) {
+            __syncthreads();
+            store(next, buf ^ 1, at(i + 1), i + 1 < steps);
+            load(next, at(i + 3));
+        };
+        int i = 0;
+        for (; i + 1 < steps; i += 2) {
+            step(i, 0, odd);
+            step(i + 1, 1, even);
+        }
+        if (i < steps) __syncthreads();                                     // the last of an odd number of steps: nothing left to fill
+        if (bias) {
 #pragma unroll
-        for (int e = 0; e < S::E; e++) bias_sums[g_row][S::E * (tid % S::CPR) + e] = bsum[e];
-    }
+            for (int e = 0; e < S::E; e++) bias_sums[g_row][S::E * (tid % S::CPR) + e] = bsum[e];
+        }
+    };
+    fill(tid, std::false_type{});
     __syncthreads();
+    // The parts of an infinity are inf, inf - inf and so on: NaN where the sum of products is an infinity.  A tile that came out with a NaN is
+    // computed again with infinities cut into themselves and zeros; looking at every element in the first pass cost 18 % (133 -> 157 us).
+    if constexpr (S::F32) {
+        if (again) {
+            int same = tid;
+            asm("" : "+v"(same));                                       // nothing of the first pass is kept in registers for the second
+            fill(same, std::true_type{});
+            __syncthreads();
+        }
+    }
 }
 
 // gw[i] = sum over the splits of part[split][i], in order; gb the same from part_b: a thread per 4 values

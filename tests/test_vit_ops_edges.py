@@ -1,12 +1,13 @@
 """scp_amd.vit_ops at calls that tests/test_vit_ops.py does not make: exact ties, lazily negated gradients, forward-mode derivatives and
 tracing, problems past a launch's limits, infinities, many steps of the pipelines.  Tolerances are bounds per element as there."""
 import ctypes
+import math
 
 import pytest
 import torch
 
 from scp_amd import vit_ops
-from test_vit_ops import BF16, FP32, U, attn_inputs, attn_reference, gen, gpu, half_step, wgrad_reference, within
+from test_vit_ops import BF16, FP32, U, attn_inputs, attn_reference, gen, gpu, half_step, spread_values, wgrad_reference, within
 
 
 # ---- cross attention: the bits of the output that its rounding drops ----------------------------------------------------------------------
@@ -190,6 +191,34 @@ def test_layer_norm_of_more_rows_than_one_launch_holds():
         ref = norm_reference(xs, None, w, b, 1e-2, xs, None, BF16)
         within(y.detach()[part], *ref["y"], "y")
         within(gx[part], *ref["gx"], "gx")
+
+
+# ---- 8-bit checkpoints --------------------------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(200, 40, 48), (200, 37, 41), (1000, 333, 144), (9000, 1536, 384), (9001, 1535, 383)], ids=str)
+def test_weight_grad8_of_infinities(shape, dtype):
+    """an infinite gradient gives what the sum of products gives: an infinity where the input is not 0, NaN where it is, or where infinities
+    of both signs meet; a NaN gives NaN; every other column is untouched"""
+    rows, n, k = shape
+    x = spread_values(rows, k, dtype, 3).clamp(-50, 50)
+    gy = torch.randn(rows, n, generator=gen(4), device="cuda").to(dtype)
+    gy[7, 3], gy[rows - 1, 5], gy[64, 9], gy[65, 9], gy[100, 11] = math.inf, -math.inf, math.inf, -math.inf, math.nan
+    x[7, 2] = 0.0
+    p = vit_ops.pack8(x)
+    x8 = p.unpack(FP32).double()
+    gw, gb = vit_ops.weight_grad8(gy, p)
+    hit = torch.tensor([3, 5, 9, 11], device="cuda")
+    ref = (gy.double()[:, hit, None] * x8[:, None]).sum(0)
+    assert torch.isinf(ref[0]).any() and torch.isnan(ref[0, 2])
+    signs = lambda t: torch.nan_to_num(t.double(), 0.0, 1.0, -1.0)
+    assert torch.equal(torch.isnan(gw[hit]), torch.isnan(ref)) and torch.equal(signs(gw[hit]), signs(ref))
+    assert gb[3] == math.inf and gb[5] == -math.inf and gb[9].isnan() and gb[11].isnan()
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[hit] = False
+    ref_w, ref_b = wgrad_reference(gy[:, rest].contiguous(), x8)
+    within(gw[rest], *ref_w, "gw")
+    within(gb[rest], *ref_b, "gb")
 
 
 # ---- linear8 ----------------------------------------------------------------------------------------------------------------------------------------
