@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from scp_amd import vit_ops
-from test_vit_ops import BF16, FP32, U, attn_inputs, attn_reference, gen, gpu, half_step, spread_values, wgrad_reference, within
+from test_vit_ops import BF16, FP32, U, attn_inputs, attn_reference, check_attn, gelu64, gelu_slope64, gen, gpu, half_step, spread_values, wgrad_reference, within
 
 
 # ---- cross attention: the bits of the output that its rounding drops ----------------------------------------------------------------------
@@ -89,6 +89,24 @@ def test_attention_gradients_asked_for_one_by_one(dtype, nq):
         got = torch.autograd.grad(vit_ops.cross_attention(*ls), wanted, go)
         for a, name in zip(got, [f for i, f in enumerate(("gq", "gk", "gv")) if bits >> i & 1]):
             within(a, *ref[name], "%s of %d" % (name, bits))
+
+
+WINDOWS = [  # a wavefront looks at the mask 64 tiles at a time: more keys than that, in the forms with own and with shared columns
+    (8, 700, 4500, 6, 6, BF16, 4096), (8, 700, 2300, 6, 3, FP32, 2048), (8, 1100, 9000, 1, 1, BF16, 8192), (8, 2000, 4300, 2, 2, FP32, 4096)]
+
+
+@gpu
+@pytest.mark.parametrize("case", WINDOWS, ids=lambda c: "%dx%dx%d-%s" % (c[0], c[1], c[2], "fp32" if c[5] == FP32 else "bf16"))
+def test_attention_over_several_windows_of_keys(case):
+    b, nq, nk, h, hk, dtype, window = case
+    q, k, v, go, g = attn_inputs(b, nq, nk, h, hk, 64, dtype, 19)
+    mask = torch.rand(b, nk, generator=g, device="cuda") < 0.8
+    mask[0, :window] = False                                                     # nothing in the first window
+    mask[1, window:] = False                                                     # nothing after it
+    mask[2, window - 70:window + 70] = False
+    mask[3] = torch.arange(nk, device="cuda") == nk - 1
+    k = torch.where(mask[:, :, None, None], k, torch.full_like(k, math.nan))
+    check_attn(q, k, v, go, mask)
 
 
 # ---- incoming gradients and other kinds of derivatives --------------------------------------------------------------------------------------
@@ -219,6 +237,56 @@ def test_weight_grad8_of_infinities(shape, dtype):
     ref_w, ref_b = wgrad_reference(gy[:, rest].contiguous(), x8)
     within(gw[rest], *ref_w, "gw")
     within(gb[rest], *ref_b, "gb")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("nk", [(1536, 384), (1535, 383)], ids=["aligned", "ragged"])
+@pytest.mark.parametrize("steps", [3, 4, 5, 37, 38])
+def test_weight_grad8_over_many_steps(steps, nk, dtype):
+    """rows for `steps` steps of 64 in every workgroup (about one workgroup per CU), the last one short: registers and LDS buffers are used
+    again and again from the third step on"""
+    n, k = nk
+    tiles = -(-n // (128 if dtype == FP32 else 256)) * -(-k // 128)
+    rows = 256 // tiles * steps * 64 - 29
+    x = spread_values(rows, k, dtype, steps).clamp(-50, 50)
+    gy = torch.randn(rows, n, generator=gen(steps), device="cuda").to(dtype)
+    p = vit_ops.pack8(x)
+    gw, gb = vit_ops.weight_grad8(gy, p)
+    ref_w, ref_b = wgrad_reference(gy, p.unpack(FP32).double())                  # (the codes themselves: test_pack8_is_the_format)
+    # every term is rounded in at most 64 steps of a workgroup and once per workgroup when they are added up
+    tight = (64 * steps + 64 + 256 // tiles) / (rows + 64)
+    within(gw, ref_w[0], tight * ref_w[1], "gw")
+    within(gb, ref_b[0], tight * ref_b[1], "gb")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("c", [1536, 1500])
+def test_checkpoints_of_more_values_than_threads(c, dtype):
+    """over 33.5 million values every thread takes further pieces"""
+    rows = 24001
+    x = spread_values(rows, c, dtype, c).clamp(-30, 30)
+    p = vit_ops.pack8(x)
+    t = torch.nn.functional.pad(x.float(), (0, -c % 32)).view(rows, -1, 32)
+    field = ((t.abs().amax(2, keepdim=True).view(torch.int32) >> 23) - 6).clamp(min=1)
+    step = (field << 23).view(FP32)
+    code = (t.double() / step.double()).round().clamp(-127, 127)
+    assert torch.equal(p.exps.int(), field[..., 0])
+    assert torch.equal(p.codes.double(), code.view(rows, -1)[:, :c])
+    x8 = (code * step.double()).view(rows, -1)[:, :c]
+    del code, step, t
+    assert torch.equal(p.unpack(FP32).double(), x8)
+    leaf, gy = x.requires_grad_(True), torch.randn(rows, c, generator=gen(78), device="cuda").to(dtype)
+    y = vit_ops.gelu8(leaf)
+    gx, = torch.autograd.grad(y, leaf, gy)
+    ref = gelu64(x.detach().double())                                            # bounds as in test_gelu8_matches_definition
+    err = 4e-7 * x.detach().double().abs() + 2 * U * ref.abs()
+    within(y.detach(), ref, err + half_step(dtype) * (ref.abs() + err), "y")
+    slope = gelu_slope64(x8)
+    ref = gy.double() * slope
+    err = gy.double().abs() * (4e-7 * (1 + slope.abs())) + 2 * U * ref.abs()
+    within(gx, ref, err + half_step(dtype) * (ref.abs() + err), "gx")
 
 
 # ---- linear8 ----------------------------------------------------------------------------------------------------------------------------------------
