@@ -278,11 +278,13 @@ __global__ __launch_bounds__(64 * SLICES) void layernorm_fold_kernel(const float
     }
 }
 
-// One workgroup for up to 2^15 elements: it needs no partials and no second launch, which cost a caller more than the ~8 us that one
-// compute unit takes to stream them.
-int backward_blocks(long rows, int C, int tpr) {
+// One workgroup where it needs at most 5 rounds (of 16, 4 or 1 rows): no partials and no second launch, which cost an eager caller 6.5 us (85 x 384:
+// forward + backward 58.5 us, with them 65).  A round is a memory round trip whatever the rows' width.  Kernels of forward + backward, 1 / 2 /
+// 4 / 6 / 8 / 32 rounds, fp32, 64 channels: one workgroup 5.3 / 6.3 / 7.9 / 9.1 / 10.8 / 27 us, one per 16 rows 5.3 / 7.2 / 7.4 / 7.8 / 7.4 / 8.0;
+// 384 channels 11.3 / 13.1 / 16.2 / 19.5 / 22.5 / 58 against 11.3 / 13.8 / 13.6 / 13.6 / 13.8 / 14.2.
+int backward_blocks(long rows, int tpr) {
     const long groups = THREADS / tpr, need = (rows + groups - 1) / groups;
-    if (rows * C <= 1 << 15) return 1;
+    if (need <= 5) return 1;
     return (int)(need < BWD_MAX_BLOCKS ? need : BWD_MAX_BLOCKS);
 }
 int lanes_per_row(int C) { return C <= 512 ? 16 : C <= 2048 ? 64 : 256; }
@@ -304,7 +306,7 @@ template <typename T, typename W, int TPR, int NCH> struct Launch {
         }
     }
     static void backward(const NormGradArgs& a, hipStream_t st) {
-        hipLaunchKernelGGL((layernorm_backward_kernel<T, W, TPR, NCH>), dim3(backward_blocks(a.rows, a.C, TPR)), dim3(THREADS), 0, st, a);
+        hipLaunchKernelGGL((layernorm_backward_kernel<T, W, TPR, NCH>), dim3(backward_blocks(a.rows, TPR)), dim3(THREADS), 0, st, a);
     }
 };
 
@@ -363,7 +365,7 @@ extern "C" int scp_layernorm_forward(const void* x, const void* resid, const voi
 
 extern "C" size_t scp_layernorm_backward_workspace(long rows, int C) {
     if (rows <= 0 || C <= 0 || C > MAX_C) return 0;
-    const int blocks = backward_blocks(rows, C, lanes_per_row(C));
+    const int blocks = backward_blocks(rows, lanes_per_row(C));
     return blocks > 1 ? (size_t)blocks * 2 * C * sizeof(float) : 0;
 }
 
@@ -373,7 +375,7 @@ extern "C" int scp_layernorm_backward(const void* s, const void* gamma, const vo
     if (const char* why = bad_problem(rows, C, dtype, wdtype)) return scp::fail(hipErrorInvalidValue, why);
     if (!s || !gy || !stats) return scp::fail(hipErrorInvalidValue, "layernorm_backward: null argument");
     if (!gx && !g_gamma && !g_beta) return 0;
-    const int blocks = backward_blocks(rows, C, lanes_per_row(C));
+    const int blocks = backward_blocks(rows, lanes_per_row(C));
     const bool fold = blocks > 1 && (g_gamma || g_beta);
     if (fold && (!workspace || workspace_bytes < scp_layernorm_backward_workspace(rows, C)))
         return scp::fail(hipErrorInvalidValue, "layernorm_backward: workspace too small");

@@ -195,6 +195,33 @@ def test_linear8_refuses_at_once_what_its_backward_pass_cannot_take():
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(20000, 1), (8192, 4), (32768, 1), (4096, 8), (1024, 32), (512, 64), (300, 96)], ids=str)
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+def test_layer_norm_gradients_of_narrow_rows(shape, dtype):
+    from test_vit_ops import norm_reference
+    rows, c = shape
+    g = gen(rows + c)
+    new = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    x, gy, w, b = (3 * new(rows, c) + 1).to(dtype).requires_grad_(True), new(rows, c).to(dtype), (1 + 0.3 * new(c)).requires_grad_(True), new(c).requires_grad_(True)
+    ref = norm_reference(x.detach(), None, w.detach(), b.detach(), 1e-3, gy, None, dtype)
+    y = vit_ops.layer_norm(x, w, b, eps=1e-3)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), gy)
+    for got, name in ((y.detach(), "y"), (gx, "gx"), (gw, "gw"), (gb, "gb")):
+        within(got, *ref[name], name)
+
+
+def test_layer_norm_gives_narrow_rows_to_many_workgroups():
+    """one workgroup holds 16 rows at a time: what it takes goes by the number of its rounds, whatever the rows' width.  A workspace is asked
+    for where there is more than one workgroup."""
+    from scp_amd import capi
+    size = capi.lib().scp_layernorm_backward_workspace
+    for rows, c in ((32768, 1), (4096, 8), (1024, 32), (512, 64)):
+        assert size(rows, c) > 0, (rows, c)
+    for rows, c in ((4, 384), (16, 64), (1, 8192), (3, 1001)):
+        assert size(rows, c) == 0, (rows, c)
+
+
+@gpu
 def test_layer_norm_of_more_rows_than_one_launch_holds():
     """2^28 rows and some: 2^24 workgroups of 16 rows would have 2^32 threads.  y of two channels is +-1 scaled; both ends are compared"""
     from test_vit_ops import norm_reference
