@@ -37,6 +37,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "scp_common.h"
@@ -1116,9 +1117,17 @@ struct Plan { bool share, few, two_blocks; int nsplit, keys_per_split, row_block
 // bf16, where they read the tensors: 64 x 6 x 4097 keys, 1 / 2 / 4 rows: 76 / 80 / 93 us against 74 to 75, but 32 x 6 x 1025 keys, 1 row:
 // 13.5 against 18.5, 32 x 8 heads of 128: 27 against 41; so one row only.
 constexpr int few_rows(int size) { return size == 4 ? 32 : 1; }
-// workgroups to split the keys for: a second launch for the join costs 3 to 4 us.  192 / 384 / 512: 32 x 6 x 1025 keys fp32 19.7 / 22.0 / 22.4 us,
-// bf16 15.1 / 15.9 / 16.4; 64 x 6 x 257 bf16 7.1 / 7.1 / 10.2; 16 x 6 x 4097 bf16 27.0 / 24.2 / 25.9, fp32 36.2 / 36.9 / 38.6
-constexpr int FEW_BLOCKS = 192;
+// Single queries: a workgroup walks its keys in trips of 4 x Few::KEYS, each a memory round trip of 1.5 us, and the join of a split is a second
+// launch of 2 to 3 us that reads every part.  So fewer than 4 trips are not split (32 x 6 heads x 257 keys of 64, bf16: whole 7.9 us, split
+// 10.5; 4 x 6 heads, fp32 5.8 and 7.6), parts keep 2 trips, there are at most 6 of them (4 x 6 x 4097, bf16, 1 / 4 / 6 / 12 / 16 parts: 33 / 17.7 /
+// 16.9 / 19.3 / 23.3 us) and no more workgroups than CUs, beyond which the memory's rate counts (16 x 6 x 4097, bf16, 1 / 2 / 4 / 8: 33.6 /
+// 27.3 / 24.4 / 26.3; fp32 40.1 / 36.7 / 37.7 / 38.9; 32 x 6 x 1025, 1 / 2 / 4, bf16 15.5 / 16.1 / 17.2, fp32 20.5 / 22.6 / 22.9).  Against the best
+// number of parts that costs 2.5 % on average over 72 shapes of 6 to 384 heads, 257 to 4097 keys, 32 to 128 channels, both types.
+inline int few_parts(long blocks, int keys, int few_keys) {
+    const long trips = (keys + 4l * few_keys - 1) / (4l * few_keys);
+    if (trips < 4) return 1;
+    return (int)std::min(std::min((trips + 1) / 2, 6l), std::max(1l, 256 / blocks));
+}
 // SHARE below so many wavefronts of 32 columns; fewer leave SIMDs empty (256 CUs x 4).  8 x 6 heads of 642 x 1025, bf16: backward pass OWN 72 us,
 // SHARE 97; fp32: forward OWN 92, SHARE 98, 4 x 6 heads backward OWN 130, SHARE 120; 512 to 4096 are within 10 % of each other there.
 constexpr long SHARE_BELOW = 1024;
@@ -1138,9 +1147,8 @@ inline Plan forward_plan(const Args& a, bool may_two, int shared, int max_few, i
         p.share = false;
         p.row_blocks = R <= 4 ? 1 : (R + 7) / 8;
         const long blocks = (long)a.BH * p.row_blocks;
-        long want = (FEW_BLOCKS - 1 + blocks) / blocks, most = (a.Nk + 4 * few_keys - 1) / (4 * few_keys);
-        if (want > most) want = most;
-        p.keys_per_split = ((a.Nk + (int)want - 1) / (int)want + 15) / 16 * 16;
+        const int parts = few_parts(blocks, a.Nk, few_keys);
+        p.keys_per_split = ((a.Nk + parts - 1) / parts + 15) / 16 * 16;
         p.nsplit = (a.Nk + p.keys_per_split - 1) / p.keys_per_split;
         return p;
     }

@@ -109,6 +109,31 @@ def test_attention_over_several_windows_of_keys(case):
     check_attn(q, k, v, go, mask)
 
 
+def _limits(**kw):
+    from scp_amd import capi
+    p = capi.CrossAttnParams()
+    p.batch, p.queries, p.keys, p.heads, p.kv_heads, p.head_dim, p.dtype, p.scale = 1, 1, 1, 1, 1, 8, 1, 1.0
+    for name, v in kw.items():
+        setattr(p, name, v)
+    for f, n, h in (("q_stride", p.queries, p.heads), ("k_stride", p.keys, p.kv_heads), ("v_stride", p.keys, p.kv_heads), ("g_stride", p.queries, p.heads)):
+        getattr(p, f)[:] = (n * h * p.head_dim, h * p.head_dim, p.head_dim)
+    return p
+
+
+def test_single_queries_are_split_where_that_saves_round_trips():
+    """no workspace: the keys are not split.  The choice goes by the keys that a workgroup walks and by the number of workgroups, without a
+    step between neighbouring batches"""
+    from scp_amd import capi
+
+    def split(batch, keys, dtype, dim=64):
+        p = _limits(batch=batch, heads=6, kv_heads=6, keys=keys, dtype=dtype, head_dim=dim)
+        return capi.lib().scp_cross_attention_forward_workspace(ctypes.byref(p)) // (batch * 6 * (dim + 2) * 4)
+    for dtype in (0, 1):
+        assert [split(b, 1025, dtype) for b in (30, 31, 32, 33, 64)] == [0] * 5
+        assert [split(b, 257, dtype) for b in (1, 4, 16, 32)] == [0] * 4
+        assert [split(b, 4097, dtype) for b in (1, 4, 8, 16, 31, 32)] == [6, 6, 5, 2, 0, 0]
+
+
 # ---- incoming gradients and other kinds of derivatives --------------------------------------------------------------------------------------
 def _calls(seed=71, dtype=FP32):
     """(name, output, leaves) of every operator with a gradient"""
