@@ -653,7 +653,8 @@ int scp_layernorm_backward(const void* s, const void* gamma, const void* gy, con
  *     pass it keeps the gradients exact where a few keys hold most of the softmax; without it g_out . out is taken from the rounded out.
  *   fp32 tensors are multiplied as three exact bf16 parts, which the workspace holds: an infinity that is not masked may come out as NaN.
  *   lse [batch,kv_heads,queries * heads / kv_heads]: log2 of the softmax denominator per row, kept for the backward pass; may be NULL.
- *   head_dim: a multiple of 8, <= 128.  g_q / g_k / g_v may each be NULL. */
+ *   head_dim: a multiple of 8, <= 128.  g_q / g_k / g_v may each be NULL.  A problem of 2^24 workgroups or more is refused (about 2^24 heads over
+ *   the batch, or 2^31 rows).  The backward workspace is never 0 bytes for a problem that the backward pass takes. */
 typedef struct scp_cross_attn_params {
     int batch, queries, keys, heads, kv_heads, head_dim, dtype;
     float scale;

@@ -50,6 +50,27 @@ bool tile_too_wide(const scp_cross_attn_params* p, bool backward) {
             if (st[1] < 0 || st[2] < 0 || (129 * st[1] + G * st[2]) * size >= lim) return true;
     return false;
 }
+// a launch has fewer than 2^32 threads: fewer than 2^24 workgroups of 256
+constexpr long long MOST_BLOCKS = (1ll << 24) - 1;
+long long per_group(long long n, long long group) { return (n + group - 1) / group; }
+int parts_rows(int D) { return 256 / (D <= 32 ? 4 : D <= 64 ? 8 : 16); }                     // rows per workgroup of parts_kernel
+// workgroups of the kernel that cuts q (and g_out), k and v into parts; 0 in bf16
+long long parts_blocks(const scp_cross_attn_params* p, bool backward) {
+    if (p->dtype != SCP_DTYPE_F32) return 0;
+    const long long rows = (long long)p->batch * p->queries * p->heads, keys = (long long)p->batch * p->keys * p->kv_heads;
+    return (backward ? 2 : 1) * per_group(rows, parts_rows(p->head_dim)) + 2 * per_group(keys, parts_rows(p->head_dim));
+}
+bool too_many_blocks_forward(const scp_cross_attn_params* p, const Args& a, const Plan& plan) {
+    const long long heads = a.BH >= 16 ? per_group(a.BH, 8) * 8 : a.BH;
+    return heads * plan.row_blocks * plan.nsplit > MOST_BLOCKS || (!plan.few && parts_blocks(p, false) > MOST_BLOCKS) ||
+           (plan.nsplit > 1 && per_group((long long)a.BH * a.Nq * a.G * (a.D / 4), 256) > MOST_BLOCKS);
+}
+// (for all three gradients in workgroups of 128 columns; narrower ones are taken for small problems only)
+bool too_many_blocks_backward(const scp_cross_attn_params* p) {
+    const long long R = (long long)p->queries * (p->heads / p->kv_heads), bh = (long long)p->batch * p->kv_heads, heads = bh >= 16 ? per_group(bh, 8) * 8 : bh;
+    return heads * (per_group(R, 128) + per_group(p->keys, 128)) > MOST_BLOCKS || parts_blocks(p, true) > MOST_BLOCKS ||
+           p->batch * per_group((long long)p->queries * p->heads, parts_rows(p->head_dim) * scp_attn::DELTA_ROWS) > MOST_BLOCKS;
+}
 bool misaligned(const void* p) { return (reinterpret_cast<size_t>(p) & 15) != 0; }
 
 Args make_args(const scp_cross_attn_params* p) {
@@ -76,12 +97,11 @@ size_t split_floats(const Args& a, const Plan& p) { return p.nsplit > 1 ? (size_
 
 // fp32 tensors as three bf16 parts: dst [batch][tokens][heads][3][D]; a thread per 8 channels, 256 / lanes rows per workgroup
 struct Parts { const float* src[4]; __bf16* dst[4]; long st[4][3]; int tokens[4], heads[4]; unsigned first[5]; int batch, D; };
-constexpr int parts_rows(int D) { return 256 / (D <= 32 ? 4 : D <= 64 ? 8 : 16); }
 __global__ __launch_bounds__(256) void parts_kernel(const Parts a) {
     int t = 0;
 #pragma unroll
     for (int i = 1; i < 4; i++) t += blockIdx.x >= a.first[i];
-    const int lanes = 256 / parts_rows(a.D), d = 8 * (threadIdx.x % lanes);
+    const int lanes = a.D <= 32 ? 4 : a.D <= 64 ? 8 : 16, d = 8 * (threadIdx.x % lanes);
     const unsigned heads = a.heads[t], per = (unsigned)a.tokens[t] * heads;
     const unsigned row = (blockIdx.x - a.first[t]) * (256 / lanes) + threadIdx.x / lanes;
     if (row >= per * (unsigned)a.batch || d >= a.D) return;
@@ -154,6 +174,7 @@ extern "C" int scp_cross_attention_forward(const void* q, const void* k, const v
     if (tile_too_wide(p, false)) return scp::fail(hipErrorInvalidValue, "cross_attention_forward: token stride of k or v too large");
     Args a = make_args(p);
     const Plan plan = plan_of(a, p->dtype);
+    if (too_many_blocks_forward(p, a, plan)) return scp::fail(hipErrorInvalidValue, "cross_attention_forward: more than 2^24 workgroups");
     const size_t parts = plan.few ? 0 : parts_bytes(p, false), need = parts + split_floats(a, plan) * sizeof(float);
     if (need && (!workspace || workspace_bytes < need))
         return scp::fail(hipErrorInvalidValue, "cross_attention_forward: workspace too small");
@@ -179,7 +200,7 @@ extern "C" int scp_cross_attention_forward(const void* q, const void* k, const v
 }
 
 extern "C" size_t scp_cross_attention_backward_workspace(const scp_cross_attn_params* p) {
-    if (bad_problem(p)) return 0;
+    if (bad_problem(p) || tile_too_wide(p, true) || too_many_blocks_backward(p)) return 0;
     return parts_bytes(p, true) + (size_t)p->batch * p->heads * p->queries * sizeof(float);
 }
 
@@ -191,6 +212,7 @@ extern "C" int scp_cross_attention_backward(const void* q, const void* k, const 
     if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(out_low) || misaligned(g_out) || misaligned(workspace) || misaligned(g_q) || misaligned(g_k) || misaligned(g_v))
         return scp::fail(hipErrorInvalidValue, "cross_attention_backward: tensors must be 16-byte aligned");
     if (tile_too_wide(p, true)) return scp::fail(hipErrorInvalidValue, "cross_attention_backward: token or head stride too large");
+    if (too_many_blocks_backward(p)) return scp::fail(hipErrorInvalidValue, "cross_attention_backward: more than 2^24 workgroups");
     if (!g_q && !g_k && !g_v) return 0;
     if (!workspace || workspace_bytes < scp_cross_attention_backward_workspace(p))
         return scp::fail(hipErrorInvalidValue, "cross_attention_backward: workspace too small");

@@ -212,11 +212,11 @@ py::object layer_norm(const py::object& x_, const py::object& weight_, const py:
 }
 
 // ---- cross attention -------------------------------------------------------------------------------------------------------------------
-// t itself when the kernels can address it (channels contiguous, pointer and strides multiples of 16 bytes, 128 tokens of all heads within
+// t itself when the kernels can address it (channels contiguous, pointer and strides multiples of 16 bytes, 130 tokens of all heads within
 // 2^31 bytes), else a contiguous copy (contiguous() would return a misaligned tensor as it is)
 Tensor addressable(const Tensor& t) {
     const int64_t size = t.element_size(), sb = t.stride(0), sn = t.stride(1), sh = t.stride(2);
-    if (t.stride(3) == 1 && !(((int64_t)(size_t)t.data_ptr() | sb * size | sn * size | sh * size) & 15) && (128 * sn + t.size(2) * sh) * size < 1l << 31) return t;
+    if (t.stride(3) == 1 && !(((int64_t)(size_t)t.data_ptr() | sb * size | sn * size | sh * size) & 15) && (130 * sn + t.size(2) * sh) * size < 1l << 31) return t;
     return t.clone(at::MemoryFormat::Contiguous);
 }
 void strides(const Tensor& t, long long* to) {
@@ -260,6 +260,13 @@ AttnOut attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, con
 struct CrossAttention : Function<CrossAttention> {
     static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& mask_, double scale) {
         const Tensor mask = plain(mask_);
+        if (q.numel() && k.size(1)) {                                   // the backward pass must be possible too (its gradient comes dense or is copied)
+            scp_cross_attn_params p = attention_params(q, k, v, scale);
+            p.g_stride[2] = q.size(3);
+            p.g_stride[1] = q.size(2) * p.g_stride[2];
+            p.g_stride[0] = q.size(1) * p.g_stride[1];
+            if (!lib.scp_cross_attention_backward_workspace_(&p)) refuse("cross_attention: q " + text(q.sizes()) + " with k " + text(k.sizes()) + " is too large for the backward pass");
+        }
         AttnOut r = attention_forward(q, k, v, mask, scale, true);
         ctx->save_for_backward({q, k, v, mask, r.out, r.low, r.lse});
         ctx->saved_data["scale"] = scale;

@@ -120,6 +120,36 @@ def _limits(**kw):
     return p
 
 
+def test_attention_refuses_what_a_launch_cannot_hold():
+    """a launch has fewer than 2^32 threads, so fewer than 2^24 workgroups of 256; the entry points say so before anything is launched"""
+    from scp_amd import capi
+    L = capi.lib()
+    one, ws = ctypes.c_void_p(4096), ctypes.c_size_t(1 << 60)
+    forward = lambda p: L.scp_cross_attention_forward(one, one, one, None, ctypes.byref(p), one, None, None, one, ws, None)
+    backward = lambda p: L.scp_cross_attention_backward(one, one, one, None, one, None, one, one, ctypes.byref(p), one, one, one, one, ws, None)
+    p = _limits(batch=(1 << 24) - 3)                                             # a workgroup per head, rounded up to the 8 XCDs
+    assert forward(p) != 0 and "workgroups" in L.scp_last_error().decode()
+    assert L.scp_cross_attention_backward_workspace(ctypes.byref(p)) == 0
+    p = _limits(batch=1 << 23, heads=2)                                          # two rows a head: a workgroup each in the forward pass ...
+    assert backward(p) != 0 and "workgroups" in L.scp_last_error().decode()      # ... and one more for its key in the backward pass
+    p = _limits(batch=1 << 20, queries=1 << 10, dtype=0)                         # 2^30 rows of q and of g_out to cut into parts, 64 a workgroup
+    assert backward(p) != 0 and "workgroups" in L.scp_last_error().decode()
+    assert L.scp_cross_attention_backward_workspace(ctypes.byref(_limits(batch=1 << 20, heads=4))) > 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+def test_attention_takes_backward_what_it_takes_forward(dtype):
+    """tokens so far apart that 128 of them are within 2^31 bytes and 130 are not"""
+    step = (1 << 31) // (129 * torch.finfo(dtype).bits // 8) // 8 * 8 + 8
+    q, k, v, go, _ = attn_inputs(1, 3, 3, 1, 1, 64, dtype, 10)
+    far = []
+    for t in (q, k, v):
+        wide = torch.empty(3, step, dtype=dtype, device="cuda")[None, :, None, :64]
+        far.append(wide.copy_(t))
+    check_attn(*far, go)
+
+
 def test_single_queries_are_split_where_that_saves_round_trips():
     """no workspace: the keys are not split.  The choice goes by the keys that a workgroup walks and by the number of workgroups, without a
     step between neighbouring batches"""
