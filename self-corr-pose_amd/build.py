@@ -52,13 +52,28 @@ def _echo(err):
 
 
 BINDING = os.path.join(HERE, "lib", "scp_vit_ops.so")
+BINDING_FOR = os.path.join(HERE, "build", "scp_vit_ops.for")
+
+
+def binding_for():
+    """what BINDING is compiled against beside the sources: it calls torch's C++ interface, which changes from version to version"""
+    import torch
+    return "torch %s, python %d.%d\n" % ((torch.__version__,) + sys.version_info[:2])
+
+
+def binding_stale():
+    """True where BINDING has to be compiled again: a source is newer, or it was built against another torch or Python"""
+    deps = [os.path.join(CSRC, "vit_ops_binding.cpp"), os.path.join(ROOT, "include", "scp_hip.h"), __file__]
+    if not os.path.exists(BINDING) or not os.path.exists(BINDING_FOR) or os.path.getmtime(BINDING) <= max(os.path.getmtime(d) for d in deps):
+        return True
+    with open(BINDING_FOR) as f:
+        return f.read() != binding_for()
 
 
 def start_binding(force=False, verbose=True):
     """the compilation of BINDING as a running process, or None if it is up to date"""
     src = os.path.join(CSRC, "vit_ops_binding.cpp")
-    deps = [src, os.path.join(ROOT, "include", "scp_hip.h"), __file__]
-    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) > max(os.path.getmtime(d) for d in deps):
+    if not force and not binding_stale():
         return None
     import sysconfig
     import torch
@@ -79,7 +94,7 @@ def sources():
 
 
 def needs_build():
-    if not os.path.exists(OUT) or not os.path.exists(BINDING):
+    if not os.path.exists(OUT) or binding_stale():
         return True
     t = os.path.getmtime(OUT)
     t = min(t, os.path.getmtime(BINDING))
@@ -117,6 +132,8 @@ def build(force=False, verbose=True):
             raise RuntimeError("hipcc failed on " + s)
     if binding is not None and binding.wait() != 0:
         raise RuntimeError("the compiler failed on vit_ops_binding.cpp")
+    with open(BINDING_FOR, "w") as f:
+        f.write(binding_for())
     cmd = [hipcc, "-shared", "-fPIC", "--offload-arch=" + ARCH] + objs + ["-o", OUT]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
+#include <torch/version.h>
 
 #include <stdexcept>
 #include <string>
@@ -502,6 +503,7 @@ PYBIND11_MODULE(scp_vit_ops, m) {
     SCP_ENTRIES(X)
 #undef X
     m.attr("entries") = entries;
+    m.attr("torch_version") = TORCH_VERSION;                           // of the headers
     m.def("init", &init);
     m.def("layer_norm", &layer_norm);
     m.def("cross_attention", &cross_attention);

@@ -34,6 +34,9 @@ def _load():
     spec = importlib.util.spec_from_file_location("scp_vit_ops", BINDING_PATH)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
+    if module.torch_version != torch.__version__.split("+")[0]:
+        raise RuntimeError("scp_amd: %s was built against torch %s, this is torch %s -- build it again with `python self-corr-pose_amd/build.py`"
+                           % (BINDING_PATH, module.torch_version, torch.__version__))
     module.init({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in module.entries})
     _binding = module
     return module

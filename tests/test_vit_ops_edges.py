@@ -446,3 +446,20 @@ def test_results_can_be_changed_in_place():
     o = vit_ops.cross_attention(q, q, q).mul_(3)                                 # kept for its backward pass: changing it is noticed
     with pytest.raises(RuntimeError, match="inplace"):
         torch.autograd.grad(o, x, torch.ones_like(o))
+
+
+# ---- build ------------------------------------------------------------------------------------------------------------------------------------------
+def test_the_binding_is_built_again_for_another_torch(monkeypatch):
+    """its sources may be older than it is: what it was compiled against counts too, and loading one of another version is an error"""
+    import importlib.util
+    import os
+    spec = importlib.util.spec_from_file_location("scp_build_edges", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(vit_ops.__file__))), "build.py"))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    build.build(verbose=False)
+    assert not build.binding_stale() and not build.needs_build()
+    monkeypatch.setattr(torch, "__version__", "2.99.0+rocm9.9")
+    assert build.binding_stale() and build.needs_build()
+    monkeypatch.setattr(vit_ops, "_binding", None)
+    with pytest.raises(RuntimeError, match="built against torch"):
+        vit_ops._load()
