@@ -33,6 +33,14 @@ def pytest_collection_modifyitems(config, items):
         rank = {name: i for i, name in enumerate(ORDER)}
         items.sort(key=lambda it: rank.get(os.path.splitext(os.path.basename(str(it.fspath)))[0], len(ORDER) - 1.5))   # stable
     if torch.cuda.is_available():
+        # the reference's own kernels are built from its sources (oracle/build_ref.py); where those were absent there is nothing to compare
+        # with, and a suite run with -x has to reach the other tests
+        from oracle import ref_gpu
+        if not ref_gpu.available():
+            skip = pytest.mark.skip(reason="oracle/_ref is not built: the reference's sources were not there when build() ran")
+            for item in items:
+                if os.path.basename(str(item.fspath)) == "test_softras_ref_gpu.py":
+                    item.add_marker(skip)
         return
     skip = pytest.mark.skip(reason="needs a GPU (marked gpu)")
     for item in items:
