@@ -8,6 +8,7 @@
 // The entry points come from the library that scp_amd/capi.py has loaded (init()); nothing here is linked to it.
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
@@ -15,6 +16,8 @@
 
 #include <stdexcept>
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include "scp_hip.h"
 
@@ -112,6 +115,28 @@ struct Wanted {                                                      // asked fo
 };
 // an incoming gradient as its memory holds it: autograd hands on tensors whose negation is only a bit of theirs
 Tensor resolved(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+// A backward pass that is being captured must not reach a leaf whose gradient accumulator belongs to the default stream: one made by an eager
+// graph of the same leaf that is still alive.  The engine would have the default stream wait for the capturing one, which ends the process.
+void check_capture() {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream().stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    const auto self = torch::autograd::get_current_node();
+    if (!self) return;
+    std::vector<torch::autograd::Node*> todo{self.get()};
+    std::unordered_set<torch::autograd::Node*> seen{self.get()};
+    while (!todo.empty()) {
+        torch::autograd::Node* node = todo.back();
+        todo.pop_back();
+        if (dynamic_cast<torch::autograd::AccumulateGrad*>(node)) {
+            const auto stream = node->stream();
+            if (stream && stream->id() == 0)
+                refuse("scp_amd.vit_ops: this backward pass is being captured, and a graph made on the default stream from the same leaf is alive: delete its "
+                       "results first, or capture with leaves of their own (detach().requires_grad_())");
+        }
+        for (const auto& edge : node->next_edges())
+            if (edge.function && seen.insert(edge.function.get()).second) todo.push_back(edge.function.get());
+    }
+}
 // Gradients of a backward pass that is itself recorded (create_graph) cannot be differentiated again: they get a node that says so.
 variable_list first_order(variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -150,6 +175,7 @@ struct LayerNorm : Function<LayerNorm> {
         return {r.y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_capture();
         Wanted wanted{ctx, ctx->saved_data["present"].toInt()};
         const bool want_x = wanted(), want_r = wanted(), want_w = wanted(), want_b = wanted();
         const Tensor gsum = grads.size() == 2 ? resolved(grads[0]) : Tensor(), gy = resolved(grads.back());
@@ -274,6 +300,7 @@ struct CrossAttention : Function<CrossAttention> {
         return {r.out};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_capture();
         const variable_list saved = ctx->get_saved_variables();
         const Tensor q = addressable(saved[0]), k = addressable(saved[1]), v = addressable(saved[2]);             // a hook may have moved them
         const Tensor &mask = saved[3], &out = saved[4], &low = saved[5], &lse = saved[6];
@@ -379,6 +406,7 @@ struct Gelu8 : Function<Gelu8> {
         return {y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_capture();
         const variable_list saved = ctx->get_saved_variables();
         const Tensor gy = resolved(grads[0]).contiguous();
         Tensor gx = at::empty(gy.sizes(), gy.options());
@@ -458,6 +486,7 @@ struct Linear8 : Function<Linear8> {
         return {linear(x, weight, bias)};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_capture();
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &weight = saved[0];
         Wanted wanted{ctx, ctx->saved_data["present"].toInt()};

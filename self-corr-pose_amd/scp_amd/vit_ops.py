@@ -11,7 +11,8 @@ Argument checks, allocation and autograd nodes are compiled (csrc/vit_ops_bindin
 
 float32 and bfloat16 GPU tensors on the current device only, anything else raises RuntimeError (no CPU fallback).  Statistics, softmax and
 sums are fp32; results are rounded once to the type they are returned in.  No atomics: a call repeated gives the same bits.  Launches
-go to the current stream; workspaces come from torch's allocator, so a call can be captured into a HIP graph.  Once differentiable,
+go to the current stream; workspaces come from torch's allocator, so a call can be captured into a HIP graph; a
+captured backward pass is refused while an eager graph of the same leaves is alive, which would end the process.  Once differentiable,
 in reverse mode: a forward-mode tangent is refused, and so is torch.jit.trace."""
 import ctypes
 import importlib.util

@@ -233,6 +233,39 @@ def test_tracing_is_refused():
             pytest.fail("call %d was traced" % i)
 
 
+@gpu
+@pytest.mark.child_process
+def test_a_captured_backward_pass_beside_an_eager_graph_is_refused():
+    """the eager graph's accumulator belongs to the default stream; torch's engine would end the process at it.  With the eager results gone the
+    same capture runs, and replays what the eager pass computes"""
+    for pick in range(5):
+        name, eager, leaves = _calls()[pick]
+        first = leaves[0]
+        base = first.detach().clone().requires_grad_(True)                       # a leaf behind a view, too
+        make = [lambda t: vit_ops.layer_norm(t, leaves[1], leaves[2]), lambda t: vit_ops.layer_norm(t, leaves[2], leaves[3], residual=leaves[1])[1],
+                lambda t: vit_ops.cross_attention(t, leaves[1].detach()[:, :, 0], leaves[1].detach()[:, :, 1]), vit_ops.gelu8, lambda t: vit_ops.linear8(t, leaves[1], leaves[2])][pick]
+        del eager
+        go = torch.randn(first.shape if name != "linear8" else (40, 48), generator=gen(77), device="cuda")
+        want, = torch.autograd.grad(make(base), base, go)
+        torch.cuda.synchronize()
+        for view in (False, True):
+            alive = base * 1.0 if view else make(base)                           # an eager graph of the leaf
+            graph = torch.cuda.CUDAGraph()
+            with pytest.raises(RuntimeError, match="being captured"):
+                with torch.cuda.graph(graph):
+                    torch.autograd.grad(make(base[:] if view else base), base, go)
+                    pytest.fail("%s was not refused" % name)
+            torch.cuda.synchronize()
+            del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(make(base), base, go)
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), name
+
+
 # ---- sizes ---------------------------------------------------------------------------------------------------------------------------------------
 @gpu
 def test_linear8_refuses_at_once_what_its_backward_pass_cannot_take():
