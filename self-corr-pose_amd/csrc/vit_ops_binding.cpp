@@ -119,7 +119,11 @@ Tensor resolved(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_
 // graph of the same leaf that is still alive.  The engine would have the default stream wait for the capturing one, which ends the process.
 void check_capture() {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream().stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream().stream(), &status) != hipSuccess) {
+        (void)hipGetLastError();                                        // (the default stream while another thread captures: not this call's error)
+        return;
+    }
+    if (status == hipStreamCaptureStatusNone) return;
     const auto self = torch::autograd::get_current_node();
     if (!self) return;
     std::vector<torch::autograd::Node*> todo{self.get()};
