@@ -4,7 +4,8 @@
 //
 // A matrix product whose reduction runs over the ROWS of both operands, on v_mfma_f32_32x32x16_bf16.  x8 is exact in bf16 and bf16 gy is what
 // it is, so every product is exact and only the fp32 accumulation rounds; fp32 gy is cut into three bf16 parts of 8 bits each
-// (gy = h + m + l exactly) and multiplied part by part: 3 matrix instructions for 1, still 5 times the rate of the fp32 cores.
+// (gy = h + m + l exactly; an infinity takes a second pass over its tile) and multiplied part by part: 3 matrix instructions for 1, still 5
+// times the rate of the fp32 cores.
 //   * a workgroup owns a BN x 128 tile of gw over a range of rows and walks it 64 rows at a time, with two kinds of wavefronts: eight FILL (gy and
 //     the codes go global -> registers three steps ahead, are cut / dequantised there and written to LDS row-major one step ahead) and
 //     eight MULTIPLY, so that the vector work of the one runs beside the matrix instructions of the other;
@@ -15,8 +16,8 @@
 //     order (bit-reproducible).  gb falls out of the registers of the filling wavefronts of the first column of tiles.
 // Bound by filling and multiplying together, not by memory: of 77 us for 32800 rows, 384 -> 1536, bf16 (with pack8 9 and the fold 6.5), 62 are
 // left without the products, 55 without the filling, 28 without both; steps of 64 rows instead of 32 halve the barriers (69), addresses that
-// are constants of the loop and rows past the end read as zeros: 67 us.  The kernel alone: 57 us, 680 TFLOP/s; 1536 -> 384, fp32 131 us,
-// 3 x 295.
+// are constants of the loop and rows past the end read as zeros: 64 to 68 us.  The kernel alone: 52 us, 740 TFLOP/s; 1536 -> 384, fp32 132 to
+// 146 us, 3 x 265 to 290.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>

@@ -10,7 +10,9 @@ modules; its pipeline keeps them frozen).
 Argument checks, allocation and autograd nodes are compiled (csrc/vit_ops_binding.cpp).
 
 float32 and bfloat16 GPU tensors on the current device only, anything else raises RuntimeError (no CPU fallback).  Statistics, softmax and
-sums are fp32; results are rounded once to the type they are returned in.  No atomics: a call repeated gives the same bits.  Launches
+sums are fp32, and results are rounded to the type they are returned in.  In between bfloat16 attention rounds its probabilities and score
+gradients to bfloat16 for the products they enter (not those of a single query, nor in a backward pass over at most 16 rows or keys): the
+error of its results is 1.4 times that of their own rounding.  No atomics: a call repeated gives the same bits.  Launches
 go to the current stream; workspaces come from torch's allocator, so a call can be captured into a HIP graph; a
 captured backward pass is refused while an eager graph of the same leaves is alive, which would end the process.  Once differentiable,
 in reverse mode: a forward-mode tangent is refused, and so is torch.jit.trace."""
@@ -57,7 +59,7 @@ def cross_attention(q, k, v, scale=None, key_mask=None):
     """softmax(scale * q k^T) v per head: q [B, Nq, H, D] against an encoder's k, v [B, Nk, Hkv, D] of another length -> [B, Nq, H, D]
     (contiguous).  H a multiple of Hkv: query head h reads key / value head h // (H // Hkv).  D a multiple of 8, at most 128.  `scale`
     defaults to D ** -0.5.  `key_mask` (bool [B, Nk], True = attend): an image's padding; values stored at masked keys, NaN included,
-    reach no result; a batch entry without a key gives zeros, and zero gradients.  Any strides (slices of a fused qkv projection, an
+    reach no result; a batch entry without a key gives zeros, and zero gradients (so does a query whose every score is -inf).  Any strides (slices of a fused qkv projection, an
     expanded batch); gradients for q, k and v.  float32 is multiplied as three exact bfloat16 parts: an infinity that is not masked may come
     out as NaN."""
     return (_binding or _load()).cross_attention(q, k, v, scale, key_mask)
@@ -95,7 +97,8 @@ def pack8(x):
 
 def gelu8(x):
     """erf GELU of x [..., C] (the MLP's activation, vision_transformer_flexible.py:54-70).  The backward pass takes the slope at the
-    8-bit checkpoint of x instead of keeping x: 1 + 1/32 bytes per value held between the passes.  The forward value is exact."""
+    8-bit checkpoint of x instead of keeping x: 1 + 1/32 bytes per value held between the passes.  The forward value is that of x itself,
+    within 4e-7 |x| before its rounding (the error function of Abramowitz & Stegun 7.1.26, which is good to 1.5e-7 absolute)."""
     return (_binding or _load()).gelu8(x)
 
 
