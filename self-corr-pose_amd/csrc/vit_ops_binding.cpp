@@ -501,8 +501,13 @@ struct Linear8 : Function<Linear8> {
             const OwnType own_type;
             const Tensor gy = as_matrix(resolved(grads[0]));
             if (want_x) gx = at::_unsafe_view(gy.mm(weight), with_last(grads[0], weight.size(1)));
-            if (saved[1].defined() && (want_w || want_b)) {
-                WeightGrad r = weight_grad(gy, saved[1], saved[2], want_b);
+            if (want_w || want_b) {
+                Tensor codes = saved[1], exps = saved[2];
+                if (!want_w) {                                          // a bias alone: its column sums beside the narrowest weight gradient
+                    codes = at::zeros({gy.size(0), 8}, gy.options().dtype(at::kChar));
+                    exps = at::zeros({gy.size(0), 1}, gy.options().dtype(at::kByte));
+                }
+                WeightGrad r = weight_grad(gy, codes, exps, want_b);
                 if (want_w) gw = r.gw.to(weight.scalar_type());
                 if (r.gb.defined()) gb = r.gb.to(weight.scalar_type());
             }
@@ -519,12 +524,12 @@ Tensor linear8(const py::object& x_, const py::object& weight_, const py::object
         bias = operand_like(bias_, "linear8: bias", x);
         if (bias.dim() != 1 || bias.size(0) != weight.size(0)) refuse("linear8: bias must have " + std::to_string(weight.size(0)) + " entries");
     }
-    const bool packs = wants_grad({weight, bias});
-    if (packs && (x.size(-1) > 1 << 20 || weight.size(0) > 1 << 20 || weight.numel() > 1l << 34))
+    const bool sums = wants_grad({weight, bias});
+    if (sums && (x.size(-1) > 1 << 20 || weight.size(0) > 1 << 20 || weight.numel() > 1l << 34))
         refuse("linear8: a gradient of weight " + text(weight.sizes()) + "; at most 2^20 rows and columns and 2^34 entries are possible");
     py::gil_scoped_release release;
     const OwnType own_type;
-    if (packs || wants_grad({x})) return Linear8::apply(x, weight, maybe(bias), packs)[0];
+    if (sums || wants_grad({x})) return Linear8::apply(x, weight, maybe(bias), wants_grad({weight}))[0];
     return linear(x, weight, bias);
 }
 

@@ -468,6 +468,24 @@ def test_linear8_makes_no_batched_product(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+def test_linear8_of_a_bias_alone_keeps_no_checkpoint(dtype):
+    """a frozen weight: nothing of x's size is held for the backward pass"""
+    g = gen(16)
+    x, w, gy = (torch.randn(*s, generator=g, device="cuda").to(dtype) for s in ((3, 500, 640), (72, 640), (3, 500, 72)))
+    b = torch.zeros(72, device="cuda", dtype=dtype, requires_grad=True)
+    held = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: held.append(t.numel()) or t, lambda t: t):
+        y = vit_ops.linear8(x, w, b)
+    assert max(held, default=0) <= w.numel() and w.numel() < x.numel()
+    val, bound = wgrad_reference(gy.reshape(-1, 72), torch.zeros(1500, 1, dtype=torch.float64, device="cuda"))[1]
+    got, = torch.autograd.grad(y, b, gy)
+    within(got, val, bound + (half_step(BF16) * (val.abs() + bound) if dtype == BF16 else 0), "gb")
+    full = torch.autograd.grad(vit_ops.linear8(x, w.clone().requires_grad_(True), b), b, gy)[0]      # asked for alone, the weight could have had one
+    within(full, val, bound + (half_step(BF16) * (val.abs() + bound) if dtype == BF16 else 0), "gb beside a weight")
+
+
+@gpu
 def test_results_can_be_changed_in_place():
     x, w, b = (torch.randn(*s, generator=gen(15), device="cuda").requires_grad_(True) for s in ((2, 3, 32), (16, 32), (16,)))
     for call in (lambda t: vit_ops.linear8(t, w, b), lambda t: vit_ops.linear8(t, w), lambda t: vit_ops.linear8(t[0], w, b), lambda t: vit_ops.linear8(t[0, 0], w, b), vit_ops.gelu8,
