@@ -266,6 +266,55 @@ def test_a_captured_backward_pass_beside_an_eager_graph_is_refused():
             assert torch.equal(got, want), name
 
 
+@gpu
+def test_exceptions_keep_their_type():
+    """what a saved-tensor hook raises, and torch's own errors, arrive as they are"""
+    class Stop(Exception):
+        pass
+
+    def hook(t):
+        raise Stop("stop")
+    for i, (call, args) in enumerate(_entries()[:4]):
+        with pytest.raises(Stop), torch.autograd.graph.saved_tensors_hooks(hook, lambda t: t):
+            call(*[t.requires_grad_(True) for t in args])
+    huge = torch.zeros(1, 8192, device="cuda").expand(1 << 26, 8192)             # 2 TiB as rows of their own
+    with pytest.raises(torch.OutOfMemoryError):
+        vit_ops.layer_norm(huge)
+    with pytest.raises(TypeError):
+        vit_ops.layer_norm(torch.zeros(2, 8, device="cuda"), eps="small")
+
+
+@gpu
+@pytest.mark.parametrize("reentrant", [False, True])
+@pytest.mark.parametrize("last", ["linear8", "gelu8", "attention", "norm"])
+def test_inside_a_checkpointed_block(last, reentrant):
+    """torch.utils.checkpoint ends the second forward pass by an exception of its own out of the last saved tensor"""
+    from torch.utils.checkpoint import checkpoint
+    g = gen(76)
+    new = lambda *s: torch.randn(*s, generator=g, device="cuda").requires_grad_(True)
+    x, n, w1, b1, w2 = new(2, 20, 64), new(64), new(96, 64), new(96), new(64, 96)
+
+    def block(t):
+        y = vit_ops.linear8(vit_ops.gelu8(vit_ops.linear8(vit_ops.layer_norm(t, n), w1, b1)), w2)
+        if last == "linear8":
+            return y
+        if last == "gelu8":
+            return vit_ops.gelu8(y)
+        if last == "norm":
+            return vit_ops.layer_norm(y, n, residual=t)[1]
+        return vit_ops.cross_attention(*(y.unflatten(2, (2, 32)) for _ in range(3)))
+    plain, kept = block(x), checkpoint(block, x, use_reentrant=reentrant)
+    go = torch.randn(plain.shape, generator=g, device="cuda")
+    grads = []
+    for out in (plain, kept):
+        for t in (x, n, w1, b1, w2):
+            t.grad = None
+        out.backward(go)
+        grads.append([t.grad for t in (x, n, w1, b1, w2)])
+    assert torch.equal(plain, kept)
+    assert all(torch.equal(a, c) for a, c in zip(*grads))
+
+
 # ---- sizes ---------------------------------------------------------------------------------------------------------------------------------------
 @gpu
 def test_linear8_refuses_at_once_what_its_backward_pass_cannot_take():
