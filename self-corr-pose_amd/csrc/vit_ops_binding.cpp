@@ -76,6 +76,10 @@ Tensor tensor(const py::handle& o, const char* name, std::initializer_list<at::S
     if (t.get_device() != device)
         refuse(std::string(name) + " lives on cuda:" + std::to_string(t.get_device()) + " but the current device is cuda:" + std::to_string(device) +
                " (torch.cuda.set_device first)");
+    // a subclass that answers for its operations itself, a wrapper of torch.func, a zero tensor: a null pointer would pass for an operand that is
+    // left out
+    constexpr c10::DispatchKeySet others({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::ZeroTensor});
+    if (t.key_set().has_any(others)) refuse(std::string(name) + " is a tensor without memory of its own");
     // autograd's nodes of this file know neither: without the refusal the tangent would be dropped, the traced result kept as a constant
     if (t._fw_grad(/*level=*/0).defined()) refuse(std::string(name) + " has a forward-mode tangent: the operators of scp_amd.vit_ops have no forward-mode derivative");
     if (torch::jit::tracer::isTracing()) refuse(std::string(name) + ": the operators of scp_amd.vit_ops cannot be traced (torch.jit.trace)");

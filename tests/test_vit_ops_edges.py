@@ -315,6 +315,29 @@ def test_inside_a_checkpointed_block(last, reentrant):
     assert all(torch.equal(a, c) for a, c in zip(*grads))
 
 
+@gpu
+def test_tensors_without_memory_of_their_own_are_refused():
+    """a subclass that answers for its operations itself (a distributed or a fake tensor), a zero tensor: nothing is there to be read"""
+    class Answers(torch.Tensor):
+        @staticmethod
+        def __new__(cls, t):
+            return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, f, types, args=(), kwargs=None):
+            return args[0]
+    for i, (call, args) in enumerate(_entries()):
+        with pytest.raises(RuntimeError, match="memory"):                        # torch.func's wrappers are no plain tensors either
+            torch.func.vmap(call)(*[t[None] for t in args])
+        with pytest.raises(RuntimeError, match="memory"):
+            torch.func.grad(lambda *a: call(*a).sum())(*args)
+        for j in range(len(args)):
+            for odd in (Answers(args[j]), torch._efficientzerotensor(args[j].shape, device="cuda")):
+                with pytest.raises(RuntimeError, match="memory"):
+                    call(*[odd if n == j else t for n, t in enumerate(args)])
+                    pytest.fail("operand %d of call %d was not refused" % (j, i))
+
+
 # ---- sizes ---------------------------------------------------------------------------------------------------------------------------------------
 @gpu
 def test_linear8_refuses_at_once_what_its_backward_pass_cannot_take():
