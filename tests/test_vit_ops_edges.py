@@ -398,6 +398,76 @@ def test_layer_norm_of_more_rows_than_one_launch_holds():
         within(gx[part], *ref["gx"], "gx")
 
 
+# ---- more than 2^31 elements ---------------------------------------------------------------------------------------------------------------------
+def _far(rows, c, seed):
+    return torch.empty(rows, c, dtype=BF16, device="cuda").normal_(generator=gen(seed))
+
+
+ENDS = (slice(0, 40), slice(-40, None))
+
+
+@gpu
+def test_layer_norm_past_32_bits():
+    """rows are independent: both ends are what they are alone, bit for bit"""
+    rows, c = (1 << 18) + 37, 8192
+    x, w = _far(rows, c, 1).requires_grad_(True), torch.randn(c, generator=gen(2), device="cuda")
+    total, y = vit_ops.layer_norm(x, w, residual=x.detach())
+    gx, = torch.autograd.grad((total, y), x, (x.detach(), y.detach()))
+    for part in ENDS:
+        xs = x.detach()[part].clone().requires_grad_(True)
+        ts, ys = vit_ops.layer_norm(xs, w, residual=xs.detach())
+        gs, = torch.autograd.grad((ts, ys), xs, (xs.detach(), ys.detach()))
+        assert torch.equal(total[part], ts) and torch.equal(y[part], ys) and torch.equal(gx[part], gs)
+
+
+@gpu
+@pytest.mark.parametrize("c", [32768, 32757])
+def test_checkpoints_past_32_bits(c):
+    rows = (1 << 31) // c + 50
+    x = _far(rows, c, 3).requires_grad_(True)
+    y = vit_ops.gelu8(x)
+    gx, = torch.autograd.grad(y, x, x.detach())
+    p = vit_ops.pack8(x)
+    back = p.unpack()
+    for part in ENDS:
+        xs = x.detach()[part].clone().requires_grad_(True)
+        ys, ps = vit_ops.gelu8(xs), vit_ops.pack8(xs)
+        gs, = torch.autograd.grad(ys, xs, xs.detach())
+        assert torch.equal(y[part], ys) and torch.equal(gx[part], gs) and torch.equal(p.codes[part], ps.codes) and torch.equal(p.exps[part], ps.exps) and torch.equal(back[part], ps.unpack())
+
+
+@gpu
+def test_weight_grad8_past_32_bits():
+    """the last rows alone differ from zero: what they give is what they give alone, up to the order of the sums"""
+    rows, n, k = (1 << 20) + 333, 2056, 40
+    gy, x = torch.zeros(rows, n, dtype=BF16, device="cuda"), torch.zeros(rows, k, dtype=BF16, device="cuda")
+    last = slice(rows - 300, rows)
+    gy[last], x[last] = _far(300, n, 4), _far(300, k, 5)
+    ref_w, ref_b = wgrad_reference(gy[last], vit_ops.pack8(x[last].contiguous()).unpack(FP32).double())
+    gw, gb = vit_ops.weight_grad8(gy, vit_ops.pack8(x))
+    within(gw, *ref_w, "gw")
+    within(gb, *ref_b, "gb")
+
+
+@gpu
+@pytest.mark.parametrize("dtype,nq", [(BF16, 300007), (FP32, 150011)], ids=["bf16", "fp32"])
+def test_attention_of_queries_past_32_bits(dtype, nq):
+    """the results of rows past 2^31 elements (of the parts, in fp32) against the definition; gk and gv are those of a gradient of these rows alone"""
+    h, d, nk, part = 120, 64, 40, slice(nq - 60, nq)
+    k, v = (torch.randn(1, nk, h, d, generator=gen(6 + i), device="cuda").to(dtype).requires_grad_(True) for i in range(2))
+    q = torch.empty(1, nq, h, d, dtype=dtype, device="cuda").normal_(generator=gen(8)).requires_grad_(True)
+    o = vit_ops.cross_attention(q, k, v)
+    go = torch.zeros_like(q, requires_grad=False)
+    go[:, part] = torch.randn(1, 60, h, d, generator=gen(9), device="cuda").to(dtype)
+    gq, gk, gv = torch.autograd.grad(o, (q, k, v), go)
+    ref = attn_reference(q.detach()[:, part], k.detach(), v.detach(), None, d ** -0.5, go[:, part], dtype)
+    within(o.detach()[:, part], *ref["o"], "o")
+    within(gq[:, part], *ref["gq"], "gq")
+    within(gk, *ref["gk"], "gk")                                                 # (every other term is 0)
+    within(gv, *ref["gv"], "gv")
+    assert not gq[:, :nq - 60].any()
+
+
 # ---- 8-bit checkpoints --------------------------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
