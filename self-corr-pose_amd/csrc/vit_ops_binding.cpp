@@ -10,6 +10,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 #include <torch/version.h>
@@ -130,6 +131,12 @@ void check_capture() {
     if (status == hipStreamCaptureStatusNone) return;
     const auto self = torch::autograd::get_current_node();
     if (!self) return;
+    const auto* plan = torch::autograd::get_current_graph_task_exec_info();     // empty: everything runs
+    auto runs = [&](torch::autograd::Node* node) {
+        if (!plan || plan->empty()) return true;
+        const auto it = plan->find(node);
+        return it != plan->end() && it->second.should_execute();
+    };
     std::vector<torch::autograd::Node*> todo{self.get()};
     std::unordered_set<torch::autograd::Node*> seen{self.get()};
     while (!todo.empty()) {
@@ -142,7 +149,7 @@ void check_capture() {
                        "results first, or capture with leaves of their own (detach().requires_grad_())");
         }
         for (const auto& edge : node->next_edges())
-            if (edge.function && seen.insert(edge.function.get()).second) todo.push_back(edge.function.get());
+            if (edge.function && runs(edge.function.get()) && seen.insert(edge.function.get()).second) todo.push_back(edge.function.get());
     }
 }
 // Gradients of a backward pass that is itself recorded (create_graph) cannot be differentiated again: they get a node that says so.

@@ -338,6 +338,27 @@ def test_tensors_without_memory_of_their_own_are_refused():
                     pytest.fail("operand %d of call %d was not refused" % (j, i))
 
 
+@gpu
+@pytest.mark.child_process
+def test_a_captured_backward_pass_that_does_not_reach_the_eager_leaf():
+    """gradients of x alone, while an eager graph of the weight is alive: nothing of that graph runs"""
+    g = gen(79)
+    x, w, gy = (torch.randn(*s, generator=g, device="cuda") for s in ((40, 96), (48, 96), (40, 48)))
+    w.requires_grad_(True)
+    alive = w * 1.0
+    leaf = x.clone().requires_grad_(True)
+    want, = torch.autograd.grad(vit_ops.linear8(vit_ops.gelu8(leaf), w), leaf, gy)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inner = x.detach().requires_grad_(True)
+        got, = torch.autograd.grad(vit_ops.linear8(vit_ops.gelu8(inner), w), inner, gy)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    assert alive.requires_grad
+
+
 # ---- sizes ---------------------------------------------------------------------------------------------------------------------------------------
 @gpu
 def test_linear8_refuses_at_once_what_its_backward_pass_cannot_take():
