@@ -13,7 +13,7 @@ src1.hi) return a wrong low half in ~0.6 % of the lanes while a K-doubled 16-bit
 SIMD -- every other op_sel / op_sel_hi / neg combination, the high half, 16-bit packed ops and scalar VALU are exact (self-checking
 probes over all 51 combinations, profiles/r05_packed_fp32_erratum.txt).  hipcc's SLP vectoriser emits that form for cross products
 (x1*y2 - x2*y1: the rasteriser's per-face kernel).  What keeps the overlapped schedule safe now:
-  * every file of the library that is not itself a bf16 GEMM is compiled with the packed-fp32 feature switched off (build.py NO_PACKED) and
+  * every file of the library but the erratum's self-test is compiled with the packed-fp32 feature switched off (build.py NO_PACKED) and
     a CPU test disassembles the shipped code objects: no packed-fp32 instruction with ANY op_sel in 220 kernels
     (tests/test_capi_symbols.py);
   * the library kernels of the step (ATen, rocprim, the remaining fp32 rocBLAS / hipBLASLt products, RCCL) are held by the screen below, by
